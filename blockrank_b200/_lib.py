@@ -24,7 +24,8 @@ EXPORTS = ("brk_version", "brk_last_error", "brk_launch_count", "brk_device_chec
            "brk_doc_scores_workspace_bytes",
            "brk_doc_scores", "brk_doc_scores_static", "brk_raw_scores",
            "brk_raw_scores_bwd_workspace_bytes", "brk_raw_scores_bwd", "brk_signal_rows", "brk_rank_pack", "brk_rmsnorm",
-           "brk_rope", "brk_silu_mul")
+           "brk_rope", "brk_silu_mul", "brk_cache_page_bytes", "brk_cache_write_workspace_bytes", "brk_cache_write", "brk_cache_read",
+           "brk_cache_attn_workspace_bytes", "brk_cache_attn", "brk_cache_doc_scores_workspace_bytes", "brk_cache_doc_scores")
 
 
 class View(C.Structure):
@@ -52,6 +53,23 @@ class ScoreParams(C.Structure):
                 ("temperature", C.c_float), ("q", View), ("k", View), ("rows", C.c_void_p),
                 ("blk_start", C.c_void_p), ("blk_len", C.c_void_p), ("doc_mass", C.c_void_p),
                 ("logits", C.c_void_p)]
+
+
+class Cache(C.Structure):
+    _fields_ = [("pages", C.c_void_p), ("n_pages", C.c_int32), ("Nk", C.c_int32), ("D", C.c_int32)]
+
+
+class CacheAttnParams(C.Structure):
+    _fields_ = [("dtype", C.c_int32), ("B", C.c_int32), ("N", C.c_int32), ("Lq", C.c_int32), ("M", C.c_int32), ("P", C.c_int32),
+                ("scale", C.c_float), ("cache", Cache), ("q", View), ("o", View), ("page_table", C.c_void_p),
+                ("blk_start", C.c_void_p), ("blk_len", C.c_void_p), ("q_len", C.c_void_p), ("lse", C.c_void_p), ("status", C.c_void_p)]
+
+
+class CacheScoreParams(C.Structure):
+    _fields_ = [("dtype", C.c_int32), ("B", C.c_int32), ("N", C.c_int32), ("R", C.c_int32), ("M", C.c_int32), ("P", C.c_int32),
+                ("max_block_len", C.c_int32), ("scale", C.c_float), ("temperature", C.c_float), ("cache", Cache), ("q", View),
+                ("page_table", C.c_void_p), ("blk_start", C.c_void_p), ("blk_len", C.c_void_p), ("doc_mass", C.c_void_p),
+                ("logits", C.c_void_p), ("status", C.c_void_p)]
 
 
 class BlockRankLibraryError(RuntimeError):
@@ -104,6 +122,24 @@ def lib() -> C.CDLL:
     L.brk_raw_scores_bwd.restype = C.c_int
     L.brk_raw_scores_bwd.argtypes = [C.POINTER(ScoreParams), C.c_void_p, C.POINTER(View), C.POINTER(View), C.c_int32,
                                      C.c_void_p, C.c_size_t, C.c_void_p]
+    L.brk_cache_page_bytes.restype = C.c_size_t
+    L.brk_cache_page_bytes.argtypes = [C.c_int32, C.c_int32]
+    L.brk_cache_write_workspace_bytes.restype = C.c_size_t
+    L.brk_cache_write_workspace_bytes.argtypes = [C.POINTER(Cache), C.c_int32, C.c_int32]
+    L.brk_cache_write.restype = C.c_int
+    L.brk_cache_write.argtypes = [C.c_int32, C.POINTER(Cache), C.POINTER(View), C.POINTER(View), C.c_int32, C.c_int32, C.c_void_p,
+                                  C.c_void_p, C.c_size_t, C.c_void_p, C.c_void_p]
+    L.brk_cache_read.restype = C.c_int
+    L.brk_cache_read.argtypes = [C.c_int32, C.POINTER(Cache), C.POINTER(View), C.POINTER(View), C.c_int32, C.c_int32, C.c_void_p,
+                                 C.c_void_p, C.c_void_p]
+    L.brk_cache_attn_workspace_bytes.restype = C.c_size_t
+    L.brk_cache_attn_workspace_bytes.argtypes = [C.POINTER(CacheAttnParams)]
+    L.brk_cache_attn.restype = C.c_int
+    L.brk_cache_attn.argtypes = [C.POINTER(CacheAttnParams), C.c_void_p, C.c_size_t, C.c_void_p]
+    L.brk_cache_doc_scores_workspace_bytes.restype = C.c_size_t
+    L.brk_cache_doc_scores_workspace_bytes.argtypes = [C.POINTER(CacheScoreParams)]
+    L.brk_cache_doc_scores.restype = C.c_int
+    L.brk_cache_doc_scores.argtypes = [C.POINTER(CacheScoreParams), C.c_void_p, C.c_size_t, C.c_void_p]
     L.brk_rmsnorm.restype = C.c_int
     L.brk_rmsnorm.argtypes = [C.c_int32, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int64, C.c_int32,
                               C.c_float, C.c_void_p]

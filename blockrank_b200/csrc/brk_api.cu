@@ -1,5 +1,6 @@
 // C ABI of libblockrank_b200: argument validation, error reporting and dispatch.
 // No entry point allocates device memory; all work is enqueued on the caller's stream.
+#include <math.h>
 #include <stdarg.h>
 #include <string.h>
 
@@ -171,6 +172,16 @@ int brk_status_poll(int32_t* status, void* stream) {
     set_error("a signal row lies outside the prompt's slots [0, S)");
     return BRK_E_ARG;
   }
+  if (v == kStatusBadSlot) {
+    set_error("a slot lies outside the cache: the token was left out");
+    return BRK_E_ARG;
+  }
+  if (v == kStatusBadCacheCall) {
+    set_error("malformed block spans, page table or number of rows of a call on the cache (blocks that overlap or reach past the page "
+              "table, a page outside the cache, a document longer than max_block_len, more rows than the last block has tokens): that "
+              "prompt or page was left out");
+    return BRK_E_ARG;
+  }
   set_error("a bounded device-side wait gave up (code %d: %s); the outputs of that call are incomplete", v,
             v >= kStatusSelfTest ? "self-test" : v < 20 ? "TMA warp" : v < 30 ? "MMA warp"
             : v == 34 || v == 35 || v == 38 || v == 39 ? "output warp" : v < 40 ? "softmax warp" : v < 60 ? "job ring" : "backward");
@@ -254,6 +265,112 @@ int brk_silu_mul(int32_t dtype, const void* gate_up, void* out, int64_t rows, in
   BRK_REQUIRE(rows * (inter / 8) / 256 < (1ll << 31), BRK_E_ARG, "silu_mul problem too large");
   BRK_REQUIRE((((uintptr_t)gate_up | (uintptr_t)out) & 15) == 0, BRK_E_ARG, "silu_mul buffers must be 16-byte aligned");
   return silu_mul_launch(dtype, gate_up, out, rows, inter, (cudaStream_t)stream);
+}
+
+// ---- 4-bit cache ----
+static int check_cache(const brk_cache* c) {
+  BRK_REQUIRE(c != nullptr && c->pages != nullptr, BRK_E_ARG, "cache is null");
+  BRK_REQUIRE(((uintptr_t)c->pages & 15) == 0, BRK_E_ARG, "cache must be 16-byte aligned");
+  BRK_REQUIRE(c->D == 64 || c->D == 128, BRK_E_UNSUPPORTED, "head_dim %d not supported (64 or 128)", c->D);
+  BRK_REQUIRE(c->Nk > 0 && c->n_pages > 0 && (int64_t)c->n_pages * BRK_CACHE_PAGE < (1ll << 31), BRK_E_ARG,
+              "bad cache shape: %d pages, %d KV heads", c->n_pages, c->Nk);
+  return BRK_OK;
+}
+
+static int check_cache_tokens(int32_t dtype, const brk_cache* c, const brk_view* k, const brk_view* v, int32_t B, int32_t S,
+                              const int32_t* slots) {
+  int rc = check_cache(c);
+  if (rc) return rc;
+  BRK_REQUIRE(dtype == BRK_BF16 || dtype == BRK_F32, BRK_E_UNSUPPORTED, "dtype %d not supported", dtype);
+  BRK_REQUIRE(k && v && slots, BRK_E_ARG, "null pointer");
+  BRK_REQUIRE(B > 0 && S > 0 && (int64_t)B * S < (1ll << 31), BRK_E_ARG, "bad shape B=%d S=%d", B, S);
+  BRK_REQUIRE((int64_t)B * S * c->Nk * (c->D / 8) / 256 < (1ll << 31) - 1, BRK_E_ARG, "too many tokens: B=%d S=%d", B, S);
+  if ((rc = check_view(*k, dtype, "k"))) return rc;
+  return check_view(*v, dtype, "v");
+}
+
+// what the attention and the scores share
+static int check_cache_call(const brk_cache& c, int32_t dtype, int B, int N, int rows, int M, int P, float scale, const brk_view& q,
+                            const int32_t* table, const int32_t* start, const int32_t* len) {
+  const int rc = check_cache(&c);
+  if (rc) return rc;
+  BRK_REQUIRE(dtype == BRK_BF16 || dtype == BRK_F32, BRK_E_UNSUPPORTED, "dtype %d not supported", dtype);
+  BRK_REQUIRE(B > 0 && N > 0 && rows > 0 && M > 0 && P > 0, BRK_E_ARG, "bad shape B=%d N=%d rows=%d M=%d P=%d", B, N, rows, M, P);
+  BRK_REQUIRE(N % c.Nk == 0, BRK_E_ARG, "N=%d is not a multiple of Nk=%d", N, c.Nk);
+  BRK_REQUIRE((int64_t)P * BRK_CACHE_PAGE < (1ll << 31) && (int64_t)B * N * rows < (1ll << 31), BRK_E_ARG, "too large: B=%d N=%d rows=%d P=%d",
+              B, N, rows, P);
+  BRK_REQUIRE((int64_t)B * c.Nk <= 65535, BRK_E_UNSUPPORTED, "B*Nk too large");
+  BRK_REQUIRE(scale > 0.f && scale < INFINITY, BRK_E_ARG, "softmax scale must be positive");
+  BRK_REQUIRE(table && start && len, BRK_E_ARG, "page table / block spans are null");
+  return check_view(q, dtype, "q");
+}
+
+size_t brk_cache_page_bytes(int32_t Nk, int32_t D) {
+  return Nk > 0 && (D == 64 || D == 128) ? (size_t)Nk * BRK_CACHE_PAGE * (D + D / 8) : 0;
+}
+
+size_t brk_cache_write_workspace_bytes(const brk_cache* c, int32_t B, int32_t S) {
+  return c && c->n_pages > 0 ? cache_write_workspace(*c, B, S) : 0;
+}
+
+int brk_cache_write(int32_t dtype, const brk_cache* c, const brk_view* k, const brk_view* v, int32_t B, int32_t S, const int32_t* slots,
+                    void* workspace, size_t workspace_bytes, int32_t* status, void* stream) {
+  const int rc = check_cache_tokens(dtype, c, k, v, B, S, slots);
+  if (rc) return rc;
+  const size_t need = cache_write_workspace(*c, B, S);
+  BRK_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && ((uintptr_t)workspace & 15) == 0), BRK_E_WORKSPACE,
+              "workspace %zu < %zu bytes (or not 16-byte aligned)", workspace_bytes, need);
+  return cache_write_launch(dtype, *c, *k, *v, B, S, slots, workspace, status, (cudaStream_t)stream);
+}
+
+int brk_cache_read(int32_t dtype, const brk_cache* c, const brk_view* k, const brk_view* v, int32_t B, int32_t S, const int32_t* slots,
+                   int32_t* status, void* stream) {
+  const int rc = check_cache_tokens(dtype, c, k, v, B, S, slots);
+  if (rc) return rc;
+  return cache_read_launch(dtype, *c, *k, *v, B, S, slots, status, (cudaStream_t)stream);
+}
+
+static int check_cache_attn(const brk_cache_attn_params* p) {
+  BRK_REQUIRE(p != nullptr, BRK_E_ARG, "params is null");
+  return check_cache_call(p->cache, p->dtype, p->B, p->N, p->Lq, p->M, p->P, p->scale, p->q, p->page_table, p->blk_start, p->blk_len);
+}
+
+size_t brk_cache_attn_workspace_bytes(const brk_cache_attn_params* p) {
+  return check_cache_attn(p) == BRK_OK ? cache_attn_workspace(*p) : 0;  // (the call refuses the others)
+}
+
+int brk_cache_attn(const brk_cache_attn_params* p, void* workspace, size_t workspace_bytes, void* stream) {
+  int rc = check_cache_attn(p);
+  if (rc || (rc = check_view(p->o, p->dtype, "o"))) return rc;
+  const size_t need = cache_attn_workspace(*p);
+  BRK_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && ((uintptr_t)workspace & 15) == 0), BRK_E_WORKSPACE,
+              "workspace %zu < %zu bytes (or not 16-byte aligned)", workspace_bytes, need);
+  return cache_attn_launch(*p, workspace, (cudaStream_t)stream);
+}
+
+static int check_cache_scores(const brk_cache_score_params* p) {
+  BRK_REQUIRE(p != nullptr, BRK_E_ARG, "params is null");
+  const int rc = check_cache_call(p->cache, p->dtype, p->B, p->N, p->R, p->M, p->P, p->scale, p->q, p->page_table, p->blk_start, p->blk_len);
+  if (rc) return rc;
+  BRK_REQUIRE(p->M >= 3, BRK_E_ARG, "document scores need at least one document block (M=%d)", p->M);
+  BRK_REQUIRE(p->R <= 64 && (p->N / p->cache.Nk) * p->R <= 256, BRK_E_ARG, "R=%d out of range", p->R);
+  BRK_REQUIRE(p->max_block_len > 0, BRK_E_ARG, "max_block_len=%d out of range", p->max_block_len);
+  BRK_REQUIRE(p->temperature > 0.f, BRK_E_ARG, "temperature must be positive");
+  return BRK_OK;
+}
+
+size_t brk_cache_doc_scores_workspace_bytes(const brk_cache_score_params* p) {
+  return check_cache_scores(p) == BRK_OK ? cache_scores_workspace(*p) : 0;
+}
+
+int brk_cache_doc_scores(const brk_cache_score_params* p, void* workspace, size_t workspace_bytes, void* stream) {
+  const int rc = check_cache_scores(p);
+  if (rc) return rc;
+  BRK_REQUIRE(p->doc_mass != nullptr, BRK_E_ARG, "doc_mass is null");
+  const size_t need = cache_scores_workspace(*p);
+  BRK_REQUIRE(workspace && workspace_bytes >= need && ((uintptr_t)workspace & 15) == 0, BRK_E_WORKSPACE,
+              "workspace %zu < %zu bytes (or not 16-byte aligned)", workspace_bytes, need);
+  return cache_scores_launch(*p, workspace, (cudaStream_t)stream);
 }
 
 }  // extern "C"

@@ -140,10 +140,12 @@ inline View make_view(const brk_view& v) { return View{(char*)v.ptr, v.stride_b,
 constexpr size_t kWsHeader = 256;
 // Values of the caller's status word: 10..49 (forward) and 60..80 (backward) name the bounded wait that gave up first in its thread
 // (10..19 TMA warp, 20..29 MMA warps, 34, 35, 38, 39 output warps, other 30..39 softmax warps, 40, 41 one of the last three at
-// the job ring; even numbers chain 0, odd ones chain 1), 50 malformed block spans, 51 a signal row outside the prompt, 90 the
-// self-test's wait, 91 a self-test that found something else.
+// the job ring; even numbers chain 0, odd ones chain 1), 50 malformed block spans, 51 a signal row outside the prompt, 52 a slot
+// outside the cache, 53 malformed spans, pages or rows of a call on the cache, 90 the self-test's wait, 91 a self-test that found something else.
 constexpr int kStatusBadSpans = 50;
 constexpr int kStatusBadRows = 51;
+constexpr int kStatusBadSlot = 52;
+constexpr int kStatusBadCacheCall = 53;
 constexpr int kStatusSelfTest = 90;
 
 // kernel launchers implemented in the .cu files
@@ -196,4 +198,13 @@ int rank_pack_launch(const float* logits, int B, int nd, int k, float* out, int6
 int signal_rows_launch(const void* x, int row_bytes, const int32_t* pos, const int32_t* rows, int B, int S, int R, void* x_out,
                        int32_t* pos_out, int32_t* local, int32_t* status, cudaStream_t st);
 int silu_mul_launch(int dtype, const void* gu, void* out, int64_t rows, int inter, cudaStream_t st);
+size_t cache_write_workspace(const brk_cache& c, int B, int S);
+int cache_write_launch(int dtype, const brk_cache& c, const brk_view& k, const brk_view& v, int B, int S, const int32_t* slots, void* ws,
+                       int32_t* status, cudaStream_t st);
+int cache_read_launch(int dtype, const brk_cache& c, const brk_view& k, const brk_view& v, int B, int S, const int32_t* slots,
+                      int32_t* status, cudaStream_t st);
+size_t cache_attn_workspace(const brk_cache_attn_params& p);
+int cache_attn_launch(const brk_cache_attn_params& p, void* ws, cudaStream_t st);
+size_t cache_scores_workspace(const brk_cache_score_params& p);
+int cache_scores_launch(const brk_cache_score_params& p, void* ws, cudaStream_t st);
 }  // namespace brk

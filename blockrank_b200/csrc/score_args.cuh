@@ -33,6 +33,8 @@ inline ScoreArgs make_score_args(const brk_score_params& p) {
   return a;
 }
 
+int doc_merge_launch(const ScoreArgs& a, cudaStream_t st);
+
 inline int check_score_params(const brk_score_params& p) {
   BRK_REQUIRE(p.q.ptr && p.k.ptr && p.blk_start && p.blk_len, BRK_E_ARG, "null pointer in score params");
   BRK_REQUIRE(p.B > 0 && p.N > 0 && p.Nk > 0 && p.N % p.Nk == 0 && p.S > 0 && p.M >= 1, BRK_E_ARG,

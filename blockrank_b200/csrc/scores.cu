@@ -398,6 +398,19 @@ __global__ void __launch_bounds__(kThreads, 4) doc_partial_mma_kernel(ScoreArgs 
 
 }  // namespace
 
+// Merge of every prompt's pairs (a.partial) into masses and logits.
+// The merge of one prompt: up to 16,384 pairs on one SM, more on up to eight.  One prompt of 300 documents (19,200 pairs) 31.1
+// us on one, 28.4 on eight, of 500 with 16 signal rows 220 and 133, of 2,000 with 16 rows 600 and 248; 16 prompts of 250
+// (16,000 pairs each) 101 and 104, 4 of 100 (6,400) 29.3 and 30.0.  (With every prompt on one, more than 100,000 pairs took
+// longer than when the CTA of each KV head that finished last merged its rows: 206 us for 500 with 16 rows, 411 for 2,000.)
+int doc_merge_launch(const ScoreArgs& a, cudaStream_t st) {
+  int merge_ctas = 1;
+  if ((int64_t)a.N * a.R * (a.M - 2) > 16384)
+    while (2 * merge_ctas <= std::min(a.Nk, 8)) merge_ctas *= 2;
+  if (merge_ctas == 1) return launch_dependent(doc_merge_kernel<false>, dim3(a.B), dim3(merge_threads<false>), 0, st, a);
+  return launch_dependent_clusters(merge_ctas, doc_merge_kernel<true>, dim3(merge_ctas, a.B), dim3(merge_threads<true>), 0, st, a);
+}
+
 // scratch: the [B, N, R, nd] (max, sum) pairs
 static size_t partial_bytes(const brk_score_params& p) {
   const size_t nd = p.M > 2 ? p.M - 2 : 0;
@@ -423,17 +436,7 @@ static int doc_scores_run(const brk_score_params& p, void* ws, size_t ws_bytes, 
   dim3 grid(nd, p.B * p.Nk);
   const size_t pitch = (size_t)p.D * (p.dtype == BRK_BF16 ? 2 : 4) + 16;
   const size_t sm = (size_t)G * p.R * p.D * 4 + (kThreads / 32) * kRowBatch * sizeof(float2) + (kThreads / 32) * 32 * pitch;
-  // The merge of one prompt: up to 16,384 pairs on one SM, more on up to eight.  One prompt of 300 documents (19,200 pairs) 31.1
-  // us on one, 28.4 on eight, of 500 with 16 signal rows 220 and 133, of 2,000 with 16 rows 600 and 248; 16 prompts of 250
-  // (16,000 pairs each) 101 and 104, 4 of 100 (6,400) 29.3 and 30.0.  (With every prompt on one, more than 100,000 pairs took
-  // longer than when the CTA of each KV head that finished last merged its rows: 206 us for 500 with 16 rows, 411 for 2,000.)
-  int merge_ctas = 1;
-  if ((int64_t)p.N * p.R * nd > 16384)
-    while (2 * merge_ctas <= std::min(p.Nk, 8)) merge_ctas *= 2;
-  auto merge = [&]() -> int {
-    if (merge_ctas == 1) return launch_dependent(doc_merge_kernel<false>, dim3(p.B), dim3(merge_threads<false>), 0, st, a);
-    return launch_dependent_clusters(merge_ctas, doc_merge_kernel<true>, dim3(merge_ctas, p.B), dim3(merge_threads<true>), 0, st, a);
-  };
+  auto merge = [&]() -> int { return doc_merge_launch(a, st); };
   auto launch = [&](auto kern) -> int {
     // (the kernels also hold a few KB of static shared memory, which counts against the same 48 KB default)
     if (sm + 8192 > 48 * 1024) BRK_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sm));

@@ -397,6 +397,172 @@ std::tuple<Tensor, OptTensor> attention_forward(const Tensor& q, const Tensor& k
   return {out, raw.defined() ? OptTensor(raw) : std::nullopt};
 }
 
+// ---- 4-bit cache --------------------------------------------------------------------------------
+// uint8 (n_pages, Nk, bytes of a page's head), contiguous; the number of bytes tells the head dim.
+brk_cache cache_of(const Tensor& c) {
+  BRK_VALUE(c.scalar_type() == at::kByte && c.dim() == 3 && c.is_contiguous(), "cache must be a contiguous uint8 (n_pages, kv_heads, bytes) tensor of "
+            "cache_alloc, got ", c.scalar_type(), " ", c.sizes());
+  brk_cache r{};
+  for (int d : {64, 128})
+    if (c.size(2) == (int64_t)brk_cache_page_bytes(1, d)) r.D = d;
+  BRK_VALUE(r.D != 0 && c.size(0) < (1ll << 31) && c.size(1) < (1ll << 31), "cache must be a contiguous uint8 (n_pages, kv_heads, bytes) tensor of "
+            "cache_alloc, got ", c.sizes());
+  r.pages = c.data_ptr();
+  r.n_pages = (int32_t)c.size(0);
+  r.Nk = (int32_t)c.size(1);
+  return r;
+}
+void need_device(const Tensor& of, std::initializer_list<const Tensor*> ts) {
+  for (const Tensor* t : ts)
+    if (t != nullptr && t->defined()) BRK_VALUE(t->device() == of.device(), "tensors on ", of.device(), " and ", t->device());
+}
+// view_of, for any stride of a dimension of one
+brk_view heads_view(const Tensor& t) {
+  brk_view v = view_of(t);
+  if (t.size(0) == 1) v.stride_b = 0;
+  if (t.size(1) == 1) v.stride_h = 0;
+  if (t.size(2) == 1) v.stride_s = 0;
+  return v;
+}
+int32_t* status_ptr(const Tensor& t) { return (int32_t*)status_word(t.get_device()).data_ptr(); }
+
+Tensor cache_alloc(int64_t n_pages, int64_t kv_heads, int64_t head_dim, const c10::Device& device) {
+  BRK_VALUE(n_pages > 0 && n_pages * BRK_CACHE_PAGE < (1ll << 31) && kv_heads > 0 && kv_heads < (1ll << 31), "bad cache shape: ", n_pages, " pages, ",
+            kv_heads, " KV heads");
+  BRK_VALUE(head_dim == 64 || head_dim == 128, "head_dim ", head_dim, " not supported (64 or 128)");
+  TORCH_CHECK(device.is_cuda(), "blockrank_b200 kernels run on CUDA tensors only (there is no CPU path)");
+  return at::zeros({n_pages, kv_heads, (int64_t)brk_cache_page_bytes(1, (int32_t)head_dim)}, at::TensorOptions().dtype(at::kByte).device(device));
+}
+
+void cache_write(const Tensor& k, const Tensor& v, const Tensor& cache, const Tensor& slots_in) {
+  need_cuda({&k, &v, &cache, &slots_in});
+  need_device(cache, {&k, &v, &slots_in});
+  const brk_cache c = cache_of(cache);
+  BRK_VALUE(k.dim() == 4 && v.sizes() == k.sizes() && k.size(1) == c.Nk && k.size(3) == c.D, "k and v must be (B, ", c.Nk, ", S, ", c.D, ") tensors, got ",
+            k.sizes(), " and ", v.sizes());
+  BRK_VALUE(v.scalar_type() == k.scalar_type(), "k and v must share a dtype");
+  BRK_VALUE(slots_in.scalar_type() == at::kInt && slots_in.dim() == 2 && slots_in.size(0) == k.size(0) && slots_in.size(1) == k.size(2),
+            "slots must be int32 (", k.size(0), ", ", k.size(2), "), got ", slots_in.scalar_type(), " ", slots_in.sizes());
+  const int dtype = dtype_code(k);
+  if (slots_in.numel() == 0) return;
+  BRK_VALUE(slots_in.numel() < (1ll << 31), "too many tokens: ", slots_in.numel());
+  c10::cuda::CUDAGuard guard(cache.device());
+  const Tensor slots = slots_in.contiguous();
+  const brk_view vk = heads_view(k), vv = heads_view(v);
+  const int32_t B = (int32_t)k.size(0), S = (int32_t)k.size(2);
+  const size_t nbytes = brk_cache_write_workspace_bytes(&c, B, S);
+  Tensor ws;
+  if (nbytes > 0) ws = scratch(nbytes, cache);
+  check(brk_cache_write(dtype, &c, &vk, &vv, B, S, (const int32_t*)slots.data_ptr(), nbytes > 0 ? ws.data_ptr() : nullptr, nbytes, status_ptr(cache),
+                        stream_of(cache)),
+        "brk_cache_write");
+}
+
+std::tuple<Tensor, Tensor> cache_read(const Tensor& cache, const Tensor& slots_in, at::ScalarType dtype) {
+  need_cuda({&cache, &slots_in});
+  need_device(cache, {&slots_in});
+  const brk_cache c = cache_of(cache);
+  BRK_VALUE(slots_in.scalar_type() == at::kInt && slots_in.dim() == 2, "slots must be int32 (B, S), got ", slots_in.scalar_type(), " ", slots_in.sizes());
+  const int64_t B = slots_in.size(0), S = slots_in.size(1);
+  BRK_VALUE(slots_in.numel() < (1ll << 31), "too many tokens: ", slots_in.numel());
+  c10::cuda::CUDAGuard guard(cache.device());
+  const auto opts = cache.options().dtype(dtype);
+  const Tensor k = at::empty({B, S, c.Nk, c.D}, opts).permute({0, 2, 1, 3}), v = at::empty({B, S, c.Nk, c.D}, opts).permute({0, 2, 1, 3});
+  const int code = dtype_code(k);
+  if (slots_in.numel() == 0) return {k, v};
+  const Tensor slots = slots_in.contiguous();
+  const brk_view vk = heads_view(k), vv = heads_view(v);
+  check(brk_cache_read(code, &c, &vk, &vv, (int32_t)B, (int32_t)S, (const int32_t*)slots.data_ptr(), status_ptr(cache), stream_of(cache)),
+        "brk_cache_read");
+  return {k, v};
+}
+
+// page table (B, P) and spans (B, M) of the B prompts of q
+void need_prompts(const Tensor& q, const brk_cache& c, const Tensor& table, const Tensor& start, const Tensor& length) {
+  BRK_VALUE(q.dim() == 4 && q.size(3) == c.D, "q must be (B, heads, rows, ", c.D, "), got ", q.sizes());
+  const int64_t B = q.size(0);
+  BRK_VALUE(table.scalar_type() == at::kInt && table.dim() == 2 && table.size(0) == B, "page_table must be int32 (", B, ", pages), got ", table.scalar_type(), " ",
+            table.sizes());
+  BRK_VALUE(start.scalar_type() == at::kInt && length.scalar_type() == at::kInt && start.dim() == 2 && start.size(0) == B && start.sizes() == length.sizes(),
+            "blk_start / blk_len must be int32 tensors of the same (", B, ", M) shape, got ", start.sizes(), " / ", length.sizes());
+  for (int64_t n : {q.size(0), q.size(1), q.size(2), table.size(1), start.size(1)}) BRK_VALUE(n < (1ll << 31), "too large");
+}
+
+std::tuple<Tensor, Tensor> cache_attention(const Tensor& q, const Tensor& cache, const Tensor& table_in, const Tensor& blk_start, const Tensor& blk_len,
+                                           double scale, const OptTensor& q_len_in, const OptTensor& out_in, bool return_lse) {
+  need_cuda({&q, &cache, &table_in, &blk_start, &blk_len, opt(q_len_in), opt(out_in)});
+  need_device(cache, {&q, &table_in, &blk_start, &blk_len, opt(q_len_in), opt(out_in)});
+  const brk_cache c = cache_of(cache);
+  need_prompts(q, c, table_in, blk_start, blk_len);
+  const int64_t B = q.size(0), N = q.size(1), Lq = q.size(2);
+  const int dtype = dtype_code(q);
+  if (q_len_in.has_value())
+    BRK_VALUE(q_len_in->scalar_type() == at::kInt && q_len_in->dim() == 1 && q_len_in->size(0) == B, "q_len must be int32 (", B, ",), got ",
+              q_len_in->scalar_type(), " ", q_len_in->sizes());
+  c10::cuda::CUDAGuard guard(cache.device());
+  if (out_in.has_value())
+    BRK_VALUE(out_in->sizes() == at::IntArrayRef({B, Lq, N, c.D}) && out_in->scalar_type() == q.scalar_type(), "out must be ", q.scalar_type(), " (", B, ", ", Lq,
+              ", ", N, ", ", c.D, "), got ", out_in->scalar_type(), " ", out_in->sizes());
+  Tensor out = out_in.has_value() ? *out_in : empty_bshd(q, B, Lq, N, c.D);
+  Tensor lse;
+  if (return_lse) lse = at::empty({B, N, Lq}, q.options().dtype(at::kFloat).requires_grad(false));
+  if (out.numel() == 0) return {out, lse};
+  const Tensor table = table_in.contiguous(), bs = blk_start.contiguous(), bl = blk_len.contiguous();
+  const Tensor q_len = q_len_in.has_value() ? q_len_in->contiguous() : Tensor();
+  brk_cache_attn_params p{};
+  p.dtype = dtype;
+  p.B = (int32_t)B; p.N = (int32_t)N; p.Lq = (int32_t)Lq;
+  p.M = (int32_t)bs.size(1); p.P = (int32_t)table.size(1);
+  p.scale = (float)scale;
+  p.cache = c;
+  p.q = heads_view(q);
+  p.o = heads_view(out.permute({0, 2, 1, 3}));
+  p.page_table = (const int32_t*)table.data_ptr();
+  p.blk_start = (const int32_t*)bs.data_ptr();
+  p.blk_len = (const int32_t*)bl.data_ptr();
+  p.q_len = q_len.defined() ? (const int32_t*)q_len.data_ptr() : nullptr;
+  p.lse = return_lse ? (float*)lse.data_ptr() : nullptr;
+  p.status = status_ptr(cache);
+  const size_t nbytes = brk_cache_attn_workspace_bytes(&p);
+  Tensor ws;
+  if (nbytes > 0) ws = scratch(nbytes, cache);
+  check(brk_cache_attn(&p, nbytes > 0 ? ws.data_ptr() : nullptr, nbytes, stream_of(cache)), "brk_cache_attn");
+  return {out, lse};
+}
+
+std::tuple<Tensor, Tensor> cache_doc_scores(const Tensor& q, const Tensor& cache, const Tensor& table_in, const Tensor& blk_start, const Tensor& blk_len,
+                                            double scale, int64_t max_block_len, double temperature) {
+  need_cuda({&q, &cache, &table_in, &blk_start, &blk_len});
+  need_device(cache, {&q, &table_in, &blk_start, &blk_len});
+  const brk_cache c = cache_of(cache);
+  need_prompts(q, c, table_in, blk_start, blk_len);
+  const int dtype = dtype_code(q);
+  c10::cuda::CUDAGuard guard(cache.device());
+  const Tensor table = table_in.contiguous(), bs = blk_start.contiguous(), bl = blk_len.contiguous();
+  const int64_t B = q.size(0), N = q.size(1), R = q.size(2), nd = std::max<int64_t>(0, bs.size(1) - 2);
+  const auto f32 = q.options().dtype(at::kFloat).requires_grad(false);
+  Tensor mass = at::empty({B, N, R, nd}, f32), logits = at::empty({B, nd}, f32);
+  brk_cache_score_params p{};
+  p.dtype = dtype;
+  p.B = (int32_t)B; p.N = (int32_t)N; p.R = (int32_t)R;
+  p.M = (int32_t)bs.size(1); p.P = (int32_t)table.size(1);
+  p.max_block_len = (int32_t)std::min<int64_t>(max_block_len, INT32_MAX);
+  p.scale = (float)scale;
+  p.temperature = (float)temperature;
+  p.cache = c;
+  p.q = heads_view(q);
+  p.page_table = (const int32_t*)table.data_ptr();
+  p.blk_start = (const int32_t*)bs.data_ptr();
+  p.blk_len = (const int32_t*)bl.data_ptr();
+  p.doc_mass = (float*)mass.data_ptr();
+  p.logits = (float*)logits.data_ptr();
+  p.status = status_ptr(cache);
+  const size_t nbytes = brk_cache_doc_scores_workspace_bytes(&p);
+  Tensor ws = scratch(nbytes > 16 ? nbytes : 16, cache);
+  check(brk_cache_doc_scores(&p, ws.data_ptr(), nbytes, stream_of(cache)), "brk_cache_doc_scores");
+  return {mass, logits};
+}
+
 // ---- runner helpers ---------------------------------------------------------------------------
 Tensor rmsnorm(const Tensor& x, const Tensor& weight, double eps, const OptTensor& residual, const OptTensor& out_in) {
   need_cuda({&x, &weight, opt(residual)});
@@ -700,6 +866,11 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   def("doc_scores", &doc_scores);
   def("raw_scores", &raw_scores);
   def("raw_scores_bwd", &raw_scores_bwd);
+  def("cache_alloc", &cache_alloc);
+  def("cache_write", &cache_write);
+  def("cache_read", &cache_read);
+  def("cache_attention", &cache_attention);
+  def("cache_doc_scores", &cache_doc_scores);
   def("rmsnorm", &rmsnorm);
   def("rope_", &rope_);
   def("silu_mul", &silu_mul);

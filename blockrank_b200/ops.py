@@ -109,6 +109,69 @@ def raw_scores_bwd(q: torch.Tensor, k: torch.Tensor, d_raw: torch.Tensor, blk_st
     return _lib.host().raw_scores_bwd(q, k, d_raw, blk_start, blk_len, scale, dq, dk)
 
 
+CACHE_PAGE = 64  # tokens of a page of the 4-bit cache
+
+
+def cache_alloc(n_pages: int, kv_heads: int, head_dim: int, device=None) -> torch.Tensor:
+    """A 4-bit cache of keys and values: uint8 (n_pages, kv_heads, bytes), pages of ``CACHE_PAGE`` tokens, all zeros.
+
+    What a token's key or value is held as: per 32 channels a scale s = max|x| / 7, rounded to 5 significant bits, and codes
+    round(x / s) in -7..7; the value is code * s (4.5 bits per channel, exact in bf16).  A group with NaN or an infinity
+    is held as NaN.  Finite magnitudes above 7 * 1.9375 * 2^122 are held as that.  The order of the bytes is the library's own.
+
+    A prompt is a row of a page table, int32: its slot s lies in page ``page_table[b, s // 64]`` at offset ``s % 64``.  A
+    document's keys and values depend on the instruction block and the document alone: any number of prompts can share its
+    pages.  None of the cache functions records a gradient.
+    """
+    device = torch.device("cuda" if device is None else device)
+    if device.type == "cuda" and device.index is None:
+        device = torch.device("cuda", torch.cuda.current_device())
+    return _lib.host().cache_alloc(int(n_pages), int(kv_heads), int(head_dim), device)
+
+
+def cache_write(k: torch.Tensor, v: torch.Tensor, cache: torch.Tensor, slots: torch.Tensor) -> None:
+    """Quantise keys and values into the cache.
+
+    k, v (B,Nk,S,D) views as :func:`attention` takes them; slots int32 (B,S): ``page * CACHE_PAGE + offset`` of each token, negative
+    to leave it out.  Of several tokens with the same slot the last one (in the order of ``slots``) is kept; slots
+    that nothing names keep what they hold.  A slot outside the cache is left out and raises at the next :func:`check_status`.
+    """
+    _lib.host().cache_write(k, v, cache, slots)
+
+
+def cache_read(cache: torch.Tensor, slots: torch.Tensor, dtype: torch.dtype = torch.bfloat16) -> Tuple[torch.Tensor, torch.Tensor]:
+    """The held keys and values of ``slots`` int32 (B,S), each (B,Nk,S,D) in bfloat16 or float32 (memory layout (B,S,Nk,D)): what
+    :func:`attention` takes, e.g. for a prefill whose documents are in the cache already.  Zeros for a negative slot."""
+    return _lib.host().cache_read(cache, slots, dtype)
+
+
+def cache_attention(q: torch.Tensor, cache: torch.Tensor, page_table: torch.Tensor, blk_start: torch.Tensor, blk_len: torch.Tensor,
+                    scale: float, q_len: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None,
+                    return_lse: bool = False):
+    """Attention of the last tokens of every prompt over its pages: :func:`attention`'s query block, with the cache in the place
+    of k and v (the tokens' own keys and values are written first).
+
+    q (B,N,L,D); page_table int32 (B,P); blk_start / blk_len int32 (B,M): the slots of the prompt's blocks, as for
+    :func:`attention` (slots between blocks have no influence; M = 1: one causal sequence).  Row i is the token at slot
+    ``blk_start[b,-1] + blk_len[b,-1] - q_len[b] + i`` and sees every block's slots up to its own.  ``q_len`` int32 (B,): the number
+    of rows of each prompt (None: L), from 0 to the last block's length.  Returns out (B,L,N,D) [and lse (B,N,L) fp32]; rows from
+    q_len on are zeros (lse -inf).  Malformed spans, pages or rows leave that prompt (that page) out and raise at the next
+    :func:`check_status`.
+    """
+    res = _lib.host().cache_attention(q, cache, page_table, blk_start, blk_len, scale, q_len, out, return_lse)
+    return res if return_lse else res[0]
+
+
+def cache_doc_scores(q: torch.Tensor, cache: torch.Tensor, page_table: torch.Tensor, blk_start: torch.Tensor, blk_len: torch.Tensor,
+                     scale: float, max_block_len: int, temperature: float = 0.05) -> Tuple[torch.Tensor, torch.Tensor]:
+    """:func:`doc_scores` with the document keys from the cache.
+
+    q (B,N,R,D): the signal rows' queries; page table and spans as for :func:`cache_attention` (blocks 1..M-2 are the documents), of
+    documents of up to ``max_block_len`` tokens.  Returns (doc_mass (B,N,R,num_docs) fp32, logits (B,num_docs) fp32).
+    """
+    return _lib.host().cache_doc_scores(q, cache, page_table, blk_start, blk_len, scale, int(max_block_len), temperature)
+
+
 def rmsnorm(x: torch.Tensor, weight: torch.Tensor, eps: float, residual: Optional[torch.Tensor] = None,
             out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """RMSNorm over the last dim.  With ``residual`` given: residual += x (in place), norm of the sum."""

@@ -34,7 +34,7 @@
 extern "C" {
 #endif
 
-#define BRK_VERSION 103
+#define BRK_VERSION 104
 
 #if defined(__GNUC__)
 #define BRK_API __attribute__((visibility("default")))
@@ -241,6 +241,81 @@ BRK_API int brk_raw_scores(const brk_score_params* p, void* out, void* stream);
 BRK_API size_t brk_raw_scores_bwd_workspace_bytes(const brk_score_params* p);
 BRK_API int brk_raw_scores_bwd(const brk_score_params* p, const void* d_raw, const brk_view* dq, const brk_view* dk,
                                int32_t accumulate, void* workspace, size_t workspace_bytes, void* stream);
+
+/* ---- 4-bit cache of keys and values -------------------------------------------------------------------------------------
+ * A document block's keys and values depend on the instruction prefix and the document alone, so a serving program can keep
+ * them: score new queries against them and decode answers over them.  The cache is a pool of pages of BRK_CACHE_PAGE
+ * tokens, n_pages * brk_cache_page_bytes(Nk, D) bytes, 16-byte aligned, each page with every KV head's keys and values.  A
+ * prompt is a page table: its slot s lies in page page_table[s / BRK_CACHE_PAGE] at offset s % BRK_CACHE_PAGE, and block spans
+ * say which slots its blocks occupy (as everywhere in this header; blocks need not begin at a page's first slot, and pages may
+ * be shared by any number of prompts, or appear twice in one).  No counterpart in the reference.
+ *
+ * Held values.  Per token, KV head and 32 consecutive channels: a scale s = max|x| / 7, rounded to the nearest number with 5
+ * significant bits (ties to even; multiples of 2^-130; at most 1.9375 * 2^122), and per channel a code n = x / s rounded to the
+ * nearest integer (ties to even) within -7..7 (0 where s is 0).  The value is n s, exact in bf16: 4.5 bits per channel.  A group
+ * that holds NaN or an infinity reads as NaN in all its channels.  The order of the bytes in a page is the library's own.
+ *
+ * The device checks what a call reads there: a slot outside the pool, a page number outside [0, n_pages) that a block needs,
+ * spans that overlap, are out of order or reach past the page table, too many rows -- it sets the status word (BRK_E_ARG at
+ * brk_status_poll) and leaves that token, page or prompt out. */
+#define BRK_CACHE_PAGE 64
+typedef struct brk_cache {
+  void* pages;
+  int32_t n_pages;
+  int32_t Nk, D;          /* D = 64 or 128 */
+} brk_cache;
+BRK_API size_t brk_cache_page_bytes(int32_t Nk, int32_t D);
+
+/* Quantises k and v ((B, Nk, S, D) views, dtype BRK_BF16 or BRK_F32) into slots[B * S] (page * BRK_CACHE_PAGE + offset;
+ * negative: skip).  Slots that no token names keep what they hold; one that several tokens name gets the last one's (in the order of
+ * `slots`).  Workspace: brk_cache_write_workspace_bytes (0 for up to 1024 tokens). */
+BRK_API size_t brk_cache_write_workspace_bytes(const brk_cache* c, int32_t B, int32_t S);
+BRK_API int brk_cache_write(int32_t dtype, const brk_cache* c, const brk_view* k, const brk_view* v, int32_t B, int32_t S,
+                            const int32_t* slots, void* workspace, size_t workspace_bytes, int32_t* status, void* stream);
+/* The held values of slots[B * S] into the (B, Nk, S, D) views k and v; zeros for a negative slot. */
+BRK_API int brk_cache_read(int32_t dtype, const brk_cache* c, const brk_view* k, const brk_view* v, int32_t B, int32_t S,
+                           const int32_t* slots, int32_t* status, void* stream);
+
+/* Attention of the last tokens of every prompt over its cache (brk_attn_fwd's last block, with keys and values from the cache,
+ * the tokens' own among them).  Row i < q_len[b] of q is the token at slot
+ *   blk_start[b, M-1] + blk_len[b, M-1] - q_len[b] + i
+ * and sees the slots of all blocks at or before its own.  Rows from q_len[b] on, and rows that see nothing, get zeros (lse:
+ * -infinity).  M == 1: one causal sequence.  The slots between blocks, and what their pages hold, have no influence. */
+typedef struct brk_cache_attn_params {
+  int32_t dtype;          /* BRK_BF16 or BRK_F32 (q, o) */
+  int32_t B, N, Lq;       /* prompts, query heads, rows per prompt */
+  int32_t M, P;           /* blocks per prompt, entries of a page table */
+  float scale;            /* softmax scale, positive */
+  brk_cache cache;
+  brk_view q, o;          /* (B, N, Lq, D) views */
+  const int32_t* page_table; /* device, [B * P]; entries that no block reaches are not looked at */
+  const int32_t* blk_start;  /* device, [B * M] */
+  const int32_t* blk_len;    /* device, [B * M] */
+  const int32_t* q_len;   /* device, [B], or NULL: Lq each */
+  float* lse;             /* optional [B, N, Lq] natural-log sum-exp of scaled logits */
+  int32_t* status;        /* optional, see brk_status_poll */
+} brk_cache_attn_params;
+BRK_API size_t brk_cache_attn_workspace_bytes(const brk_cache_attn_params* p);
+BRK_API int brk_cache_attn(const brk_cache_attn_params* p, void* workspace, size_t workspace_bytes, void* stream);
+
+/* brk_doc_scores with the document keys from the cache: every row of q (B, N, R, D) is a signal row. */
+typedef struct brk_cache_score_params {
+  int32_t dtype;          /* BRK_BF16 or BRK_F32 (q) */
+  int32_t B, N, R;
+  int32_t M, P;
+  int32_t max_block_len;  /* upper bound on blk_len of the documents */
+  float scale, temperature;
+  brk_cache cache;
+  brk_view q;
+  const int32_t* page_table;
+  const int32_t* blk_start;
+  const int32_t* blk_len;
+  float* doc_mass;        /* [B, N, R, M-2] */
+  float* logits;          /* optional [B, M-2] */
+  int32_t* status;
+} brk_cache_score_params;
+BRK_API size_t brk_cache_doc_scores_workspace_bytes(const brk_cache_score_params* p);
+BRK_API int brk_cache_doc_scores(const brk_cache_score_params* p, void* workspace, size_t workspace_bytes, void* stream);
 
 /* Runner helpers (the model code around the attention call; the reference
  * relies on transformers' modeling_mistral.py for these). All row-major. */

@@ -1,0 +1,106 @@
+"""The 4-bit cache without a GPU: refusals of the C ABI and the properties of what is held."""
+import ctypes as C
+
+import pytest
+import torch
+
+from blockrank_b200 import _lib, ops
+from tests import cache_helpers as ch
+
+
+def _cache(n_pages=4, Nk=2, D=64, ptr=64):
+    return _lib.Cache(ptr, n_pages, Nk, D)
+
+
+def _view(D=64, ptr=64):
+    return _lib.View(ptr, 8 * D, D, 2 * D)
+
+
+def test_sizes():
+    L = _lib.lib()
+    assert L.brk_cache_page_bytes(1, 64) == 64 * 72 and L.brk_cache_page_bytes(8, 128) == 8 * 64 * 144
+    assert L.brk_cache_page_bytes(1, 96) == 0 and L.brk_cache_page_bytes(0, 64) == 0
+    c = _cache()
+    assert L.brk_cache_write_workspace_bytes(C.byref(c), 4, 256) == 0
+    assert L.brk_cache_write_workspace_bytes(C.byref(c), 4, 257) == 4 * 64 * 4
+    assert L.brk_cache_attn_workspace_bytes(None) == 0 and L.brk_cache_doc_scores_workspace_bytes(None) == 0
+
+
+@pytest.mark.parametrize("change,code", [
+    (dict(cache=None), -1), (dict(ptr=0), -1), (dict(ptr=72), -1), (dict(D=96), -2), (dict(n_pages=0), -1), (dict(Nk=0), -1),
+    (dict(n_pages=2 ** 25), -1), (dict(dtype=2), -2), (dict(slots=None), -1), (dict(S=0), -1), (dict(B=2 ** 16, S=2 ** 16), -1),
+    (dict(view=0), -1), (dict(view=8), -1), (dict(S=2000), -3)])
+def test_refusals_of_write(change, code):
+    """(every one of them is refused in front of any launch)"""
+    L = _lib.lib()
+    a = dict(ptr=64, n_pages=4, Nk=2, D=64, dtype=0, B=1, S=3, slots=64, view=64, cache=True)
+    a.update(change)
+    c = _cache(a["n_pages"], a["Nk"], a["D"], a["ptr"])
+    v = _view(ptr=a["view"])
+    args = (a["dtype"], C.byref(c) if a["cache"] else None, C.byref(v), C.byref(v), a["B"], a["S"], a["slots"])
+    assert L.brk_cache_write(*args, None, 0, None, None) == code, L.brk_last_error()
+    if code != -3:
+        assert L.brk_cache_read(*args, None, None) == code, L.brk_last_error()
+
+
+def _attn(**change):
+    p = _lib.CacheAttnParams()
+    p.dtype, p.B, p.N, p.Lq, p.M, p.P, p.scale = 0, 1, 4, 1, 1, 1, 1.0
+    p.cache, p.q, p.o = _cache(), _view(), _view()
+    p.page_table = p.blk_start = p.blk_len = 64
+    for k, v in change.items():
+        setattr(p, k, v)
+    return p
+
+
+@pytest.mark.parametrize("change,code", [
+    (dict(dtype=3), -2), (dict(B=0), -1), (dict(N=5), -1), (dict(Lq=0), -1), (dict(M=0), -1), (dict(P=0), -1), (dict(P=2 ** 25), -1),
+    (dict(scale=0.0), -1), (dict(scale=float("nan")), -1), (dict(scale=float("inf")), -1), (dict(page_table=None), -1),
+    (dict(blk_len=None), -1), (dict(B=40000), -2), (dict(B=30000, Lq=2 ** 16), -1), (dict(q=_view(ptr=8)), -1), (dict(o=_view(ptr=0)), -1),
+    (dict(cache=_cache(D=32)), -2)])
+def test_refusals_of_attention(change, code):
+    L = _lib.lib()
+    p = _attn(**change)
+    assert L.brk_cache_attn(C.byref(p), None, 0, None) == code, L.brk_last_error()
+    assert L.brk_cache_attn(None, None, 0, None) == -1
+
+
+def test_a_workspace_that_is_too_small_is_refused():
+    L = _lib.lib()
+    p = _attn(P=4096)
+    need = L.brk_cache_attn_workspace_bytes(C.byref(p))
+    assert need > 0 and L.brk_cache_attn(C.byref(p), 64, need - 1, None) == -3
+
+
+@pytest.mark.parametrize("change,code", [
+    (dict(M=2), -1), (dict(R=65), -1), (dict(max_block_len=0), -1), (dict(temperature=0.0), -1), (dict(doc_mass=None), -1), (dict(N=3), -1), ({}, -3)])
+def test_refusals_of_scores(change, code):
+    L = _lib.lib()
+    p = _lib.CacheScoreParams()
+    p.dtype, p.B, p.N, p.R, p.M, p.P, p.max_block_len, p.scale, p.temperature = 0, 1, 4, 1, 3, 1, 64, 1.0, 0.05
+    p.cache, p.q = _cache(), _view()
+    p.page_table = p.blk_start = p.blk_len = p.doc_mass = 64
+    for k, v in change.items():
+        setattr(p, k, v)
+    assert L.brk_cache_doc_scores(C.byref(p), None, 0, None) == code, L.brk_last_error()
+
+
+def test_cpu_tensors_are_refused():
+    i = torch.zeros(1, 1, dtype=torch.int32)
+    x = torch.zeros(1, 1, 1, 64)
+    c = torch.zeros(1, 1, 64 * 72, dtype=torch.uint8)
+    for call in (lambda: ops.cache_alloc(1, 1, 64, "cpu"), lambda: ops.cache_write(x, x, c, i), lambda: ops.cache_read(c, i),
+                 lambda: ops.cache_attention(x, c, i, i, i, 1.0), lambda: ops.cache_doc_scores(x, c, i, i, i, 1.0, 1)):
+        with pytest.raises(RuntimeError, match="CUDA tensors"):
+            call()
+
+
+def test_what_is_held():
+    """Held values are exact in bf16, held as themselves when written again, and half a step of their scale off at most."""
+    g = torch.Generator().manual_seed(0)
+    x = torch.randn(500, 3, 128, generator=g) * torch.exp(8 * torch.randn(500, 3, 1, generator=g))
+    h = ch.held(x)
+    assert torch.equal(h, h.float().double()) and torch.equal(h, h.bfloat16().double())
+    assert torch.equal(ch.held(h), h)
+    s = ch.scales(x).repeat_interleave(32, -1)
+    assert bool(((h - x.double()).abs() <= s / 2 + 1e-300).all())

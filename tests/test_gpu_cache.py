@@ -1,0 +1,518 @@
+"""The 4-bit cache on the GPU against the same in 64 bits."""
+import pytest
+import torch
+
+from tests import cache_helpers as ch
+
+pytestmark = pytest.mark.gpu
+
+if torch.cuda.is_available():
+    from blockrank_b200 import _lib, ops
+
+BF16, F32 = torch.bfloat16, torch.float32
+PAGE = ch.PAGE
+
+
+def _rand(*shape, seed, dtype, spread=0.5):
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn(*shape, generator=g) * torch.exp(spread * torch.randn(*shape[:-2], 1, shape[-1], generator=g))
+    return x.to(dtype)
+
+
+def _filled(pool, Nk, D, seed, dtype=BF16):
+    """A pool of which every slot is written; returns the cache and the held values, fp64 (slots, Nk, D)."""
+    k, v = (_rand(pool * PAGE, Nk, D, seed=seed + i, dtype=dtype) for i in (0, 1))
+    cache = ops.cache_alloc(pool, Nk, D, "cuda")
+    every = torch.arange(pool * PAGE, dtype=torch.int32, device="cuda")[None]
+    ops.cache_write(k[None].transpose(1, 2).cuda(), v[None].transpose(1, 2).cuda(), cache, every)
+    return cache, ch.held(k), ch.held(v)
+
+
+def _table(B, P, pool, seed):
+    return torch.randperm(pool, generator=torch.Generator().manual_seed(seed))[:B * P].reshape(B, P).to(torch.int32)
+
+
+def _check(out, lse, ref, ref_lse, size, v, steps):
+    """Rounding of the output to its type (half a step), and in front of it: a logit is off by its products' and sums' roundings (at
+    most 24 accumulations of 2^-23 of sum |q||k|), a probability by twice that, by its exponential (2^-21) and by what its bf16
+    pieces leave out (2^-16 for two), the sums by 2^-23 for each of `steps` accumulations."""
+    rel = 2 * float(size.max()) * 24 * 2.0 ** -23 + 2.0 ** -21 + (2.0 ** -16 if out.dtype == BF16 else 0.0) + steps * 2.0 ** -23
+    err = (out.double().cpu() - ref).abs()
+    allowed = ref.abs() * torch.finfo(out.dtype).eps / 2 + 2 * rel * float(v.abs().max())
+    assert bool((err <= allowed).all()), (err - allowed).max()
+    if lse is not None:
+        dead = ref_lse == -torch.inf
+        assert torch.equal(lse.cpu() == -torch.inf, dead)
+        err = (lse.double().cpu() - ref_lse)[~dead].abs()
+        assert bool((err <= rel + ref_lse[~dead].abs() * 2.0 ** -22).all()), err.max()
+
+
+# ---- writing and reading -------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("B,Nk,S", [(1, 1, 1), (2, 3, 5), (3, 8, 37), (2, 7, 700)])
+def test_written_values_are_read_back(dtype, D, B, Nk, S):
+    pool = -(-B * S // PAGE) + 2
+    k, v = (_rand(B, S, Nk, D, seed=S + i, dtype=dtype, spread=2.0) for i in (0, 1))
+    slots = torch.randperm(pool * PAGE, generator=torch.Generator().manual_seed(S))[:B * S].reshape(B, S).to(torch.int32)
+    slots[:, ::5] = -1
+    cache = ops.cache_alloc(pool, Nk, D, "cuda")
+    # (views of a fused projection: heads of a wider row)
+    kv = torch.cat([k, v], 2).cuda()
+    ops.cache_write(kv[:, :, :Nk].transpose(1, 2), kv[:, :, Nk:].transpose(1, 2), cache, slots.cuda())
+    for t in (BF16, F32):
+        gk, gv = ops.cache_read(cache, slots.cuda(), t)
+        assert gk.dtype == t and gk.shape == (B, Nk, S, D)
+        for got, x in ((gk, k), (gv, v)):
+            ref = torch.where((slots >= 0)[:, None, :, None], ch.held(x).transpose(1, 2), 0.0)
+            assert torch.equal(got.double().cpu(), ref)
+    ops.check_status()
+
+
+def test_values_at_the_ends_of_the_range():
+    """Zeros, ties of codes and scales, subnormal and huge magnitudes, NaN and infinities."""
+    D, Nk = 64, 1
+    rows = []
+    half = torch.arange(32) * 0.5 - 8  # s = 1 with the 7 below: every tie
+    half[0] = 7.0
+    rows.append(half.clamp(-7, 7))
+    rows.append(torch.zeros(32))
+    rows.append(torch.full((32,), -0.0))
+    rows += [torch.linspace(-1, 1, 32) * 2.0 ** e for e in (-149, -140, -133, -130, -126, -100, 100, 122, 126)]
+    rows.append(torch.full((32,), torch.finfo(F32).max))
+    rows.append(torch.cat([torch.tensor([7 * 1.03125]), torch.linspace(-7.2, 7.2, 31)]))  # s between two 5-bit numbers
+    for bad in (torch.nan, torch.inf, -torch.inf):
+        r = torch.linspace(-1, 1, 32)
+        r[17] = bad
+        rows.append(r)
+    x = torch.stack(rows)
+    x = torch.cat([x, x.flip(0)], -1).reshape(1, 1, -1, D)  # (B, Nk, S, D): two groups each
+    for dtype in (F32, BF16):
+        y = x.to(dtype)
+        cache = ops.cache_alloc(1, Nk, D, "cuda")
+        slots = torch.arange(y.shape[2], dtype=torch.int32)[None]
+        ops.cache_write(y.cuda(), (-y).cuda(), cache, slots.cuda())
+        gk, gv = ops.cache_read(cache, slots.cuda(), F32)
+        for got, src in ((gk, y), (gv, -y)):
+            ref = ch.held(src)
+            got = got.double().cpu()
+            assert torch.equal(got.isnan(), ref.isnan())
+            assert torch.equal(got.nan_to_num(nan=0.0), ref.nan_to_num(nan=0.0))
+
+
+@pytest.mark.parametrize("S", [7, 1025, 3000])
+def test_of_tokens_with_the_same_slot_the_last_one_is_kept(S):
+    Nk, D, pool = 2, 64, 3
+    k, v = (_rand(1, S, Nk, D, seed=i, dtype=F32) for i in (0, 1))
+    slots = torch.randint(-1, 40, (1, S), generator=torch.Generator().manual_seed(S), dtype=torch.int32)
+    cache, hk, hv = _filled(pool, Nk, D, 5)
+    ops.cache_write(k.transpose(1, 2).cuda(), v.transpose(1, 2).cuda(), cache, slots.cuda())
+    for i, s in enumerate(slots[0].tolist()):
+        if s >= 0:
+            hk[s], hv[s] = ch.held(k[0, i]), ch.held(v[0, i])
+    every = torch.arange(pool * PAGE, dtype=torch.int32, device="cuda")[None]
+    gk, gv = ops.cache_read(cache, every, F32)  # what was not named is what it was
+    assert torch.equal(gk[0].transpose(0, 1).double().cpu(), hk) and torch.equal(gv[0].transpose(0, 1).double().cpu(), hv)
+
+
+@pytest.mark.parametrize("S", [9, 1500])
+def test_slots_outside_the_cache_are_left_out_and_reported(S):
+    Nk, D, pool = 1, 128, S // PAGE + 1
+    k, v = (_rand(1, S, Nk, D, seed=i, dtype=BF16) for i in (0, 1))
+    slots = torch.arange(S, dtype=torch.int32)[None].clone()
+    slots[0, 3], slots[0, 5] = pool * PAGE, 2 ** 31 - 1
+    cache = ops.cache_alloc(pool, Nk, D, "cuda")
+    ops.check_status()
+    ops.cache_write(k.transpose(1, 2).cuda(), v.transpose(1, 2).cuda(), cache, slots.cuda())
+    with pytest.raises(ValueError, match="slot lies outside the cache"):
+        ops.check_status()
+    gk, _ = ops.cache_read(cache, slots.cuda())
+    with pytest.raises(ValueError, match="slot lies outside the cache"):
+        ops.check_status()
+    ref = ch.held(k).transpose(1, 2)
+    ref[:, :, 3] = ref[:, :, 5] = 0
+    assert torch.equal(gk.double().cpu(), ref)
+
+
+# ---- attention -----------------------------------------------------------------------------------
+LENS = {
+    "one_token": [[1], [1]],
+    "one_block": [[130], [64], [1]],
+    "docs": [[5, 64, 1, 100, 33, 20], [1, 63, 65, 128, 2, 9]],
+    "empty_docs": [[5, 0, 70, 0, 0, 3], [0, 0, 0, 0, 0, 2], [0, 64, 0, 0, 64, 64]],
+    "long": [[40, 900, 700, 12], [40, 1, 1300, 31]],
+}
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("N,Nk,D", [(8, 2, 128), (6, 2, 64), (4, 4, 64), (16, 2, 128)])
+@pytest.mark.parametrize("name", list(LENS))
+@pytest.mark.parametrize("paged", [True, False])
+def test_one_row(dtype, N, Nk, D, name, paged):
+    start, length, P = ch.spans(LENS[name], paged, gap=0 if paged else 3)
+    B = len(LENS[name])
+    cache, hk, hv = _filled(B * P + 2, Nk, D, 11, dtype)
+    table = _table(B, P, B * P + 2, 3)
+    q = _rand(B, 1, N, D, seed=2, dtype=dtype).transpose(1, 2)
+    out, lse = ops.cache_attention(q.cuda(), cache, table.cuda(), start.cuda(), length.cuda(), D ** -0.5, return_lse=True)
+    ref, ref_lse, size = ch.attention(q, hk, hv, table, start, length, D ** -0.5)
+    assert out.shape == (B, 1, N, D) and out.dtype == dtype
+    _check(out, lse, ref, ref_lse, size, hv, 3 * P + 8)
+    ops.check_status()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("N,Nk,D", [(8, 2, 128), (6, 2, 64), (3, 3, 128)])
+@pytest.mark.parametrize("rows", [2, 3, 17, 70])
+def test_several_rows_of_different_number(dtype, N, Nk, D, rows):
+    lens = [[5, 64, 1, 100, rows + 30], [1, 63, 65, 128, rows], [9, 0, 0, 3, rows + 64], [2, 3, 4, 0, 80]]
+    q_len = torch.tensor([rows, rows, rows // 2, 0], dtype=torch.int32)
+    start, length, P = ch.spans(lens, False)
+    cache, hk, hv = _filled(4 * P + 1, Nk, D, 21, dtype)
+    table = _table(4, P, 4 * P + 1, 4)
+    q = _rand(4, rows, N, D, seed=6, dtype=dtype).transpose(1, 2)
+    out, lse = ops.cache_attention(q.cuda(), cache, table.cuda(), start.cuda(), length.cuda(), D ** -0.5, q_len=q_len.cuda(), return_lse=True)
+    ref, ref_lse, size = ch.attention(q, hk, hv, table, start, length, D ** -0.5, q_len)
+    _check(out, lse, ref, ref_lse, size, hv, 3 * P + 8)
+    assert not out[3].any() and not out[2, rows // 2:].any()
+    ops.check_status()
+
+
+@pytest.mark.parametrize("tokens,capacity,B", [(3000, 4096, 1), (70000, 70016, 1), (200, 60000, 2), (33000, 33024, 3)])
+def test_long_caches_and_tables_far_longer_than_the_prompt(tokens, capacity, B):
+    N, Nk, D, P = 4, 1, 64, -(-capacity // PAGE)
+    used = -(-tokens // PAGE)
+    cache, hk, hv = _filled(B * used, Nk, D, 31)
+    table = torch.full((B, P), -1, dtype=torch.int32)  # entries that no block reaches are never looked at
+    table[:, :used] = _table(B, used, B * used, 5)
+    start, length = torch.zeros(B, 1, dtype=torch.int32), torch.full((B, 1), tokens, dtype=torch.int32)
+    length[-1] -= 77
+    q = _rand(B, 2, N, D, seed=7, dtype=BF16).transpose(1, 2)
+    out, lse = ops.cache_attention(q.cuda(), cache, table.cuda(), start.cuda(), length.cuda(), D ** -0.5, return_lse=True)
+    ref, ref_lse, size = ch.attention(q, hk, hv, table, start, length, D ** -0.5)
+    _check(out, lse, ref, ref_lse, size, hv, 12 * used)
+    ops.check_status()
+
+
+def test_views_and_a_given_output():
+    N, Nk, D, B, R = 4, 2, 64, 2, 3
+    start, length, P = ch.spans([[3, 70, 9], [64, 1, 5]], True)
+    cache, hk, hv = _filled(B * P, Nk, D, 41)
+    table = _table(B, P, B * P, 6)
+    wide = _rand(B, R, N + 2, D, seed=8, dtype=BF16)
+    q = wide[:, :, 1:N + 1].transpose(1, 2)
+    room = torch.full((B, R + 2, N, D + 16), 7.0, dtype=BF16, device="cuda")
+    out = room[:, 1:R + 1, :, :D]
+    # page table and spans as columns of something wider
+    tab = torch.stack([table, table], -1).cuda()[..., 0]
+    st, ln = (torch.stack([x, x], -1).cuda()[..., 0] for x in (start, length))
+    got = ops.cache_attention(wide.cuda()[:, :, 1:N + 1].transpose(1, 2), cache, tab, st, ln, 0.2, out=out)
+    assert got.data_ptr() == out.data_ptr()
+    ref, _, size = ch.attention(q, hk, hv, table, start, length, 0.2)
+    _check(out, None, ref, None, size, hv, 3 * P + 8)
+    assert (room[:, 0] == 7).all() and (room[:, -1] == 7).all() and (room[..., D:] == 7).all()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_what_no_row_sees_has_no_influence(dtype):
+    """Pages of NaN scales and arbitrary codes outside the blocks; NaN and infinities in tokens behind a row's own."""
+    N, Nk, D, B, R = 4, 2, 128, 2, 5
+    lens = [[3, 70, 9, 12], [64, 1, 0, 5]]
+    start, length, P = ch.spans(lens, True, gap=PAGE)
+    cache, hk, hv = _filled(B * P + 1, Nk, D, 51, dtype)
+    table = _table(B, P, B * P + 1, 7)
+    inside = torch.zeros(B * P * PAGE + PAGE, dtype=torch.bool)
+    for b in range(B):
+        for s, n in zip(start[b].tolist(), length[b].tolist()):
+            inside[ch.slots_of(table[b], torch.arange(s, s + n))] = True
+    kept_k, kept_v = (x.clone() for x in ops.cache_read(cache, inside.nonzero().T.int().cuda(), F32))
+    cache.fill_(255)
+    ops.cache_write(kept_k, kept_v, cache, inside.nonzero().T.int().contiguous().cuda())  # (held values are held as they are)
+    q = _rand(B, R, N, D, seed=9, dtype=dtype).transpose(1, 2)
+    args = (q.cuda(), cache, table.cuda(), start.cuda(), length.cuda(), D ** -0.5)
+    ref, ref_lse, size = ch.attention(q, hk, hv, table, start, length, D ** -0.5)
+    out, lse = ops.cache_attention(*args, return_lse=True)
+    _check(out, lse, ref, ref_lse, size, hv, 3 * P + 8)
+    # the last token but one of each prompt: NaN in one group of V's first head, an infinity in K's second
+    last = (start[:, -1] + length[:, -1] - 2).tolist()
+    at = torch.tensor([[int(ch.slots_of(table[b], torch.tensor(last[b])))] for b in range(B)], dtype=torch.int32).cuda()
+    k1, v1 = ops.cache_read(cache, at, F32)
+    v1[:, 0, 0, 40] = torch.nan
+    k1[:, 1, 0, 3] = torch.inf
+    ops.cache_write(k1, v1, cache, at)
+    bad, bad_lse = ops.cache_attention(*args, return_lse=True)
+    assert torch.equal(bad[:, :R - 2], out[:, :R - 2]) and torch.equal(bad_lse[:, :, :R - 2], lse[:, :, :R - 2])
+    g = N // Nk
+    assert bad[:, R - 2:, :g, 32:64].isnan().all() and bad[:, R - 2:, g:].isnan().all() and bad_lse[:, g:, R - 2:].isnan().all()
+    assert torch.equal(bad[:, R - 2:, :g, :32], out[:, R - 2:, :g, :32]) and torch.equal(bad[:, R - 2:, :g, 64:], out[:, R - 2:, :g, 64:])
+
+
+def test_malformed_prompts_are_left_out_and_reported():
+    N, Nk, D, B = 4, 2, 64, 6
+    start, length, P = ch.spans([[3, 70, 9]] * B, True)
+    cache, hk, hv = _filled(B * P, Nk, D, 61)
+    table = _table(B, P, B * P, 8)
+    start[1, 1] = 2              # overlaps the first block
+    length[2, 2] = P * PAGE      # past the page table
+    length[3, 0] = -1
+    q_len = torch.tensor([2, 2, 2, 2, 10, 2], dtype=torch.int32)  # prompt 4: more rows than q has and than the last block's 9
+    table[5, 0] = B * P          # a page outside the cache: left out, the rest of the prompt is seen
+    q = _rand(B, 3, N, D, seed=10, dtype=BF16).transpose(1, 2)
+    ops.check_status()
+    out = ops.cache_attention(q.cuda(), cache, table.cuda(), start.cuda(), length.cuda(), 0.3, q_len=q_len.cuda())
+    with pytest.raises(ValueError, match="of a call on the cache"):
+        ops.check_status()
+    assert not out[1:5].any()
+    for b in (0, 5):
+        ln = length[b:b + 1].clone()
+        if b == 5:
+            ln[0, 0] = 0
+        ref, _, size = ch.attention(q[b:b + 1], hk, hv, table[b:b + 1], start[b:b + 1], ln, 0.3, q_len[b:b + 1])
+        _check(out[b:b + 1], None, ref, None, size, hv, 32)
+
+
+def test_pages_beyond_the_reach_of_32_bits():
+    """The last pages of a pool of more than 2^32 bytes."""
+    N, Nk, D = 8, 8, 128
+    pool = 2 ** 32 // 73728 + 40
+    cache = ops.cache_alloc(pool, Nk, D, "cuda")
+    assert cache.numel() > 2 ** 32
+    P, T = 3, 150
+    table = torch.tensor([[pool - 1, 5, pool - 2]], dtype=torch.int32)
+    k, v = (_rand(1, T, Nk, D, seed=i, dtype=BF16) for i in (1, 2))
+    slots = ch.slots_of(table[0], torch.arange(T))[None].int()
+    ops.cache_write(k.transpose(1, 2).cuda(), v.transpose(1, 2).cuda(), cache, slots.cuda())
+    gk, gv = ops.cache_read(cache, slots.cuda(), F32)
+    assert torch.equal(gk.double().cpu(), ch.held(k).transpose(1, 2)) and torch.equal(gv.double().cpu(), ch.held(v).transpose(1, 2))
+    q = _rand(1, 1, N, D, seed=3, dtype=BF16).transpose(1, 2)
+    start, length = torch.zeros(1, 1, dtype=torch.int32), torch.full((1, 1), T, dtype=torch.int32)
+    out = ops.cache_attention(q.cuda(), cache, table.cuda(), start.cuda(), length.cuda(), 0.1)
+    local = torch.arange(P, dtype=torch.int32)[None]
+    pad = lambda x: torch.cat([ch.held(x)[0], torch.zeros(P * PAGE - T, Nk, D, dtype=torch.float64)])
+    ref, _, size = ch.attention(q, pad(k), pad(v), local, start, length, 0.1)
+    _check(out, None, ref, None, size, ch.held(v), 32)
+    ops.check_status()
+
+
+# ---- document scores -----------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("N,Nk,D,R", [(8, 2, 128, 2), (6, 2, 64, 1), (4, 4, 64, 2), (16, 2, 128, 3)])
+@pytest.mark.parametrize("name", ["docs", "empty_docs", "long"])
+@pytest.mark.parametrize("paged", [True, False])
+def test_document_scores(dtype, N, Nk, D, R, name, paged):
+    start, length, P = ch.spans(LENS[name], paged, gap=0 if paged else 3)
+    B = len(LENS[name])
+    cache, hk, _ = _filled(B * P + 2, Nk, D, 71, dtype)
+    table = _table(B, P, B * P + 2, 9)
+    q = _rand(B, R, N, D, seed=12, dtype=dtype).transpose(1, 2)
+    mass, logits = ops.cache_doc_scores(q.cuda(), cache, table.cuda(), start.cuda(), length.cuda(), D ** -0.5, int(length.max()))
+    ref = ch.doc_mass(q, hk, table, start, length, D ** -0.5)
+    # a probability is off by twice its logit's error (24 accumulations of 2^-23 of sum |q||k|), its exponentials' and the sums'
+    size = float((q.double().abs().amax() * hk.abs().sum(-1).amax()) * D ** -0.5)
+    rel = 2 * size * 24 * 2.0 ** -23 + 64 * 2.0 ** -23
+    assert bool(((mass.double().cpu() - ref).abs() <= rel * ref + 2.0 ** -40).all())
+    want = ref.mean((1, 2)) / 0.05
+    assert bool(((logits.double().cpu() - want).abs() <= 2 * rel * want + 2.0 ** -40).all())
+    ops.check_status()
+
+
+def test_document_scores_are_those_of_the_values_read_back():
+    """The cached epilogue against the uncached one on the same numbers."""
+    N, Nk, D, R = 32, 8, 128, 2
+    lens = [[27, 40, 90, 64, 1, 77, 19], [27, 35, 35, 128, 64, 2, 30]]
+    start, length, P = ch.spans(lens, False)
+    cache, _, _ = _filled(2 * P, Nk, D, 81)
+    table = _table(2, P, 2 * P, 10)
+    slots = torch.stack([ch.slots_of(table[b], torch.arange(P * PAGE)) for b in range(2)]).int().cuda()
+    k, _ = ops.cache_read(cache, slots)
+    rows = torch.tensor([[P * PAGE - 2, P * PAGE - 1]] * 2, dtype=torch.int32).cuda()
+    q = _rand(2, P * PAGE, N, D, seed=13, dtype=BF16).transpose(1, 2).cuda()
+    want, want_logits = ops.doc_scores(q, k, start.cuda(), length.cuda(), rows, D ** -0.5)
+    got, got_logits = ops.cache_doc_scores(q[:, :, -2:], cache, table.cuda(), start.cuda(), length.cuda(), D ** -0.5, int(length.max()))
+    assert torch.allclose(got, want, rtol=2e-5, atol=1e-9) and torch.allclose(got_logits, want_logits, rtol=2e-5)
+
+
+def test_malformed_documents_are_left_out_and_reported():
+    N, Nk, D = 4, 2, 64
+    start, length, P = ch.spans([[3, 70, 60, 9]] * 3, True)
+    cache, hk, _ = _filled(3 * P, Nk, D, 91)
+    table = _table(3, P, 3 * P, 11)
+    q = _rand(3, 1, N, D, seed=14, dtype=BF16).transpose(1, 2)
+    ops.check_status()
+    length[1, 1] = 200            # runs into the next block, longer than max_block_len
+    table[2, start[2, 1] // PAGE] = -3
+    mass, _ = ops.cache_doc_scores(q.cuda(), cache, table.cuda(), start.cuda(), length.cuda(), 0.2, 70)
+    with pytest.raises(ValueError, match="of a call on the cache"):
+        ops.check_status()
+    ref = ch.doc_mass(q[:1], hk, table[:1], start[:1], length[:1], 0.2)
+    assert torch.allclose(mass[:1].double().cpu(), ref, rtol=1e-4)
+    assert not mass[1, :, :, 0].any()
+
+
+# ---- together ------------------------------------------------------------------------------------
+def test_a_prompt_is_cached_ranked_and_answered():
+    """Prefill, the cache filled from its keys and values, document scores, and three decoding steps; two prompts share the pages
+    of the instruction and of one document."""
+    N, Nk, D = 8, 2, 128
+    lens = [[30, 64, 100, 40], [30, 64, 7, 25]]
+    start, length, P = ch.spans(lens, True)
+    B, S = 2, P * PAGE
+    q, k, v = (_rand(B, S, n, D, seed=i, dtype=BF16) for i, n in ((1, N), (2, Nk), (3, Nk)))
+    k[1, :128], v[1, :128] = k[0, :128], v[0, :128]  # the same instruction and first document
+    table = torch.arange(2 * P, dtype=torch.int32).reshape(2, P).clone()
+    table[1, :2] = table[0, :2]
+    scale = D ** -0.5
+    logical = torch.arange(S)
+    inside = [torch.isin(logical, torch.cat([torch.arange(a, a + n) for a, n in zip(start[b].tolist(), length[b].tolist())])) for b in range(B)]
+    slots = torch.stack([torch.where(inside[b], ch.slots_of(table[b], logical), -1) for b in range(B)]).int()
+    cache = ops.cache_alloc(2 * P, Nk, D, "cuda")
+    ops.cache_write(k.cuda().transpose(1, 2), v.cuda().transpose(1, 2), cache, slots.cuda())
+    ck, cv = ops.cache_read(cache, slots.cuda())
+    st, ln, tab = start.cuda(), length.cuda(), table.cuda()
+    # the query block's rows: the prefill attention on what was read back and the cached one agree
+    full = ops.attention(q.cuda().transpose(1, 2), ck, cv, st, ln, scale, int(length.max()))
+    rows = int(length[:, -1].max())
+    qq = torch.zeros(B, rows, N, D, dtype=BF16)
+    for b in range(B):
+        a, n = int(start[b, -1]), int(length[b, -1])
+        qq[b, :n] = q[b, a:a + n]
+    got = ops.cache_attention(qq.cuda().transpose(1, 2), cache, tab, st, ln, scale, q_len=ln[:, -1].contiguous())
+    for b in range(B):
+        a, n = int(start[b, -1]), int(length[b, -1])
+        d = (got[b, :n].float() - full[b, a:a + n].float()).abs().max()
+        assert d <= 2 ** -7 * float(cv.abs().max())
+    mass, logits = ops.cache_doc_scores(qq.cuda().transpose(1, 2)[:, :, :2], cache, tab, st, ln, scale, int(length.max()))
+    assert torch.allclose(mass.sum(-1), torch.ones_like(mass.sum(-1)), atol=1e-5) and logits.shape == (B, 2)
+    hk, hv = (torch.zeros(2 * P * PAGE, Nk, D, dtype=torch.float64) for _ in range(2))
+    for b in range(B):
+        hk[slots[b][inside[b]].long()], hv[slots[b][inside[b]].long()] = ch.held(k[b][inside[b]]), ch.held(v[b][inside[b]])
+    for step in range(3):
+        length[:, -1] += 1
+        ln = length.cuda()
+        q1, k1, v1 = (_rand(B, 1, n, D, seed=20 + step + i, dtype=BF16) for i, n in ((1, N), (2, Nk), (3, Nk)))
+        at = torch.stack([ch.slots_of(table[b], start[b, -1:].long() + length[b, -1:].long() - 1) for b in range(B)]).int()
+        ops.cache_write(k1.cuda().transpose(1, 2), v1.cuda().transpose(1, 2), cache, at.cuda())
+        hk[at[:, 0].long()], hv[at[:, 0].long()] = ch.held(k1[:, 0]), ch.held(v1[:, 0])
+        out = ops.cache_attention(q1.cuda().transpose(1, 2), cache, tab, st, ln, scale)
+        ref, _, size = ch.attention(q1.transpose(1, 2), hk, hv, table, start, length, scale)
+        _check(out, None, ref, None, size, hv, 32)
+    ops.check_status()
+
+
+def test_a_captured_step_replays_on_new_inputs():
+    N, Nk, D, B = 8, 2, 128, 2
+    start, length, P = ch.spans([[30, 64, 500, 40], [30, 64, 7, 25]], True)
+    cache, hk, hv = _filled(B * P, Nk, D, 101)
+    table = _table(B, P, B * P, 12)
+    st, ln, tab = start.cuda(), length.cuda(), table.cuda()
+    k1, v1, q1 = (torch.zeros(B, 1, n, D, dtype=BF16, device="cuda").transpose(1, 2) for n in (Nk, Nk, N))
+    at = torch.zeros(B, 1, dtype=torch.int32, device="cuda")
+    ops.status_word("cuda")
+
+    def step():
+        ops.cache_write(k1, v1, cache, at)
+        return ops.cache_attention(q1, cache, tab, st, ln, 0.1), ops.cache_doc_scores(q1, cache, tab, st, ln, 0.1, 512)[0]
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        at.fill_(-1)
+        step()
+    torch.cuda.synchronize()
+    graphs = []
+    for _ in range(2):  # two graphs of the same step
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = step()
+        graphs.append((graph, out))
+    for i in range(4):
+        length[:, -1] += 1
+        ln.copy_(length)
+        new = [_rand(B, 1, n, D, seed=30 + 3 * i + j, dtype=BF16) for j, n in enumerate((Nk, Nk, N))]
+        for dst, src in zip((k1, v1, q1), new):
+            dst.copy_(src.transpose(1, 2))
+        slot = torch.stack([ch.slots_of(table[b], start[b, -1:].long() + length[b, -1:].long() - 1) for b in range(B)])
+        at.copy_(slot)
+        hk[slot[:, 0]], hv[slot[:, 0]] = ch.held(new[0][:, 0]), ch.held(new[1][:, 0])
+        graph, (out, mass) = graphs[i % 2]
+        graph.replay()
+        ref, _, size = ch.attention(new[2].transpose(1, 2), hk, hv, table, start, length, 0.1)
+        _check(out, None, ref, None, size, hv, 64)
+        assert torch.allclose(mass.double().cpu(), ch.doc_mass(new[2].transpose(1, 2), hk, table, start, length, 0.1), rtol=1e-3, atol=1e-6)
+    ops.check_status()
+
+
+def test_calls_on_two_streams_at_once():
+    N, Nk, D, B = 8, 2, 128, 2
+    start, length, P = ch.spans([[30, 900, 40], [30, 64, 25]], True)
+    cache, hk, hv = _filled(B * P, Nk, D, 111)
+    table = _table(B, P, B * P, 13)
+    qs = [_rand(B, 1, N, D, seed=40 + i, dtype=BF16).transpose(1, 2) for i in range(2)]
+    dev = [q.cuda() for q in qs]
+    st, ln, tab = start.cuda(), length.cuda(), table.cuda()
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    outs = [[], []]
+    for _ in range(20):
+        for i in range(2):
+            with torch.cuda.stream(streams[i]):
+                outs[i].append(ops.cache_attention(dev[i], cache, tab, st, ln, 0.1))
+    torch.cuda.synchronize()
+    for i in range(2):
+        ref, _, size = ch.attention(qs[i], hk, hv, table, start, length, 0.1)
+        for out in outs[i]:
+            assert torch.equal(out, outs[i][0])
+        _check(outs[i][0], None, ref, None, size, hv, 64)
+
+
+def test_calls_of_nothing():
+    cache, _, _ = _filled(2, 2, 64, 121)
+    z = lambda *s: torch.zeros(*s, dtype=torch.int32, device="cuda")
+    e = lambda *s: torch.zeros(*s, dtype=BF16, device="cuda")
+    before = cache.clone()
+    ops.cache_write(e(2, 2, 0, 64), e(2, 2, 0, 64), cache, z(2, 0))
+    ops.cache_write(e(0, 2, 3, 64), e(0, 2, 3, 64), cache, z(0, 3))
+    assert torch.equal(cache, before)
+    assert ops.cache_read(cache, z(3, 0))[0].shape == (3, 2, 0, 64)
+    assert ops.cache_attention(e(2, 4, 0, 64), cache, z(2, 1), z(2, 1), z(2, 1), 1.0).shape == (2, 0, 4, 64)
+    assert ops.cache_attention(e(0, 4, 1, 64), cache, z(0, 1), z(0, 1), z(0, 1), 1.0).shape == (0, 1, 4, 64)
+    out, lse = ops.cache_attention(e(2, 4, 3, 64), cache, z(2, 1), z(2, 1), z(2, 1), 1.0, q_len=z(2), return_lse=True)
+    assert not out.any() and (lse == -torch.inf).all()
+    ops.check_status()
+
+
+def test_refused_calls():
+    cache = ops.cache_alloc(2, 2, 64, "cuda")
+    z = lambda *s: torch.zeros(*s, dtype=torch.int32, device="cuda")
+    e = lambda *s, dtype=BF16: torch.zeros(*s, dtype=dtype, device="cuda")
+    bad = [
+        lambda: ops.cache_alloc(0, 2, 64, "cuda"),
+        lambda: ops.cache_alloc(2, 2, 96, "cuda"),
+        lambda: ops.cache_write(e(1, 2, 3, 64), e(1, 2, 3, 64), cache, z(1, 2)),
+        lambda: ops.cache_write(e(1, 2, 3, 64), e(1, 2, 3, 64), cache, z(1, 3).long()),
+        lambda: ops.cache_write(e(1, 3, 3, 64), e(1, 3, 3, 64), cache, z(1, 3)),
+        lambda: ops.cache_write(e(1, 2, 3, 128), e(1, 2, 3, 128), cache, z(1, 3)),
+        lambda: ops.cache_write(e(1, 2, 3, 64), e(1, 2, 3, 64, dtype=F32), cache, z(1, 3)),
+        lambda: ops.cache_write(e(1, 2, 3, 64, dtype=torch.float16), e(1, 2, 3, 64, dtype=torch.float16), cache, z(1, 3)),
+        lambda: ops.cache_write(e(1, 2, 3, 65)[..., 1:], e(1, 2, 3, 64), cache, z(1, 3)),
+        lambda: ops.cache_read(cache, z(3)),
+        lambda: ops.cache_read(cache, z(1, 3), torch.float16),
+        lambda: ops.cache_read(cache.view(2, 2, 72, 64), z(1, 3)),
+        lambda: ops.cache_read(cache[:, :1], z(1, 3)),
+        lambda: ops.cache_attention(e(1, 3, 1, 64), cache, z(1, 1), z(1, 1), z(1, 1), 1.0),
+        lambda: ops.cache_attention(e(1, 4, 1, 64), cache, z(2, 1), z(1, 1), z(1, 1), 1.0),
+        lambda: ops.cache_attention(e(1, 4, 1, 64), cache, z(1, 1), z(1, 1), z(1, 2), 1.0),
+        lambda: ops.cache_attention(e(1, 4, 1, 64), cache, z(1, 0), z(1, 1), z(1, 1), 1.0),
+        lambda: ops.cache_attention(e(1, 4, 1, 64), cache, z(1, 1), z(1, 1), z(1, 1), 0.0),
+        lambda: ops.cache_attention(e(1, 4, 1, 64), cache, z(1, 1), z(1, 1), z(1, 1), float("nan")),
+        lambda: ops.cache_attention(e(1, 4, 1, 64), cache, z(1, 1), z(1, 1), z(1, 1), 1.0, q_len=z(2)),
+        lambda: ops.cache_attention(e(1, 4, 1, 64), cache, z(1, 1), z(1, 1), z(1, 1), 1.0, out=e(1, 4, 1, 64)),
+        lambda: ops.cache_doc_scores(e(1, 4, 1, 64), cache, z(1, 1), z(1, 2), z(1, 2), 1.0, 64),
+        lambda: ops.cache_doc_scores(e(1, 4, 1, 64), cache, z(1, 1), z(1, 3), z(1, 3), 1.0, 0),
+        lambda: ops.cache_doc_scores(e(1, 4, 65, 64), cache, z(1, 1), z(1, 3), z(1, 3), 1.0, 64),
+        lambda: ops.cache_doc_scores(e(1, 4, 1, 64), cache, z(1, 1), z(1, 3), z(1, 3), 1.0, 64, temperature=0.0),
+    ]
+    for i, call in enumerate(bad):
+        with pytest.raises(ValueError):
+            call()
+            pytest.fail(f"call {i} was not refused")
+    with pytest.raises(RuntimeError, match="CUDA tensors"):
+        ops.cache_read(cache, torch.zeros(1, 3, dtype=torch.int32))
