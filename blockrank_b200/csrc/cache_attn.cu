@@ -14,6 +14,7 @@
 // fp32 queries as three.  The held values are exact in bf16, so these are the only roundings in front of the 32-bit sums.
 #include <algorithm>
 #include <atomic>
+#include <type_traits>
 
 #include "cache_layout.cuh"
 #include "tc_ptx.cuh"
@@ -25,8 +26,8 @@ using namespace cache;
 
 constexpr int kWarps = 4;
 constexpr int kThreads = 32 * kWarps;
-constexpr int kStages = 2;        // pages a warp has in shared memory
-constexpr int kShare = 512;       // pages a CTA takes at most
+constexpr int kParts = 3;         // K or V parts of pages that a warp has room for in shared memory: two K, one V
+constexpr int kShare = 128;       // pages a CTA takes at most
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 struct CacheAttnArgs {
@@ -42,6 +43,7 @@ struct CacheAttnArgs {
   float2* part_ml;       // [B, N, Lq, shares] (maximum in log2 units, sum)
   int n_pages, B, N, Nk, Lq, M, P, shares;
   float scale;
+  Codes codes;
 };
 
 // rows of prompt b, or -1 if its spans or its number of rows are malformed (all threads of the CTA)
@@ -54,25 +56,30 @@ __device__ __forceinline__ int checked_rows(const CacheAttnArgs& a, int b) {
   return __syncthreads_or(bad) ? -1 : rows;
 }
 
-template <typename T, int D, int kTiles>
-__global__ void __launch_bounds__(kThreads) cache_attn_kernel(CacheAttnArgs a) {
+template <typename T, int kTiles>
+constexpr int ctas_per_sm = kTiles == 1 && sizeof(T) == 2 ? 4 : 2;
+
+// kTwice: up to 4 rows, each in columns c and c + 4: the higher 8 bits of P go into one, the rest into the other, and one MMA takes
+// both.
+template <typename T, int D, int kTiles, bool kTwice>
+__global__ void __launch_bounds__(kThreads, ctas_per_sm<T, kTiles>) cache_attn_kernel(CacheAttnArgs a) {
   using L = Layout<D>;
   constexpr bool kF32 = sizeof(T) == 4;
-  constexpr int kQ = kF32 ? 3 : 1, kP = kF32 ? 3 : 2;
-  constexpr int kCols = 8 * kTiles;
-  extern __shared__ __align__(16) unsigned char smem[];  // [kWarps][kStages][page]; at the end the warps' outputs
+  constexpr int kP = kF32 ? 3 : 2, kMmas = kTwice ? 1 : kP;
+  constexpr int kCols = 8 * kTiles, kRows = kTwice ? 4 : kCols;
+  extern __shared__ __align__(16) unsigned char smem[];  // [kWarps][kParts][part]; at the end the warps' outputs
   __shared__ uint32_t s_mask[2 * kShare];                // which tokens of the CTA's pages lie in a block
   __shared__ int32_t s_page[kShare];
   __shared__ float2 s_ml[kWarps][kCols];
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-  const int share = blockIdx.x, b = blockIdx.y / a.Nk, kvh = blockIdx.y % a.Nk, row0 = blockIdx.z * kCols;
+  const int share = blockIdx.x, b = blockIdx.y / a.Nk, kvh = blockIdx.y % a.Nk, row0 = blockIdx.z * kRows;
   const int G = a.N / a.Nk;
   ptx::grid_dependency_launch();
   ptx::grid_dependency_wait();  // (inputs of this call; the workspace of the one in front)
   const int checked = checked_rows(a, b), rows = max(checked, 0);
   if (checked < 0 && tid == 0 && a.status) atomicCAS(a.status, 0, kStatusBadCacheCall);
-  const int n_rows = min(rows * G - row0, kCols);  // of this CTA
+  const int n_rows = min(rows * G - row0, kRows);  // of this CTA
   const int32_t *start = a.blk_start + (int64_t)b * a.M, *len = a.blk_len + (int64_t)b * a.M;
   const int first_slot = start[a.M - 1] + len[a.M - 1] - rows;  // of the prompt's row 0
   // this CTA's pages: an even share of those up to the last row's slot
@@ -118,23 +125,25 @@ __global__ void __launch_bounds__(kThreads) cache_attn_kernel(CacheAttnArgs a) {
   __syncthreads();
 
   // ---- the rows ----
-  uint32_t q[kTiles][kQ][D / 32][2][2];
+  QueryRows<T, D, kTiles> q;
+  q.load([&](int c) -> const T* {
+    if (kTwice) c &= 3;
+    const int r = row0 + c;
+    if (c >= n_rows) return nullptr;
+    return reinterpret_cast<const T*>(a.q.ptr) + (int64_t)b * a.q.sb + (int64_t)(kvh * G + r % G) * a.q.sh + (int64_t)(r / G) * a.q.ss;
+  }, g, t);
   int lim[kTiles][2];  // last slot that this lane's columns see
+  float sl2[kTiles][2];
 #pragma unroll
-  for (int c = 0; c < kTiles; ++c) {
-    const int r = row0 + 8 * c + g;
-    const T* p = nullptr;
-    if (8 * c + g < n_rows)
-      p = reinterpret_cast<const T*>(a.q.ptr) + (int64_t)b * a.q.sb + (int64_t)(kvh * G + r % G) * a.q.sh + (int64_t)(r / G) * a.q.ss;
-    load_query<D, kQ>(p, t, q[c]);
+  for (int c = 0; c < kTiles; ++c)
 #pragma unroll
     for (int x = 0; x < 2; ++x) {
-      const int col = 8 * c + 2 * t + x;
+      const int col = 8 * c + (kTwice ? 2 * (t & 1) : 2 * t) + x;
       lim[c][x] = col < n_rows ? first_slot + (row0 + col) / G : INT_MAX;
+      sl2[c][x] = a.scale * kLog2e * q.unit[c][x];
     }
-  }
   const int first_lim = first_slot + row0 / G;  // the least of the CTA's rows
-  const float sl2 = a.scale * kLog2e;
+  const Codes codes = a.codes;
   float o[kTiles][L::kGroups][2][4] = {};
   float mx[kTiles][2], sum[kTiles][2];
 #pragma unroll
@@ -145,34 +154,38 @@ __global__ void __launch_bounds__(kThreads) cache_attn_kernel(CacheAttnArgs a) {
       sum[c][x] = 0.f;
     }
 
-  unsigned char* const ring = smem + warp * kStages * L::kBytes;
-  const unsigned char* const head = a.pages + (int64_t)kvh * L::kBytes + lane * 16;
+  // Copies are requested in the order K0 K1 V0 K2 V1 K3 ..., each into the place of the part that has just been used.
+  unsigned char* const ring = smem + warp * kParts * L::kHalf;
+  const unsigned char* const head = a.pages + (int64_t)kvh * L::kBytes;
   auto next = [&](int i) {  // the warp's next page with a token in it
     while (i < n && s_page[i] < 0) i += kWarps;
     return i;
   };
-  auto request = [&](int i, int stage) {
+  auto request = [&](int i, int half, int place) {
     if (i < n) {
-      const unsigned char* src = head + (int64_t)s_page[i] * a.Nk * L::kBytes;
-      unsigned char* dst = ring + stage * L::kBytes + lane * 16;
+      const unsigned char* src = head + (int64_t)s_page[i] * a.Nk * L::kBytes + half * L::kHalf + lane * 16;
+      unsigned char* dst = ring + place * L::kHalf + lane * 16;
 #pragma unroll
-      for (int x = 0; x < L::kBytes / 512; ++x) cp_async16(dst + 512 * x, src + 512 * x);
+      for (int x = 0; x < L::kHalf; x += 512)
+        if (x + 512 <= L::kHalf || lane * 16 < L::kHalf - x) cp_async16(dst + x, src + x);
     }
     cp_async_commit();
   };
-  int ahead = next(warp);
-#pragma unroll
-  for (int s = 0; s < kStages; ++s) {
-    request(ahead, s);
+  int i = next(warp), ahead = next(i + kWarps);  // the page in hand, and the one whose K is requested next
+  request(i, 0, 0);
+  request(ahead, 0, 1);
+  request(i, 1, 2);
+  int place = 0;  // of the page's K
+  while (i < n) {
+    const int i1 = ahead;
     ahead = next(ahead + kWarps);
-  }
-  int stage = 0;
-  for (int i = next(warp); i < n; i = next(i + kWarps)) {
-    cp_async_wait<kStages - 1>();
+    cp_async_wait<2>();
     __syncwarp();
-    const unsigned char* const page = ring + stage * L::kBytes;
     float s[kTiles][4][4];
-    page_logits<D, kTiles, kQ>(page, q, g, t, s);
+    q.logits(ring + place * L::kHalf, g, t, s);
+    __syncwarp();
+    request(ahead, 0, place);
+    place ^= 1;
 
     // ---- softmax ----
     const int slot0 = (page0 + i) * kPage;
@@ -203,8 +216,8 @@ __global__ void __launch_bounds__(kThreads) cache_attn_kernel(CacheAttnArgs a) {
         for (int k = 0; k < 4; ++k) top = fmaxf(top, fmaxf(s[c][k][x], s[c][k][2 + x]));
 #pragma unroll
         for (int off = 4; off <= 16; off <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
-        const float ref = top == -INFINITY ? 0.f : top * sl2;
-        scale_o[c][x] = ptx::ex2(mx[c][x] * sl2 - ref);  // (2^-inf = 0 in front of the first page)
+        const float ref = top == -INFINITY ? 0.f : top * sl2[c][x];
+        scale_o[c][x] = ptx::ex2(mx[c][x] * sl2[c][x] - ref);  // (2^-inf = 0 in front of the first page)
         grown |= top > mx[c][x];
         mx[c][x] = top;
         sum[c][x] *= scale_o[c][x];
@@ -212,7 +225,7 @@ __global__ void __launch_bounds__(kThreads) cache_attn_kernel(CacheAttnArgs a) {
         for (int k = 0; k < 4; ++k)
 #pragma unroll
           for (int y = 0; y < 2; ++y) {
-            const float p = ptx::ex2(fmaf(s[c][k][2 * y + x], sl2, -ref));
+            const float p = ptx::ex2(fmaf(s[c][k][2 * y + x], sl2[c][x], -ref));
             s[c][k][2 * y + x] = p;
             sum[c][x] += p;
           }
@@ -229,16 +242,24 @@ __global__ void __launch_bounds__(kThreads) cache_attn_kernel(CacheAttnArgs a) {
     }
 
     // ---- O^T += V^T P^T ----
+    cp_async_wait<1>();
+    __syncwarp();
+    const unsigned char* const page = ring + 2 * L::kHalf - L::kHalf;  // (offsets count from a page's beginning)
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-      uint32_t pt[kTiles][2][kP];
+      uint32_t pt[kTiles][2][kMmas];
 #pragma unroll
       for (int c = 0; c < kTiles; ++c)
 #pragma unroll
         for (int y = 0; y < 2; ++y) {
-          split2<kP>(s[c][k][2 * y], s[c][k][2 * y + 1], pt[c][y]);
+          uint32_t piece[kP];
+          split2<kP>(s[c][k][2 * y], s[c][k][2 * y + 1], piece);
+          if constexpr (kTwice) {
+            pt[c][y][0] = transpose8(t < 2 ? piece[0] : piece[1]);
+          } else {
 #pragma unroll
-          for (int x = 0; x < kP; ++x) pt[c][y][x] = transpose8(pt[c][y][x]);
+            for (int x = 0; x < kP; ++x) pt[c][y][x] = transpose8(piece[x]);
+          }
         }
       // pairs of tokens 16 k + 2 t (v[0]) and 16 k + 8 + 2 t (v[1]); words of the even token, then of the odd one
       uint32_t v[2][2 * (L::kGroups / 2)], sv[2][L::kGroups];
@@ -312,20 +333,19 @@ __global__ void __launch_bounds__(kThreads) cache_attn_kernel(CacheAttnArgs a) {
           for (int y = 0; y < 2; ++y) c2[y] = scale_offset(sv[y][j]);
 #pragma unroll
           for (int u = 0; u < 2; ++u) {  // channels 4 g + 2 u, 4 g + 2 u + 1 of group j
-            const uint32_t e0 = held(x[0][2 * z + u], sv[0][j], c2[0]), e1 = held(x[0][2 * z + u] >> 4, sv[0][j], c2[0]);
-            const uint32_t f0 = held(x[1][2 * z + u], sv[1][j], c2[1]), f1 = held(x[1][2 * z + u] >> 4, sv[1][j], c2[1]);
+            const uint32_t e0 = held(codes, x[0][2 * z + u], sv[0][j], c2[0]), e1 = held(codes, x[0][2 * z + u] >> 4, sv[0][j], c2[0]);
+            const uint32_t f0 = held(codes, x[1][2 * z + u], sv[1][j], c2[1]), f1 = held(codes, x[1][2 * z + u] >> 4, sv[1][j], c2[1]);
 #pragma unroll
             for (int c = 0; c < kTiles; ++c)
 #pragma unroll
-              for (int p = 0; p < kP; ++p) mma(o[c][j][u], e0, e1, f0, f1, pt[c][0][p], pt[c][1][p]);
+              for (int p = 0; p < kMmas; ++p) mma(o[c][j][u], e0, e1, f0, f1, pt[c][0][p], pt[c][1][p]);
           }
         }
       }
     }
     __syncwarp();
-    request(ahead, stage);
-    ahead = next(ahead + kWarps);
-    stage = stage + 1 == kStages ? 0 : stage + 1;
+    request(i1, 1, 2);
+    i = i1;
   }
   cp_async_wait<0>();
 
@@ -336,7 +356,7 @@ __global__ void __launch_bounds__(kThreads) cache_attn_kernel(CacheAttnArgs a) {
     for (int x = 0; x < 2; ++x) {
 #pragma unroll
       for (int off = 4; off <= 16; off <<= 1) sum[c][x] += __shfl_xor_sync(0xffffffffu, sum[c][x], off);
-      if (g == 0) s_ml[warp][8 * c + 2 * t + x] = make_float2(mx[c][x] * sl2, sum[c][x]);
+      if (g == 0) s_ml[warp][8 * c + 2 * t + x] = make_float2(mx[c][x] * sl2[c][x], sum[c][x]);
     }
   __syncthreads();  // every page has been used
   float* const s_o = reinterpret_cast<float*>(smem);  // [kWarps][kCols][D]
@@ -349,7 +369,7 @@ __global__ void __launch_bounds__(kThreads) cache_attn_kernel(CacheAttnArgs a) {
         *reinterpret_cast<float4*>(s_o + (warp * kCols + 8 * c + 2 * t + x) * D + 32 * j + 4 * g) =
             make_float4(o[c][j][0][x], o[c][j][0][2 + x], o[c][j][1][x], o[c][j][1][2 + x]);
   __syncthreads();
-  for (int i = tid; i < kCols * (D / 4); i += kThreads) {
+  for (int i = tid; i < kRows * (D / 4); i += kThreads) {
     const int col = i / (D / 4), d = i % (D / 4) * 4;
     const int r = row0 + col, tok = r / G, hd = kvh * G + r % G;
     if (tok >= a.Lq) break;
@@ -363,7 +383,11 @@ __global__ void __launch_bounds__(kThreads) cache_attn_kernel(CacheAttnArgs a) {
       for (int w = 0; w < kWarps; ++w) {
         const float2 ml = s_ml[w][col];
         const float f = ptx::ex2(ml.x - ref);
-        const float4 x = *reinterpret_cast<const float4*>(s_o + (w * kCols + col) * D + d);
+        float4 x = *reinterpret_cast<const float4*>(s_o + (w * kCols + col) * D + d);
+        if constexpr (kTwice) {
+          const float4 y = *reinterpret_cast<const float4*>(s_o + (w * kCols + col + 4) * D + d);
+          x.x += y.x; x.y += y.y; x.z += y.z; x.w += y.w;
+        }
         l = fmaf(ml.y, f, l);
         acc.x = fmaf(x.x, f, acc.x); acc.y = fmaf(x.y, f, acc.y); acc.z = fmaf(x.z, f, acc.z); acc.w = fmaf(x.w, f, acc.w);
       }
@@ -382,52 +406,82 @@ __global__ void __launch_bounds__(kThreads) cache_attn_kernel(CacheAttnArgs a) {
   }
 }
 
-// One warp per row.  A share without pages has written its statistics and nothing else.
+// One CTA per row; D / 4 threads read a share's part, 4 channels each.  A share without pages has written its statistics alone.
+// Bound by latency: a thread's first parts are requested together with the statistics.
 template <typename T, int D>
 __global__ void __launch_bounds__(128) cache_join_kernel(CacheAttnArgs a) {
-  const int lane = threadIdx.x & 31;
-  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);  // (b, head, token)
+  constexpr int kLanes = D / 4, kAtOnce = 128 / kLanes, kHeld = 4;
+  __shared__ float4 s_acc[128];
+  const int tid = threadIdx.x, lane = tid & 31, sub = tid / kLanes, d = tid % kLanes * 4;
+  const int64_t row = blockIdx.x;  // (b, head, token)
   ptx::grid_dependency_wait();
-  if (row >= (int64_t)a.B * a.N * a.Lq) return;
   const int tok = (int)(row % a.Lq), hd = (int)(row / a.Lq % a.N), b = (int)(row / a.Lq / a.N);
   const int rows = a.q_len ? a.q_len[b] : a.Lq;
-  constexpr int kPer = D / 32;
-  float acc[kPer] = {}, l = 0.f, ref = 0.f;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  float l = 0.f, ref = 0.f;
   if (tok < rows) {
-    const float2* ml = a.part_ml + row * a.shares;
+    const float2* const ml = a.part_ml + row * a.shares;
+    const float* const part = a.part_o + row * a.shares * D + d;
+    float4 held[kHeld];
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i)
+      if (sub + i * kAtOnce < a.shares) held[i] = load4(part + (int64_t)(sub + i * kAtOnce) * D);
     float m = -INFINITY;
     for (int c = lane; c < a.shares; c += 32) m = fmaxf(m, ml[c].x);
 #pragma unroll
     for (int off = 16; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, off));
     ref = m == -INFINITY ? 0.f : m;
-    for (int c = 0; c < a.shares; ++c) {
-      const float2 x = ml[c];
-      if (x.y == 0.f) continue;
-      const float f = ptx::ex2(x.x - ref);
-      l = fmaf(x.y, f, l);
-      const float* p = a.part_o + (row * a.shares + c) * D + lane;
+    for (int c = lane; c < a.shares; c += 32) l = fmaf(ml[c].y, ptx::ex2(ml[c].x - ref), l);
 #pragma unroll
-      for (int i = 0; i < kPer; ++i) acc[i] = fmaf(p[32 * i], f, acc[i]);
-    }
+    for (int off = 16; off > 0; off >>= 1) l += __shfl_xor_sync(0xffffffffu, l, off);
+    auto add = [&](int c, float4 x) {
+      const float2 w = ml[c];
+      if (w.y == 0.f) return;
+      const float f = ptx::ex2(w.x - ref);
+      acc.x = fmaf(x.x, f, acc.x); acc.y = fmaf(x.y, f, acc.y); acc.z = fmaf(x.z, f, acc.z); acc.w = fmaf(x.w, f, acc.w);
+    };
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i)
+      if (sub + i * kAtOnce < a.shares) add(sub + i * kAtOnce, held[i]);
+    for (int c = sub + kHeld * kAtOnce; c < a.shares; c += kAtOnce) add(c, load4(part + (int64_t)c * D));
+  }
+  s_acc[tid] = acc;
+  __syncthreads();
+  if (sub != 0) return;
+#pragma unroll
+  for (int i = 1; i < kAtOnce; ++i) {
+    const float4 x = s_acc[tid + i * kLanes];
+    acc.x += x.x; acc.y += x.y; acc.z += x.z; acc.w += x.w;
   }
   const float inv = l != 0.f ? 1.f / l : 0.f;
-  T* dst = reinterpret_cast<T*>(a.o.ptr) + (int64_t)b * a.o.sb + (int64_t)hd * a.o.sh + (int64_t)tok * a.o.ss + lane;
-#pragma unroll
-  for (int i = 0; i < kPer; ++i) Elem<T>::store(dst + 32 * i, acc[i] * inv);
-  if (a.lse && lane == 0) a.lse[row] = l != 0.f ? (ref + log2f(l)) * kLn2 : -INFINITY;
+  store4(reinterpret_cast<T*>(a.o.ptr) + (int64_t)b * a.o.sb + (int64_t)hd * a.o.sh + (int64_t)tok * a.o.ss + d,
+         make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv));
+  if (a.lse && tid == 0) a.lse[row] = l != 0.f ? (ref + log2f(l)) * kLn2 : -INFINITY;
 }
 
-// Rows of a CTA: 8 or 16.
-int row_tiles(const brk_cache_attn_params& p) { return (int64_t)p.Lq * (p.N / p.cache.Nk) > 8 ? 2 : 1; }
+// Rows of a CTA: 4 (bf16), 8 or 16.
+int rows_per_cta(const brk_cache_attn_params& p) {
+  const int64_t rows = (int64_t)p.Lq * (p.N / p.cache.Nk);
+  return rows <= 4 && p.dtype == BRK_BF16 ? 4 : rows <= 8 ? 8 : 16;
+}
+int64_t row_groups(const brk_cache_attn_params& p) {
+  return ((int64_t)p.Lq * (p.N / p.cache.Nk) + rows_per_cta(p) - 1) / rows_per_cta(p);
+}
 
-// Shares of a prompt's pages: CTAs for every SM several times over, as long as a share has a page for each warp, and none
-// beyond kShare pages.
+// Shares of a prompt's pages, at most kShare pages each.  A round of CTAs (three per SM) takes as long as its share, with about
+// six pages' time for beginning and end; what is left over of the SMs in the last round is lost.
 int shares_of(const brk_cache_attn_params& p) {
-  const int64_t tiles = ((int64_t)p.Lq * (p.N / p.cache.Nk) + 8 * row_tiles(p) - 1) / (8 * row_tiles(p));
-  const int64_t ctas = (int64_t)p.B * p.cache.Nk * tiles;
-  const int64_t want = (3 * (int64_t)std::max(1, sm_count()) + ctas - 1) / ctas;
-  const int64_t most = (p.P + kWarps - 1) / kWarps, least = (p.P + kShare - 1) / kShare;
-  return (int)std::max(least, std::min(want, most));
+  const int64_t ctas = (int64_t)p.B * p.cache.Nk * row_groups(p), room = (p.dtype == BRK_BF16 && rows_per_cta(p) <= 8 ? 4 : 2) * (int64_t)std::max(1, sm_count());
+  const int64_t least = (p.P + kShare - 1) / kShare, most = std::max<int64_t>(least, std::min<int64_t>(64, (p.P + kWarps - 1) / kWarps));
+  int64_t best = least, best_cost = INT64_MAX;
+  for (int64_t s = least; s <= most; ++s) {
+    const int64_t cost = (ctas * s + room - 1) / room * ((p.P + s - 1) / s + 6) + (s > 1 ? 4 + s / 8 : 0);
+    if (cost < best_cost) {
+      best_cost = cost;
+      best = s;
+    }
+  }
+  return (int)best;
 }
 
 }  // namespace
@@ -454,12 +508,11 @@ int cache_attn_launch(const brk_cache_attn_params& p, void* ws, cudaStream_t st)
   const size_t rows = (size_t)p.B * p.N * p.Lq;
   a.part_o = static_cast<float*>(ws);
   a.part_ml = reinterpret_cast<float2*>(a.part_o + rows * a.shares * p.cache.D);
-  const int tiles = row_tiles(p);
-  const int64_t z = ((int64_t)p.Lq * (p.N / a.Nk) + 8 * tiles - 1) / (8 * tiles);
+  const int64_t z = row_groups(p);
   BRK_REQUIRE(z <= 65535, BRK_E_UNSUPPORTED, "Lq * N / Nk = %lld rows are too many for one call", (long long)p.Lq * (p.N / a.Nk));
   const dim3 grid(a.shares, p.B * a.Nk, (unsigned)z);
   auto run = [&](auto kern, std::atomic<bool>* configured) -> int {
-    const int bytes = kWarps * kStages * (int)head_page_bytes(p.cache.D);
+    const int bytes = kWarps * kParts * (int)head_page_bytes(p.cache.D) / 2;
     int dev = 0;
     BRK_CUDA(cudaGetDevice(&dev));
     if (dev < 0 || dev >= 64 || !configured[dev].load(std::memory_order_acquire)) {
@@ -469,18 +522,18 @@ int cache_attn_launch(const brk_cache_attn_params& p, void* ws, cudaStream_t st)
     }
     return launch_dependent(kern, grid, dim3(kThreads), bytes, st, a);
   };
-  static std::atomic<bool> done[8][64] = {};
-  int rc;
+  static std::atomic<bool> done[10][64] = {};
   const bool f32 = p.dtype == BRK_F32;
-  if (p.cache.D == 128) {
-    if (f32) rc = tiles == 1 ? run(cache_attn_kernel<float, 128, 1>, done[0]) : run(cache_attn_kernel<float, 128, 2>, done[1]);
-    else rc = tiles == 1 ? run(cache_attn_kernel<__nv_bfloat16, 128, 1>, done[2]) : run(cache_attn_kernel<__nv_bfloat16, 128, 2>, done[3]);
-  } else {
-    if (f32) rc = tiles == 1 ? run(cache_attn_kernel<float, 64, 1>, done[4]) : run(cache_attn_kernel<float, 64, 2>, done[5]);
-    else rc = tiles == 1 ? run(cache_attn_kernel<__nv_bfloat16, 64, 1>, done[6]) : run(cache_attn_kernel<__nv_bfloat16, 64, 2>, done[7]);
-  }
+  const int per = rows_per_cta(p);
+  auto of_head_dim = [&](auto d, std::atomic<bool>(*flags)[64]) -> int {
+    constexpr int D = decltype(d)::value;
+    if (f32) return per == 8 ? run(cache_attn_kernel<float, D, 1, false>, flags[0]) : run(cache_attn_kernel<float, D, 2, false>, flags[1]);
+    if (per == 4) return run(cache_attn_kernel<__nv_bfloat16, D, 1, true>, flags[2]);
+    return per == 8 ? run(cache_attn_kernel<__nv_bfloat16, D, 1, false>, flags[3]) : run(cache_attn_kernel<__nv_bfloat16, D, 2, false>, flags[4]);
+  };
+  const int rc = p.cache.D == 128 ? of_head_dim(std::integral_constant<int, 128>(), done) : of_head_dim(std::integral_constant<int, 64>(), done + 5);
   if (rc || a.shares == 1) return rc;
-  const dim3 joins((unsigned)((rows + 3) / 4)), block(128);
+  const dim3 joins((unsigned)rows), block(128);
   if (p.cache.D == 128)
     return f32 ? launch_dependent(cache_join_kernel<float, 128>, joins, block, 0, st, a)
                : launch_dependent(cache_join_kernel<__nv_bfloat16, 128>, joins, block, 0, st, a);

@@ -108,7 +108,7 @@ __global__ void __launch_bounds__(kIoThreads) cache_write_kernel(IoArgs a) {
   if (slot < 0) return;
   unsigned char* const page = a.pages + ((int64_t)(slot / kPage) * a.Nk + h) * L::kBytes;
   const int at = slot % kPage;
-  *reinterpret_cast<uint32_t*>(page + L::k_word(at, j, t)) = rotl(wk, 3);
+  *reinterpret_cast<uint32_t*>(page + L::k_word(at, j, t)) = wk;
   *reinterpret_cast<uint32_t*>(page + L::v_word(at, 2 * t + (j & 1), j >> 1)) = rotl(word, 3);
   if (t == 0) *reinterpret_cast<__nv_bfloat16*>(page + L::k_scale(at, j)) = __float2bfloat16_rn(sk);
   if (t == 1) *reinterpret_cast<__nv_bfloat16*>(page + L::v_scale(at, j)) = __float2bfloat16_rn(sv);
@@ -132,7 +132,7 @@ __global__ void __launch_bounds__(kIoThreads) cache_read_kernel(IoArgs a) {
   if (slot >= 0) {
     const unsigned char* const page = a.pages + ((int64_t)(slot / kPage) * a.Nk + h) * L::kBytes;
     const int at = slot % kPage;
-    const uint32_t wk = rotr(*reinterpret_cast<const uint32_t*>(page + L::k_word(at, j, t)), 3);
+    const uint32_t wk = *reinterpret_cast<const uint32_t*>(page + L::k_word(at, j, t));
     const uint32_t w0 = rotr(*reinterpret_cast<const uint32_t*>(page + L::v_word(at, 2 * t, j >> 1)), 3);
     const uint32_t w1 = rotr(*reinterpret_cast<const uint32_t*>(page + L::v_word(at, 2 * t + 1, j >> 1)), 3);
     const uint32_t wv = __byte_perm(w0, w1, (j & 1) ? 0x7632 : 0x5410);

@@ -4,18 +4,22 @@
 // there is a scale s with 5 significant bits and 8 exponent bits (stored as bf16) and a code u = n + 8 per channel, n in -7..7;
 // the value is n s.
 //
-// 3 bits of n times 5 bits of s fit the 8 significant bits of bf16, so the tensor cores get the held values themselves, unrounded,
-// and one instruction per two values makes them: with u in bits 3..6 of a bf16 whose exponent is that of 16, the number is
-// 16 + u = 24 + n, and fma(24 + n, s, -24 s) = n s is exact (24 s has 7 significant bits).  Hence every 32-bit word of codes is
-// stored rotated by 3 bits to the left: a shift by a multiple of 4 brings any code there.  (A scale with all 8 bits of bf16
-// would have to be applied behind the product: for V once per group of 32 channels to each probability and both parts that
-// it is split into, for K to every accumulator; counted from the source 351 instructions per 16 keys instead of 287.)
+// Both products take the codes as they are, without rounding:
 //
-// The order inside a row follows the fragments of mma.m16n8k16, lane = 4 g + t, so that every lane's codes are one load:
+// V: 3 bits of n times 5 bits of s fit the 8 significant bits of bf16, and one instruction per two values makes them: with u in bits
+// 3..6 of a bf16 whose exponent is that of 16, the number is 16 + u = 24 + n, and fma(24 + n, s, -24 s) = n s is exact (24 s has 7
+// significant bits).
+//
+// K: the scale of a group can wait for the sum over its channels, so the codes go in as numbers: the low 8 bits of a bf16, its
+// mantissa and its lowest exponent bit, are one even grid (subnormals and the binade above them), so a code in bits 0..3 is u 2^-133 and
+// one in bits 4..7 16 u 2^-133 by a mask alone.  The query is scaled by a power of two (exact) that brings its largest magnitude to
+// 2^120, and by 1/16 where it meets the latter; -8 sum(q) s, summed over the groups, is one more product, of the scales.
+// The order inside a row follows the MMA fragments, lane = 4 g + t, so that every lane's codes are one load:
 //   K  row r (D/2 bytes): word t (D/32) + j holds channels 32 j + 8 t + 0..7.  Lane (g, t) reads the D/32 words of key g from
-//      its quarter on: A (16 keys x 16 channels), where a step's channels are two of each t's, in whatever order Q has too.
+//      its quarter on: A (16 keys x the channels of group j), in whatever order Q has them too.
 //   V  tokens 2p, 2p + 1 (D bytes): piece g (D/8 bytes) holds channels 32 j + 4 g + 0..3 of both tokens, first all of 2p's.
-//      Lane (g, t) reads the piece g of pair t: A (16 channels x 16 keys), two keys of a register side by side.
+//      Lane (g, t) reads the piece g of pair t: A (16 channels x 16 keys), two keys of a register side by side.  Words are
+//      stored rotated by 3 bits to the left: whole bytes and shifts by 4 bring any code to bits 3..6.
 //   scales: K [64][D/32]; V [32 pairs][D/32][2 tokens].
 #pragma once
 #include "brk_common.cuh"
@@ -45,7 +49,11 @@ struct Layout {
 };
 inline size_t head_page_bytes(int D) { return D == 128 ? Layout<128>::kBytes : Layout<64>::kBytes; }
 
-constexpr uint32_t kCodeMask = 0x00780078u, kCodeBase = 0x41804180u;  // bits 3..6 of both halves; 16.0 in both
+// For V: bits 3..6 of both halves of a word, and 16.0 in both.  An argument of the kernels: of constants that it knows the assembler makes
+// two instructions for every (x & mask) | base, since only one operand can be a constant.
+struct Codes {
+  uint32_t mask = 0x00780078u, base = 0x41804180u;
+};
 
 __device__ __forceinline__ uint32_t rotr(uint32_t x, int n) { return __funnelshift_r(x, x, n); }
 __device__ __forceinline__ uint32_t rotl(uint32_t x, int n) { return __funnelshift_l(x, x, n); }
@@ -62,7 +70,9 @@ __device__ __forceinline__ uint32_t scale_offset(uint32_t s2) {
   return d;
 }
 // two codes in bits 3..6 and 19..22 of x (others are ignored) -> their values
-__device__ __forceinline__ uint32_t held(uint32_t x, uint32_t s2, uint32_t c2) { return fma_bf2((x & kCodeMask) | kCodeBase, s2, c2); }
+__device__ __forceinline__ uint32_t held(const Codes& k, uint32_t x, uint32_t s2, uint32_t c2) {
+  return fma_bf2((x & k.mask) | k.base, s2, c2);
+}
 
 // C (16 x 8) += A (16 x 16) B (16 x 8)
 __device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -92,80 +102,130 @@ __device__ __forceinline__ void split2(float x0, float x1, uint32_t (&piece)[kPi
   }
 }
 
-// The K part of a page (in shared memory) times kTiles x 8 query rows: s[n][i] is the C fragment of keys 16 i .. 16 i + 15 and
-// rows 8 n .. 8 n + 7.  q[n][piece][j][h]: B fragment of group j's step h, channels 32 j + 8 t + 2 h + {0, 4} and {1, 5}.
-template <int D, int kTiles, int kPieces>
-__device__ __forceinline__ void page_logits(const unsigned char* page, const uint32_t (&q)[kTiles][kPieces][D / 32][2][2], int g, int t,
-                                            float (&s)[kTiles][4][4]) {
-  using L = Layout<D>;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    uint32_t wa[L::kGroups], wb[L::kGroups], sa[L::kGroups / 2], sb[L::kGroups / 2];
-    const unsigned char *ka = page + L::k_word(16 * i + g, 0, t), *kb = page + L::k_word(16 * i + 8 + g, 0, t);
-    const unsigned char *ca = page + L::k_scale(16 * i + g, 0), *cb = page + L::k_scale(16 * i + 8 + g, 0);
-    if constexpr (D == 128) {
-      *reinterpret_cast<uint4*>(wa) = *reinterpret_cast<const uint4*>(ka);
-      *reinterpret_cast<uint4*>(wb) = *reinterpret_cast<const uint4*>(kb);
-      *reinterpret_cast<uint2*>(sa) = *reinterpret_cast<const uint2*>(ca);
-      *reinterpret_cast<uint2*>(sb) = *reinterpret_cast<const uint2*>(cb);
-    } else {
-      *reinterpret_cast<uint2*>(wa) = *reinterpret_cast<const uint2*>(ka);
-      *reinterpret_cast<uint2*>(wb) = *reinterpret_cast<const uint2*>(kb);
-      sa[0] = *reinterpret_cast<const uint32_t*>(ca);
-      sb[0] = *reinterpret_cast<const uint32_t*>(cb);
-    }
-#pragma unroll
-    for (int n = 0; n < kTiles; ++n)
-#pragma unroll
-      for (int x = 0; x < 4; ++x) s[n][i][x] = 0.f;
-#pragma unroll
-    for (int j = 0; j < L::kGroups; ++j) {
-      const uint32_t s2a = __byte_perm(sa[j / 2], 0, j % 2 ? 0x3232 : 0x1010), s2b = __byte_perm(sb[j / 2], 0, j % 2 ? 0x3232 : 0x1010);
-      const uint32_t c2a = scale_offset(s2a), c2b = scale_offset(s2b);
-      uint32_t a[4], b[4];
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        a[k] = held(rotr(wa[j], 4 * k), s2a, c2a);
-        b[k] = held(rotr(wb[j], 4 * k), s2b, c2b);
-      }
-#pragma unroll
-      for (int h = 0; h < 2; ++h)
-#pragma unroll
-        for (int n = 0; n < kTiles; ++n)
-#pragma unroll
-          for (int p = 0; p < kPieces; ++p) mma(s[n][i], a[2 * h], b[2 * h], a[2 * h + 1], b[2 * h + 1], q[n][p][j][h][0], q[n][p][j][h][1]);
-    }
-  }
+template <int D>
+__device__ __forceinline__ void load_words(const unsigned char* p, uint32_t (&w)[D / 32]) {
+  if constexpr (D == 128) *reinterpret_cast<uint4*>(w) = *reinterpret_cast<const uint4*>(p);
+  else *reinterpret_cast<uint2*>(w) = *reinterpret_cast<const uint2*>(p);
+}
+template <int D>
+__device__ __forceinline__ void load_scales(const unsigned char* p, uint32_t (&w)[D / 64]) {
+  if constexpr (D == 128) *reinterpret_cast<uint2*>(w) = *reinterpret_cast<const uint2*>(p);
+  else w[0] = *reinterpret_cast<const uint32_t*>(p);
 }
 
-// The B fragments of one query row for page_logits: this lane's channels 32 j + 8 t + 0..7 of the row at `p` (null: zeros).
-template <int D, int kPieces>
-__device__ __forceinline__ void load_query(const __nv_bfloat16* p, int t, uint32_t (&q)[kPieces][D / 32][2][2]) {
-  static_assert(kPieces == 1, "bf16 needs no splitting");
+// The rows of a warp as the 8-column operand: 8 kTiles columns of queries, one row each, and their products with pages of keys.
+// A bf16 query is one bf16 number, an fp32 one three.  Logits are to be multiplied by `unit` (by tile and by which of the two
+// columns of a C fragment): each row's power of two.
+template <typename T, int D, int kTiles>
+struct QueryRows {
+  using L = Layout<D>;
+  static constexpr int kPieces = sizeof(T) == 4 ? 3 : 1;
+  uint32_t q[kTiles][kPieces][L::kGroups][2][2];  // [group][step][register]: channels 8 t + 2 step + {0, 4}, {1, 5}
+  uint32_t shift[kTiles][2];                      // B of the product of the scales: -8 2^-133 sum(q) of the groups, in three bf16 numbers
+  float unit[kTiles][2];
+
+  // row(c): column c's query, null for none
+  template <typename F>
+  __device__ __forceinline__ void load(F row, int g, int t) {
 #pragma unroll
-  for (int j = 0; j < D / 32; ++j) {
-    const uint4 w = p ? *reinterpret_cast<const uint4*>(p + 32 * j + 8 * t) : make_uint4(0, 0, 0, 0);
-    q[0][j][0][0] = __byte_perm(w.x, w.z, 0x5410);
-    q[0][j][0][1] = __byte_perm(w.x, w.z, 0x7632);
-    q[0][j][1][0] = __byte_perm(w.y, w.w, 0x5410);
-    q[0][j][1][1] = __byte_perm(w.y, w.w, 0x7632);
-  }
-}
-template <int D, int kPieces>
-__device__ __forceinline__ void load_query(const float* p, int t, uint32_t (&q)[kPieces][D / 32][2][2]) {
+    for (int n = 0; n < kTiles; ++n) {
+      const T* const p = row(8 * n + g);
+      float x[L::kGroups][8], top = 0.f;
 #pragma unroll
-  for (int j = 0; j < D / 32; ++j) {
-    float x[8] = {};
-    if (p) load8(p + 32 * j + 8 * t, x);
+      for (int j = 0; j < L::kGroups; ++j) {
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      uint32_t piece[kPieces];
-      split2<kPieces>(x[k], x[k + 4], piece);
+        for (int k = 0; k < 8; ++k) x[j][k] = 0.f;
+        if (p) load8(p + 32 * j + 8 * t, x[j]);
 #pragma unroll
-      for (int i = 0; i < kPieces; ++i) q[i][j][k / 2][k % 2] = piece[i];
+        for (int k = 0; k < 8; ++k) top = isnan(x[j][k]) ? INFINITY : fmaxf(top, fabsf(x[j][k]));
+      }
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      // 2^up = 2^120 / 2^(exponent of top), as float exponent fields; in two factors, since it can be 2^246
+      const bool finite = top < INFINITY;
+      const int up = 120 + 127 - (int)max(__float_as_uint(top) >> 23, 1u);
+      const float up0 = __uint_as_float((uint32_t)(up / 2 + 127) << 23), up1 = __uint_as_float((uint32_t)(up - up / 2 + 127) << 23);
+      float total[L::kGroups];
+#pragma unroll
+      for (int j = 0; j < L::kGroups; ++j) {
+        total[j] = 0.f;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          x[j][k] = finite ? x[j][k] * up0 * up1 : 0.f;
+          total[j] += x[j][k];
+        }
+        total[j] += __shfl_xor_sync(0xffffffffu, total[j], 1);
+        total[j] += __shfl_xor_sync(0xffffffffu, total[j], 2);
+        total[j] *= -0x1p-126f * 0x1p-4f;  // (about 2^-5)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          uint32_t piece[kPieces];
+          const float f = k % 2 ? 0.0625f : 1.f;
+          split2<kPieces>(x[j][k] * f, x[j][k + 4] * f, piece);
+#pragma unroll
+          for (int i = 0; i < kPieces; ++i) q[n][i][j][k / 2][k % 2] = piece[i];
+        }
+      }
+      // The scales stand side by side in A as they do in memory, the groups' four times (D 128) or eight times over.
+      uint32_t w[3][L::kGroups / 2];
+#pragma unroll
+      for (int j = 0; j < L::kGroups; j += 2) {
+        uint32_t piece[3];
+        split2<3>(total[j], total[j + 1], piece);
+#pragma unroll
+        for (int i = 0; i < 3; ++i) w[i][j / 2] = piece[i];
+      }
+      if constexpr (D == 128) {
+        shift[n][0] = t == 0 ? w[0][0] : t == 1 ? w[0][1] : t == 2 ? w[1][0] : w[1][1];
+        shift[n][1] = t == 0 ? w[2][0] : t == 1 ? w[2][1] : 0u;
+      } else {
+        shift[n][0] = t == 0 ? w[0][0] : t == 1 ? w[1][0] : t == 2 ? w[2][0] : 0u;
+        shift[n][1] = 0u;
+      }
+      // 2^(133 - up), up >= -7: a row with NaN or an infinity has a unit of NaN, one from 2^121 on of infinity
+      const float down = !finite ? NAN : 133 - up > 127 ? INFINITY : up > 133 + 126 ? 0.f : __uint_as_float((uint32_t)(133 - up + 127) << 23);
+#pragma unroll
+      for (int y = 0; y < 2; ++y) unit[n][y] = __shfl_sync(0xffffffffu, down, 4 * (2 * t + y));
     }
   }
-}
+  // s[n][i]: the C fragment of keys 16 i .. 16 i + 15 of the page and the columns of tile n
+  __device__ __forceinline__ void logits(const unsigned char* page, int g, int t, float (&s)[kTiles][4][4]) const {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      uint32_t wa[L::kGroups], wb[L::kGroups], sa[L::kGroups / 2], sb[L::kGroups / 2];
+      load_words<D>(page + L::k_word(16 * i + g, 0, t), wa);
+      load_words<D>(page + L::k_word(16 * i + 8 + g, 0, t), wb);
+      load_scales<D>(page + L::k_scale(16 * i + g, 0), sa);
+      load_scales<D>(page + L::k_scale(16 * i + 8 + g, 0), sb);
+      {
+        const uint32_t a = D == 128 && t % 2 ? sa[L::kGroups / 2 - 1] : sa[0], b = D == 128 && t % 2 ? sb[L::kGroups / 2 - 1] : sb[0];
+#pragma unroll
+        for (int n = 0; n < kTiles; ++n) {
+#pragma unroll
+          for (int x = 0; x < 4; ++x) s[n][i][x] = 0.f;
+          mma(s[n][i], a, b, a, b, shift[n][0], shift[n][1]);
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < L::kGroups; ++j) {
+        const float fa = j % 2 ? bf_hi(sa[j / 2]) : bf_lo(sa[j / 2]), fb = j % 2 ? bf_hi(sb[j / 2]) : bf_lo(sb[j / 2]);
+        const uint32_t a8 = wa[j] >> 8, b8 = wb[j] >> 8;
+        const uint32_t a[4] = {wa[j] & 0x000F000Fu, wa[j] & 0x00F000F0u, a8 & 0x000F000Fu, a8 & 0x00F000F0u};  // codes k and k + 4
+        const uint32_t b[4] = {wb[j] & 0x000F000Fu, wb[j] & 0x00F000F0u, b8 & 0x000F000Fu, b8 & 0x00F000F0u};
+#pragma unroll
+        for (int n = 0; n < kTiles; ++n) {
+          float x[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int p = 0; p < kPieces; ++p)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) mma(x, a[2 * h], b[2 * h], a[2 * h + 1], b[2 * h + 1], q[n][p][j][h][0], q[n][p][j][h][1]);
+#pragma unroll
+          for (int z = 0; z < 4; ++z) s[n][i][z] = fmaf(x[z], z < 2 ? fa : fb, s[n][i][z]);
+        }
+      }
+    }
+  }
+};
 
 // One prompt's block spans, read by all threads of a CTA: `bad` if a block lies outside [0, slots), has a negative length or
 // begins before the end of the one in front of it.

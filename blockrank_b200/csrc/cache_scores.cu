@@ -34,9 +34,8 @@ struct CacheScoreArgs {
 };
 
 template <typename T, int D, int kTiles>
-__global__ void __launch_bounds__(kThreads) cache_scores_kernel(CacheScoreArgs a) {
+__global__ void __launch_bounds__(kThreads, kTiles == 1 && sizeof(T) == 2 ? 4 : 2) cache_scores_kernel(CacheScoreArgs a) {
   using L = Layout<D>;
-  constexpr int kQ = sizeof(T) == 4 ? 3 : 1;
   constexpr int kCols = 8 * kTiles;
   extern __shared__ __align__(16) unsigned char smem[];  // [kWarps][kStages][K part of a page]
   __shared__ float2 s_ml[kWarps][kCols];
@@ -88,21 +87,18 @@ __global__ void __launch_bounds__(kThreads) cache_scores_kernel(CacheScoreArgs a
 #pragma unroll
   for (int s = 0; s < kStages; ++s) request(part + s * a.split, s);
 
-  uint32_t q[kTiles][kQ][D / 32][2][2];
-#pragma unroll
-  for (int c = 0; c < kTiles; ++c) {
-    const int r = row0 + 8 * c + g;
-    const T* p = nullptr;
-    if (r < GR)
-      p = reinterpret_cast<const T*>(a.q.ptr) + (int64_t)b * a.q.sb + (int64_t)(kvh * G + r / a.R) * a.q.sh + (int64_t)(r % a.R) * a.q.ss;
-    load_query<D, kQ>(p, t, q[c]);
-  }
-  const float sl2 = a.scale * kLog2e;
-  float mx[kTiles][2], sum[kTiles][2];  // this lane's keys
+  QueryRows<T, D, kTiles> q;
+  q.load([&](int c) -> const T* {
+    const int r = row0 + c;
+    if (r >= GR) return nullptr;
+    return reinterpret_cast<const T*>(a.q.ptr) + (int64_t)b * a.q.sb + (int64_t)(kvh * G + r / a.R) * a.q.sh + (int64_t)(r % a.R) * a.q.ss;
+  }, g, t);
+  float sl2[kTiles][2], mx[kTiles][2], sum[kTiles][2];  // this lane's keys
 #pragma unroll
   for (int c = 0; c < kTiles; ++c)
 #pragma unroll
     for (int x = 0; x < 2; ++x) {
+      sl2[c][x] = a.scale * kLog2e * q.unit[c][x];
       mx[c][x] = -INFINITY;
       sum[c][x] = 0.f;
     }
@@ -112,7 +108,7 @@ __global__ void __launch_bounds__(kThreads) cache_scores_kernel(CacheScoreArgs a
     __syncwarp();
     if (!((absent >> stage) & 1)) {
       float s[kTiles][4][4];
-      page_logits<D, kTiles, kQ>(ring + stage * L::kHalf, q, g, t, s);
+      q.logits(ring + stage * L::kHalf, g, t, s);
       const int from = start - (page0 + i) * kPage, to = start + len - (page0 + i) * kPage;  // the document's tokens in this page
       if (from > 0 || to < kPage) {
 #pragma unroll
@@ -133,13 +129,13 @@ __global__ void __launch_bounds__(kThreads) cache_scores_kernel(CacheScoreArgs a
           float top = mx[c][x];
 #pragma unroll
           for (int k = 0; k < 4; ++k) top = fmaxf(top, fmaxf(s[c][k][x], s[c][k][2 + x]));
-          const float ref = top == -INFINITY ? 0.f : top * sl2;
-          sum[c][x] *= ptx::ex2(mx[c][x] * sl2 - ref);
+          const float ref = top == -INFINITY ? 0.f : top * sl2[c][x];
+          sum[c][x] *= ptx::ex2(mx[c][x] * sl2[c][x] - ref);
           mx[c][x] = top;
 #pragma unroll
           for (int k = 0; k < 4; ++k)
 #pragma unroll
-            for (int y = 0; y < 2; ++y) sum[c][x] += ptx::ex2(fmaf(s[c][k][2 * y + x], sl2, -ref));
+            for (int y = 0; y < 2; ++y) sum[c][x] += ptx::ex2(fmaf(s[c][k][2 * y + x], sl2[c][x], -ref));
         }
     }
     __syncwarp();
@@ -151,7 +147,7 @@ __global__ void __launch_bounds__(kThreads) cache_scores_kernel(CacheScoreArgs a
   for (int c = 0; c < kTiles; ++c)
 #pragma unroll
     for (int x = 0; x < 2; ++x) {
-      float m = mx[c][x] * sl2, l = sum[c][x];
+      float m = mx[c][x] * sl2[c][x], l = sum[c][x];
 #pragma unroll
       for (int off = 4; off <= 16; off <<= 1) {
         const float m2 = __shfl_xor_sync(0xffffffffu, m, off), l2 = __shfl_xor_sync(0xffffffffu, l, off);
