@@ -272,7 +272,7 @@ static int check_cache(const brk_cache* c) {
   BRK_REQUIRE(c != nullptr && c->pages != nullptr, BRK_E_ARG, "cache is null");
   BRK_REQUIRE(((uintptr_t)c->pages & 15) == 0, BRK_E_ARG, "cache must be 16-byte aligned");
   BRK_REQUIRE(c->D == 64 || c->D == 128, BRK_E_UNSUPPORTED, "head_dim %d not supported (64 or 128)", c->D);
-  BRK_REQUIRE(c->Nk > 0 && c->n_pages > 0 && (int64_t)c->n_pages * BRK_CACHE_PAGE < (1ll << 31), BRK_E_ARG,
+  BRK_REQUIRE(c->Nk > 0 && c->Nk <= 4096 && c->n_pages > 0 && (int64_t)c->n_pages * BRK_CACHE_PAGE < (1ll << 31), BRK_E_ARG,
               "bad cache shape: %d pages, %d KV heads", c->n_pages, c->Nk);
   return BRK_OK;
 }

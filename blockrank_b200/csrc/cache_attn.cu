@@ -57,7 +57,7 @@ __device__ __forceinline__ int checked_rows(const CacheAttnArgs& a, int b) {
 }
 
 template <typename T, int kTiles>
-constexpr int ctas_per_sm = kTiles == 1 && sizeof(T) == 2 ? 4 : 2;
+constexpr int ctas_per_sm = kTiles == 1 && sizeof(T) == 2 ? 3 : 2;
 
 // kTwice: up to 4 rows, each in columns c and c + 4: the higher 8 bits of P go into one, the rest into the other, and one MMA takes
 // both.
@@ -471,7 +471,7 @@ int64_t row_groups(const brk_cache_attn_params& p) {
 // Shares of a prompt's pages, at most kShare pages each.  A round of CTAs (three per SM) takes as long as its share, with about
 // six pages' time for beginning and end; what is left over of the SMs in the last round is lost.
 int shares_of(const brk_cache_attn_params& p) {
-  const int64_t ctas = (int64_t)p.B * p.cache.Nk * row_groups(p), room = (p.dtype == BRK_BF16 && rows_per_cta(p) <= 8 ? 4 : 2) * (int64_t)std::max(1, sm_count());
+  const int64_t ctas = (int64_t)p.B * p.cache.Nk * row_groups(p), room = (p.dtype == BRK_BF16 && rows_per_cta(p) <= 8 ? 3 : 2) * (int64_t)std::max(1, sm_count());
   const int64_t least = (p.P + kShare - 1) / kShare, most = std::max<int64_t>(least, std::min<int64_t>(64, (p.P + kWarps - 1) / kWarps));
   int64_t best = least, best_cost = INT64_MAX;
   for (int64_t s = least; s <= most; ++s) {

@@ -427,7 +427,7 @@ brk_view heads_view(const Tensor& t) {
 int32_t* status_ptr(const Tensor& t) { return (int32_t*)status_word(t.get_device()).data_ptr(); }
 
 Tensor cache_alloc(int64_t n_pages, int64_t kv_heads, int64_t head_dim, const c10::Device& device) {
-  BRK_VALUE(n_pages > 0 && n_pages * BRK_CACHE_PAGE < (1ll << 31) && kv_heads > 0 && kv_heads < (1ll << 31), "bad cache shape: ", n_pages, " pages, ",
+  BRK_VALUE(n_pages > 0 && n_pages * BRK_CACHE_PAGE < (1ll << 31) && kv_heads > 0 && kv_heads <= 4096, "bad cache shape: ", n_pages, " pages, ",
             kv_heads, " KV heads");
   BRK_VALUE(head_dim == 64 || head_dim == 128, "head_dim ", head_dim, " not supported (64 or 128)");
   TORCH_CHECK(device.is_cuda(), "blockrank_b200 kernels run on CUDA tensors only (there is no CPU path)");
