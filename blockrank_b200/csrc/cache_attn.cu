@@ -28,6 +28,7 @@ constexpr int kWarps = 4;
 constexpr int kThreads = 32 * kWarps;
 constexpr int kParts = 3;         // K or V parts of pages that a warp has room for in shared memory: two K, one V
 constexpr int kShare = 128;       // pages a CTA takes at most
+constexpr int kCluster = 8;       // shares that a cluster joins, at most
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 struct CacheAttnArgs {
@@ -42,19 +43,10 @@ struct CacheAttnArgs {
   float* part_o;         // [B, N, Lq, shares, D]
   float2* part_ml;       // [B, N, Lq, shares] (maximum in log2 units, sum)
   int n_pages, B, N, Nk, Lq, M, P, shares;
+  bool cluster;          // a prompt's shares are a cluster, which joins its parts itself
   float scale;
   Codes codes;
 };
-
-// rows of prompt b, or -1 if its spans or its number of rows are malformed (all threads of the CTA)
-__device__ __forceinline__ int checked_rows(const CacheAttnArgs& a, int b) {
-  const int32_t *start = a.blk_start + (int64_t)b * a.M, *len = a.blk_len + (int64_t)b * a.M;
-  bool bad = false;
-  for (int m = threadIdx.x; m < a.M; m += blockDim.x) bad |= span_is_bad(start, len, m, (int64_t)a.P * kPage);
-  const int rows = a.q_len ? a.q_len[b] : a.Lq;
-  bad |= rows < 0 || rows > a.Lq || rows > len[a.M - 1];
-  return __syncthreads_or(bad) ? -1 : rows;
-}
 
 template <typename T, int kTiles>
 constexpr int ctas_per_sm = kTiles == 1 && sizeof(T) == 2 ? 3 : 2;
@@ -77,25 +69,47 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<T, kTiles>) cache_attn_k
   const int G = a.N / a.Nk;
   ptx::grid_dependency_launch();
   ptx::grid_dependency_wait();  // (inputs of this call; the workspace of the one in front)
-  const int checked = checked_rows(a, b), rows = max(checked, 0);
-  if (checked < 0 && tid == 0 && a.status) atomicCAS(a.status, 0, kStatusBadCacheCall);
-  const int n_rows = min(rows * G - row0, kRows);  // of this CTA
+
+  // ---- everything that has to be read first, at once: spans, the number of rows, the rows ----
   const int32_t *start = a.blk_start + (int64_t)b * a.M, *len = a.blk_len + (int64_t)b * a.M;
-  const int first_slot = start[a.M - 1] + len[a.M - 1] - rows;  // of the prompt's row 0
-  // this CTA's pages: an even share of those up to the last row's slot
+  const int64_t slots = (int64_t)a.P * kPage;
+  const int last_start = start[a.M - 1], last_len = len[a.M - 1], given = a.q_len ? a.q_len[b] : a.Lq;
+  int my_start = 0, my_len = 0;
+  bool bad = false;
+  typename QueryRows<T, D, kTiles>::Raw raw;
+  QueryRows<T, D, kTiles>::fetch([&](int c) -> const T* {  // (rows from q_len on among them: they are not used)
+    const int r = row0 + (kTwice ? c & 3 : c);
+    if (r >= a.Lq * G) return nullptr;
+    return reinterpret_cast<const T*>(a.q.ptr) + (int64_t)b * a.q.sb + (int64_t)(kvh * G + r % G) * a.q.sh + (int64_t)(r / G) * a.q.ss;
+  }, g, t, raw);
+  if (tid < a.M) {
+    my_start = start[tid];
+    my_len = len[tid];
+    bad = span_is_bad(start, len, tid, slots);
+  }
+  for (int m = tid + kThreads; m < a.M; m += kThreads) bad |= span_is_bad(start, len, m, slots);
+  s_mask[tid] = s_mask[tid + kThreads] = 0;
+  bad |= given < 0 || given > a.Lq || given > last_len;
+  bad = __syncthreads_or(bad);
+  if (bad && tid == 0 && a.status) atomicCAS(a.status, 0, kStatusBadCacheCall);
+
+  // ---- this CTA's rows, and its pages: an even share of those up to the last row's slot ----
+  const int rows = bad ? 0 : given, n_rows = min(rows * G - row0, kRows);
+  const int first_slot = bad ? 0 : last_start + last_len - rows;  // of the prompt's row 0
   const int last_tok = n_rows > 0 ? (row0 + n_rows - 1) / G : -1;
   const int live = n_rows > 0 ? (first_slot + last_tok) / kPage + 1 : 0;
   const int per = max((live + a.shares - 1) / a.shares, min(live, kWarps));
   const int page0 = min(live, share * per), n = min(live, page0 + per) - page0;
+  int page_id = -1;
+  if (tid < n) page_id = a.table[(int64_t)b * a.P + page0 + tid];
 
   // ---- which tokens of these pages lie in a block ----
-  for (int i = tid; i < 2 * n; i += kThreads) s_mask[i] = 0;
-  __syncthreads();
+  static_assert(kShare == kThreads, "a thread per page");
   if (n > 0) {
     const int lo = page0 * kPage, hi = (page0 + n) * kPage;
     for (int m0 = warp * 32; m0 < a.M; m0 += kThreads) {
       const int m = m0 + lane;
-      const int s = m < a.M ? start[m] : 0, e = m < a.M ? s + len[m] : 0;
+      const int s = m0 < kThreads ? my_start : m < a.M ? start[m] : 0, e = s + (m0 < kThreads ? my_len : m < a.M ? len[m] : 0);
       unsigned todo = __ballot_sync(0xffffffffu, max(s, lo) < min(e, hi));
       while (todo) {
         const int src = __ffs(todo) - 1;
@@ -107,52 +121,17 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<T, kTiles>) cache_attn_k
         }
       }
     }
-    __syncthreads();
-    bool bad = false;
-    for (int i = tid; i < n; i += kThreads) {
-      int page = -1;
-      if (s_mask[2 * i] | s_mask[2 * i + 1]) {
-        page = a.table[(int64_t)b * a.P + page0 + i];
-        if (page < 0 || page >= a.n_pages) {
-          bad = true;
-          page = -1;
-        }
-      }
-      s_page[i] = page;
-    }
-    if (bad && a.status) atomicCAS(a.status, 0, kStatusBadCacheCall);
   }
   __syncthreads();
-
-  // ---- the rows ----
-  QueryRows<T, D, kTiles> q;
-  q.load([&](int c) -> const T* {
-    if (kTwice) c &= 3;
-    const int r = row0 + c;
-    if (c >= n_rows) return nullptr;
-    return reinterpret_cast<const T*>(a.q.ptr) + (int64_t)b * a.q.sb + (int64_t)(kvh * G + r % G) * a.q.sh + (int64_t)(r / G) * a.q.ss;
-  }, g, t);
-  int lim[kTiles][2];  // last slot that this lane's columns see
-  float sl2[kTiles][2];
-#pragma unroll
-  for (int c = 0; c < kTiles; ++c)
-#pragma unroll
-    for (int x = 0; x < 2; ++x) {
-      const int col = 8 * c + (kTwice ? 2 * (t & 1) : 2 * t) + x;
-      lim[c][x] = col < n_rows ? first_slot + (row0 + col) / G : INT_MAX;
-      sl2[c][x] = a.scale * kLog2e * q.unit[c][x];
+  if (tid < n) {
+    const bool needed = (s_mask[2 * tid] | s_mask[2 * tid + 1]) != 0;
+    if (needed && (page_id < 0 || page_id >= a.n_pages)) {
+      if (a.status) atomicCAS(a.status, 0, kStatusBadCacheCall);
+      page_id = -1;
     }
-  const int first_lim = first_slot + row0 / G;  // the least of the CTA's rows
-  const Codes codes = a.codes;
-  float o[kTiles][L::kGroups][2][4] = {};
-  float mx[kTiles][2], sum[kTiles][2];
-#pragma unroll
-  for (int c = 0; c < kTiles; ++c)
-#pragma unroll
-    for (int x = 0; x < 2; ++x) {
-      mx[c][x] = -INFINITY;
-      sum[c][x] = 0.f;
-    }
+    s_page[tid] = needed ? page_id : -1;
+  }
+  __syncthreads();
 
   // Copies are requested in the order K0 K1 V0 K2 V1 K3 ..., each into the place of the part that has just been used.
   unsigned char* const ring = smem + warp * kParts * L::kHalf;
@@ -175,6 +154,32 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<T, kTiles>) cache_attn_k
   request(i, 0, 0);
   request(ahead, 0, 1);
   request(i, 1, 2);
+
+  // ---- the rows ----
+  QueryRows<T, D, kTiles> q;
+  q.make(raw, g, t);
+  int lim[kTiles][2];  // last slot that this lane's columns see
+  float sl2[kTiles][2];
+#pragma unroll
+  for (int c = 0; c < kTiles; ++c)
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      const int col = 8 * c + (kTwice ? 2 * (t & 1) : 2 * t) + x;
+      lim[c][x] = col < n_rows ? first_slot + (row0 + col) / G : INT_MAX;
+      sl2[c][x] = a.scale * kLog2e * q.unit[c][x];
+    }
+  const int first_lim = first_slot + row0 / G;  // the least of the CTA's rows
+  const Codes codes = a.codes;
+  float o[kTiles][L::kGroups][2][4] = {};
+  float mx[kTiles][2], sum[kTiles][2];
+#pragma unroll
+  for (int c = 0; c < kTiles; ++c)
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      mx[c][x] = -INFINITY;
+      sum[c][x] = 0.f;
+    }
+
   int place = 0;  // of the page's K
   while (i < n) {
     const int i1 = ahead;
@@ -369,41 +374,86 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<T, kTiles>) cache_attn_k
         *reinterpret_cast<float4*>(s_o + (warp * kCols + 8 * c + 2 * t + x) * D + 32 * j + 4 * g) =
             make_float4(o[c][j][0][x], o[c][j][0][2 + x], o[c][j][1][x], o[c][j][1][2 + x]);
   __syncthreads();
+  // the CTA's statistics and output of column `col`, channels d .. d + 3
+  auto part = [&](int col, int d, float& m, float& l, float4& acc) {
+    m = -INFINITY;
+    l = 0.f;
+    acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) m = fmaxf(m, s_ml[w][col].x);
+    const float ref = m == -INFINITY ? 0.f : m;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      const float2 ml = s_ml[w][col];
+      const float f = ptx::ex2(ml.x - ref);
+      float4 x = *reinterpret_cast<const float4*>(s_o + (w * kCols + col) * D + d);
+      if constexpr (kTwice) {
+        const float4 y = *reinterpret_cast<const float4*>(s_o + (w * kCols + col + 4) * D + d);
+        x.x += y.x; x.y += y.y; x.z += y.z; x.w += y.w;
+      }
+      l = fmaf(ml.y, f, l);
+      acc.x = fmaf(x.x, f, acc.x); acc.y = fmaf(x.y, f, acc.y); acc.z = fmaf(x.z, f, acc.z); acc.w = fmaf(x.w, f, acc.w);
+    }
+  };
+  auto write = [&](int tok, int hd, int d, float m, float l, float4 acc) {
+    const float inv = l != 0.f ? 1.f / l : 0.f;  // (a sum that is NaN stays one)
+    store4(reinterpret_cast<T*>(a.o.ptr) + (int64_t)b * a.o.sb + (int64_t)hd * a.o.sh + (int64_t)tok * a.o.ss + d,
+           make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv));
+    if (a.lse && d == 0) a.lse[((int64_t)b * a.N + hd) * a.Lq + tok] = l != 0.f ? (m + log2f(l)) * kLn2 : -INFINITY;
+  };
+  float* const s_part = s_o + kWarps * kCols * D;  // [kRows][D], then the rows' statistics: what the cluster's other CTAs read
   for (int i = tid; i < kRows * (D / 4); i += kThreads) {
     const int col = i / (D / 4), d = i % (D / 4) * 4;
     const int r = row0 + col, tok = r / G, hd = kvh * G + r % G;
     if (tok >= a.Lq) break;
-    float m = -INFINITY, l = 0.f;
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (col < n_rows) {
-#pragma unroll
-      for (int w = 0; w < kWarps; ++w) m = fmaxf(m, s_ml[w][col].x);
-      const float ref = m == -INFINITY ? 0.f : m;
-#pragma unroll
-      for (int w = 0; w < kWarps; ++w) {
-        const float2 ml = s_ml[w][col];
-        const float f = ptx::ex2(ml.x - ref);
-        float4 x = *reinterpret_cast<const float4*>(s_o + (w * kCols + col) * D + d);
-        if constexpr (kTwice) {
-          const float4 y = *reinterpret_cast<const float4*>(s_o + (w * kCols + col + 4) * D + d);
-          x.x += y.x; x.y += y.y; x.z += y.z; x.w += y.w;
-        }
-        l = fmaf(ml.y, f, l);
-        acc.x = fmaf(x.x, f, acc.x); acc.y = fmaf(x.y, f, acc.y); acc.z = fmaf(x.z, f, acc.z); acc.w = fmaf(x.w, f, acc.w);
-      }
+    float m, l;
+    float4 acc;
+    part(col, d, m, l, acc);
+    if (col >= n_rows) {
+      m = -INFINITY;
+      l = 0.f;
+      acc = make_float4(0.f, 0.f, 0.f, 0.f);
     }
-    const int64_t row = ((int64_t)b * a.N + hd) * a.Lq + tok;
-    if (a.shares > 1) {
-      if (col >= n_rows && checked >= 0) continue;  // (the join looks at q_len: a malformed prompt's rows get statistics, of nothing)
+    if (a.cluster) {
+      *reinterpret_cast<float4*>(s_part + col * D + d) = acc;
+      if (d == 0) reinterpret_cast<float2*>(s_part + kRows * D)[col] = make_float2(m, l);
+    } else if (a.shares > 1) {
+      if (col >= n_rows && !bad) continue;  // (the join looks at q_len: a malformed prompt's rows get statistics, of nothing)
+      const int64_t row = ((int64_t)b * a.N + hd) * a.Lq + tok;
       if (n > 0) store4(a.part_o + (row * a.shares + share) * D + d, acc);
       if (d == 0) a.part_ml[row * a.shares + share] = make_float2(m, l);
     } else {
-      const float inv = l != 0.f ? 1.f / l : 0.f;  // (a sum that is NaN stays one)
-      store4(reinterpret_cast<T*>(a.o.ptr) + (int64_t)b * a.o.sb + (int64_t)hd * a.o.sh + (int64_t)tok * a.o.ss + d,
-             make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv));
-      if (a.lse && d == 0) a.lse[row] = l != 0.f ? (m + log2f(l)) * kLn2 : -INFINITY;
+      write(tok, hd, d, m, l, acc);
     }
   }
+  if (!a.cluster) return;
+  ptx::cluster_sync();
+  for (int i = tid * a.shares + share; i < kRows * (D / 4); i += kThreads * a.shares) {
+    const int col = i / (D / 4), d = i % (D / 4) * 4;
+    const int r = row0 + col, tok = r / G;
+    if (tok >= a.Lq) break;
+    const uint32_t at_ml = ptx::smem_u32(reinterpret_cast<float2*>(s_part + kRows * D) + col), at_o = ptx::smem_u32(s_part + col * D + d);
+    float2 ml[kCluster];
+    float m = -INFINITY;
+#pragma unroll
+    for (int c = 0; c < kCluster; ++c) {
+      ml[c] = c < a.shares ? ptx::ld_cluster_f32x2(at_ml, c) : make_float2(-INFINITY, 0.f);
+      m = fmaxf(m, ml[c].x);
+    }
+    const float ref = m == -INFINITY ? 0.f : m;
+    float l = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int c = 0; c < kCluster; ++c) {
+      if (c >= a.shares) continue;
+      const float f = ptx::ex2(ml[c].x - ref);
+      const float4 x = ptx::ld_cluster_f32x4(at_o, c);
+      l = fmaf(ml[c].y, f, l);
+      acc.x = fmaf(x.x, f, acc.x); acc.y = fmaf(x.y, f, acc.y); acc.z = fmaf(x.z, f, acc.z); acc.w = fmaf(x.w, f, acc.w);
+    }
+    write(tok, kvh * G + r % G, d, m, l, acc);
+  }
+  ptx::cluster_sync();  // nobody leaves while its part is read
 }
 
 // One CTA per row; D / 4 threads read a share's part, 4 channels each.  A share without pages has written its statistics alone.
@@ -475,7 +525,7 @@ int shares_of(const brk_cache_attn_params& p) {
   const int64_t least = (p.P + kShare - 1) / kShare, most = std::max<int64_t>(least, std::min<int64_t>(64, (p.P + kWarps - 1) / kWarps));
   int64_t best = least, best_cost = INT64_MAX;
   for (int64_t s = least; s <= most; ++s) {
-    const int64_t cost = (ctas * s + room - 1) / room * ((p.P + s - 1) / s + 6) + (s > 1 ? 4 + s / 8 : 0);
+    const int64_t cost = (ctas * s + room - 1) / room * ((p.P + s - 1) / s + 6) + (s > kCluster ? 6 + s / 8 : s > 1 ? 2 : 0);
     if (cost < best_cost) {
       best_cost = cost;
       best = s;
@@ -488,7 +538,7 @@ int shares_of(const brk_cache_attn_params& p) {
 
 size_t cache_attn_workspace(const brk_cache_attn_params& p) {
   const size_t n = shares_of(p);
-  return n > 1 ? (size_t)p.B * p.N * p.Lq * n * (p.cache.D * sizeof(float) + sizeof(float2)) : 0;
+  return n > (size_t)kCluster ? (size_t)p.B * p.N * p.Lq * n * (p.cache.D * sizeof(float) + sizeof(float2)) : 0;
 }
 
 int cache_attn_launch(const brk_cache_attn_params& p, void* ws, cudaStream_t st) {
@@ -505,6 +555,7 @@ int cache_attn_launch(const brk_cache_attn_params& p, void* ws, cudaStream_t st)
   a.n_pages = p.cache.n_pages; a.B = p.B; a.N = p.N; a.Nk = p.cache.Nk; a.Lq = p.Lq; a.M = p.M; a.P = p.P;
   a.shares = shares_of(p);
   a.scale = p.scale;
+  a.cluster = a.shares > 1 && a.shares <= kCluster;
   const size_t rows = (size_t)p.B * p.N * p.Lq;
   a.part_o = static_cast<float*>(ws);
   a.part_ml = reinterpret_cast<float2*>(a.part_o + rows * a.shares * p.cache.D);
@@ -520,7 +571,7 @@ int cache_attn_launch(const brk_cache_attn_params& p, void* ws, cudaStream_t st)
       BRK_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributePreferredSharedMemoryCarveout, (int)cudaSharedmemCarveoutMaxShared));
       if (dev >= 0 && dev < 64) configured[dev].store(true, std::memory_order_release);
     }
-    return launch_dependent(kern, grid, dim3(kThreads), bytes, st, a);
+    return launch_dependent_clusters(a.cluster ? a.shares : 1, kern, grid, dim3(kThreads), bytes, st, a);
   };
   static std::atomic<bool> done[10][64] = {};
   const bool f32 = p.dtype == BRK_F32;
@@ -532,7 +583,7 @@ int cache_attn_launch(const brk_cache_attn_params& p, void* ws, cudaStream_t st)
     return per == 8 ? run(cache_attn_kernel<__nv_bfloat16, D, 1, false>, flags[3]) : run(cache_attn_kernel<__nv_bfloat16, D, 2, false>, flags[4]);
   };
   const int rc = p.cache.D == 128 ? of_head_dim(std::integral_constant<int, 128>(), done) : of_head_dim(std::integral_constant<int, 64>(), done + 5);
-  if (rc || a.shares == 1) return rc;
+  if (rc || a.shares <= kCluster) return rc;
   const dim3 joins((unsigned)rows), block(128);
   if (p.cache.D == 128)
     return f32 ? launch_dependent(cache_join_kernel<float, 128>, joins, block, 0, st, a)

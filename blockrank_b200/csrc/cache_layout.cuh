@@ -124,18 +124,30 @@ struct QueryRows {
   uint32_t shift[kTiles][2];                      // B of the product of the scales: -8 2^-133 sum(q) of the groups, in three bf16 numbers
   float unit[kTiles][2];
 
+  // this lane's channels of the queries as they are in memory, so that they can be on their way while something else is done
+  struct Raw {
+    uint4 w[kTiles][L::kGroups][sizeof(T) / 2];
+  };
   // row(c): column c's query, null for none
   template <typename F>
-  __device__ __forceinline__ void load(F row, int g, int t) {
+  static __device__ __forceinline__ void fetch(F row, int g, int t, Raw& raw) {
 #pragma unroll
     for (int n = 0; n < kTiles; ++n) {
       const T* const p = row(8 * n + g);
+#pragma unroll
+      for (int j = 0; j < L::kGroups; ++j)
+#pragma unroll
+        for (int i = 0; i < (int)sizeof(T) / 2; ++i)
+          raw.w[n][j][i] = p ? *(reinterpret_cast<const uint4*>(p + 32 * j + 8 * t) + i) : make_uint4(0, 0, 0, 0);
+    }
+  }
+  __device__ __forceinline__ void make(const Raw& raw, int g, int t) {
+#pragma unroll
+    for (int n = 0; n < kTiles; ++n) {
       float x[L::kGroups][8], top = 0.f;
 #pragma unroll
       for (int j = 0; j < L::kGroups; ++j) {
-#pragma unroll
-        for (int k = 0; k < 8; ++k) x[j][k] = 0.f;
-        if (p) load8(p + 32 * j + 8 * t, x[j]);
+        load8(reinterpret_cast<const T*>(raw.w[n][j]), x[j]);
 #pragma unroll
         for (int k = 0; k < 8; ++k) top = isnan(x[j][k]) ? INFINITY : fmaxf(top, fabsf(x[j][k]));
       }

@@ -1,10 +1,12 @@
 // Document scores from the 4-bit cache: the signal rows against the held keys of every document.
 //
-// A warp takes a document (or a part of its pages, where there are few documents) for one KV head and up to 8 kTiles (head, signal
-// row) pairs and keeps a running (maximum, sum) per pair; the pairs of a prompt's documents are merged by the kernel that
-// merges those of doc_scores.  Bound by the read of the keys (72 bytes per token and KV head at head_dim 128).
+// A CTA takes some of a prompt's documents, about as many pages as every other CTA, for one KV head and up to 8 kTiles (head, signal
+// row) pairs; its warps take equal parts of those pages, whatever documents they belong to, and keep a running (maximum, sum) per
+// pair and document.  The pairs of a prompt's documents are merged by the kernel that merges those of doc_scores.
+// Bound by the read of the keys (72 bytes per token and KV head at head_dim 128).
 #include <algorithm>
 #include <atomic>
+#include <type_traits>
 
 #include "cache_layout.cuh"
 #include "score_args.cuh"
@@ -18,6 +20,7 @@ using namespace cache;
 constexpr int kWarps = 4;
 constexpr int kThreads = 32 * kWarps;
 constexpr int kStages = 3;  // pages (their K parts) a warp has in shared memory
+constexpr int kDocs = 32;   // documents at a time: one per lane
 constexpr float kLog2e = 1.4426950408889634f;
 
 struct CacheScoreArgs {
@@ -29,70 +32,95 @@ struct CacheScoreArgs {
   float2* partial;  // [B, N, R, M - 2]
   int32_t* status;
   int n_pages, N, Nk, R, M, P, max_block_len;
-  int split;  // warps per document: 1 or kWarps
   float scale;
 };
 
+__device__ __forceinline__ float2 merged(float2 a, float2 b) {
+  const float top = fmaxf(a.x, b.x), ref = top == -INFINITY ? 0.f : top;
+  return make_float2(top, a.y * ptx::ex2(a.x - ref) + b.y * ptx::ex2(b.x - ref));
+}
+
 template <typename T, int D, int kTiles>
-__global__ void __launch_bounds__(kThreads, kTiles == 1 && sizeof(T) == 2 ? 4 : 2) cache_scores_kernel(CacheScoreArgs a) {
+__global__ void __launch_bounds__(kThreads, kTiles == 1 && sizeof(T) == 2 ? 3 : 2) cache_scores_kernel(CacheScoreArgs a) {
   using L = Layout<D>;
   constexpr int kCols = 8 * kTiles;
   extern __shared__ __align__(16) unsigned char smem[];  // [kWarps][kStages][K part of a page]
-  __shared__ float2 s_ml[kWarps][kCols];
+  __shared__ float2 s_ml[kWarps][kDocs][kCols];
+  __shared__ int s_scan[kWarps], s_before[2];
   ptx::grid_dependency_wait();
   ptx::grid_dependency_launch();
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
   const int b = blockIdx.y / a.Nk, kvh = blockIdx.y % a.Nk, row0 = blockIdx.z * kCols;
   const int G = a.N / a.Nk, GR = G * a.R, nd = a.M - 2;
-  const int doc = (blockIdx.x * kWarps + warp) / a.split, part = warp % a.split;
+  const int32_t *const bs = a.blk_start + (int64_t)b * a.M, *const bl = a.blk_len + (int64_t)b * a.M;
 
-  int start = 0, len = 0;
-  if (doc < nd) {
-    const int32_t *bs = a.blk_start + (int64_t)b * a.M, *bl = a.blk_len + (int64_t)b * a.M;
-    start = bs[doc + 1];
-    len = bl[doc + 1];
-    if (span_is_bad(bs, bl, doc + 1, (int64_t)a.P * kPage) || len > a.max_block_len) {
-      if (lane == 0 && a.status) atomicCAS(a.status, 0, kStatusBadCacheCall);
+  // document d's span (length 0 if it is malformed) and its pages
+  auto span = [&](int d, int& start, int& len) {
+    start = bs[d + 1];
+    len = bl[d + 1];
+    if (span_is_bad(bs, bl, d + 1, (int64_t)a.P * kPage) || len > a.max_block_len) {
+      if (a.status) atomicCAS(a.status, 0, kStatusBadCacheCall);
       len = 0;
     }
-  }
-  const int page0 = start / kPage, n = len > 0 ? (start + len - 1) / kPage - page0 + 1 : 0;  // the document's pages
-
-  unsigned char* const ring = smem + warp * kStages * L::kHalf;
-  const unsigned char* const head = a.pages + (int64_t)kvh * L::kBytes;
-  int ids = -1, ids0 = -32;  // page numbers of the pages ids0 .. ids0 + 31, one per lane
-  auto page_of = [&](int i) {
-    if (i >= ids0 + 32) {
-      ids0 = i;
-      ids = i + lane < n ? a.table[(int64_t)b * a.P + page0 + i + lane] : 0;
-      if (__any_sync(0xffffffffu, ids < 0 || ids >= a.n_pages)) {
-        if (lane == 0 && a.status) atomicCAS(a.status, 0, kStatusBadCacheCall);
-        if (ids >= a.n_pages) ids = -1;
-      }
-    }
-    return __shfl_sync(0xffffffffu, ids, i - ids0);
+    return len > 0 ? (start + len - 1) / kPage - start / kPage + 1 : 0;
   };
-  uint32_t absent = 0;  // bit s: the page in stage s does not exist
-  auto request = [&](int i, int stage) {
-    if (i < n) {
-      const int page = page_of(i);
-      absent = page < 0 ? absent | (1u << stage) : absent & ~(1u << stage);
-      if (page >= 0) {
-        const unsigned char* src = head + (int64_t)page * a.Nk * L::kBytes;
-        for (int x = lane * 16; x < L::kHalf; x += 512) cp_async16(ring + stage * L::kHalf + x, src + x);
-      }
-    }
-    cp_async_commit();
-  };
+  auto warp_scan = [&](int x) {
 #pragma unroll
-  for (int s = 0; s < kStages; ++s) request(part + s * a.split, s);
+    for (int off = 1; off < 32; off <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, x, off);
+      if (lane >= off) x += y;
+    }
+    return x;
+  };
 
-  QueryRows<T, D, kTiles> q;
-  q.load([&](int c) -> const T* {
+  // ---- this CTA's documents: those whose first page is in its share of all documents' pages ----
+  int my_start = 0, my_len = 0;
+  const int n0 = tid < nd ? span(tid, my_start, my_len) : 0;
+  typename QueryRows<T, D, kTiles>::Raw raw;
+  QueryRows<T, D, kTiles>::fetch([&](int c) -> const T* {
     const int r = row0 + c;
     if (r >= GR) return nullptr;
     return reinterpret_cast<const T*>(a.q.ptr) + (int64_t)b * a.q.sb + (int64_t)(kvh * G + r / a.R) * a.q.sh + (int64_t)(r % a.R) * a.q.ss;
-  }, g, t);
+  }, g, t, raw);
+  int64_t total = 0, lo = 0, hi = 0;
+  if (tid < 2) s_before[tid] = 0;
+#pragma unroll 1
+  for (int pass = 0; pass < 2; ++pass) {  // all pages; then the number of documents that begin before the share, and before its end
+    int64_t before = 0;
+#pragma unroll 1
+    for (int d0 = 0; d0 < nd; d0 += kThreads) {
+      int s, l;
+      const int n = d0 == 0 ? n0 : d0 + tid < nd ? span(d0 + tid, s, l) : 0;
+      const int x = warp_scan(n);
+      if (lane == 31) s_scan[warp] = x;
+      __syncthreads();
+      int sum = 0, first = x - n;
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) {
+        if (w < warp) first += s_scan[w];
+        sum += s_scan[w];
+      }
+      if (pass == 1) {
+        const unsigned below = __ballot_sync(0xffffffffu, d0 + tid < nd && before + first < lo);
+        const unsigned below_end = __ballot_sync(0xffffffffu, d0 + tid < nd && (before + first < hi || blockIdx.x + 1 == gridDim.x));
+        if (lane == 0) {
+          atomicAdd(&s_before[0], __popc(below));
+          atomicAdd(&s_before[1], __popc(below_end));
+        }
+      }
+      before += sum;
+      __syncthreads();
+    }
+    if (pass == 0) {
+      total = before;
+      lo = total * blockIdx.x / gridDim.x;
+      hi = total * (blockIdx.x + 1) / gridDim.x;
+    }
+  }
+  const int doc_end = s_before[1];
+
+  QueryRows<T, D, kTiles> q;
+  q.make(raw, g, t);
   float sl2[kTiles][2], mx[kTiles][2], sum[kTiles][2];  // this lane's keys
 #pragma unroll
   for (int c = 0; c < kTiles; ++c)
@@ -102,73 +130,129 @@ __global__ void __launch_bounds__(kThreads, kTiles == 1 && sizeof(T) == 2 ? 4 : 
       mx[c][x] = -INFINITY;
       sum[c][x] = 0.f;
     }
-  int stage = 0;
-  for (int i = part; i < n; i += a.split) {
-    cp_async_wait<kStages - 1>();
+  unsigned char* const ring = smem + warp * kStages * L::kHalf;
+  const unsigned char* const head = a.pages + (int64_t)kvh * L::kBytes;
+  const int32_t* const table = a.table + (int64_t)b * a.P;
+
+#pragma unroll 1
+  for (int doc0 = s_before[0]; doc0 < doc_end; doc0 += kDocs) {
+    const int n_docs = min(kDocs, doc_end - doc0);
+    int start = 0, len = 0;  // lane l: of document doc0 + l
+    const int n = lane < n_docs ? span(doc0 + lane, start, len) : 0;
+    const int end = warp_scan(n), pages = __shfl_sync(0xffffffffu, end, 31);
+    const int from = (int)((int64_t)pages * warp / kWarps), to = (int)((int64_t)pages * (warp + 1) / kWarps);
+    for (int i = lane; i < kDocs * kCols; i += 32) (&s_ml[warp][0][0])[i] = make_float2(-INFINITY, 0.f);
     __syncwarp();
-    if (!((absent >> stage) & 1)) {
-      float s[kTiles][4][4];
-      q.logits(ring + stage * L::kHalf, g, t, s);
-      const int from = start - (page0 + i) * kPage, to = start + len - (page0 + i) * kPage;  // the document's tokens in this page
-      if (from > 0 || to < kPage) {
-#pragma unroll
-        for (int k = 0; k < 4; ++k)
-#pragma unroll
-          for (int y = 0; y < 2; ++y) {
-            const int key = 16 * k + 8 * y + g;
-            if (key < from || key >= to) {
-#pragma unroll
-              for (int c = 0; c < kTiles; ++c) s[c][k][2 * y] = s[c][k][2 * y + 1] = -INFINITY;
-            }
-          }
+
+    // A walk over the pages from .. to - 1; page numbers are read one page before they are needed, pages kStages - 1 before.
+    struct Walk {
+      int at, doc, next, slot0, start, len;  // page at is of document doc0 + doc, as are all before next; its first slot
+    };
+    auto enter = [&](Walk& w) {  // the document of page w.at
+      w.doc = __popc(__ballot_sync(0xffffffffu, end <= w.at));
+      w.next = __shfl_sync(0xffffffffu, end, w.doc);
+      w.start = __shfl_sync(0xffffffffu, start, w.doc);
+      w.len = __shfl_sync(0xffffffffu, len, w.doc);
+      w.slot0 = (w.start / kPage + w.at - (w.next - __shfl_sync(0xffffffffu, n, w.doc))) * kPage;
+    };
+    auto step = [&](Walk& w) {
+      ++w.at;
+      w.slot0 += kPage;
+      if (w.at < to && w.at >= w.next) enter(w);
+    };
+    Walk ahead = {from, 0, 0, 0, 0, 0}, here = ahead;
+    if (from < to) {
+      enter(ahead);
+      here = ahead;
+    }
+    int id = from < to ? table[ahead.slot0 / kPage] : 0;
+    uint32_t absent = 0;  // bit s: the page in stage s does not exist
+    auto request = [&](int stage) {
+      if (ahead.at < to) {
+        const int page = id;
+        step(ahead);
+        if (ahead.at < to) id = table[ahead.slot0 / kPage];
+        if (page >= 0 && page < a.n_pages) {
+          absent &= ~(1u << stage);
+          const unsigned char* src = head + (int64_t)page * a.Nk * L::kBytes;
+          for (int x = lane * 16; x < L::kHalf; x += 512) cp_async16(ring + stage * L::kHalf + x, src + x);
+        } else {
+          absent |= 1u << stage;
+          if (lane == 0 && a.status) atomicCAS(a.status, 0, kStatusBadCacheCall);
+        }
       }
+      cp_async_commit();
+    };
 #pragma unroll
-      for (int c = 0; c < kTiles; ++c)
-#pragma unroll
-        for (int x = 0; x < 2; ++x) {
-          float top = mx[c][x];
-#pragma unroll
-          for (int k = 0; k < 4; ++k) top = fmaxf(top, fmaxf(s[c][k][x], s[c][k][2 + x]));
-          const float ref = top == -INFINITY ? 0.f : top * sl2[c][x];
-          sum[c][x] *= ptx::ex2(mx[c][x] * sl2[c][x] - ref);
-          mx[c][x] = top;
+    for (int s = 0; s < kStages - 1; ++s) request(s);
+
+    int stage = 0;
+#pragma unroll 1
+    while (here.at < to) {
+      cp_async_wait<kStages - 2>();
+      __syncwarp();
+      request(stage == 0 ? kStages - 1 : stage - 1);  // into the place of the page before
+      if (!((absent >> stage) & 1)) {
+        float s[kTiles][4][4];
+        q.logits(ring + stage * L::kHalf, g, t, s);
+        const int first = here.start - here.slot0, last = first + here.len;  // the document's tokens in this page
+        if (first > 0 || last < kPage) {
 #pragma unroll
           for (int k = 0; k < 4; ++k)
 #pragma unroll
-            for (int y = 0; y < 2; ++y) sum[c][x] += ptx::ex2(fmaf(s[c][k][2 * y + x], sl2[c][x], -ref));
+            for (int y = 0; y < 2; ++y) {
+              const int key = 16 * k + 8 * y + g;
+              if (key < first || key >= last) {
+#pragma unroll
+                for (int c = 0; c < kTiles; ++c) s[c][k][2 * y] = s[c][k][2 * y + 1] = -INFINITY;
+              }
+            }
         }
-    }
-    __syncwarp();
-    request(i + kStages * a.split, stage);
-    stage = stage + 1 == kStages ? 0 : stage + 1;
-  }
-  cp_async_wait<0>();
 #pragma unroll
-  for (int c = 0; c < kTiles; ++c)
+        for (int c = 0; c < kTiles; ++c)
 #pragma unroll
-    for (int x = 0; x < 2; ++x) {
-      float m = mx[c][x] * sl2[c][x], l = sum[c][x];
+          for (int x = 0; x < 2; ++x) {
+            float top = mx[c][x];
 #pragma unroll
-      for (int off = 4; off <= 16; off <<= 1) {
-        const float m2 = __shfl_xor_sync(0xffffffffu, m, off), l2 = __shfl_xor_sync(0xffffffffu, l, off);
-        const float top = fmaxf(m, m2), ref = top == -INFINITY ? 0.f : top;
-        l = l * ptx::ex2(m - ref) + l2 * ptx::ex2(m2 - ref);
-        m = top;
+            for (int k = 0; k < 4; ++k) top = fmaxf(top, fmaxf(s[c][k][x], s[c][k][2 + x]));
+            const float ref = top == -INFINITY ? 0.f : top * sl2[c][x];
+            sum[c][x] *= ptx::ex2(mx[c][x] * sl2[c][x] - ref);
+            mx[c][x] = top;
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+#pragma unroll
+              for (int y = 0; y < 2; ++y) sum[c][x] += ptx::ex2(fmaf(s[c][k][2 * y + x], sl2[c][x], -ref));
+          }
       }
-      if (g == 0) s_ml[warp][8 * c + 2 * t + x] = make_float2(m, l);
+      stage = stage + 1 == kStages ? 0 : stage + 1;
+      const int doc = here.doc;
+      step(here);
+      if (here.at >= to || here.doc != doc) {  // the last of this warp's pages of the document
+#pragma unroll
+        for (int c = 0; c < kTiles; ++c)
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            float2 ml = make_float2(mx[c][x] * sl2[c][x], sum[c][x]);
+#pragma unroll
+            for (int off = 4; off <= 16; off <<= 1)
+              ml = merged(ml, make_float2(__shfl_xor_sync(0xffffffffu, ml.x, off), __shfl_xor_sync(0xffffffffu, ml.y, off)));
+            if (g == 0) s_ml[warp][doc][8 * c + 2 * t + x] = ml;
+            mx[c][x] = -INFINITY;
+            sum[c][x] = 0.f;
+          }
+      }
     }
-  if (a.split > 1) __syncthreads();
-  else __syncwarp();
-  if (doc >= nd || part != 0) return;
-  for (int col = lane; col < kCols && row0 + col < GR; col += 32) {
-    float2 ml = s_ml[warp][col];
-    for (int w = 1; w < a.split; ++w) {
-      const float2 x = s_ml[warp + w][col];
-      const float top = fmaxf(ml.x, x.x), ref = top == -INFINITY ? 0.f : top;
-      ml = make_float2(top, ml.y * ptx::ex2(ml.x - ref) + x.y * ptx::ex2(x.x - ref));
+    cp_async_wait<0>();
+    __syncthreads();
+    for (int i = tid; i < kDocs * kCols; i += kThreads) {
+      const int doc = i % kDocs, r = row0 + i / kDocs;
+      if (doc >= n_docs || r >= GR) continue;
+      float2 ml = s_ml[0][doc][i / kDocs];
+#pragma unroll
+      for (int w = 1; w < kWarps; ++w) ml = merged(ml, s_ml[w][doc][i / kDocs]);
+      a.partial[(((int64_t)b * a.N + kvh * G + r / a.R) * a.R + r % a.R) * nd + doc0 + doc] = ml;
     }
-    const int r = row0 + col;
-    a.partial[(((int64_t)b * a.N + kvh * G + r / a.R) * a.R + r % a.R) * nd + doc] = ml;
+    __syncthreads();
   }
 }
 
@@ -190,8 +274,19 @@ int cache_scores_launch(const brk_cache_score_params& p, void* ws, cudaStream_t 
   a.scale = p.scale;
   const int nd = p.M - 2, rows = p.N / a.Nk * p.R, tiles = rows > 8 ? 2 : 1;
   const int z = (rows + 8 * tiles - 1) / (8 * tiles);
-  a.split = (int64_t)nd * p.B * a.Nk * z < 8 * (int64_t)std::max(1, sm_count()) || p.max_block_len > 16 * kPage ? kWarps : 1;
-  const dim3 grid((nd * a.split + kWarps - 1) / kWarps, p.B * a.Nk, z);
+  // Shares of a prompt's documents, at least a page for each warp: a round of CTAs takes as long as its share, with about eight pages' time
+  // for beginning and end.
+  const int64_t ctas = (int64_t)p.B * a.Nk * z, room = (tiles == 1 && p.dtype == BRK_BF16 ? 3 : 2) * (int64_t)std::max(1, sm_count());
+  const int64_t most = std::min<int64_t>(nd, (p.P + kWarps - 1) / kWarps);
+  int64_t shares = 1, best = INT64_MAX;
+  for (int64_t s = 1; s <= std::min<int64_t>(most, 256); ++s) {
+    const int64_t cost = (ctas * s + room - 1) / room * ((p.P + s - 1) / s + 8);
+    if (cost < best) {
+      best = cost;
+      shares = s;
+    }
+  }
+  const dim3 grid((unsigned)shares, p.B * a.Nk, z);
   auto run = [&](auto kern, std::atomic<bool>* configured) -> int {
     const int bytes = kWarps * kStages * (int)head_page_bytes(p.cache.D) / 2;
     int dev = 0;
@@ -204,15 +299,12 @@ int cache_scores_launch(const brk_cache_score_params& p, void* ws, cudaStream_t 
     return launch_dependent(kern, grid, dim3(kThreads), bytes, st, a);
   };
   static std::atomic<bool> done[8][64] = {};
-  int rc;
-  const bool f32 = p.dtype == BRK_F32;
-  if (p.cache.D == 128) {
-    if (f32) rc = tiles == 1 ? run(cache_scores_kernel<float, 128, 1>, done[0]) : run(cache_scores_kernel<float, 128, 2>, done[1]);
-    else rc = tiles == 1 ? run(cache_scores_kernel<__nv_bfloat16, 128, 1>, done[2]) : run(cache_scores_kernel<__nv_bfloat16, 128, 2>, done[3]);
-  } else {
-    if (f32) rc = tiles == 1 ? run(cache_scores_kernel<float, 64, 1>, done[4]) : run(cache_scores_kernel<float, 64, 2>, done[5]);
-    else rc = tiles == 1 ? run(cache_scores_kernel<__nv_bfloat16, 64, 1>, done[6]) : run(cache_scores_kernel<__nv_bfloat16, 64, 2>, done[7]);
-  }
+  auto of_head_dim = [&](auto d, std::atomic<bool>(*flags)[64]) -> int {
+    constexpr int D = decltype(d)::value;
+    if (p.dtype == BRK_F32) return tiles == 1 ? run(cache_scores_kernel<float, D, 1>, flags[0]) : run(cache_scores_kernel<float, D, 2>, flags[1]);
+    return tiles == 1 ? run(cache_scores_kernel<__nv_bfloat16, D, 1>, flags[2]) : run(cache_scores_kernel<__nv_bfloat16, D, 2>, flags[3]);
+  };
+  const int rc = p.cache.D == 128 ? of_head_dim(std::integral_constant<int, 128>(), done) : of_head_dim(std::integral_constant<int, 64>(), done + 4);
   if (rc) return rc;
   ScoreArgs m = {};
   m.partial = a.partial;
