@@ -16,8 +16,7 @@
 #include <atomic>
 #include <type_traits>
 
-#include "cache_layout.cuh"
-#include "tc_ptx.cuh"
+#include "cache_share.cuh"
 
 namespace brk {
 namespace {
@@ -27,26 +26,7 @@ using namespace cache;
 constexpr int kWarps = 4;
 constexpr int kThreads = 32 * kWarps;
 constexpr int kParts = 3;         // K or V parts of pages that a warp has room for in shared memory: two K, one V
-constexpr int kShare = 128;       // pages a CTA takes at most
 constexpr int kCluster = 8;       // shares that a cluster joins, at most
-constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
-
-struct CacheAttnArgs {
-  const unsigned char* pages;
-  View q, o;  // (B, N, Lq, D)
-  const int32_t* table;  // [B, P]
-  const int32_t* blk_start;
-  const int32_t* blk_len;
-  const int32_t* q_len;  // [B] or null: Lq each
-  float* lse;            // [B, N, Lq] or null
-  int32_t* status;
-  float* part_o;         // [B, N, Lq, shares, D]
-  float2* part_ml;       // [B, N, Lq, shares] (maximum in log2 units, sum)
-  int n_pages, B, N, Nk, Lq, M, P, shares;
-  bool cluster;          // a prompt's shares are a cluster, which joins its parts itself
-  float scale;
-  Codes codes;
-};
 
 template <typename T, int kTiles>
 constexpr int ctas_per_sm = kTiles == 1 && sizeof(T) == 2 ? 3 : 2;
@@ -70,68 +50,15 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<T, kTiles>) cache_attn_k
   ptx::grid_dependency_launch();
   ptx::grid_dependency_wait();  // (inputs of this call; the workspace of the one in front)
 
-  // ---- everything that has to be read first, at once: spans, the number of rows, the rows ----
-  const int32_t *start = a.blk_start + (int64_t)b * a.M, *len = a.blk_len + (int64_t)b * a.M;
-  const int64_t slots = (int64_t)a.P * kPage;
-  const int last_start = start[a.M - 1], last_len = len[a.M - 1], given = a.q_len ? a.q_len[b] : a.Lq;
-  int my_start = 0, my_len = 0;
-  bool bad = false;
   typename QueryRows<T, D, kTiles>::Raw raw;
-  QueryRows<T, D, kTiles>::fetch([&](int c) -> const T* {  // (rows from q_len on among them: they are not used)
-    const int r = row0 + (kTwice ? c & 3 : c);
-    if (r >= a.Lq * G) return nullptr;
-    return reinterpret_cast<const T*>(a.q.ptr) + (int64_t)b * a.q.sb + (int64_t)(kvh * G + r % G) * a.q.sh + (int64_t)(r / G) * a.q.ss;
-  }, g, t, raw);
-  if (tid < a.M) {
-    my_start = start[tid];
-    my_len = len[tid];
-    bad = span_is_bad(start, len, tid, slots);
-  }
-  for (int m = tid + kThreads; m < a.M; m += kThreads) bad |= span_is_bad(start, len, m, slots);
-  s_mask[tid] = s_mask[tid + kThreads] = 0;
-  bad |= given < 0 || given > a.Lq || given > last_len;
-  bad = __syncthreads_or(bad);
-  if (bad && tid == 0 && a.status) atomicCAS(a.status, 0, kStatusBadCacheCall);
-
-  // ---- this CTA's rows, and its pages: an even share of those up to the last row's slot ----
-  const int rows = bad ? 0 : given, n_rows = min(rows * G - row0, kRows);
-  const int first_slot = bad ? 0 : last_start + last_len - rows;  // of the prompt's row 0
-  const int last_tok = n_rows > 0 ? (row0 + n_rows - 1) / G : -1;
-  const int live = n_rows > 0 ? (first_slot + last_tok) / kPage + 1 : 0;
-  const int per = max((live + a.shares - 1) / a.shares, min(live, kWarps));
-  const int page0 = min(live, share * per), n = min(live, page0 + per) - page0;
-  int page_id = -1;
-  if (tid < n) page_id = a.table[(int64_t)b * a.P + page0 + tid];
-
-  // ---- which tokens of these pages lie in a block ----
-  static_assert(kShare == kThreads, "a thread per page");
-  if (n > 0) {
-    const int lo = page0 * kPage, hi = (page0 + n) * kPage;
-    for (int m0 = warp * 32; m0 < a.M; m0 += kThreads) {
-      const int m = m0 + lane;
-      const int s = m0 < kThreads ? my_start : m < a.M ? start[m] : 0, e = s + (m0 < kThreads ? my_len : m < a.M ? len[m] : 0);
-      unsigned todo = __ballot_sync(0xffffffffu, max(s, lo) < min(e, hi));
-      while (todo) {
-        const int src = __ffs(todo) - 1;
-        todo &= todo - 1;
-        const int bs = max(__shfl_sync(0xffffffffu, s, src), lo) - lo, be = min(__shfl_sync(0xffffffffu, e, src), hi) - lo;
-        for (int w = bs / 32 + lane; w * 32 < be; w += 32) {  // a word of 32 tokens per lane
-          const int from = max(bs - w * 32, 0), to = min(be - w * 32, 32);
-          atomicOr(&s_mask[w], (to == 32 ? ~0u : (1u << to) - 1) & (~0u << from));
-        }
-      }
-    }
-  }
-  __syncthreads();
-  if (tid < n) {
-    const bool needed = (s_mask[2 * tid] | s_mask[2 * tid + 1]) != 0;
-    if (needed && (page_id < 0 || page_id >= a.n_pages)) {
-      if (a.status) atomicCAS(a.status, 0, kStatusBadCacheCall);
-      page_id = -1;
-    }
-    s_page[tid] = needed ? page_id : -1;
-  }
-  __syncthreads();
+  const Share sh = find_share<kThreads>(a, b, row0, kRows, share, kWarps, s_mask, s_page, [&] {
+    QueryRows<T, D, kTiles>::fetch([&](int c) -> const T* {  // (rows from q_len on among them: they are not used)
+      const int r = row0 + (kTwice ? c & 3 : c);
+      if (r >= a.Lq * G) return nullptr;
+      return reinterpret_cast<const T*>(a.q.ptr) + (int64_t)b * a.q.sb + (int64_t)(kvh * G + r % G) * a.q.sh + (int64_t)(r / G) * a.q.ss;
+    }, g, t, raw);
+  });
+  const int n = sh.n, n_rows = sh.n_rows, page0 = sh.page0, first_slot = sh.first_slot;
 
   // Copies are requested in the order K0 K1 V0 K2 V1 K3 ..., each into the place of the part that has just been used.
   unsigned char* const ring = smem + warp * kParts * L::kHalf;
@@ -186,6 +113,9 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<T, kTiles>) cache_attn_k
     ahead = next(ahead + kWarps);
     cp_async_wait<2>();
     __syncwarp();
+    const int slot0 = (page0 + i) * kPage;
+    const uint32_t m_lo = s_mask[2 * i], m_hi = s_mask[2 * i + 1];
+    const bool ragged = (m_lo & m_hi) != ~0u, late = slot0 + kPage - 1 > first_lim;  // tokens that no row sees, that some do not see
     float s[kTiles][4][4];
     q.logits(ring + place * L::kHalf, g, t, s);
     __syncwarp();
@@ -193,21 +123,30 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<T, kTiles>) cache_attn_k
     place ^= 1;
 
     // ---- softmax ----
-    const int slot0 = (page0 + i) * kPage;
-    const uint32_t m_lo = s_mask[2 * i], m_hi = s_mask[2 * i + 1];
-    const bool whole = (m_lo & m_hi) == ~0u && slot0 + kPage - 1 <= first_lim;
-    if (!whole) {
+    // (A page's last tokens are worked on whether they count or not: left out 16 at a time, with a branch each, two contexts of
+    // 131,072 tokens took 77 us, not 69; with code of their own for pages that end early 16 prompts of 100 documents 100, not 87.)
+    if (ragged) {
+      const uint32_t lo = m_lo >> g, hi = m_hi >> g;  // this lane's keys: every eighth bit
 #pragma unroll
       for (int k = 0; k < 4; ++k)
 #pragma unroll
-        for (int y = 0; y < 2; ++y) {
-          const int key = 16 * k + 8 * y + g;
-          const bool in = ((key < 32 ? m_lo : m_hi) >> (key & 31)) & 1;
+        for (int y = 0; y < 2; ++y)
+          if (!((k < 2 ? lo : hi) & (1u << (16 * (k & 1) + 8 * y)))) {
 #pragma unroll
-          for (int c = 0; c < kTiles; ++c)
+            for (int c = 0; c < kTiles; ++c) s[c][k][2 * y] = s[c][k][2 * y + 1] = -INFINITY;
+          }
+    }
+    if (late) {
 #pragma unroll
-            for (int x = 0; x < 2; ++x)
-              if (!in || slot0 + key > lim[c][x]) s[c][k][2 * y + x] = -INFINITY;
+      for (int c = 0; c < kTiles; ++c)
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          const int last = lim[c][x] - slot0 - g;
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+#pragma unroll
+            for (int y = 0; y < 2; ++y)
+              if (16 * k + 8 * y > last) s[c][k][2 * y + x] = -INFINITY;
         }
     }
     float scale_o[kTiles][2];
@@ -252,7 +191,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<T, kTiles>) cache_attn_k
     const unsigned char* const page = ring + 2 * L::kHalf - L::kHalf;  // (offsets count from a page's beginning)
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-      uint32_t pt[kTiles][2][kMmas];
+        uint32_t pt[kTiles][2][kMmas];
 #pragma unroll
       for (int c = 0; c < kTiles; ++c)
 #pragma unroll
@@ -280,9 +219,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<T, kTiles>) cache_attn_k
           *reinterpret_cast<uint2*>(sv[y]) = *reinterpret_cast<const uint2*>(ps);
         }
       }
-      if (!whole) {
-        // Values of tokens that no row sees are zeros: 0 x NaN would reach every row.  One that some rows see and others do
-        // not is dealt with below.
+      if (ragged) {  // values of tokens that no row sees are zeros: 0 x NaN would reach every row
 #pragma unroll
         for (int y = 0; y < 2; ++y) {
           const int tok = 16 * k + 8 * y + 2 * t;
@@ -291,6 +228,8 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<T, kTiles>) cache_attn_k
 #pragma unroll
           for (int j = 0; j < L::kGroups; ++j) sv[y][j] &= keep;
         }
+      }
+      if (late) {
         uint32_t nan = 0;  // (a scale of all ones in the exponent is NaN)
 #pragma unroll
         for (int y = 0; y < 2; ++y)
@@ -418,7 +357,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<T, kTiles>) cache_attn_k
       *reinterpret_cast<float4*>(s_part + col * D + d) = acc;
       if (d == 0) reinterpret_cast<float2*>(s_part + kRows * D)[col] = make_float2(m, l);
     } else if (a.shares > 1) {
-      if (col >= n_rows && !bad) continue;  // (the join looks at q_len: a malformed prompt's rows get statistics, of nothing)
+      if (col >= n_rows && !sh.bad) continue;  // (the join looks at q_len: a malformed prompt's rows get statistics, of nothing)
       const int64_t row = ((int64_t)b * a.N + hd) * a.Lq + tok;
       if (n > 0) store4(a.part_o + (row * a.shares + share) * D + d, acc);
       if (d == 0) a.part_ml[row * a.shares + share] = make_float2(m, l);

@@ -194,8 +194,8 @@ __global__ void __launch_bounds__(kThreads, kTiles == 1 && sizeof(T) == 2 ? 3 : 
       request(stage == 0 ? kStages - 1 : stage - 1);  // into the place of the page before
       if (!((absent >> stage) & 1)) {
         float s[kTiles][4][4];
-        q.logits(ring + stage * L::kHalf, g, t, s);
         const int first = here.start - here.slot0, last = first + here.len;  // the document's tokens in this page
+        q.logits(ring + stage * L::kHalf, g, t, s);
         if (first > 0 || last < kPage) {
 #pragma unroll
           for (int k = 0; k < 4; ++k)
