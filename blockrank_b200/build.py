@@ -22,7 +22,7 @@ HOST_SOURCE = os.path.join(CSRC, "torch_host.cpp")
 HEADER = os.path.join(os.path.dirname(PKG), "include", "blockrank_b200.h")
 SOURCES = ["brk_api.cu", "attn_simt.cu", "attn_f32.cu", "attn_tc.cu", "attn_bwd.cu", "attn_bwd_mma.cu", "attn_bwd_tc.cu", "attn_bwd_f32.cu",
            "scores.cu",
-           "raw_scores.cu", "elementwise.cu", "cache_io.cu", "cache_attn.cu", "cache_scores.cu"]
+           "raw_scores.cu", "elementwise.cu", "cache_io.cu", "cache_attn.cu", "cache_attn_tc.cu", "cache_scores.cu"]
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
               "-Xcompiler", "-fPIC", "-Xcompiler", "-fvisibility=hidden", "--expt-relaxed-constexpr"]
 

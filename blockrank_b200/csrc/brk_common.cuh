@@ -141,11 +141,13 @@ constexpr size_t kWsHeader = 256;
 // Values of the caller's status word: 10..49 (forward) and 60..80 (backward) name the bounded wait that gave up first in its thread
 // (10..19 TMA warp, 20..29 MMA warps, 34, 35, 38, 39 output warps, other 30..39 softmax warps, 40, 41 one of the last three at
 // the job ring; even numbers chain 0, odd ones chain 1), 50 malformed block spans, 51 a signal row outside the prompt, 52 a slot
-// outside the cache, 53 malformed spans, pages or rows of a call on the cache, 90 the self-test's wait, 91 a self-test that found something else.
+// outside the cache, 53 malformed spans, pages or rows of a call on the cache, 85 a wait of its
+// attention, 90 the self-test's wait, 91 a self-test that found something else.
 constexpr int kStatusBadSpans = 50;
 constexpr int kStatusBadRows = 51;
 constexpr int kStatusBadSlot = 52;
 constexpr int kStatusBadCacheCall = 53;
+constexpr int kStatusCacheWait = 85;
 constexpr int kStatusSelfTest = 90;
 
 // kernel launchers implemented in the .cu files

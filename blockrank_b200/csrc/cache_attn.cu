@@ -448,23 +448,31 @@ __global__ void __launch_bounds__(128) cache_join_kernel(CacheAttnArgs a) {
   if (a.lse && tid == 0) a.lse[row] = l != 0.f ? (ref + log2f(l)) * kLn2 : -INFINITY;
 }
 
-// Rows of a CTA: 4 (bf16), 8 or 16.
+// More rows than this go to the tcgen05 kernel (bf16).
+constexpr int kManyRows = 32;
+
+// Rows of a CTA: 4 (bf16), 8 or 16; 256 in the tcgen05 kernel.
 int rows_per_cta(const brk_cache_attn_params& p) {
   const int64_t rows = (int64_t)p.Lq * (p.N / p.cache.Nk);
+  if (p.dtype == BRK_BF16 && rows > kManyRows) return 256;
   return rows <= 4 && p.dtype == BRK_BF16 ? 4 : rows <= 8 ? 8 : 16;
 }
 int64_t row_groups(const brk_cache_attn_params& p) {
   return ((int64_t)p.Lq * (p.N / p.cache.Nk) + rows_per_cta(p) - 1) / rows_per_cta(p);
 }
 
-// Shares of a prompt's pages, at most kShare pages each.  A round of CTAs (three per SM) takes as long as its share, with about
-// six pages' time for beginning and end; what is left over of the SMs in the last round is lost.
+// Shares of a prompt's pages, at most kShare pages each.  A round of CTAs takes as long as its share, with about six pages' time for
+// beginning and end (in the tcgen05 kernel four); what is left over of the SMs in the last round is lost.
 int shares_of(const brk_cache_attn_params& p) {
-  const int64_t ctas = (int64_t)p.B * p.cache.Nk * row_groups(p), room = (p.dtype == BRK_BF16 && rows_per_cta(p) <= 8 ? 3 : 2) * (int64_t)std::max(1, sm_count());
-  const int64_t least = (p.P + kShare - 1) / kShare, most = std::max<int64_t>(least, std::min<int64_t>(64, (p.P + kWarps - 1) / kWarps));
+  const bool many = rows_per_cta(p) == 256;
+  const int per_sm = many ? 1 : p.dtype == BRK_BF16 && rows_per_cta(p) <= 8 ? 3 : 2;
+  const int64_t ctas = (int64_t)p.B * p.cache.Nk * row_groups(p), room = per_sm * (int64_t)std::max(1, sm_count());
+  const int64_t least = (p.P + kShare - 1) / kShare, pages = many ? 4 : kWarps;
+  const int64_t most = std::max<int64_t>(least, std::min<int64_t>(64, (p.P + pages - 1) / pages));
   int64_t best = least, best_cost = INT64_MAX;
   for (int64_t s = least; s <= most; ++s) {
-    const int64_t cost = (ctas * s + room - 1) / room * ((p.P + s - 1) / s + 6) + (s > kCluster ? 6 + s / 8 : s > 1 ? 2 : 0);
+    const int64_t join = s == 1 ? 0 : s > kCluster || many ? 6 + s / 8 : 2;
+    const int64_t cost = (ctas * s + room - 1) / room * ((p.P + s - 1) / s + (many ? 4 : 6)) + join;
     if (cost < best_cost) {
       best_cost = cost;
       best = s;
@@ -472,12 +480,14 @@ int shares_of(const brk_cache_attn_params& p) {
   }
   return (int)best;
 }
+// Its cluster joins the parts of a prompt's shares; otherwise a kernel does.
+bool cluster_joins(const brk_cache_attn_params& p, int shares) { return shares <= kCluster && rows_per_cta(p) != 256; }
 
 }  // namespace
 
 size_t cache_attn_workspace(const brk_cache_attn_params& p) {
   const size_t n = shares_of(p);
-  return n > (size_t)kCluster ? (size_t)p.B * p.N * p.Lq * n * (p.cache.D * sizeof(float) + sizeof(float2)) : 0;
+  return n > 1 && !cluster_joins(p, (int)n) ? (size_t)p.B * p.N * p.Lq * n * (p.cache.D * sizeof(float) + sizeof(float2)) : 0;
 }
 
 int cache_attn_launch(const brk_cache_attn_params& p, void* ws, cudaStream_t st) {
@@ -494,7 +504,7 @@ int cache_attn_launch(const brk_cache_attn_params& p, void* ws, cudaStream_t st)
   a.n_pages = p.cache.n_pages; a.B = p.B; a.N = p.N; a.Nk = p.cache.Nk; a.Lq = p.Lq; a.M = p.M; a.P = p.P;
   a.shares = shares_of(p);
   a.scale = p.scale;
-  a.cluster = a.shares > 1 && a.shares <= kCluster;
+  a.cluster = a.shares > 1 && cluster_joins(p, a.shares);
   const size_t rows = (size_t)p.B * p.N * p.Lq;
   a.part_o = static_cast<float*>(ws);
   a.part_ml = reinterpret_cast<float2*>(a.part_o + rows * a.shares * p.cache.D);
@@ -521,8 +531,10 @@ int cache_attn_launch(const brk_cache_attn_params& p, void* ws, cudaStream_t st)
     if (per == 4) return run(cache_attn_kernel<__nv_bfloat16, D, 1, true>, flags[2]);
     return per == 8 ? run(cache_attn_kernel<__nv_bfloat16, D, 1, false>, flags[3]) : run(cache_attn_kernel<__nv_bfloat16, D, 2, false>, flags[4]);
   };
-  const int rc = p.cache.D == 128 ? of_head_dim(std::integral_constant<int, 128>(), done) : of_head_dim(std::integral_constant<int, 64>(), done + 5);
-  if (rc || a.shares <= kCluster) return rc;
+  const int rc = per == 256 ? cache_attn_tc_launch(a, p.cache.D, st)
+                 : p.cache.D == 128 ? of_head_dim(std::integral_constant<int, 128>(), done)
+                                    : of_head_dim(std::integral_constant<int, 64>(), done + 5);
+  if (rc || a.shares == 1 || a.cluster) return rc;
   const dim3 joins((unsigned)rows), block(128);
   if (p.cache.D == 128)
     return f32 ? launch_dependent(cache_join_kernel<float, 128>, joins, block, 0, st, a)

@@ -1,0 +1,375 @@
+// Attention of many rows (a whole query block) over the 4-bit cache, on the tcgen05 tensor cores; bf16.
+//
+// A CTA takes a share of one prompt's pages for one KV head and up to 256 rows (query heads of the group at one token after the other), two
+// tiles of 128.  Per page: four warps bring the codes out of the cache and write n s, exact in bf16, as the K and V operands
+// (128-byte swizzle); one thread issues S = Q K^T and O += P V per tile; a thread per row makes P from S in tensor memory, in two
+// bf16 parts (16 bits) that take the place of the 64 logits.  S is held twice, K and V three times, so that a page's Q K^T runs while
+// the softmax is at the page before and the next one is being unpacked.
+// 128 x 64 x D products three times per tile and page (S once, P in two parts); the softmax's instructions come second.
+//
+// Tensor memory: per tile S (64 columns) twice and O (D columns).  Shared memory: Q 64 KB, K and V 3 x 32 KB at head_dim 128.
+// Every wait is bounded (ptx::BoundedWaits).
+#include <algorithm>
+#include <atomic>
+
+#include "cache_share.cuh"
+
+namespace brk {
+namespace {
+
+using namespace cache;
+
+constexpr int kTile = 128;                 // rows of a tile
+constexpr int kSoftWarps = 8, kUnpackWarps = 4;
+constexpr int kMmaWarp = kSoftWarps + kUnpackWarps;
+constexpr int kThreads = 32 * (kMmaWarp + 1);
+constexpr int kBufs = 3;
+constexpr int kTmemCols = 512, kTileCols = 256, kColO = 128;
+constexpr float kLazy = 8.f;               // O is brought in line when the reference moves by more than 2^8
+constexpr int kWaitBudget = 1 << 18;
+// barriers
+constexpr int kKVFull = 0, kKVEmpty = kKVFull + kBufs, kSFull = kKVEmpty + kBufs, kPFull = kSFull + 4, kODone = kPFull + 4, kNumBars = kODone + 2;
+
+template <int D>
+struct Smem {
+  static constexpr int kQChunk = kTile * 128, kQ = kTile * D * 2;   // 64 channels of a tile; a tile
+  static constexpr int kChunk = kPage * 128, kHalf = kPage * D * 2; // 64 channels of a page's K (or V); all of it
+  static constexpr int kKV = 2 * kQ, kBars = kKV + kBufs * 2 * kHalf, kBytes = kBars + kNumBars * 8 + 16;
+};
+
+__device__ __forceinline__ uint32_t low_part(uint32_t hi, float x, float y) { return pack_bf16(x - bf_lo(hi), y - bf_hi(hi)); }
+
+template <int D>
+__global__ void __launch_bounds__(kThreads, 1) cache_attn_tc_kernel(CacheAttnArgs a) {
+  using L = Layout<D>;
+  using SM = Smem<D>;
+  constexpr int kG = L::kGroups;
+  extern __shared__ unsigned char smem_raw[];
+  __shared__ uint32_t s_mask[2 * kShare];
+  __shared__ int32_t s_page[kShare];
+  __shared__ int s_list[kShare], s_live;  // the pages with a token in a block, in order
+  __shared__ uint32_t s_nan[kBufs][kG][2];  // pages that some rows see in part: tokens whose value is NaN, by group
+  unsigned char* const smem = smem_raw + ((1024u - (ptx::smem_u32(smem_raw) & 1023u)) & 1023u);
+  const uint32_t sbase = ptx::smem_u32(smem);
+  uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(smem + SM::kBars + kNumBars * 8);
+  auto bar = [&](int i) { return sbase + SM::kBars + (uint32_t)i * 8u; };
+
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int share = blockIdx.x, b = blockIdx.y / a.Nk, kvh = blockIdx.y % a.Nk, row0 = blockIdx.z * 2 * kTile;
+  const int G = a.N / a.Nk;
+  if (tid == 0) {
+    for (int i = 0; i < kNumBars; ++i)
+      ptx::mbar_init(bar(i), i < kKVEmpty || (i >= kPFull && i < kODone) ? 4u : 1u);  // (by the warps that write K and V, or P)
+    ptx::fence_barrier_init();
+  }
+  if (warp == kMmaWarp) {
+    __syncwarp();
+    ptx::tmem_alloc(ptx::smem_u32(tmem_slot), kTmemCols);
+    ptx::tmem_relinquish();
+  }
+  ptx::grid_dependency_launch();
+  ptx::grid_dependency_wait();
+  const Share sh = find_share<kThreads>(a, b, row0, 2 * kTile, share, 1, s_mask, s_page, [&] {
+    // Q as the K-major A operand: rows of 128 bytes, their 16-byte units swizzled
+#pragma unroll 2
+    for (int i = tid; i < 2 * kTile * (D / 8); i += kThreads) {
+      const int u = i % (D / 8), rr = i / (D / 8), r = row0 + rr;
+      uint4 x = make_uint4(0, 0, 0, 0);
+      if (r < a.Lq * G)
+        x = *reinterpret_cast<const uint4*>(reinterpret_cast<const __nv_bfloat16*>(a.q.ptr) + (int64_t)b * a.q.sb +
+                                            (int64_t)(kvh * G + r % G) * a.q.sh + (int64_t)(r / G) * a.q.ss + 8 * u);
+      *reinterpret_cast<uint4*>(smem + (rr / kTile) * SM::kQ + (u >> 3) * SM::kQChunk + (rr % kTile) * 128 + (((u & 7) ^ (rr & 7)) << 4)) = x;
+    }
+  });
+  if (warp == 0) {
+    int live = 0;
+    for (int i = lane; i < kShare; i += 32) {
+      const unsigned there = __ballot_sync(0xffffffffu, i < sh.n && s_page[i] >= 0);
+      if (i < sh.n && s_page[i] >= 0) s_list[live + __popc(there & ((1u << lane) - 1))] = i;
+      live += __popc(there);
+    }
+    if (lane == 0) s_live = live;
+  }
+  ptx::fence_proxy_async_smem();
+  ptx::tc_fence_before_sync();
+  __syncthreads();
+  ptx::tc_fence_after_sync();
+  const uint32_t tmem = *tmem_slot;
+  const int live = s_live;
+  const int tiles = sh.n_rows > kTile ? 2 : 1;
+  const int first_lim = sh.first_slot + row0 / G;  // the last slot that the CTA's first row sees
+  ptx::BoundedWaits waits(kWaitBudget);
+  auto wait = [&](int i, uint32_t parity) { waits(bar(i), parity & 1u, 1); };
+
+  if (warp < kSoftWarps) {
+    // =============================== softmax: a thread per row ===========================================
+    const int x = warp >> 2, rr = tid & (kTile - 1), r = row0 + x * kTile + rr, tok = r / G, hd = kvh * G + r % G;
+    const bool there = x * kTile + rr < sh.n_rows;
+    const uint32_t tm = tmem + ((uint32_t)((warp & 3) * 32) << 16) + (uint32_t)x * kTileCols;
+    const int lim = sh.first_slot + tok;
+    const float sl2 = a.scale * kLog2e;
+    float m_run = -INFINITY, l_run = 0.f;
+    unsigned poison = 0;  // groups of channels in which this row has seen NaN
+    const int pages = x < tiles ? live : 0;
+#pragma unroll 1
+    for (int k = 0; k < pages; ++k) {
+      const int i = s_list[k], slot0 = (sh.page0 + i) * kPage;
+      unsigned v0 = s_mask[2 * i], v1 = s_mask[2 * i + 1];
+      const bool late = slot0 + kPage - 1 > first_lim;
+      wait(kSFull + 2 * x + (k & 1), k >> 1);
+      ptx::tc_fence_after_sync();
+      __syncwarp();
+      uint32_t sr[64];
+      ptx::tmem_ld32(tm + (uint32_t)(k & 1) * 64, *reinterpret_cast<uint32_t (*)[32]>(&sr[0]));
+      ptx::tmem_ld32(tm + (uint32_t)(k & 1) * 64 + 32, *reinterpret_cast<uint32_t (*)[32]>(&sr[32]));
+      ptx::tmem_wait_ld(sr);
+      if (late || (v0 & v1) != ~0u) {  // (warp-uniform)
+        if (late) {
+          const int n = there ? max(0, min(64, lim - slot0 + 1)) : 64;
+          v0 &= n >= 32 ? ~0u : (1u << n) - 1u;
+          v1 &= n >= 64 ? ~0u : n > 32 ? (1u << (n - 32)) - 1u : 0u;
+          wait(kKVFull + k % kBufs, k / kBufs);  // (long since: what the unpacking warps wrote beside K and V is visible behind it)
+#pragma unroll
+          for (int j = 0; j < kG; ++j)
+            if ((s_nan[k % kBufs][j][0] & v0) | (s_nan[k % kBufs][j][1] & v1)) poison |= 1u << j;
+          __syncwarp();
+        }
+#pragma unroll
+        for (int c = 0; c < 64; ++c) sr[c] = ((c < 32 ? v0 : v1) & (1u << (c & 31))) ? sr[c] : 0xff800000u;
+      }
+      float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+      for (int c = 0; c < 64; c += 2) mx4[(c >> 1) & 3] = ptx::max3(mx4[(c >> 1) & 3], __uint_as_float(sr[c]), __uint_as_float(sr[c + 1]));
+      const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * sl2;
+      float m_new = fmaxf(m_run, mx);
+      if (m_run != -INFINITY && m_new - m_run <= kLazy) m_new = m_run;
+      const float ref = m_new == -INFINITY ? 0.f : m_new;
+      const float corr = ptx::ex2(m_run - ref);
+      const bool changed = m_new != m_run;
+      m_run = m_new;
+      const ptx::f32x2 sc2 = ptx::pack2(sl2, sl2), nr2 = ptx::pack2(-ref, -ref);
+      ptx::f32x2 sum2[2] = {0ull, 0ull};
+      uint32_t hi[32], lo[32];
+#pragma unroll
+      for (int c = 0; c < 64; c += 2) {
+        float t0, t1;
+        ptx::unpack2(ptx::fma2(ptx::pack2(__uint_as_float(sr[c]), __uint_as_float(sr[c + 1])), sc2, nr2), t0, t1);
+        const float p0 = ptx::ex2(t0), p1 = ptx::ex2(t1);
+        sum2[(c >> 1) & 1] = ptx::add2(sum2[(c >> 1) & 1], ptx::pack2(p0, p1));
+        hi[c >> 1] = pack_bf16(p0, p1);
+        lo[c >> 1] = low_part(hi[c >> 1], p0, p1);
+      }
+      ptx::tmem_st32(tm + (uint32_t)(k & 1) * 64, hi);
+      ptx::tmem_st32(tm + (uint32_t)(k & 1) * 64 + 32, lo);
+      if (k > 0 && __any_sync(0xffffffffu, changed)) {  // (rare)
+        wait(kODone + x, k - 1);
+        ptx::tc_fence_after_sync();
+        __syncwarp();
+#pragma unroll 1
+        for (int ch = 0; ch < D / 32; ++ch) {
+          uint32_t o[32];
+          ptx::tmem_ld32(tm + kColO + (uint32_t)ch * 32, o);
+          ptx::tmem_wait_ld(o);
+#pragma unroll
+          for (int c = 0; c < 32; ++c) o[c] = __float_as_uint(__uint_as_float(o[c]) * corr);
+          ptx::tmem_st32(tm + kColO + (uint32_t)ch * 32, o);
+        }
+      }
+      float s0, s1, s2, s3;
+      ptx::unpack2(sum2[0], s0, s1);
+      ptx::unpack2(sum2[1], s2, s3);
+      l_run = l_run * corr + ((s0 + s1) + (s2 + s3));
+      ptx::tmem_wait_st();
+      ptx::tc_fence_before_sync();
+      __syncwarp();
+      ptx::mbar_arrive_warp(bar(kPFull + 2 * x + (k & 1)));
+    }
+    // ---- output ----
+    if (pages > 0) {
+      wait(kODone + x, pages - 1);
+      ptx::tc_fence_after_sync();
+      __syncwarp();
+    }
+    const int64_t row = ((int64_t)b * a.N + hd) * a.Lq + tok;
+    const float inv = a.shares > 1 ? 1.f : l_run != 0.f ? 1.f / l_run : 0.f;  // (a sum that is NaN stays one)
+#pragma unroll 1
+    for (int ch = 0; ch < D / 32; ++ch) {
+      uint32_t o[32];
+      if (pages > 0) {
+        ptx::tmem_ld32(tm + kColO + (uint32_t)ch * 32, o);
+        ptx::tmem_wait_ld(o);
+      } else {
+#pragma unroll
+        for (int c = 0; c < 32; ++c) o[c] = 0;
+      }
+      if (tok < a.Lq) {
+        if (!there) {
+#pragma unroll
+          for (int c = 0; c < 32; ++c) o[c] = 0;
+        }
+        if (there && (poison >> ch & 1)) {
+#pragma unroll
+          for (int c = 0; c < 32; ++c) o[c] = 0x7FC00000u;
+        }
+        if (a.shares > 1) {
+          if (there && pages > 0) {
+            float4* const p = reinterpret_cast<float4*>(a.part_o + (row * a.shares + share) * D + ch * 32);
+#pragma unroll
+            for (int c = 0; c < 32; c += 4)
+              p[c / 4] = make_float4(__uint_as_float(o[c]), __uint_as_float(o[c + 1]), __uint_as_float(o[c + 2]), __uint_as_float(o[c + 3]));
+          }
+        } else {
+          __nv_bfloat16* const p = reinterpret_cast<__nv_bfloat16*>(a.o.ptr) + (int64_t)b * a.o.sb + (int64_t)hd * a.o.sh + (int64_t)tok * a.o.ss + ch * 32;
+#pragma unroll
+          for (int c = 0; c < 32; c += 8) {
+            float v[8];
+#pragma unroll
+            for (int y = 0; y < 8; ++y) v[y] = __uint_as_float(o[c + y]) * inv;
+            store8(p + c, v);
+          }
+        }
+      }
+      __syncwarp();
+    }
+    if (tok < a.Lq) {
+      if (!there) m_run = -INFINITY, l_run = 0.f;
+      if (a.shares > 1) {
+        if (there || sh.bad) a.part_ml[row * a.shares + share] = make_float2(m_run, l_run);
+      } else if (a.lse) {
+        a.lse[row] = l_run != 0.f ? (m_run + log2f(l_run)) * kLn2 : -INFINITY;
+      }
+    }
+  } else if (warp < kMmaWarp) {
+    // =============================== codes -> K and V ===========================================
+    const int p = tid - 32 * kSoftWarps, t = p & 3, line = p >> 2;  // keys `line`, `line` + 32; token pair `line`
+    const unsigned char* const head = a.pages + (int64_t)kvh * L::kBytes;
+    const Codes codes = a.codes;
+    uint32_t kw[2][kG], ks[2][kG / 2], vw[2][kG], vs[kG];
+    auto fetch = [&](int k) {
+      const unsigned char* const page = head + (int64_t)s_page[s_list[k]] * a.Nk * L::kBytes;
+#pragma unroll
+      for (int y = 0; y < 2; ++y) {
+        load_words<D>(page + L::k_word(line + 32 * y, 0, t), kw[y]);
+        load_scales<D>(page + L::k_scale(line + 32 * y, 0), ks[y]);
+        load_words<D>(page + L::v_word(2 * line, 2 * t + y, 0), vw[y]);  // the even token's words, then the odd one's
+      }
+      load_words<D>(page + L::v_scale(2 * line, 0), vs);
+    };
+    if (live > 0) fetch(0);
+#pragma unroll 1
+    for (int k = 0; k < live; ++k) {
+      const int buf = k % kBufs, i = s_list[k], slot0 = (sh.page0 + i) * kPage;
+      const uint32_t in = s_mask[2 * i + (line >> 4)] >> (2 * line & 31);  // of this pair of tokens
+      const bool late = slot0 + kPage - 1 > first_lim;
+      if (k >= kBufs) wait(kKVEmpty + buf, k / kBufs - 1);
+      unsigned char* const out_k = smem + SM::kKV + buf * 2 * SM::kHalf;
+      unsigned char* const out_v = out_k + SM::kHalf;
+      auto place = [&](int key, int j) { return ((4 * j + t) >> 3) * SM::kChunk + key * 128 + ((((4 * j + t) & 7) ^ (key & 7)) << 4); };
+      auto write = [&](unsigned char* to, uint32_t w, uint32_t s2) {
+        const Pairs x = pairs_of(codes, w, s2);
+        const uint2 lo = low_values(x), hi = high_values(x);
+        *reinterpret_cast<uint4*>(to) = make_uint4(lo.x, lo.y, hi.x, hi.y);
+      };
+#pragma unroll
+      for (int y = 0; y < 2; ++y)
+#pragma unroll
+        for (int j = 0; j < kG; ++j) write(out_k + place(line + 32 * y, j), kw[y][j], __byte_perm(ks[y][j / 2], 0, j % 2 ? 0x3232 : 0x1010));
+      // values of tokens in no block are zeros (0 x NaN would reach every row); so are NaN that some rows see and others do not:
+      // those rows are told
+      const uint32_t keep = ((in & 1) ? 0xFFFFu : 0u) | ((in & 2) ? 0xFFFF0000u : 0u);
+#pragma unroll
+      for (int j = 0; j < kG; ++j) vs[j] &= keep;
+      if (late) {
+        if (p < 2 * kG) s_nan[buf][p / 2][p % 2] = 0;
+        asm volatile("bar.sync 1, 128;" ::: "memory");
+#pragma unroll
+        for (int j = 0; j < kG; ++j) {
+          const uint32_t is = __vcmpeq2(vs[j] & 0x7F807F80u, 0x7F807F80u);
+          if (is) atomicOr(&s_nan[buf][j][line >> 4], ((is & 1u) | ((is >> 31) << 1)) << (2 * line & 31));
+          vs[j] &= ~is;
+        }
+      }
+#pragma unroll
+      for (int y = 0; y < 2; ++y)
+#pragma unroll
+        for (int j = 0; j < kG; ++j)
+          write(out_v + place(2 * line + y, j), __byte_perm(rotr(vw[0][y * (kG / 2) + j / 2], 3), rotr(vw[1][y * (kG / 2) + j / 2], 3), j % 2 ? 0x7632 : 0x5410),
+                __byte_perm(vs[j], 0, y ? 0x3232 : 0x1010));
+      if (k + 1 < live) fetch(k + 1);
+      ptx::fence_proxy_async_smem();
+      __syncwarp();
+      ptx::mbar_arrive_warp(bar(kKVFull + buf));
+    }
+  } else {
+    // =============================== MMA ===========================================
+    const uint32_t idesc_qk = ptx::idesc_bf16(kTile, kPage, 0, 0), idesc_pv = ptx::idesc_bf16(kTile, D, 0, 1);
+    const uint64_t q_desc = ptx::smem_desc_sw128(sbase, 16, 1024), k_desc = ptx::smem_desc_sw128(sbase + SM::kKV, 16, 1024);
+    const uint64_t v_desc = ptx::smem_desc_sw128(sbase + SM::kKV + SM::kHalf, SM::kChunk, 1024);
+    auto issue_qk = [&](int k) {
+      const int buf = k % kBufs;
+      wait(kKVFull + buf, k / kBufs);
+      ptx::tc_fence_after_sync();
+      __syncwarp();
+      if (ptx::elect_one()) {
+#pragma unroll 1
+        for (int x = 0; x < tiles; ++x) {
+          const uint32_t d = tmem + (uint32_t)x * kTileCols + (uint32_t)(k & 1) * 64;
+#pragma unroll 1
+          for (int s = 0; s < D / 16; ++s)
+            ptx::mma_ss_lohi(d, (uint32_t)q_desc + (uint32_t)x * (SM::kQ >> 4) + (uint32_t)(s >> 2) * (SM::kQChunk >> 4) + (uint32_t)(s & 3) * 2,
+                             (uint32_t)(q_desc >> 32), (uint32_t)k_desc + (uint32_t)buf * (2 * SM::kHalf >> 4) + (uint32_t)(s >> 2) * (SM::kChunk >> 4) + (uint32_t)(s & 3) * 2,
+                             (uint32_t)(k_desc >> 32), idesc_qk, s > 0);
+          ptx::mma_commit(bar(kSFull + 2 * x + (k & 1)));
+        }
+      }
+      __syncwarp();
+    };
+    if (live > 0) issue_qk(0);
+#pragma unroll 1
+    for (int k = 0; k < live; ++k) {
+      if (k + 1 < live) issue_qk(k + 1);
+      const int buf = k % kBufs;
+#pragma unroll 1
+      for (int x = 0; x < tiles; ++x) {
+        wait(kPFull + 2 * x + (k & 1), k >> 1);
+        ptx::tc_fence_after_sync();
+        __syncwarp();
+        if (ptx::elect_one()) {
+          const uint32_t s = tmem + (uint32_t)x * kTileCols + (uint32_t)(k & 1) * 64, d = tmem + (uint32_t)x * kTileCols + kColO;
+#pragma unroll 1
+          for (int ks = 0; ks < kPage / 16; ++ks) {
+            const uint32_t v = (uint32_t)v_desc + (uint32_t)buf * (2 * SM::kHalf >> 4) + (uint32_t)ks * (16 * 128 >> 4);
+            ptx::mma_ts_lohi(d, s + ks * 8, v, (uint32_t)(v_desc >> 32), idesc_pv, k > 0 || ks > 0);
+            ptx::mma_ts_lohi(d, s + 32 + ks * 8, v, (uint32_t)(v_desc >> 32), idesc_pv, 1u);
+          }
+          ptx::mma_commit(bar(kODone + x));
+          if (x + 1 == tiles) ptx::mma_commit(bar(kKVEmpty + buf));
+        }
+        __syncwarp();
+      }
+    }
+  }
+  ptx::tc_fence_before_sync();
+  ptx::end_of_waits(waits, [](int) { return kStatusCacheWait; }, a.status);
+  if (warp == kMmaWarp) ptx::tmem_dealloc(tmem, kTmemCols);
+}
+
+}  // namespace
+
+int cache_attn_tc_launch(const cache::CacheAttnArgs& a, int D, cudaStream_t st) {
+  const int64_t rows = (int64_t)a.Lq * (a.N / a.Nk), z = (rows + 2 * kTile - 1) / (2 * kTile);
+  const dim3 grid(a.shares, a.B * a.Nk, (unsigned)z);
+  auto run = [&](auto kern, int bytes, std::atomic<bool>* configured) -> int {
+    int dev = 0;
+    BRK_CUDA(cudaGetDevice(&dev));
+    if (dev < 0 || dev >= 64 || !configured[dev].load(std::memory_order_acquire)) {
+      BRK_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+      if (dev >= 0 && dev < 64) configured[dev].store(true, std::memory_order_release);
+    }
+    return launch_dependent(kern, grid, dim3(kThreads), bytes, st, a);
+  };
+  static std::atomic<bool> done128[64] = {}, done64[64] = {};
+  return D == 128 ? run(cache_attn_tc_kernel<128>, Smem<128>::kBytes + 1024, done128) : run(cache_attn_tc_kernel<64>, Smem<64>::kBytes + 1024, done64);
+}
+
+}  // namespace brk

@@ -294,19 +294,6 @@ __global__ void __launch_bounds__(kIoThreads) cache_write_kernel(IoArgs a) {
   }
 }
 
-// a word of 8 codes -> their values, k and k + 4 in one register
-struct Pairs {
-  uint32_t x[4];
-};
-__device__ __forceinline__ Pairs pairs_of(const Codes& codes, uint32_t w, uint32_t s2) {
-  const uint32_t c2 = scale_offset(s2);
-  Pairs p;
-#pragma unroll
-  for (int k = 0; k < 4; ++k) p.x[k] = held(codes, rotl(w, (35 - 4 * k) % 32), s2, c2);
-  return p;
-}
-__device__ __forceinline__ uint2 low_values(const Pairs& p) { return make_uint2(__byte_perm(p.x[0], p.x[1], 0x5410), __byte_perm(p.x[2], p.x[3], 0x5410)); }
-__device__ __forceinline__ uint2 high_values(const Pairs& p) { return make_uint2(__byte_perm(p.x[0], p.x[1], 0x7632), __byte_perm(p.x[2], p.x[3], 0x7632)); }
 // four values as bf16 -> memory
 __device__ __forceinline__ void write4(__nv_bfloat16* p, uint2 x) { __stcs(reinterpret_cast<uint2*>(p), x); }
 __device__ __forceinline__ void write4(float* p, uint2 x) {

@@ -74,6 +74,20 @@ __device__ __forceinline__ uint32_t held(const Codes& k, uint32_t x, uint32_t s2
   return fma_bf2((x & k.mask) | k.base, s2, c2);
 }
 
+// a word of 8 codes -> their values, k and k + 4 in one register
+struct Pairs {
+  uint32_t x[4];
+};
+__device__ __forceinline__ Pairs pairs_of(const Codes& codes, uint32_t w, uint32_t s2) {
+  const uint32_t c2 = scale_offset(s2);
+  Pairs p;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) p.x[k] = held(codes, rotl(w, (35 - 4 * k) % 32), s2, c2);
+  return p;
+}
+__device__ __forceinline__ uint2 low_values(const Pairs& p) { return make_uint2(__byte_perm(p.x[0], p.x[1], 0x5410), __byte_perm(p.x[2], p.x[3], 0x5410)); }
+__device__ __forceinline__ uint2 high_values(const Pairs& p) { return make_uint2(__byte_perm(p.x[0], p.x[1], 0x7632), __byte_perm(p.x[2], p.x[3], 0x7632)); }
+
 // C (16 x 8) += A (16 x 16) B (16 x 8)
 __device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"

@@ -105,4 +105,7 @@ __device__ __forceinline__ Share find_share(const CacheAttnArgs& a, int b, int r
 }
 
 }  // namespace cache
+
+int cache_attn_tc_launch(const cache::CacheAttnArgs& a, int D, cudaStream_t st);
+
 }  // namespace brk
