@@ -7,7 +7,8 @@
 // the softmax is at the page before and the next one is being unpacked.
 // 128 x 64 x D products three times per tile and page (S once, P in two parts); the softmax's instructions come second.
 //
-// Tensor memory: per tile S (64 columns) twice and O (D columns).  Shared memory: Q 64 KB, K and V 3 x 32 KB at head_dim 128.
+// Tensor memory: per tile S (64 columns) twice and O (D columns).  Shared memory at head_dim 128: Q 64 KB, K and V 3 x 32 KB, codes on
+// their way 4 x 12 KB.
 // Every wait is bounded (ptx::BoundedWaits).
 #include <algorithm>
 #include <atomic>
@@ -24,6 +25,7 @@ constexpr int kSoftWarps = 8, kUnpackWarps = 4;
 constexpr int kMmaWarp = kSoftWarps + kUnpackWarps;
 constexpr int kThreads = 32 * (kMmaWarp + 1);
 constexpr int kBufs = 3;
+constexpr int kAhead = 4;                  // pages whose codes are on their way
 constexpr int kTmemCols = 512, kTileCols = 256, kColO = 128;
 constexpr float kLazy = 8.f;               // O is brought in line when the reference moves by more than 2^8
 constexpr int kWaitBudget = 1 << 18;
@@ -34,9 +36,17 @@ template <int D>
 struct Smem {
   static constexpr int kQChunk = kTile * 128, kQ = kTile * D * 2;   // 64 channels of a tile; a tile
   static constexpr int kChunk = kPage * 128, kHalf = kPage * D * 2; // 64 channels of a page's K (or V); all of it
-  static constexpr int kKV = 2 * kQ, kBars = kKV + kBufs * 2 * kHalf, kBytes = kBars + kNumBars * 8 + 16;
+  // What an unpacking thread copies of a page, every piece in a cell of its own: K words and V words twice, V scales; K scales twice.
+  static constexpr int kCell = D / 8, kScales = D / 16, kThread = 5 * kCell + 2 * kScales, kStage = kThread * 32 * kUnpackWarps;
+  static constexpr int kKV = 2 * kQ, kCodes = kKV + kBufs * 2 * kHalf, kBars = kCodes + kAhead * kStage, kBytes = kBars + kNumBars * 8 + 16;
 };
 
+template <int kBytes>
+__device__ __forceinline__ void cp_async(void* dst, const void* src) {
+  const uint32_t d = ptx::smem_u32(dst);
+  if constexpr (kBytes == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(d), "l"(src) : "memory");
+  else asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(d), "l"(src), "n"(kBytes) : "memory");
+}
 __device__ __forceinline__ uint32_t low_part(uint32_t hi, float x, float y) { return pack_bf16(x - bf_lo(hi), y - bf_hi(hi)); }
 
 template <int D>
@@ -244,23 +254,42 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attn_tc_kernel(CacheAttnArg
     const int p = tid - 32 * kSoftWarps, t = p & 3, line = p >> 2;  // keys `line`, `line` + 32; token pair `line`
     const unsigned char* const head = a.pages + (int64_t)kvh * L::kBytes;
     const Codes codes = a.codes;
-    uint32_t kw[2][kG], ks[2][kG / 2], vw[2][kG], vs[kG];
-    auto fetch = [&](int k) {
-      const unsigned char* const page = head + (int64_t)s_page[s_list[k]] * a.Nk * L::kBytes;
+    unsigned char* const cells = smem + SM::kCodes + p * SM::kCell;  // cell c of stage s: s kStage + c 128 kCell on
+    unsigned char* const scale_cells = smem + SM::kCodes + 5 * 128 * SM::kCell + p * SM::kScales;
+    auto request = [&](int k) {
+      if (k < live) {
+        const unsigned char* const page = head + (int64_t)s_page[s_list[k]] * a.Nk * L::kBytes;
+        const int stage = k % kAhead * SM::kStage;
 #pragma unroll
-      for (int y = 0; y < 2; ++y) {
-        load_words<D>(page + L::k_word(line + 32 * y, 0, t), kw[y]);
-        load_scales<D>(page + L::k_scale(line + 32 * y, 0), ks[y]);
-        load_words<D>(page + L::v_word(2 * line, 2 * t + y, 0), vw[y]);  // the even token's words, then the odd one's
+        for (int y = 0; y < 2; ++y) {
+          cp_async<SM::kCell>(cells + stage + y * 128 * SM::kCell, page + L::k_word(line + 32 * y, 0, t));
+          cp_async<SM::kCell>(cells + stage + (2 + y) * 128 * SM::kCell, page + L::v_word(2 * line, 2 * t + y, 0));
+          cp_async<SM::kScales>(scale_cells + stage + y * 128 * SM::kScales, page + L::k_scale(line + 32 * y, 0));
+        }
+        cp_async<SM::kCell>(cells + stage + 4 * 128 * SM::kCell, page + L::v_scale(2 * line, 0));
       }
-      load_words<D>(page + L::v_scale(2 * line, 0), vs);
+      cp_async_commit();
     };
-    if (live > 0) fetch(0);
+#pragma unroll 1
+    for (int k = 0; k < kAhead - 1; ++k) request(k);
 #pragma unroll 1
     for (int k = 0; k < live; ++k) {
       const int buf = k % kBufs, i = s_list[k], slot0 = (sh.page0 + i) * kPage;
       const uint32_t in = s_mask[2 * i + (line >> 4)] >> (2 * line & 31);  // of this pair of tokens
       const bool late = slot0 + kPage - 1 > first_lim;
+      request(k + kAhead - 1);
+      cp_async_wait<kAhead - 1>();  // this thread's cells of page k have landed
+      uint32_t kw[2][kG], ks[2][kG / 2], vw[2][kG], vs[kG];
+      {
+        const int stage = k % kAhead * SM::kStage;
+#pragma unroll
+        for (int y = 0; y < 2; ++y) {
+          load_words<D>(cells + stage + y * 128 * SM::kCell, kw[y]);
+          load_words<D>(cells + stage + (2 + y) * 128 * SM::kCell, vw[y]);  // the even token's words, then the odd one's
+          load_scales<D>(scale_cells + stage + y * 128 * SM::kScales, ks[y]);
+        }
+        load_words<D>(cells + stage + 4 * 128 * SM::kCell, vs);
+      }
       if (k >= kBufs) wait(kKVEmpty + buf, k / kBufs - 1);
       unsigned char* const out_k = smem + SM::kKV + buf * 2 * SM::kHalf;
       unsigned char* const out_v = out_k + SM::kHalf;
@@ -295,11 +324,11 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attn_tc_kernel(CacheAttnArg
         for (int j = 0; j < kG; ++j)
           write(out_v + place(2 * line + y, j), __byte_perm(rotr(vw[0][y * (kG / 2) + j / 2], 3), rotr(vw[1][y * (kG / 2) + j / 2], 3), j % 2 ? 0x7632 : 0x5410),
                 __byte_perm(vs[j], 0, y ? 0x3232 : 0x1010));
-      if (k + 1 < live) fetch(k + 1);
       ptx::fence_proxy_async_smem();
       __syncwarp();
       ptx::mbar_arrive_warp(bar(kKVFull + buf));
     }
+    cp_async_wait<0>();
   } else {
     // =============================== MMA ===========================================
     const uint32_t idesc_qk = ptx::idesc_bf16(kTile, kPage, 0, 0), idesc_pv = ptx::idesc_bf16(kTile, D, 0, 1);
