@@ -19,9 +19,13 @@ void set_error(const char* fmt, ...) {
 }
 
 int sm_count() {
+  static std::atomic<int> known[64];
   int dev = 0, n = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) return 0;
+  const bool kept = dev >= 0 && dev < 64;
+  if (kept && (n = known[dev].load(std::memory_order_relaxed)) > 0) return n;
   if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 0;
+  if (kept) known[dev].store(n, std::memory_order_relaxed);
   return n;
 }
 

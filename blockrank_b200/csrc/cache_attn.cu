@@ -470,7 +470,8 @@ int shares_of(const brk_cache_attn_params& p) {
   const int64_t least = (p.P + kShare - 1) / kShare, pages = many ? 4 : kWarps;
   const int64_t most = std::max<int64_t>(least, std::min<int64_t>(64, (p.P + pages - 1) / pages));
   int64_t best = least, best_cost = INT64_MAX;
-  for (int64_t s = least; s <= most; ++s) {
+  for (int64_t round = 0; round <= 8; ++round) {  // (the most shares of so many rounds, and the fewest)
+    const int64_t s = std::min(most, std::max(least, round * room / ctas));
     const int64_t join = s == 1 ? 0 : s > kCluster || many ? 6 + s / 8 : 2;
     const int64_t cost = (ctas * s + room - 1) / room * ((p.P + s - 1) / s + (many ? 4 : 6)) + join;
     if (cost < best_cost) {

@@ -29,8 +29,9 @@ constexpr int kAhead = 4;                  // pages whose codes are on their way
 constexpr int kTmemCols = 512, kTileCols = 256, kColO = 128;
 constexpr float kLazy = 8.f;               // O is brought in line when the reference moves by more than 2^8
 constexpr int kWaitBudget = 1 << 18;
-// barriers
-constexpr int kKVFull = 0, kKVEmpty = kKVFull + kBufs, kSFull = kKVEmpty + kBufs, kPFull = kSFull + 4, kODone = kPFull + 4, kNumBars = kODone + 2;
+// Barriers.  S, P and O have two per tile, for even and odd pages: by the time that a page's S is there only the page before last is
+// sure to have reached O, so a single one's parity would not tell the last two pages apart.
+constexpr int kKVFull = 0, kKVEmpty = kKVFull + kBufs, kSFull = kKVEmpty + kBufs, kPFull = kSFull + 4, kODone = kPFull + 4, kNumBars = kODone + 4;
 
 template <int D>
 struct Smem {
@@ -172,7 +173,7 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attn_tc_kernel(CacheAttnArg
       ptx::tmem_st32(tm + (uint32_t)(k & 1) * 64, hi);
       ptx::tmem_st32(tm + (uint32_t)(k & 1) * 64 + 32, lo);
       if (k > 0 && __any_sync(0xffffffffu, changed)) {  // (rare)
-        wait(kODone + x, k - 1);
+        wait(kODone + 2 * x + ((k - 1) & 1), (k - 1) >> 1);
         ptx::tc_fence_after_sync();
         __syncwarp();
 #pragma unroll 1
@@ -196,7 +197,7 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attn_tc_kernel(CacheAttnArg
     }
     // ---- output ----
     if (pages > 0) {
-      wait(kODone + x, pages - 1);
+      wait(kODone + 2 * x + ((pages - 1) & 1), (pages - 1) >> 1);
       ptx::tc_fence_after_sync();
       __syncwarp();
     }
@@ -371,7 +372,7 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attn_tc_kernel(CacheAttnArg
             ptx::mma_ts_lohi(d, s + ks * 8, v, (uint32_t)(v_desc >> 32), idesc_pv, k > 0 || ks > 0);
             ptx::mma_ts_lohi(d, s + 32 + ks * 8, v, (uint32_t)(v_desc >> 32), idesc_pv, 1u);
           }
-          ptx::mma_commit(bar(kODone + x));
+          ptx::mma_commit(bar(kODone + 2 * x + (k & 1)));
           if (x + 1 == tiles) ptx::mma_commit(bar(kKVEmpty + buf));
         }
         __syncwarp();

@@ -279,7 +279,8 @@ int cache_scores_launch(const brk_cache_score_params& p, void* ws, cudaStream_t 
   const int64_t ctas = (int64_t)p.B * a.Nk * z, room = (tiles == 1 && p.dtype == BRK_BF16 ? 3 : 2) * (int64_t)std::max(1, sm_count());
   const int64_t most = std::min<int64_t>(nd, (p.P + kWarps - 1) / kWarps);
   int64_t shares = 1, best = INT64_MAX;
-  for (int64_t s = 1; s <= std::min<int64_t>(most, 256); ++s) {
+  for (int64_t round = 0; round <= 8; ++round) {  // (the most shares of so many rounds, and the fewest)
+    const int64_t s = std::min(most, std::max<int64_t>(1, round * room / ctas));
     const int64_t cost = (ctas * s + room - 1) / room * ((p.P + s - 1) / s + 8);
     if (cost < best) {
       best = cost;

@@ -6,6 +6,7 @@
 // same steps cost 40-60 us per attention call, more than its kernels take on a short prompt.
 #include <ATen/cuda/CUDAContext.h>
 #include <ATen/cuda/CUDAEvent.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <ATen/cuda/tunable/Tunable.h>
 #include <ATen/ops/addmm_cuda_dispatch.h>
 #include <ATen/ops/mm_cuda_dispatch.h>
@@ -416,13 +417,19 @@ void need_device(const Tensor& of, std::initializer_list<const Tensor*> ts) {
   for (const Tensor* t : ts)
     if (t != nullptr && t->defined()) BRK_VALUE(t->device() == of.device(), "tensors on ", of.device(), " and ", t->device());
 }
-// view_of, for any stride of a dimension of one
-brk_view heads_view(const Tensor& t) {
-  brk_view v = view_of(t);
+// view_of (view_bshd), for any stride of a dimension of one
+brk_view heads_view(const Tensor& t, bool bshd = false) {
+  brk_view v = bshd ? view_bshd(t) : view_of(t);
   if (t.size(0) == 1) v.stride_b = 0;
-  if (t.size(1) == 1) v.stride_h = 0;
-  if (t.size(2) == 1) v.stride_s = 0;
+  if (t.size(bshd ? 2 : 1) == 1) v.stride_h = 0;
+  if (t.size(bshd ? 1 : 2) == 1) v.stride_s = 0;
   return v;
+}
+// at::empty without its dispatch: a step's call is as long as its host path (reading back one document 6.9 us of it, now XX)
+Tensor fresh(at::IntArrayRef sizes, at::ScalarType type, const Tensor& like) { return at::detail::empty_cuda(sizes, type, like.device(), std::nullopt); }
+// (B, heads, S, D) with the memory layout (B, S, heads, D)
+Tensor fresh_heads(int64_t B, int64_t heads, int64_t S, int64_t D, at::ScalarType type, const Tensor& like) {
+  return at::detail::empty_strided_cuda({B, heads, S, D}, {S * heads * D, D, heads * D, 1}, type, like.device());
 }
 int32_t* status_ptr(const Tensor& t) { return (int32_t*)status_word(t.get_device()).data_ptr(); }
 
@@ -452,7 +459,7 @@ void cache_write(const Tensor& k, const Tensor& v, const Tensor& cache, const Te
   const int32_t B = (int32_t)k.size(0), S = (int32_t)k.size(2);
   const size_t nbytes = brk_cache_write_workspace_bytes(&c, B, S);
   Tensor ws;
-  if (nbytes > 0) ws = scratch(nbytes, cache);
+  if (nbytes > 0) ws = fresh({(int64_t)nbytes}, at::kByte, cache);
   check(brk_cache_write(dtype, &c, &vk, &vv, B, S, (const int32_t*)slots.data_ptr(), nbytes > 0 ? ws.data_ptr() : nullptr, nbytes, status_ptr(cache),
                         stream_of(cache)),
         "brk_cache_write");
@@ -466,8 +473,7 @@ std::tuple<Tensor, Tensor> cache_read(const Tensor& cache, const Tensor& slots_i
   const int64_t B = slots_in.size(0), S = slots_in.size(1);
   BRK_VALUE(slots_in.numel() < (1ll << 31), "too many tokens: ", slots_in.numel());
   c10::cuda::CUDAGuard guard(cache.device());
-  const auto opts = cache.options().dtype(dtype);
-  const Tensor k = at::empty({B, S, c.Nk, c.D}, opts).permute({0, 2, 1, 3}), v = at::empty({B, S, c.Nk, c.D}, opts).permute({0, 2, 1, 3});
+  const Tensor k = fresh_heads(B, c.Nk, S, c.D, dtype, cache), v = fresh_heads(B, c.Nk, S, c.D, dtype, cache);
   const int code = dtype_code(k);
   if (slots_in.numel() == 0) return {k, v};
   const Tensor slots = slots_in.contiguous();
@@ -503,9 +509,9 @@ std::tuple<Tensor, Tensor> cache_attention(const Tensor& q, const Tensor& cache,
   if (out_in.has_value())
     BRK_VALUE(out_in->sizes() == at::IntArrayRef({B, Lq, N, c.D}) && out_in->scalar_type() == q.scalar_type(), "out must be ", q.scalar_type(), " (", B, ", ", Lq,
               ", ", N, ", ", c.D, "), got ", out_in->scalar_type(), " ", out_in->sizes());
-  Tensor out = out_in.has_value() ? *out_in : empty_bshd(q, B, Lq, N, c.D);
+  Tensor out = out_in.has_value() ? *out_in : fresh({B, Lq, N, c.D}, q.scalar_type(), q);
   Tensor lse;
-  if (return_lse) lse = at::empty({B, N, Lq}, q.options().dtype(at::kFloat).requires_grad(false));
+  if (return_lse) lse = fresh({B, N, Lq}, at::kFloat, q);
   if (out.numel() == 0) return {out, lse};
   const Tensor table = table_in.contiguous(), bs = blk_start.contiguous(), bl = blk_len.contiguous();
   const Tensor q_len = q_len_in.has_value() ? q_len_in->contiguous() : Tensor();
@@ -516,7 +522,7 @@ std::tuple<Tensor, Tensor> cache_attention(const Tensor& q, const Tensor& cache,
   p.scale = (float)scale;
   p.cache = c;
   p.q = heads_view(q);
-  p.o = heads_view(out.permute({0, 2, 1, 3}));
+  p.o = heads_view(out, true);
   p.page_table = (const int32_t*)table.data_ptr();
   p.blk_start = (const int32_t*)bs.data_ptr();
   p.blk_len = (const int32_t*)bl.data_ptr();
@@ -525,7 +531,7 @@ std::tuple<Tensor, Tensor> cache_attention(const Tensor& q, const Tensor& cache,
   p.status = status_ptr(cache);
   const size_t nbytes = brk_cache_attn_workspace_bytes(&p);
   Tensor ws;
-  if (nbytes > 0) ws = scratch(nbytes, cache);
+  if (nbytes > 0) ws = fresh({(int64_t)nbytes}, at::kByte, cache);
   check(brk_cache_attn(&p, nbytes > 0 ? ws.data_ptr() : nullptr, nbytes, stream_of(cache)), "brk_cache_attn");
   return {out, lse};
 }
@@ -540,8 +546,7 @@ std::tuple<Tensor, Tensor> cache_doc_scores(const Tensor& q, const Tensor& cache
   c10::cuda::CUDAGuard guard(cache.device());
   const Tensor table = table_in.contiguous(), bs = blk_start.contiguous(), bl = blk_len.contiguous();
   const int64_t B = q.size(0), N = q.size(1), R = q.size(2), nd = std::max<int64_t>(0, bs.size(1) - 2);
-  const auto f32 = q.options().dtype(at::kFloat).requires_grad(false);
-  Tensor mass = at::empty({B, N, R, nd}, f32), logits = at::empty({B, nd}, f32);
+  Tensor mass = fresh({B, N, R, nd}, at::kFloat, q), logits = fresh({B, nd}, at::kFloat, q);
   brk_cache_score_params p{};
   p.dtype = dtype;
   p.B = (int32_t)B; p.N = (int32_t)N; p.R = (int32_t)R;
@@ -558,7 +563,7 @@ std::tuple<Tensor, Tensor> cache_doc_scores(const Tensor& q, const Tensor& cache
   p.logits = (float*)logits.data_ptr();
   p.status = status_ptr(cache);
   const size_t nbytes = brk_cache_doc_scores_workspace_bytes(&p);
-  Tensor ws = scratch(nbytes > 16 ? nbytes : 16, cache);
+  Tensor ws = fresh({(int64_t)std::max<size_t>(nbytes, 16)}, at::kByte, cache);
   check(brk_cache_doc_scores(&p, ws.data_ptr(), nbytes, stream_of(cache)), "brk_cache_doc_scores");
   return {mass, logits};
 }

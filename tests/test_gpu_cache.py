@@ -163,7 +163,7 @@ def test_one_row(dtype, N, Nk, D, name, paged):
 
 @pytest.mark.parametrize("dtype", [BF16, F32])
 @pytest.mark.parametrize("N,Nk,D", [(8, 2, 128), (6, 2, 64), (3, 3, 128)])
-@pytest.mark.parametrize("rows", [2, 3, 17, 70])
+@pytest.mark.parametrize("rows", [2, 3, 17, 33, 70])
 def test_several_rows_of_different_number(dtype, N, Nk, D, rows):
     lens = [[5, 64, 1, 100, rows + 30], [1, 63, 65, 128, rows], [9, 0, 0, 3, rows + 64], [2, 3, 4, 0, 80]]
     q_len = torch.tensor([rows, rows, rows // 2, 0], dtype=torch.int32)
@@ -213,11 +213,11 @@ def test_views_and_a_given_output():
     assert (room[:, 0] == 7).all() and (room[:, -1] == 7).all() and (room[..., D:] == 7).all()
 
 
-@pytest.mark.parametrize("dtype", [BF16, F32])
-def test_what_no_row_sees_has_no_influence(dtype):
+@pytest.mark.parametrize("dtype,N,R", [(BF16, 4, 5), (F32, 4, 5), (BF16, 4, 3), (BF16, 16, 5), (BF16, 4, 30)])
+def test_what_no_row_sees_has_no_influence(dtype, N, R):
     """Pages of NaN scales and arbitrary codes outside the blocks; NaN and infinities in tokens behind a row's own."""
-    N, Nk, D, B, R = 4, 2, 128, 2, 5
-    lens = [[3, 70, 9, 12], [64, 1, 0, 5]]
+    Nk, D, B = 2, 128, 2
+    lens = [[3, 70, 9, R + 7], [64, 1, 0, R]]
     start, length, P = ch.spans(lens, True, gap=PAGE)
     cache, hk, hv = _filled(B * P + 1, Nk, D, 51, dtype)
     table = _table(B, P, B * P + 1, 7)
@@ -516,3 +516,40 @@ def test_refused_calls():
             pytest.fail(f"call {i} was not refused")
     with pytest.raises(RuntimeError, match="CUDA tensors"):
         ops.cache_read(cache, torch.zeros(1, 3, dtype=torch.int32))
+
+
+@pytest.mark.parametrize("N,Nk,D,rows,tokens", [(8, 2, 128, 70, 700), (16, 2, 64, 33, 5000), (4, 1, 128, 9, 9000), (8, 1, 64, 100, 131)])
+def test_many_rows_over_shares_of_the_pages(N, Nk, D, rows, tokens):
+    """Query blocks long enough for the tensor cores' rows, over as many pages as several CTAs take: the same every time."""
+    lens = [[40, tokens // 3, tokens // 2, rows], [3, tokens // 4, 64, rows + 7]]
+    start, length, P = ch.spans(lens, False)
+    cache, hk, hv = _filled(2 * P + 1, Nk, D, 131)
+    table = _table(2, P, 2 * P + 1, 14)
+    q_len = torch.tensor([rows, rows - 5], dtype=torch.int32)
+    q = 3 * _rand(2, rows, N, D, seed=15, dtype=BF16).transpose(1, 2)
+    args = (q.cuda(), cache, table.cuda(), start.cuda(), length.cuda(), D ** -0.5)
+    ref, ref_lse, size = ch.attention(q, hk, hv, table, start, length, D ** -0.5, q_len)
+    first = None
+    for _ in range(30):
+        out, lse = ops.cache_attention(*args, q_len=q_len.cuda(), return_lse=True)
+        first = first if first is not None else (out, lse)
+        assert torch.equal(out, first[0]) and torch.equal(lse, first[1])
+    _check(*first, ref, ref_lse, size, hv, 3 * P + 8)
+    ops.check_status()
+
+
+def test_logits_that_keep_growing():
+    """Later pages outweigh earlier ones by far more than a probability can hold: what was summed is brought in line."""
+    N, Nk, D, P = 8, 1, 128, 9
+    cache, hk, hv = _filled(P, Nk, D, 141)
+    k, v = ops.cache_read(cache, torch.arange(P * PAGE, dtype=torch.int32, device="cuda")[None], F32)
+    k *= torch.exp2(torch.arange(P * PAGE, device="cuda") / 64.0)[:, None]
+    ops.cache_write(k, v, cache, torch.arange(P * PAGE, dtype=torch.int32, device="cuda")[None])
+    hk = ch.held(k[0].transpose(0, 1).cpu())
+    table = torch.arange(P, dtype=torch.int32)[None]
+    start, length = torch.zeros(1, 1, dtype=torch.int32), torch.full((1, 1), P * PAGE - 3, dtype=torch.int32)
+    for rows in (1, 2, 9):
+        q = _rand(1, rows, N, D, seed=16, dtype=BF16).transpose(1, 2)
+        out, lse = ops.cache_attention(q.cuda(), cache, table.cuda(), start.cuda(), length.cuda(), 0.05, return_lse=True)
+        ref, ref_lse, size = ch.attention(q, hk, hv, table, start, length, 0.05)
+        _check(out, lse, ref, ref_lse, size, hv, 64)
