@@ -189,6 +189,12 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<T, kTiles>) cache_attn_k
     cp_async_wait<1>();
     __syncwarp();
     const unsigned char* const page = ring + 2 * L::kHalf - L::kHalf;  // (offsets count from a page's beginning)
+    // The tensor cores cut a sum off rather than round it, so in 32 bits a page has sums of its own.
+    float fresh[kF32 ? kTiles : 1][L::kGroups][2][4] = {};
+    auto& sums = [&]() -> float (&)[kTiles][L::kGroups][2][4] {
+      if constexpr (kF32) return fresh;
+      else return o;
+    }();
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
         uint32_t pt[kTiles][2][kMmas];
@@ -282,10 +288,20 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<T, kTiles>) cache_attn_k
 #pragma unroll
             for (int c = 0; c < kTiles; ++c)
 #pragma unroll
-              for (int p = 0; p < kMmas; ++p) mma(o[c][j][u], e0, e1, f0, f1, pt[c][0][p], pt[c][1][p]);
+              for (int p = kMmas - 1; p >= 0; --p) mma(sums[c][j][u], e0, e1, f0, f1, pt[c][0][p], pt[c][1][p]);
           }
         }
       }
+    }
+    if constexpr (kF32) {
+#pragma unroll
+      for (int c = 0; c < kTiles; ++c)
+#pragma unroll
+        for (int j = 0; j < L::kGroups; ++j)
+#pragma unroll
+          for (int y = 0; y < 2; ++y)
+#pragma unroll
+            for (int x = 0; x < 4; ++x) o[c][j][y][x] += fresh[c][j][y][x];
     }
     __syncwarp();
     request(i1, 1, 2);

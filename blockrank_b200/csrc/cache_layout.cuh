@@ -63,6 +63,11 @@ __device__ __forceinline__ uint32_t fma_bf2(uint32_t a, uint32_t b, uint32_t c) 
   asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
   return d;
 }
+__device__ __forceinline__ uint32_t add_bf2(uint32_t a, uint32_t b) {
+  uint32_t d;
+  asm("add.rn.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+  return d;
+}
 // -24 s, for two scales
 __device__ __forceinline__ uint32_t scale_offset(uint32_t s2) {
   uint32_t d;
@@ -134,6 +139,10 @@ template <typename T, int D, int kTiles>
 struct QueryRows {
   using L = Layout<D>;
   static constexpr int kPieces = sizeof(T) == 4 ? 3 : 1;
+  // fp32: -8 is added to the codes instead (-8 2^-133 and -128 2^-133): of sums of n q, not of u q, fewer bits cancel.  (Output's error
+  // against 64 bits, 2 prompts of 100 documents, head_dim 64: 1.1e-6 with the codes as they are and one sum per group,
+  // 0.6e-6 so and with sums of 16 channels; plain fp32 0.5e-6.)
+  static constexpr bool kSigned = sizeof(T) == 4;
   uint32_t q[kTiles][kPieces][L::kGroups][2][2];  // [group][step][register]: channels 8 t + 2 step + {0, 4}, {1, 5}
   uint32_t shift[kTiles][2];                      // B of the product of the scales: -8 2^-133 sum(q) of the groups, in three bf16 numbers
   float unit[kTiles][2];
@@ -223,7 +232,12 @@ struct QueryRows {
       load_words<D>(page + L::k_word(16 * i + 8 + g, 0, t), wb);
       load_scales<D>(page + L::k_scale(16 * i + g, 0), sa);
       load_scales<D>(page + L::k_scale(16 * i + 8 + g, 0), sb);
-      {
+      if constexpr (kSigned) {
+#pragma unroll
+        for (int n = 0; n < kTiles; ++n)
+#pragma unroll
+          for (int x = 0; x < 4; ++x) s[n][i][x] = 0.f;
+      } else {
         const uint32_t a = D == 128 && t % 2 ? sa[L::kGroups / 2 - 1] : sa[0], b = D == 128 && t % 2 ? sb[L::kGroups / 2 - 1] : sb[0];
 #pragma unroll
         for (int n = 0; n < kTiles; ++n) {
@@ -236,15 +250,35 @@ struct QueryRows {
       for (int j = 0; j < L::kGroups; ++j) {
         const float fa = j % 2 ? bf_hi(sa[j / 2]) : bf_lo(sa[j / 2]), fb = j % 2 ? bf_hi(sb[j / 2]) : bf_lo(sb[j / 2]);
         const uint32_t a8 = wa[j] >> 8, b8 = wb[j] >> 8;
-        const uint32_t a[4] = {wa[j] & 0x000F000Fu, wa[j] & 0x00F000F0u, a8 & 0x000F000Fu, a8 & 0x00F000F0u};  // codes k and k + 4
-        const uint32_t b[4] = {wb[j] & 0x000F000Fu, wb[j] & 0x00F000F0u, b8 & 0x000F000Fu, b8 & 0x00F000F0u};
+        uint32_t a[4] = {wa[j] & 0x000F000Fu, wa[j] & 0x00F000F0u, a8 & 0x000F000Fu, a8 & 0x00F000F0u};  // codes k and k + 4
+        uint32_t b[4] = {wb[j] & 0x000F000Fu, wb[j] & 0x00F000F0u, b8 & 0x000F000Fu, b8 & 0x00F000F0u};
+        if constexpr (kSigned) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            a[k] = add_bf2(a[k], k % 2 ? 0x80808080u : 0x80088008u);
+            b[k] = add_bf2(b[k], k % 2 ? 0x80808080u : 0x80088008u);
+          }
+        }
 #pragma unroll
         for (int n = 0; n < kTiles; ++n) {
+          // The tensor cores cut a sum off where it would have to be rounded: in fp32 the products with the first pieces, 16 channels each, are
+          // sums of their own, added in 32 bits.
           float x[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-          for (int p = 0; p < kPieces; ++p)
+          for (int p = kPieces - 1; p >= 0; --p)
 #pragma unroll
-            for (int h = 0; h < 2; ++h) mma(x, a[2 * h], b[2 * h], a[2 * h + 1], b[2 * h + 1], q[n][p][j][h][0], q[n][p][j][h][1]);
+            for (int h = 0; h < 2; ++h) {
+              if constexpr (kPieces == 1) {
+                mma(x, a[2 * h], b[2 * h], a[2 * h + 1], b[2 * h + 1], q[n][p][j][h][0], q[n][p][j][h][1]);
+              } else {
+                float y[4] = {0.f, 0.f, 0.f, 0.f};
+                float (&sum)[4] = p > 0 ? x : y;
+                mma(sum, a[2 * h], b[2 * h], a[2 * h + 1], b[2 * h + 1], q[n][p][j][h][0], q[n][p][j][h][1]);
+#pragma unroll
+                for (int z = 0; z < 4; ++z)
+                  if (p == 0) x[z] += y[z];
+              }
+            }
 #pragma unroll
           for (int z = 0; z < 4; ++z) s[n][i][z] = fmaf(x[z], z < 2 ? fa : fb, s[n][i][z]);
         }
