@@ -467,11 +467,13 @@ __global__ void __launch_bounds__(128) cache_join_kernel(CacheAttnArgs a) {
 // More rows than this go to the tcgen05 kernel (bf16).
 constexpr int kManyRows = 32;
 
-// Rows of a CTA: 4 (bf16), 8 or 16; 256 in the tcgen05 kernel.
+// Rows of a CTA: 4 (bf16), 8 or 16; 256 in the tcgen05 kernel.  (fp32 at head_dim 128 has no registers for 16: 2 prompts of 100 documents,
+// 16 rows 47 us, with 8 to a CTA 36; 64 rows 135 and 113.  At head_dim 64 32 rows 35 and 42, 16 rows 23 and 24.)
 int rows_per_cta(const brk_cache_attn_params& p) {
   const int64_t rows = (int64_t)p.Lq * (p.N / p.cache.Nk);
   if (p.dtype == BRK_BF16 && rows > kManyRows) return 256;
-  return rows <= 4 && p.dtype == BRK_BF16 ? 4 : rows <= 8 ? 8 : 16;
+  if (p.dtype == BRK_F32) return rows <= 8 || p.cache.D == 128 ? 8 : 16;
+  return rows <= 4 ? 4 : rows <= 8 ? 8 : 16;
 }
 int64_t row_groups(const brk_cache_attn_params& p) {
   return ((int64_t)p.Lq * (p.N / p.cache.Nk) + rows_per_cta(p) - 1) / rows_per_cta(p);
@@ -544,7 +546,9 @@ int cache_attn_launch(const brk_cache_attn_params& p, void* ws, cudaStream_t st)
   const int per = rows_per_cta(p);
   auto of_head_dim = [&](auto d, std::atomic<bool>(*flags)[64]) -> int {
     constexpr int D = decltype(d)::value;
-    if (f32) return per == 8 ? run(cache_attn_kernel<float, D, 1, false>, flags[0]) : run(cache_attn_kernel<float, D, 2, false>, flags[1]);
+    if constexpr (D == 64)
+      if (f32 && per == 16) return run(cache_attn_kernel<float, D, 2, false>, flags[1]);
+    if (f32) return run(cache_attn_kernel<float, D, 1, false>, flags[0]);
     if (per == 4) return run(cache_attn_kernel<__nv_bfloat16, D, 1, true>, flags[2]);
     return per == 8 ? run(cache_attn_kernel<__nv_bfloat16, D, 1, false>, flags[3]) : run(cache_attn_kernel<__nv_bfloat16, D, 2, false>, flags[4]);
   };
