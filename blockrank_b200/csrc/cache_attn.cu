@@ -25,6 +25,7 @@ using namespace cache;
 
 constexpr int kWarps = 4;
 constexpr int kThreads = 32 * kWarps;
+constexpr int kShare = 128;       // pages a CTA takes at most
 constexpr int kParts = 3;         // K or V parts of pages that a warp has room for in shared memory: two K, one V
 constexpr int kCluster = 8;       // shares that a cluster joins, at most
 
@@ -51,7 +52,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<T, kTiles>) cache_attn_k
   ptx::grid_dependency_wait();  // (inputs of this call; the workspace of the one in front)
 
   typename QueryRows<T, D, kTiles>::Raw raw;
-  const Share sh = find_share<kThreads>(a, b, row0, kRows, share, kWarps, s_mask, s_page, [&] {
+  const Share sh = find_share<kThreads, kShare>(a, b, row0, kRows, share, kWarps, s_mask, s_page, [&] {
     QueryRows<T, D, kTiles>::fetch([&](int c) -> const T* {  // (rows from q_len on among them: they are not used)
       const int r = row0 + (kTwice ? c & 3 : c);
       if (r >= a.Lq * G) return nullptr;
@@ -485,7 +486,7 @@ int shares_of(const brk_cache_attn_params& p) {
   const bool many = rows_per_cta(p) == 256;
   const int per_sm = many ? 1 : p.dtype == BRK_BF16 && rows_per_cta(p) <= 8 ? 3 : 2;
   const int64_t ctas = (int64_t)p.B * p.cache.Nk * row_groups(p), room = per_sm * (int64_t)std::max(1, sm_count());
-  const int64_t least = (p.P + kShare - 1) / kShare, pages = many ? 4 : kWarps;
+  const int64_t largest = many ? kManyShare : kShare, least = (p.P + largest - 1) / largest, pages = many ? 4 : kWarps;
   const int64_t most = std::max<int64_t>(least, std::min<int64_t>(64, (p.P + pages - 1) / pages));
   int64_t best = least, best_cost = INT64_MAX;
   for (int64_t round = 0; round <= 8; ++round) {  // (the most shares of so many rounds, and the fewest)

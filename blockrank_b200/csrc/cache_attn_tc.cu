@@ -20,6 +20,7 @@ namespace {
 
 using namespace cache;
 
+constexpr int kShare = kManyShare;
 constexpr int kTile = 128;                 // rows of a tile
 constexpr int kSoftWarps = 8, kUnpackWarps = 4;
 constexpr int kMmaWarp = kSoftWarps + kUnpackWarps;
@@ -80,7 +81,7 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attn_tc_kernel(CacheAttnArg
   }
   ptx::grid_dependency_launch();
   ptx::grid_dependency_wait();
-  const Share sh = find_share<kThreads>(a, b, row0, 2 * kTile, share, 1, s_mask, s_page, [&] {
+  const Share sh = find_share<kThreads, kShare>(a, b, row0, 2 * kTile, share, 1, s_mask, s_page, [&] {
     // Q as the K-major A operand: rows of 128 bytes, their 16-byte units swizzled
 #pragma unroll 2
     for (int i = tid; i < 2 * kTile * (D / 8); i += kThreads) {

@@ -6,7 +6,7 @@
 namespace brk {
 namespace cache {
 
-constexpr int kShare = 128;  // pages a CTA takes at most
+constexpr int kManyShare = 256;  // pages a CTA of the tcgen05 kernel takes at most
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 struct CacheAttnArgs {
@@ -35,31 +35,21 @@ struct Share {
 };
 
 // Rows row0 .. row0 + max_rows - 1 of prompt b (query heads of a group at one token after the other) against an even share, of at
-// least min_pages, of the pages up to the last row's slot.  s_mask [2 kShare]: which tokens of these pages lie in a block; s_page [kShare]: the pages' numbers,
-// -1 for one without such a token.  The latencies are paid once each: spans and number of rows, with what `meanwhile` requests and the
-// first entries of the page table; the other entries.
-template <int kThreads, typename F>
+// least min_pages, of the pages up to the last row's slot.  s_mask [2 kShare]: which tokens of these pages lie in a block; s_page [kShare]: the pages'
+// numbers, -1 for one without such a token.  The latencies are paid once each: spans and number of rows, with what `meanwhile` requests and
+// the first entries of the page table; the other entries.
+template <int kThreads, int kShare, typename F>
 __device__ __forceinline__ Share find_share(const CacheAttnArgs& a, int b, int row0, int max_rows, int share, int min_pages, uint32_t* s_mask,
                                             int32_t* s_page, F meanwhile) {
-  static_assert(kThreads >= kShare, "a thread per page");
-  __shared__ int32_t s_table[kShare];
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, G = a.N / a.Nk;
+  const int tid = threadIdx.x, G = a.N / a.Nk;
   const int32_t *start = a.blk_start + (int64_t)b * a.M, *len = a.blk_len + (int64_t)b * a.M, *table = a.table + (int64_t)b * a.P;
   const int64_t slots = (int64_t)a.P * kPage;
   const int last_start = start[a.M - 1], last_len = len[a.M - 1], given = a.q_len ? a.q_len[b] : a.Lq;
-  const int early = tid < kShare && tid < a.P ? table[tid] : -1;
+  __shared__ int32_t s_table[kThreads];
+  s_table[tid] = tid < a.P ? table[tid] : -1;
   meanwhile();
-  int my_start = 0, my_len = 0;
-  bool bad = false;
-  if (tid < a.M) {
-    my_start = start[tid];
-    my_len = len[tid];
-    bad = span_is_bad(start, len, tid, slots);
-  }
-  for (int m = tid + kThreads; m < a.M; m += kThreads) bad |= span_is_bad(start, len, m, slots);
-  for (int i = tid; i < 2 * kShare; i += kThreads) s_mask[i] = 0;
-  if (tid < kShare) s_table[tid] = early;
-  bad |= given < 0 || given > a.Lq || given > last_len;
+  bool bad = given < 0 || given > a.Lq || given > last_len;
+  for (int m = tid; m < a.M; m += kThreads) bad |= span_is_bad(start, len, m, slots);
   Share r;
   r.bad = __syncthreads_or(bad);
   if (r.bad && tid == 0 && a.status) atomicCAS(a.status, 0, kStatusBadCacheCall);
@@ -71,34 +61,36 @@ __device__ __forceinline__ Share find_share(const CacheAttnArgs& a, int b, int r
   const int per = max((live + a.shares - 1) / a.shares, min(live, min_pages));
   r.page0 = min(live, share * per);
   r.n = min(live, r.page0 + per) - r.page0;
-  int page = -1;
-  if (tid < r.n) page = r.page0 + tid < kShare ? s_table[r.page0 + tid] : table[r.page0 + tid];
-
-  if (r.n > 0) {
-    const int lo = r.page0 * kPage, hi = (r.page0 + r.n) * kPage;
-    for (int m0 = warp * 32; m0 < a.M; m0 += kThreads) {
-      const int m = m0 + lane;
-      const int s = m0 < kThreads ? my_start : m < a.M ? start[m] : 0, e = s + (m0 < kThreads ? my_len : m < a.M ? len[m] : 0);
-      unsigned todo = __ballot_sync(0xffffffffu, max(s, lo) < min(e, hi));
-      while (todo) {
-        const int src = __ffs(todo) - 1;
-        todo &= todo - 1;
-        const int bs = max(__shfl_sync(0xffffffffu, s, src), lo) - lo, be = min(__shfl_sync(0xffffffffu, e, src), hi) - lo;
-        for (int w = bs / 32 + lane; w * 32 < be; w += 32) {  // a word of 32 tokens per lane
-          const int from = max(bs - w * 32, 0), to = min(be - w * 32, 32);
-          atomicOr(&s_mask[w], (to == 32 ? ~0u : (1u << to) - 1) & (~0u << from));
-        }
+  for (int i = tid; i < r.n; i += kThreads) {
+    const int at = r.page0 + i, lo = at * kPage;
+    int page = at < kThreads ? s_table[at] : table[at];
+    int m = 0;  // the first block that ends behind the page's first token (blocks are in order)
+    for (int size = a.M; size > 0;) {
+      const int half = size / 2;
+      if (start[m + half] + len[m + half] <= lo) {
+        m += half + 1;
+        size -= half + 1;
+      } else {
+        size = half;
       }
     }
-  }
-  __syncthreads();
-  if (tid < r.n) {
-    const bool needed = (s_mask[2 * tid] | s_mask[2 * tid + 1]) != 0;
+    uint32_t w[2] = {0, 0};
+    for (; m < a.M && start[m] < lo + kPage; ++m) {
+      const int from = max(start[m] - lo, 0), to = min(start[m] + len[m] - lo, kPage);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int f = max(from - 32 * h, 0), t = min(to - 32 * h, 32);
+        if (f < t) w[h] |= (t == 32 ? ~0u : (1u << t) - 1) & (~0u << f);
+      }
+    }
+    const bool needed = (w[0] | w[1]) != 0;
     if (needed && (page < 0 || page >= a.n_pages)) {
       if (a.status) atomicCAS(a.status, 0, kStatusBadCacheCall);
       page = -1;
     }
-    s_page[tid] = needed ? page : -1;
+    s_mask[2 * i] = w[0];
+    s_mask[2 * i + 1] = w[1];
+    s_page[i] = needed ? page : -1;
   }
   __syncthreads();
   return r;
