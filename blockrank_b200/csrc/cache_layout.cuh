@@ -63,17 +63,18 @@ __device__ __forceinline__ uint32_t fma_bf2(uint32_t a, uint32_t b, uint32_t c) 
   asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
   return d;
 }
+__device__ __forceinline__ uint32_t mul_bf2(uint32_t a, uint32_t b) {
+  uint32_t d;
+  asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+  return d;
+}
 __device__ __forceinline__ uint32_t add_bf2(uint32_t a, uint32_t b) {
   uint32_t d;
   asm("add.rn.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
   return d;
 }
 // -24 s, for two scales
-__device__ __forceinline__ uint32_t scale_offset(uint32_t s2) {
-  uint32_t d;
-  asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(s2), "r"(0xC1C0C1C0u));
-  return d;
-}
+__device__ __forceinline__ uint32_t scale_offset(uint32_t s2) { return mul_bf2(s2, 0xC1C0C1C0u); }
 // two codes in bits 3..6 and 19..22 of x (others are ignored) -> their values
 __device__ __forceinline__ uint32_t held(const Codes& k, uint32_t x, uint32_t s2, uint32_t c2) {
   return fma_bf2((x & k.mask) | k.base, s2, c2);
@@ -167,39 +168,64 @@ struct QueryRows {
   __device__ __forceinline__ void make(const Raw& raw, int g, int t) {
 #pragma unroll
     for (int n = 0; n < kTiles; ++n) {
-      float x[L::kGroups][8], top = 0.f;
+      // the bits of the row's largest magnitude (NaN is above infinity)
+      uint32_t top = 0;
 #pragma unroll
-      for (int j = 0; j < L::kGroups; ++j) {
-        load8(reinterpret_cast<const T*>(raw.w[n][j]), x[j]);
+      for (int j = 0; j < L::kGroups; ++j)
 #pragma unroll
-        for (int k = 0; k < 8; ++k) top = isnan(x[j][k]) ? INFINITY : fmaxf(top, fabsf(x[j][k]));
-      }
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      // 2^up = 2^120 / 2^(exponent of top), as float exponent fields; in two factors, since it can be 2^246
-      const bool finite = top < INFINITY;
-      const int up = 120 + 127 - (int)max(__float_as_uint(top) >> 23, 1u);
-      const float up0 = __uint_as_float((uint32_t)(up / 2 + 127) << 23), up1 = __uint_as_float((uint32_t)(up - up / 2 + 127) << 23);
+        for (int i = 0; i < (int)sizeof(T) / 2; ++i) {
+          const uint4 w = raw.w[n][j][i];
+          if constexpr (sizeof(T) == 2) {
+            const uint32_t k = 0x7FFF7FFFu;
+            top = __vmaxu2(top, __vmaxu2(__vmaxu2(w.x & k, w.y & k), __vmaxu2(w.z & k, w.w & k)));
+          } else {
+            const uint32_t k = 0x7FFFFFFFu;
+            top = max(top, max(max(w.x & k, w.y & k), max(w.z & k, w.w & k)));
+          }
+        }
+      if constexpr (sizeof(T) == 2) top = max(top & 0xFFFF0000u, top << 16);
+      top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      // 2^up = 2^120 / 2^(exponent of top); in two factors, since it can be 2^246
+      const bool finite = top < 0x7F800000u;
+      const int up = 120 + 127 - (int)max(top >> 23, 1u);
+      const uint32_t up0 = (uint32_t)(up / 2 + 127) << 23, up1 = (uint32_t)(up - up / 2 + 127) << 23;  // (as numbers)
       float total[L::kGroups];
 #pragma unroll
       for (int j = 0; j < L::kGroups; ++j) {
-        total[j] = 0.f;
+        if constexpr (sizeof(T) == 2) {
+          // powers of two leave bf16 as it is: packed
+          const uint32_t u0 = up0 | up0 >> 16, u1 = up1 | up1 >> 16, none = finite ? ~0u : 0u;
+          const uint4 w = raw.w[n][j][0];
+          const uint32_t x[4] = {mul_bf2(mul_bf2(w.x & none, u0), u1), mul_bf2(mul_bf2(w.y & none, u0), u1),
+                                 mul_bf2(mul_bf2(w.z & none, u0), u1), mul_bf2(mul_bf2(w.w & none, u0), u1)};
+          total[j] = ((bf_lo(x[0]) + bf_hi(x[0])) + (bf_lo(x[1]) + bf_hi(x[1]))) + ((bf_lo(x[2]) + bf_hi(x[2])) + (bf_lo(x[3]) + bf_hi(x[3])));
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          x[j][k] = finite ? x[j][k] * up0 * up1 : 0.f;
-          total[j] += x[j][k];
+          for (int h = 0; h < 2; ++h) {
+            q[n][0][j][h][0] = __byte_perm(x[h], x[h + 2], 0x5410);
+            q[n][0][j][h][1] = mul_bf2(__byte_perm(x[h], x[h + 2], 0x7632), 0x3D803D80u);  // 1/16
+          }
+        } else {
+          float x[8];
+          load8(reinterpret_cast<const float*>(raw.w[n][j]), x);
+          total[j] = 0.f;
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            x[k] = finite ? x[k] * __uint_as_float(up0) * __uint_as_float(up1) : 0.f;
+            total[j] += x[k];
+          }
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            uint32_t piece[kPieces];
+            const float f = k % 2 ? 0.0625f : 1.f;
+            split2<kPieces>(x[k] * f, x[k + 4] * f, piece);
+#pragma unroll
+            for (int i = 0; i < kPieces; ++i) q[n][i][j][k / 2][k % 2] = piece[i];
+          }
         }
         total[j] += __shfl_xor_sync(0xffffffffu, total[j], 1);
         total[j] += __shfl_xor_sync(0xffffffffu, total[j], 2);
         total[j] *= -0x1p-126f * 0x1p-4f;  // (about 2^-5)
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          uint32_t piece[kPieces];
-          const float f = k % 2 ? 0.0625f : 1.f;
-          split2<kPieces>(x[j][k] * f, x[j][k + 4] * f, piece);
-#pragma unroll
-          for (int i = 0; i < kPieces; ++i) q[n][i][j][k / 2][k % 2] = piece[i];
-        }
       }
       // The scales stand side by side in A as they do in memory, the groups' four times (D 128) or eight times over.
       uint32_t w[3][L::kGroups / 2];
