@@ -47,12 +47,16 @@ __global__ void __launch_bounds__(kThreads, kTiles == 1 && sizeof(T) == 2 ? 3 : 
   extern __shared__ __align__(16) unsigned char smem[];  // [kWarps][kStages][K part of a page]
   __shared__ float2 s_ml[kWarps][kDocs][kCols];
   __shared__ int s_scan[kWarps], s_before[2];
+  __shared__ int2 s_span[kThreads];      // (start, length) of the first documents
+  __shared__ int32_t s_table[kThreads];  // the first page numbers
   ptx::grid_dependency_wait();
   ptx::grid_dependency_launch();
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
   const int b = blockIdx.y / a.Nk, kvh = blockIdx.y % a.Nk, row0 = blockIdx.z * kCols;
   const int G = a.N / a.Nk, GR = G * a.R, nd = a.M - 2;
   const int32_t *const bs = a.blk_start + (int64_t)b * a.M, *const bl = a.blk_len + (int64_t)b * a.M;
+
+  const int32_t* const table = a.table + (int64_t)b * a.P;
 
   // document d's span (length 0 if it is malformed) and its pages
   auto span = [&](int d, int& start, int& len) {
@@ -62,8 +66,8 @@ __global__ void __launch_bounds__(kThreads, kTiles == 1 && sizeof(T) == 2 ? 3 : 
       if (a.status) atomicCAS(a.status, 0, kStatusBadCacheCall);
       len = 0;
     }
-    return len > 0 ? (start + len - 1) / kPage - start / kPage + 1 : 0;
   };
+  auto pages_of = [](int start, int len) { return len > 0 ? (start + len - 1) / kPage - start / kPage + 1 : 0; };
   auto warp_scan = [&](int x) {
 #pragma unroll
     for (int off = 1; off < 32; off <<= 1) {
@@ -75,23 +79,27 @@ __global__ void __launch_bounds__(kThreads, kTiles == 1 && sizeof(T) == 2 ? 3 : 
 
   // ---- this CTA's documents: those whose first page is in its share of all documents' pages ----
   int my_start = 0, my_len = 0;
-  const int n0 = tid < nd ? span(tid, my_start, my_len) : 0;
+  s_table[tid] = tid < a.P ? table[tid] : -1;
+  if (tid < nd) span(tid, my_start, my_len);
+  s_span[tid] = make_int2(my_start, my_len);
   typename QueryRows<T, D, kTiles>::Raw raw;
   QueryRows<T, D, kTiles>::fetch([&](int c) -> const T* {
     const int r = row0 + c;
     if (r >= GR) return nullptr;
     return reinterpret_cast<const T*>(a.q.ptr) + (int64_t)b * a.q.sb + (int64_t)(kvh * G + r / a.R) * a.q.sh + (int64_t)(r % a.R) * a.q.ss;
   }, g, t, raw);
-  int64_t total = 0, lo = 0, hi = 0;
+  int64_t lo = 0, hi = 0;
   if (tid < 2) s_before[tid] = 0;
+  // All pages (pass 0); then the number of documents that begin before the share, and before its end.  Up to kThreads documents are
+  // looked at once.
 #pragma unroll 1
-  for (int pass = 0; pass < 2; ++pass) {  // all pages; then the number of documents that begin before the share, and before its end
+  for (int pass = 0; pass < 2; ++pass) {
     int64_t before = 0;
 #pragma unroll 1
     for (int d0 = 0; d0 < nd; d0 += kThreads) {
-      int s, l;
-      const int n = d0 == 0 ? n0 : d0 + tid < nd ? span(d0 + tid, s, l) : 0;
-      const int x = warp_scan(n);
+      int st = my_start, ln = my_len;
+      if (d0 > 0 && d0 + tid < nd) span(d0 + tid, st, ln);
+      const int n = d0 + tid < nd ? pages_of(st, ln) : 0, x = warp_scan(n);
       if (lane == 31) s_scan[warp] = x;
       __syncthreads();
       int sum = 0, first = x - n;
@@ -100,21 +108,26 @@ __global__ void __launch_bounds__(kThreads, kTiles == 1 && sizeof(T) == 2 ? 3 : 
         if (w < warp) first += s_scan[w];
         sum += s_scan[w];
       }
-      if (pass == 1) {
+      const bool only = nd <= kThreads;
+      if (only) {
+        lo = (int64_t)sum * blockIdx.x / gridDim.x;
+        hi = (int64_t)sum * (blockIdx.x + 1) / gridDim.x;
+      }
+      if (pass == 1 || only) {
         const unsigned below = __ballot_sync(0xffffffffu, d0 + tid < nd && before + first < lo);
         const unsigned below_end = __ballot_sync(0xffffffffu, d0 + tid < nd && (before + first < hi || blockIdx.x + 1 == gridDim.x));
         if (lane == 0) {
           atomicAdd(&s_before[0], __popc(below));
           atomicAdd(&s_before[1], __popc(below_end));
         }
+        if (only) pass = 1;
       }
       before += sum;
       __syncthreads();
     }
     if (pass == 0) {
-      total = before;
-      lo = total * blockIdx.x / gridDim.x;
-      hi = total * (blockIdx.x + 1) / gridDim.x;
+      lo = before * blockIdx.x / gridDim.x;
+      hi = before * (blockIdx.x + 1) / gridDim.x;
     }
   }
   const int doc_end = s_before[1];
@@ -132,13 +145,21 @@ __global__ void __launch_bounds__(kThreads, kTiles == 1 && sizeof(T) == 2 ? 3 : 
     }
   unsigned char* const ring = smem + warp * kStages * L::kHalf;
   const unsigned char* const head = a.pages + (int64_t)kvh * L::kBytes;
-  const int32_t* const table = a.table + (int64_t)b * a.P;
+  auto page_number = [&](int i) { return i < kThreads ? s_table[i] : table[i]; };
 
 #pragma unroll 1
   for (int doc0 = s_before[0]; doc0 < doc_end; doc0 += kDocs) {
     const int n_docs = min(kDocs, doc_end - doc0);
     int start = 0, len = 0;  // lane l: of document doc0 + l
-    const int n = lane < n_docs ? span(doc0 + lane, start, len) : 0;
+    if (lane < n_docs) {
+      if (doc0 + lane < kThreads) {
+        start = s_span[doc0 + lane].x;
+        len = s_span[doc0 + lane].y;
+      } else {
+        span(doc0 + lane, start, len);
+      }
+    }
+    const int n = pages_of(start, len);
     const int end = warp_scan(n), pages = __shfl_sync(0xffffffffu, end, 31);
     const int from = (int)((int64_t)pages * warp / kWarps), to = (int)((int64_t)pages * (warp + 1) / kWarps);
     for (int i = lane; i < kDocs * kCols; i += 32) (&s_ml[warp][0][0])[i] = make_float2(-INFINITY, 0.f);
@@ -165,13 +186,13 @@ __global__ void __launch_bounds__(kThreads, kTiles == 1 && sizeof(T) == 2 ? 3 : 
       enter(ahead);
       here = ahead;
     }
-    int id = from < to ? table[ahead.slot0 / kPage] : 0;
+    int id = from < to ? page_number(ahead.slot0 / kPage) : 0;
     uint32_t absent = 0;  // bit s: the page in stage s does not exist
     auto request = [&](int stage) {
       if (ahead.at < to) {
         const int page = id;
         step(ahead);
-        if (ahead.at < to) id = table[ahead.slot0 / kPage];
+        if (ahead.at < to) id = page_number(ahead.slot0 / kPage);
         if (page >= 0 && page < a.n_pages) {
           absent &= ~(1u << stage);
           const unsigned char* src = head + (int64_t)page * a.Nk * L::kBytes;
