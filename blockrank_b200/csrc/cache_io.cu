@@ -151,14 +151,14 @@ constexpr int kTile = 32;  // tokens of a CTA, at most
 constexpr int kScan = 1024;
 
 __global__ void __launch_bounds__(256) owner_clear_kernel(const int32_t* slots, int tokens, int64_t n_slots, int32_t* owner) {
-  const int i = blockIdx.x * blockDim.x + threadIdx.x;
+  const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
   ptx::grid_dependency_wait();
   if (i < tokens && slots[i] >= 0 && slots[i] < n_slots) owner[slots[i]] = -1;
 }
 __global__ void __launch_bounds__(256) owner_claim_kernel(const int32_t* slots, int tokens, int64_t n_slots, int32_t* owner) {
-  const int i = blockIdx.x * blockDim.x + threadIdx.x;
+  const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
   ptx::grid_dependency_wait();
-  if (i < tokens && slots[i] >= 0 && slots[i] < n_slots) atomicMax(owner + slots[i], i);
+  if (i < tokens && slots[i] >= 0 && slots[i] < n_slots) atomicMax(owner + slots[i], (int)i);
 }
 
 // Where the CTA's tokens are: element offsets of their rows in k and v, and the byte offset of head 0's page and the place in it

@@ -316,6 +316,25 @@ def test_document_scores(dtype, N, Nk, D, R, name, paged):
     ops.check_status()
 
 
+@pytest.mark.parametrize("paged", [True, False])
+def test_scores_of_very_many_documents(paged):
+    """More than a CTA looks at in one go, most of them short, some empty, one long."""
+    N, Nk, D, R = 4, 2, 64, 2
+    g = torch.Generator().manual_seed(3)
+    lens = [torch.randint(0, 12, (330,), generator=g).tolist() for _ in range(2)]
+    lens[0][17], lens[1][300], lens[1][301] = 900, 2000, 0
+    lens = [[7] + x + [5] for x in lens]
+    start, length, P = ch.spans(lens, paged)
+    cache, hk, _ = _filled(2 * P, Nk, D, 151)
+    table = _table(2, P, 2 * P, 17)
+    q = _rand(2, R, N, D, seed=18, dtype=BF16).transpose(1, 2)
+    mass, logits = ops.cache_doc_scores(q.cuda(), cache, table.cuda(), start.cuda(), length.cuda(), 0.1, 2000)
+    ref = ch.doc_mass(q, hk, table, start, length, 0.1)
+    assert torch.allclose(mass.double().cpu(), ref, rtol=1e-4, atol=1e-9)
+    assert torch.allclose(logits.double().cpu(), ref.mean((1, 2)) / 0.05, rtol=1e-4, atol=1e-8)
+    ops.check_status()
+
+
 def test_document_scores_are_those_of_the_values_read_back():
     """The cached epilogue against the uncached one on the same numbers."""
     N, Nk, D, R = 32, 8, 128, 2
@@ -553,3 +572,186 @@ def test_logits_that_keep_growing():
         out, lse = ops.cache_attention(q.cuda(), cache, table.cuda(), start.cuda(), length.cuda(), 0.05, return_lse=True)
         ref, ref_lse, size = ch.attention(q, hk, hv, table, start, length, 0.05)
         _check(out, lse, ref, ref_lse, size, hv, 64)
+
+
+@pytest.mark.parametrize("dtype,N,Nk,D,rows", [(BF16, 8, 2, 128, 130), (BF16, 20, 1, 64, 33), (F32, 8, 2, 64, 40), (BF16, 64, 1, 128, 1)])
+def test_more_rows_than_a_cta_takes(dtype, N, Nk, D, rows):
+    """Several CTAs' rows, their borders inside a token's heads; a prompt without rows, one with fewer than the others."""
+    lens = [[40, 130, 0, 61, rows + 2], [3, 5, 64, 1, rows], [1, 700, 2, 2, rows]]
+    start, length, P = ch.spans(lens, True)
+    cache, hk, hv = _filled(3 * P, Nk, D, 161, dtype)
+    table = _table(3, P, 3 * P, 18)
+    q_len = torch.tensor([rows, 0, max(1, rows - 9)], dtype=torch.int32)
+    q = _rand(3, rows, N, D, seed=19, dtype=dtype).transpose(1, 2)
+    out, lse = ops.cache_attention(q.cuda(), cache, table.cuda(), start.cuda(), length.cuda(), D ** -0.5, q_len=q_len.cuda(), return_lse=True)
+    ref, ref_lse, size = ch.attention(q, hk, hv, table, start, length, D ** -0.5, q_len)
+    _check(out, lse, ref, ref_lse, size, hv, 3 * P + 8)
+    ops.check_status()
+
+
+@pytest.mark.parametrize("dtype,rows", [(BF16, 1), (BF16, 9), (BF16, 20), (F32, 3)])
+def test_more_blocks_than_a_cta_has_threads(dtype, rows):
+    N, Nk, D = 4, 2, 64
+    g = torch.Generator().manual_seed(4)
+    lens = [[9] + torch.randint(0, 20, (498,), generator=g).tolist() + [rows] for _ in range(2)]
+    start, length, P = ch.spans(lens, False, gap=1)
+    cache, hk, hv = _filled(2 * P, Nk, D, 171, dtype)
+    table = _table(2, P, 2 * P, 20)
+    q = _rand(2, rows, N, D, seed=21, dtype=dtype).transpose(1, 2)
+    out, lse = ops.cache_attention(q.cuda(), cache, table.cuda(), start.cuda(), length.cuda(), 0.1, return_lse=True)
+    ref, ref_lse, size = ch.attention(q, hk, hv, table, start, length, 0.1)
+    _check(out, lse, ref, ref_lse, size, hv, 3 * P + 8)
+    ops.check_status()
+
+
+def test_a_long_list_of_short_prompts():
+    N, Nk, D, B = 4, 2, 64, 600
+    lens = [[1 + b % 70] for b in range(B)]
+    start, length, P = ch.spans(lens, False)
+    cache, hk, hv = _filled(200, Nk, D, 181)
+    table = torch.randint(0, 200, (B, P), generator=torch.Generator().manual_seed(5), dtype=torch.int32)  # (prompts share pages)
+    q = _rand(B, 1, N, D, seed=22, dtype=BF16).transpose(1, 2)
+    out, lse = ops.cache_attention(q.cuda(), cache, table.cuda(), start.cuda(), length.cuda(), 0.1, return_lse=True)
+    ref, ref_lse, size = ch.attention(q, hk, hv, table, start, length, 0.1)
+    _check(out, lse, ref, ref_lse, size, hv, 64)
+
+
+@pytest.mark.parametrize("dtype,rows,width", [(BF16, 2, 1), (BF16, 40, 1), (BF16, 2, 4000), (BF16, 40, 4000), (F32, 2, 1), (F32, 40, 4000)])
+def test_rows_that_see_nothing(dtype, rows, width):
+    """No page of the prompt exists: zeros and -inf, no NaN; the prompts next to it are whole.  Wide tables: parts joined by a kernel."""
+    N, Nk, D, B = 4, 2, 64, 4
+    start, length, P = ch.spans([[3, 70, rows]] * B, True)
+    cache, hk, hv = _filled(B * P, Nk, D, 191, dtype)
+    table = torch.full((B, max(P, width)), -1, dtype=torch.int32)
+    table[:, :P] = _table(B, P, B * P, 23)
+    table[1, :P] = -7
+    table[2, :P] = B * P + 5
+    q = _rand(B, rows, N, D, seed=24, dtype=dtype).transpose(1, 2)
+    ops.check_status()
+    out, lse = ops.cache_attention(q.cuda(), cache, table.cuda(), start.cuda(), length.cuda(), 0.1, return_lse=True)
+    with pytest.raises(ValueError, match="of a call on the cache"):
+        ops.check_status()
+    mass, logits = ops.cache_doc_scores(q[:, :, :2].cuda(), cache, table.cuda(), start.cuda(), length.cuda(), 0.1, 70)
+    with pytest.raises(ValueError, match="of a call on the cache"):
+        ops.check_status()
+    assert not out[1:3].any() and (lse[1:3] == -torch.inf).all() and not mass[1:3].any() and not logits[1:3].any()
+    length[1:3] = 0
+    start[1:3] = 0
+    q_len = torch.tensor([rows, 0, 0, rows], dtype=torch.int32)
+    ref, ref_lse, size = ch.attention(q, hk, hv, table, start, length, 0.1, q_len)
+    _check(out, lse, ref, ref_lse, size, hv, 64)
+    want = ch.doc_mass(q[:, :, :2], hk, table, start, length, 0.1)
+    assert torch.allclose(mass.double().cpu(), want, rtol=1e-4)
+
+
+@pytest.mark.parametrize("width", [1, 4000])
+def test_malformed_prompts_of_many_rows(width):
+    N, Nk, D, B, rows = 4, 2, 64, 5, 40
+    start, length, P = ch.spans([[3, 70, rows + 2]] * B, True)
+    cache, hk, hv = _filled(B * P, Nk, D, 201)
+    table = torch.full((B, max(P, width)), -1, dtype=torch.int32)
+    table[:, :P] = _table(B, P, B * P, 25)
+    start[1, 1] = 2
+    length[2, 2] = 2 ** 31 - 1
+    length[3, 1] = -1
+    q_len = torch.tensor([rows, rows, rows, rows, rows + 3], dtype=torch.int32)
+    q = _rand(B, rows + 5, N, D, seed=26, dtype=BF16).transpose(1, 2)
+    ops.check_status()
+    out, lse = ops.cache_attention(q.cuda(), cache, table.cuda(), start.cuda(), length.cuda(), 0.1, q_len=q_len.cuda(), return_lse=True)
+    with pytest.raises(ValueError, match="of a call on the cache"):
+        ops.check_status()
+    assert not out[1:].any() and (lse[1:] == -torch.inf).all()
+    ref, ref_lse, size = ch.attention(q[:1], hk, hv, table[:1], start[:1], length[:1], 0.1, q_len[:1])
+    _check(out[:1], lse[:1], ref, ref_lse, size, hv, 64)
+
+
+def test_captured_prompts_replay_on_new_inputs():
+    """Calls that take workspaces, as one graph: over a thousand tokens written, read back, a block of many rows over a wide table, one row
+    over a long one, scores."""
+    N, Nk, D, B, rows = 8, 2, 128, 2, 40
+    start, length, P = ch.spans([[30, 500, 300, rows], [30, 64, 700, rows]], True)
+    S = P * PAGE
+    st, ln = start.cuda(), length.cuda()
+    table = torch.full((B, 4000), -1, dtype=torch.int32)
+    table[:, :P] = _table(B, P, B * P, 27)
+    tab = table.cuda()
+    cache = ops.cache_alloc(B * P, Nk, D, "cuda")
+    slots = torch.stack([ch.slots_of(table[b], torch.arange(S)) for b in range(B)]).int().cuda()
+    k, v = (torch.zeros(B, S, Nk, D, dtype=BF16, device="cuda").transpose(1, 2) for _ in range(2))
+    q = torch.zeros(B, rows, N, D, dtype=BF16, device="cuda").transpose(1, 2)
+    ops.status_word("cuda")
+
+    def run():
+        ops.cache_write(k, v, cache, slots)
+        ck, _ = ops.cache_read(cache, slots)
+        return (ck, ops.cache_attention(q, cache, tab, st, ln, 0.1), ops.cache_attention(q[:, :, :1], cache, tab, st, ln, 0.1),
+                ops.cache_doc_scores(q[:, :, :2], cache, tab, st, ln, 0.1, 700)[0])
+    with torch.cuda.stream(torch.cuda.Stream()):
+        run()
+    torch.cuda.synchronize()
+    graphs = []
+    for _ in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = run()
+        graphs.append((graph, out))
+    for i in range(4):
+        nk, nv = (_rand(B, S, Nk, D, seed=50 + 2 * i + j, dtype=BF16) for j in range(2))
+        nq = _rand(B, rows, N, D, seed=60 + i, dtype=BF16).transpose(1, 2)
+        for dst, src in ((k, nk.transpose(1, 2)), (v, nv.transpose(1, 2)), (q, nq)):
+            dst.copy_(src)
+        graph, (ck, many, one, mass) = graphs[i % 2]
+        graph.replay()
+        assert torch.equal(ck.double().cpu(), ch.held(nk).transpose(1, 2))
+        hk, hv = (torch.zeros(B * P * PAGE, Nk, D, dtype=torch.float64) for _ in range(2))
+        hk[slots.cpu().long().flatten()], hv[slots.cpu().long().flatten()] = ch.held(nk).flatten(0, 1), ch.held(nv).flatten(0, 1)
+        for got, x in ((many, nq), (one, nq[:, :, :1])):
+            ref, _, size = ch.attention(x, hk, hv, table, start, length, 0.1)
+            _check(got, None, ref, None, size, hv, 3 * P + 8)
+        assert torch.allclose(mass.double().cpu(), ch.doc_mass(nq[:, :, :2], hk, table, start, length, 0.1), rtol=1e-3, atol=1e-6)
+    ops.check_status()
+
+
+def test_calls_with_workspaces_on_two_streams_at_once():
+    N, Nk, D, rows = 8, 2, 128, 40
+    start, length, P = ch.spans([[30, 900, rows]], True)
+    table = torch.full((1, 4000), -1, dtype=torch.int32)
+    table[:, :P] = torch.arange(P, dtype=torch.int32)
+    T = P * PAGE
+    slots = torch.arange(T, dtype=torch.int32)[None].repeat(1, 2)  # every slot twice: the second counts
+    data = []
+    for i in range(2):
+        k, v = (_rand(1, 2 * T, Nk, D, seed=70 + 2 * i + j, dtype=BF16) for j in range(2))
+        q = _rand(1, rows, N, D, seed=80 + i, dtype=BF16).transpose(1, 2)
+        data.append((k, v, q, ops.cache_alloc(P, Nk, D, "cuda"), k.cuda().transpose(1, 2), v.cuda().transpose(1, 2), q.cuda()))
+    st, ln, tab, sl = start.cuda(), length.cuda(), table.cuda(), slots.cuda()
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    outs = [[], []]
+    for _ in range(10):
+        for i, (_, _, _, cache, k, v, q) in enumerate(data):
+            with torch.cuda.stream(streams[i]):
+                ops.cache_write(k, v, cache, sl)
+                outs[i].append((ops.cache_attention(q, cache, tab, st, ln, 0.1), ops.cache_attention(q[:, :, :1], cache, tab, st, ln, 0.1)))
+    torch.cuda.synchronize()
+    for i, (k, v, q, *_) in enumerate(data):
+        hk, hv = ch.held(k)[0, T:], ch.held(v)[0, T:]
+        for n, x in enumerate((q, q[:, :, :1])):
+            for out in outs[i]:
+                assert torch.equal(out[n], outs[i][0][n])
+            ref, _, size = ch.attention(x, hk, hv, table, start, length, 0.1)
+            _check(outs[i][0][n], None, ref, None, size, hv, 3 * P + 8)
+    ops.check_status()
+
+
+def test_very_many_heads():
+    Nk, D, S = 300, 64, 5
+    k, v = (_rand(1, S, Nk, D, seed=90 + i, dtype=BF16) for i in range(2))
+    cache = ops.cache_alloc(2, Nk, D, "cuda")
+    slots = torch.tensor([[70, 3, -1, 127, 64]], dtype=torch.int32)
+    ops.cache_write(k.cuda().transpose(1, 2), v.cuda().transpose(1, 2), cache, slots.cuda())
+    gk, gv = ops.cache_read(cache, slots.cuda(), F32)
+    keep = (slots >= 0)[:, None, :, None]
+    assert torch.equal(gk.double().cpu(), torch.where(keep, ch.held(k).transpose(1, 2), 0.0))
+    assert torch.equal(gv.double().cpu(), torch.where(keep, ch.held(v).transpose(1, 2), 0.0))
+    ops.check_status()
