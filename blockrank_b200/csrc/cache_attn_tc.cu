@@ -4,8 +4,16 @@
 // tiles of 128.  Per page: four warps bring the codes out of the cache and write n s, exact in bf16, as the K and V operands
 // (128-byte swizzle); one thread issues S = Q K^T and O += P V per tile; a thread per row makes P from S in tensor memory, in two
 // bf16 parts (16 bits) that take the place of the 64 logits.  S is held twice, K and V three times, so that a page's Q K^T runs while
-// the softmax is at the page before and the next one is being unpacked.
-// 128 x 64 x D products three times per tile and page (S once, P in two parts); the softmax's instructions come second.
+// the softmax is at the page before and the next one is being unpacked.  With up to 128 rows both groups of softmax threads work on the
+// one tile, at every other page each, and put their outputs together at the end.
+//
+// Channels stand in K and V in whatever order the codes come out in, without a permutation: Q's are brought into K's order once, O's
+// columns are given their names as they are written.
+//
+// Bound by the integer instructions of softmax and unpacking together (of a page's 2,350 cycles with two tiles about 1,700; the products
+// take 1,950 of them beside it): 4 prompts of 100 documents of 160 tokens, 45 tokens by 4 heads in the longest: 110 us.  On the way there:
+// products issued in a loop 131 us, unrolled 125; Q by asynchronous copies 120.6; one tile by both groups, outputs through
+// shared memory 117; no permutations 110.  (Q in tensor memory, one S to a tile: 124 where this took 125.)
 //
 // Tensor memory: per tile S (64 columns) twice and O (D columns).  Shared memory at head_dim 128: Q 64 KB, K and V 3 x 32 KB, codes on
 // their way 4 x 12 KB.
@@ -49,6 +57,10 @@ __device__ __forceinline__ void cp_async(void* dst, const void* src) {
   if constexpr (kBytes == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(d), "l"(src) : "memory");
   else asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(d), "l"(src), "n"(kBytes) : "memory");
 }
+// 16 bytes, or zeros
+__device__ __forceinline__ void cp_async_or_zero(uint32_t dst, const void* src, bool there) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
+}
 __device__ __forceinline__ uint32_t low_part(uint32_t hi, float x, float y) { return pack_bf16(x - bf_lo(hi), y - bf_hi(hi)); }
 
 template <int D>
@@ -81,26 +93,45 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attn_tc_kernel(CacheAttnArg
   }
   ptx::grid_dependency_launch();
   ptx::grid_dependency_wait();
+  constexpr int kQUnits = D / 8, kQStep = kThreads / kQUnits;  // 16 bytes of a row to a thread
+  const int q_unit = tid % kQUnits;
+  auto q_place = [&](int rr) {
+    return smem + (rr / kTile) * SM::kQ + (q_unit >> 3) * SM::kQChunk + (rr % kTile) * 128 + (((q_unit & 7) ^ (rr & 7)) << 4);
+  };
   const Share sh = find_share<kThreads, kShare>(a, b, row0, 2 * kTile, share, 1, s_mask, s_page, [&] {
     // Q as the K-major A operand: rows of 128 bytes, their 16-byte units swizzled
-#pragma unroll 2
-    for (int i = tid; i < 2 * kTile * (D / 8); i += kThreads) {
-      const int u = i % (D / 8), rr = i / (D / 8), r = row0 + rr;
-      uint4 x = make_uint4(0, 0, 0, 0);
-      if (r < a.Lq * G)
-        x = *reinterpret_cast<const uint4*>(reinterpret_cast<const __nv_bfloat16*>(a.q.ptr) + (int64_t)b * a.q.sb +
-                                            (int64_t)(kvh * G + r % G) * a.q.sh + (int64_t)(r / G) * a.q.ss + 8 * u);
-      *reinterpret_cast<uint4*>(smem + (rr / kTile) * SM::kQ + (u >> 3) * SM::kQChunk + (rr % kTile) * 128 + (((u & 7) ^ (rr & 7)) << 4)) = x;
+    const __nv_bfloat16* const q = reinterpret_cast<const __nv_bfloat16*>(a.q.ptr);
+    const int step_tok = kQStep / G, step_head = kQStep % G;
+    int tok = (row0 + tid / kQUnits) / G, head = (row0 + tid / kQUnits) % G;
+#pragma unroll 1
+    for (int rr = tid / kQUnits; rr < 2 * kTile; rr += kQStep) {
+      const bool there = tok < a.Lq;
+      cp_async_or_zero(ptx::smem_u32(q_place(rr)),
+                       there ? q + (int64_t)b * a.q.sb + (int64_t)(kvh * G + head) * a.q.sh + (int64_t)tok * a.q.ss + 8 * q_unit : q, there);
+      tok += step_tok;
+      head += step_head;
+      if (head >= G) {
+        head -= G;
+        ++tok;
+      }
     }
+    cp_async_commit();
   });
   if (warp == 0) {
     int live = 0;
-    for (int i = lane; i < kShare; i += 32) {
+    for (int i = lane; i - lane < sh.n; i += 32) {
       const unsigned there = __ballot_sync(0xffffffffu, i < sh.n && s_page[i] >= 0);
       if (i < sh.n && s_page[i] >= 0) s_list[live + __popc(there & ((1u << lane) - 1))] = i;
       live += __popc(there);
     }
     if (lane == 0) s_live = live;
+  }
+  cp_async_wait<0>();
+#pragma unroll 2
+  for (int rr = tid / kQUnits; rr < 2 * kTile; rr += kQStep) {  // (what this thread has copied) channels in the order of K's
+    uint4* const p = reinterpret_cast<uint4*>(q_place(rr));
+    const uint4 x = *p;
+    *p = make_uint4(__byte_perm(x.x, x.z, 0x5410), __byte_perm(x.x, x.z, 0x7632), __byte_perm(x.y, x.w, 0x5410), __byte_perm(x.y, x.w, 0x7632));
   }
   ptx::fence_proxy_async_smem();
   ptx::tc_fence_before_sync();
@@ -108,32 +139,33 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attn_tc_kernel(CacheAttnArg
   ptx::tc_fence_after_sync();
   const uint32_t tmem = *tmem_slot;
   const int live = s_live;
-  const int tiles = sh.n_rows > kTile ? 2 : 1;
+  const bool split = sh.n_rows <= kTile;  // one tile: the softmax groups take its pages in turn
   const int first_lim = sh.first_slot + row0 / G;  // the last slot that the CTA's first row sees
   ptx::BoundedWaits waits(kWaitBudget);
   auto wait = [&](int i, uint32_t parity) { waits(bar(i), parity & 1u, 1); };
 
   if (warp < kSoftWarps) {
     // =============================== softmax: a thread per row ===========================================
-    const int x = warp >> 2, rr = tid & (kTile - 1), r = row0 + x * kTile + rr, tok = r / G, hd = kvh * G + r % G;
-    const bool there = x * kTile + rr < sh.n_rows;
+    const int x = warp >> 2, rr = tid & (kTile - 1);
+    int r = row0 + (split ? rr : tid);  // the thread's row
+    bool there = r - row0 < sh.n_rows;
     const uint32_t tm = tmem + ((uint32_t)((warp & 3) * 32) << 16) + (uint32_t)x * kTileCols;
-    const int lim = sh.first_slot + tok;
+    const int lim = sh.first_slot + r / G;
     const float sl2 = a.scale * kLog2e;
     float m_run = -INFINITY, l_run = 0.f;
     unsigned poison = 0;  // groups of channels in which this row has seen NaN
-    const int pages = x < tiles ? live : 0;
+    int pages = split ? (live + 1 - x) / 2 : live;
 #pragma unroll 1
-    for (int k = 0; k < pages; ++k) {
-      const int i = s_list[k], slot0 = (sh.page0 + i) * kPage;
+    for (int j = 0; j < pages; ++j) {
+      const int k = split ? 2 * j + x : j, i = s_list[k], slot0 = (sh.page0 + i) * kPage;
       unsigned v0 = s_mask[2 * i], v1 = s_mask[2 * i + 1];
       const bool late = slot0 + kPage - 1 > first_lim;
-      wait(kSFull + 2 * x + (k & 1), k >> 1);
+      wait(kSFull + 2 * x + (j & 1), j >> 1);
       ptx::tc_fence_after_sync();
       __syncwarp();
       uint32_t sr[64];
-      ptx::tmem_ld32(tm + (uint32_t)(k & 1) * 64, *reinterpret_cast<uint32_t (*)[32]>(&sr[0]));
-      ptx::tmem_ld32(tm + (uint32_t)(k & 1) * 64 + 32, *reinterpret_cast<uint32_t (*)[32]>(&sr[32]));
+      ptx::tmem_ld32(tm + (uint32_t)(j & 1) * 64, *reinterpret_cast<uint32_t (*)[32]>(&sr[0]));
+      ptx::tmem_ld32(tm + (uint32_t)(j & 1) * 64 + 32, *reinterpret_cast<uint32_t (*)[32]>(&sr[32]));
       ptx::tmem_wait_ld(sr);
       if (late || (v0 & v1) != ~0u) {  // (warp-uniform)
         if (late) {
@@ -142,8 +174,8 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attn_tc_kernel(CacheAttnArg
           v1 &= n >= 64 ? ~0u : n > 32 ? (1u << (n - 32)) - 1u : 0u;
           wait(kKVFull + k % kBufs, k / kBufs);  // (long since: what the unpacking warps wrote beside K and V is visible behind it)
 #pragma unroll
-          for (int j = 0; j < kG; ++j)
-            if ((s_nan[k % kBufs][j][0] & v0) | (s_nan[k % kBufs][j][1] & v1)) poison |= 1u << j;
+          for (int c = 0; c < kG; ++c)
+            if ((s_nan[k % kBufs][c][0] & v0) | (s_nan[k % kBufs][c][1] & v1)) poison |= 1u << c;
           __syncwarp();
         }
 #pragma unroll
@@ -171,10 +203,10 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attn_tc_kernel(CacheAttnArg
         hi[c >> 1] = pack_bf16(p0, p1);
         lo[c >> 1] = low_part(hi[c >> 1], p0, p1);
       }
-      ptx::tmem_st32(tm + (uint32_t)(k & 1) * 64, hi);
-      ptx::tmem_st32(tm + (uint32_t)(k & 1) * 64 + 32, lo);
-      if (k > 0 && __any_sync(0xffffffffu, changed)) {  // (rare)
-        wait(kODone + 2 * x + ((k - 1) & 1), (k - 1) >> 1);
+      ptx::tmem_st32(tm + (uint32_t)(j & 1) * 64, hi);
+      ptx::tmem_st32(tm + (uint32_t)(j & 1) * 64 + 32, lo);
+      if (j > 0 && __any_sync(0xffffffffu, changed)) {  // (rare)
+        wait(kODone + 2 * x + ((j - 1) & 1), (j - 1) >> 1);
         ptx::tc_fence_after_sync();
         __syncwarp();
 #pragma unroll 1
@@ -194,52 +226,123 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attn_tc_kernel(CacheAttnArg
       ptx::tmem_wait_st();
       ptx::tc_fence_before_sync();
       __syncwarp();
-      ptx::mbar_arrive_warp(bar(kPFull + 2 * x + (k & 1)));
+      ptx::mbar_arrive_warp(bar(kPFull + 2 * x + (j & 1)));
     }
-    // ---- output ----
     if (pages > 0) {
       wait(kODone + 2 * x + ((pages - 1) & 1), (pages - 1) >> 1);
       ptx::tc_fence_after_sync();
       __syncwarp();
     }
+    // ---- the groups' parts of one tile: the second's through the place of K and V into the first's ----
+    float4* const box = reinterpret_cast<float4*>(smem + SM::kKV);  // [D / 4][kTile]
+    float4* const box_ml = box + D / 4 * kTile;                    // [kTile]: maximum, sum, groups with NaN
+    float f0 = 1.f, f1 = 0.f;
+    if (split) {
+      asm volatile("bar.sync 2, 256;" ::: "memory");  // (every product has been made)
+      if (x == 1) {
+#pragma unroll 1
+        for (int ch = 0; ch < D / 32; ++ch) {
+          uint32_t o[32];
+          if (pages > 0) {
+            ptx::tmem_ld32(tm + kColO + (uint32_t)ch * 32, o);
+            ptx::tmem_wait_ld(o);
+          } else {
+#pragma unroll
+            for (int c = 0; c < 32; ++c) o[c] = 0;
+          }
+#pragma unroll
+          for (int c = 0; c < 32; c += 4)
+            box[(ch * 8 + c / 4) * kTile + rr] =
+                make_float4(__uint_as_float(o[c]), __uint_as_float(o[c + 1]), __uint_as_float(o[c + 2]), __uint_as_float(o[c + 3]));
+        }
+        box_ml[rr] = make_float4(m_run, l_run, __uint_as_float(poison), 0.f);
+      }
+      asm volatile("bar.sync 2, 256;" ::: "memory");
+      if (x == 0) {
+        const float4 other = box_ml[rr];
+        const float top = fmaxf(m_run, other.x), ref = top == -INFINITY ? 0.f : top;
+        f0 = ptx::ex2(m_run - ref);
+        f1 = ptx::ex2(other.x - ref);
+        m_run = top;
+        l_run = l_run * f0 + other.y * f1;
+        poison |= __float_as_uint(other.z);
+      } else {  // a row that is not there
+        r = row0 + tid;
+        there = false;
+        pages = 0;
+      }
+    }
+    // ---- output: 32 columns at a time through the tile's place of Q, so that rows are written in pieces of 16 channels ----
+    // Column 64 w + 8 g + 2 k + h of O is channel 32 (2 w + h) + 4 g + k: the order in which V's codes lie in a word.
+    const int tok = r / G, hd = kvh * G + r % G;
     const int64_t row = ((int64_t)b * a.N + hd) * a.Lq + tok;
     const float inv = a.shares > 1 ? 1.f : l_run != 0.f ? 1.f / l_run : 0.f;  // (a sum that is NaN stays one)
+    f0 *= inv;
+    f1 *= inv;
+    char* to = nullptr;
+    if (tok < a.Lq) {
+      if (a.shares == 1)
+        to = reinterpret_cast<char*>(reinterpret_cast<__nv_bfloat16*>(a.o.ptr) + (int64_t)b * a.o.sb + (int64_t)hd * a.o.sh + (int64_t)tok * a.o.ss);
+      else if (there && live > 0) to = reinterpret_cast<char*>(a.part_o + (row * a.shares + share) * D);
+    }
+    char* line_to[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      line_to[i] = reinterpret_cast<char*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(to), 4 * i + (lane >> 3)));
+    unsigned char* const stage = smem + x * SM::kQ + (warp & 3) * 4096;
 #pragma unroll 1
     for (int ch = 0; ch < D / 32; ++ch) {
-      uint32_t o[32];
-      if (pages > 0) {
-        ptx::tmem_ld32(tm + kColO + (uint32_t)ch * 32, o);
-        ptx::tmem_wait_ld(o);
+      float v[32];
+      {
+        uint32_t o[32];
+        if (pages > 0) {
+          ptx::tmem_ld32(tm + kColO + (uint32_t)ch * 32, o);
+          ptx::tmem_wait_ld(o);
+        }
+#pragma unroll
+        for (int c = 0; c < 32; ++c) v[c] = __uint_as_float(o[c]) * f0;
+      }
+      if (split && x == 0) {
+#pragma unroll
+        for (int c = 0; c < 8; ++c) {
+          const float4 w = box[(ch * 8 + c) * kTile + rr];
+          v[4 * c] = fmaf(w.x, f1, v[4 * c]);
+          v[4 * c + 1] = fmaf(w.y, f1, v[4 * c + 1]);
+          v[4 * c + 2] = fmaf(w.z, f1, v[4 * c + 2]);
+          v[4 * c + 3] = fmaf(w.w, f1, v[4 * c + 3]);
+        }
+      }
+      const unsigned nan = poison >> (2 * (ch >> 1)) & 3;
+      if (nan) {
+#pragma unroll
+        for (int c = 0; c < 32; ++c)
+          if (nan >> (c & 1) & 1) v[c] = NAN;
+      }
+      if (!there || pages == 0) {
+#pragma unroll
+        for (int c = 0; c < 32; ++c) v[c] = 0.f;
+      }
+#pragma unroll
+      for (int c = 0; c < 8; ++c) {  // channels 16 (ch % 2) + 4 (c % 4) + 0..3 of group 2 (ch / 2) + c / 4
+        const int k = 8 * (c & 3) + (c >> 2);
+        *reinterpret_cast<float4*>(stage + lane * 128 + ((c ^ (lane & 7)) << 4)) = make_float4(v[k], v[k + 2], v[k + 4], v[k + 6]);
+      }
+      __syncwarp();
+      float4 piece[8];
+      const int c = lane & 7, channel = 64 * (ch >> 1) + 32 * (c >> 2) + 16 * (ch & 1) + 4 * (c & 3);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int line = 4 * i + (lane >> 3);
+        piece[i] = *reinterpret_cast<const float4*>(stage + line * 128 + ((c ^ (line & 7)) << 4));
+      }
+      if (a.shares > 1) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (line_to[i]) store4(reinterpret_cast<float*>(line_to[i]) + channel, piece[i]);
       } else {
 #pragma unroll
-        for (int c = 0; c < 32; ++c) o[c] = 0;
-      }
-      if (tok < a.Lq) {
-        if (!there) {
-#pragma unroll
-          for (int c = 0; c < 32; ++c) o[c] = 0;
-        }
-        if (there && (poison >> ch & 1)) {
-#pragma unroll
-          for (int c = 0; c < 32; ++c) o[c] = 0x7FC00000u;
-        }
-        if (a.shares > 1) {
-          if (there && pages > 0) {
-            float4* const p = reinterpret_cast<float4*>(a.part_o + (row * a.shares + share) * D + ch * 32);
-#pragma unroll
-            for (int c = 0; c < 32; c += 4)
-              p[c / 4] = make_float4(__uint_as_float(o[c]), __uint_as_float(o[c + 1]), __uint_as_float(o[c + 2]), __uint_as_float(o[c + 3]));
-          }
-        } else {
-          __nv_bfloat16* const p = reinterpret_cast<__nv_bfloat16*>(a.o.ptr) + (int64_t)b * a.o.sb + (int64_t)hd * a.o.sh + (int64_t)tok * a.o.ss + ch * 32;
-#pragma unroll
-          for (int c = 0; c < 32; c += 8) {
-            float v[8];
-#pragma unroll
-            for (int y = 0; y < 8; ++y) v[y] = __uint_as_float(o[c + y]) * inv;
-            store8(p + c, v);
-          }
-        }
+        for (int i = 0; i < 8; ++i)
+          if (line_to[i]) store4(reinterpret_cast<__nv_bfloat16*>(line_to[i]) + channel, piece[i]);
       }
       __syncwarp();
     }
@@ -253,7 +356,8 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attn_tc_kernel(CacheAttnArg
     }
   } else if (warp < kMmaWarp) {
     // =============================== codes -> K and V ===========================================
-    const int p = tid - 32 * kSoftWarps, t = p & 3, line = p >> 2;  // keys `line`, `line` + 32; token pair `line`
+    const int p = tid - 32 * kSoftWarps, t = p & 3, line = p >> 2;  // token pair `line`, and (eight lanes that write at once: other banks):
+    const int key = (line & ~7) | (line & 1) << 2 | (line >> 1 & 3), flip = line & 1;  // keys `key`, `key` + 32; V's pieces 2 t + flip, then the other
     const unsigned char* const head = a.pages + (int64_t)kvh * L::kBytes;
     const Codes codes = a.codes;
     unsigned char* const cells = smem + SM::kCodes + p * SM::kCell;  // cell c of stage s: s kStage + c 128 kCell on
@@ -264,9 +368,9 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attn_tc_kernel(CacheAttnArg
         const int stage = k % kAhead * SM::kStage;
 #pragma unroll
         for (int y = 0; y < 2; ++y) {
-          cp_async<SM::kCell>(cells + stage + y * 128 * SM::kCell, page + L::k_word(line + 32 * y, 0, t));
-          cp_async<SM::kCell>(cells + stage + (2 + y) * 128 * SM::kCell, page + L::v_word(2 * line, 2 * t + y, 0));
-          cp_async<SM::kScales>(scale_cells + stage + y * 128 * SM::kScales, page + L::k_scale(line + 32 * y, 0));
+          cp_async<SM::kCell>(cells + stage + y * 128 * SM::kCell, page + L::k_word(key + 32 * y, 0, t));
+          cp_async<SM::kCell>(cells + stage + (2 + y) * 128 * SM::kCell, page + L::v_word(2 * line, 2 * t + (y ^ flip), 0));
+          cp_async<SM::kScales>(scale_cells + stage + y * 128 * SM::kScales, page + L::k_scale(key + 32 * y, 0));
         }
         cp_async<SM::kCell>(cells + stage + 4 * 128 * SM::kCell, page + L::v_scale(2 * line, 0));
       }
@@ -295,16 +399,14 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attn_tc_kernel(CacheAttnArg
       if (k >= kBufs) wait(kKVEmpty + buf, k / kBufs - 1);
       unsigned char* const out_k = smem + SM::kKV + buf * 2 * SM::kHalf;
       unsigned char* const out_v = out_k + SM::kHalf;
-      auto place = [&](int key, int j) { return ((4 * j + t) >> 3) * SM::kChunk + key * 128 + ((((4 * j + t) & 7) ^ (key & 7)) << 4); };
-      auto write = [&](unsigned char* to, uint32_t w, uint32_t s2) {
-        const Pairs x = pairs_of(codes, w, s2);
-        const uint2 lo = low_values(x), hi = high_values(x);
-        *reinterpret_cast<uint4*>(to) = make_uint4(lo.x, lo.y, hi.x, hi.y);
-      };
+      auto place = [&](int row, int unit) { return (unit >> 3) * SM::kChunk + row * 128 + (((unit & 7) ^ (row & 7)) << 4); };
 #pragma unroll
       for (int y = 0; y < 2; ++y)
 #pragma unroll
-        for (int j = 0; j < kG; ++j) write(out_k + place(line + 32 * y, j), kw[y][j], __byte_perm(ks[y][j / 2], 0, j % 2 ? 0x3232 : 0x1010));
+        for (int j = 0; j < kG; ++j) {
+          const Pairs x = pairs_of(codes, kw[y][j], __byte_perm(ks[y][j / 2], 0, j % 2 ? 0x3232 : 0x1010));
+          *reinterpret_cast<uint4*>(out_k + place(key + 32 * y, 4 * j + t)) = make_uint4(x.x[0], x.x[1], x.x[2], x.x[3]);
+        }
       // values of tokens in no block are zeros (0 x NaN would reach every row); so are NaN that some rows see and others do not:
       // those rows are told
       const uint32_t keep = ((in & 1) ? 0xFFFFu : 0u) | ((in & 2) ? 0xFFFF0000u : 0u);
@@ -321,11 +423,17 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attn_tc_kernel(CacheAttnArg
         }
       }
 #pragma unroll
-      for (int y = 0; y < 2; ++y)
+      for (int w = 0; w < kG / 2; ++w)
 #pragma unroll
-        for (int j = 0; j < kG; ++j)
-          write(out_v + place(2 * line + y, j), __byte_perm(rotr(vw[0][y * (kG / 2) + j / 2], 3), rotr(vw[1][y * (kG / 2) + j / 2], 3), j % 2 ? 0x7632 : 0x5410),
-                __byte_perm(vs[j], 0, y ? 0x3232 : 0x1010));
+        for (int h = 0; h < 2; ++h) {  // the even and the odd token
+          const uint32_t s2 = __byte_perm(vs[2 * w], vs[2 * w + 1], h ? 0x7632 : 0x5410), c2 = scale_offset(s2);
+#pragma unroll
+          for (int y = 0; y < 2; ++y) {
+            const uint32_t x = vw[y][h * (kG / 2) + w];
+            *reinterpret_cast<uint4*>(out_v + place(2 * line + h, 8 * w + 2 * t + (y ^ flip))) =
+                make_uint4(held(codes, x, s2, c2), held(codes, rotr(x, 4), s2, c2), held(codes, rotr(x, 8), s2, c2), held(codes, rotr(x, 12), s2, c2));
+          }
+        }
       ptx::fence_proxy_async_smem();
       __syncwarp();
       ptx::mbar_arrive_warp(bar(kKVFull + buf));
@@ -336,47 +444,57 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attn_tc_kernel(CacheAttnArg
     const uint32_t idesc_qk = ptx::idesc_bf16(kTile, kPage, 0, 0), idesc_pv = ptx::idesc_bf16(kTile, D, 0, 1);
     const uint64_t q_desc = ptx::smem_desc_sw128(sbase, 16, 1024), k_desc = ptx::smem_desc_sw128(sbase + SM::kKV, 16, 1024);
     const uint64_t v_desc = ptx::smem_desc_sw128(sbase + SM::kKV + SM::kHalf, SM::kChunk, 1024);
-    auto issue_qk = [&](int k) {
+    // Page k for group x's tile: its j-th.
+    auto issue_qk = [&](int k, int x, int j) {
       const int buf = k % kBufs;
       wait(kKVFull + buf, k / kBufs);
       ptx::tc_fence_after_sync();
       __syncwarp();
       if (ptx::elect_one()) {
-#pragma unroll 1
-        for (int x = 0; x < tiles; ++x) {
-          const uint32_t d = tmem + (uint32_t)x * kTileCols + (uint32_t)(k & 1) * 64;
-#pragma unroll 1
-          for (int s = 0; s < D / 16; ++s)
-            ptx::mma_ss_lohi(d, (uint32_t)q_desc + (uint32_t)x * (SM::kQ >> 4) + (uint32_t)(s >> 2) * (SM::kQChunk >> 4) + (uint32_t)(s & 3) * 2,
-                             (uint32_t)(q_desc >> 32), (uint32_t)k_desc + (uint32_t)buf * (2 * SM::kHalf >> 4) + (uint32_t)(s >> 2) * (SM::kChunk >> 4) + (uint32_t)(s & 3) * 2,
-                             (uint32_t)(k_desc >> 32), idesc_qk, s > 0);
-          ptx::mma_commit(bar(kSFull + 2 * x + (k & 1)));
-        }
+        const uint32_t d = tmem + (uint32_t)x * kTileCols + (uint32_t)(j & 1) * 64, q = (uint32_t)q_desc + (split ? 0u : (uint32_t)x * (SM::kQ >> 4));
+        const uint32_t key = (uint32_t)k_desc + (uint32_t)buf * (2 * SM::kHalf >> 4);
+#pragma unroll
+        for (int s = 0; s < D / 16; ++s)
+          ptx::mma_ss_lohi(d, q + (s >> 2) * (SM::kQChunk >> 4) + (s & 3) * 2, (uint32_t)(q_desc >> 32), key + (s >> 2) * (SM::kChunk >> 4) + (s & 3) * 2,
+                           (uint32_t)(k_desc >> 32), idesc_qk, s > 0);
+        ptx::mma_commit(bar(kSFull + 2 * x + (j & 1)));
       }
       __syncwarp();
     };
-    if (live > 0) issue_qk(0);
-#pragma unroll 1
-    for (int k = 0; k < live; ++k) {
-      if (k + 1 < live) issue_qk(k + 1);
+    auto issue_pv = [&](int k, int x, int j, bool last) {
       const int buf = k % kBufs;
-#pragma unroll 1
-      for (int x = 0; x < tiles; ++x) {
-        wait(kPFull + 2 * x + (k & 1), k >> 1);
-        ptx::tc_fence_after_sync();
-        __syncwarp();
-        if (ptx::elect_one()) {
-          const uint32_t s = tmem + (uint32_t)x * kTileCols + (uint32_t)(k & 1) * 64, d = tmem + (uint32_t)x * kTileCols + kColO;
-#pragma unroll 1
-          for (int ks = 0; ks < kPage / 16; ++ks) {
-            const uint32_t v = (uint32_t)v_desc + (uint32_t)buf * (2 * SM::kHalf >> 4) + (uint32_t)ks * (16 * 128 >> 4);
-            ptx::mma_ts_lohi(d, s + ks * 8, v, (uint32_t)(v_desc >> 32), idesc_pv, k > 0 || ks > 0);
-            ptx::mma_ts_lohi(d, s + 32 + ks * 8, v, (uint32_t)(v_desc >> 32), idesc_pv, 1u);
-          }
-          ptx::mma_commit(bar(kODone + 2 * x + (k & 1)));
-          if (x + 1 == tiles) ptx::mma_commit(bar(kKVEmpty + buf));
+      wait(kPFull + 2 * x + (j & 1), j >> 1);
+      ptx::tc_fence_after_sync();
+      __syncwarp();
+      if (ptx::elect_one()) {
+        const uint32_t s = tmem + (uint32_t)x * kTileCols + (uint32_t)(j & 1) * 64, d = tmem + (uint32_t)x * kTileCols + kColO;
+        const uint32_t v = (uint32_t)v_desc + (uint32_t)buf * (2 * SM::kHalf >> 4);
+#pragma unroll
+        for (int ks = 0; ks < kPage / 16; ++ks) {
+          ptx::mma_ts_lohi(d, s + ks * 8, v + ks * (16 * 128 >> 4), (uint32_t)(v_desc >> 32), idesc_pv, j > 0 || ks > 0);
+          ptx::mma_ts_lohi(d, s + 32 + ks * 8, v + ks * (16 * 128 >> 4), (uint32_t)(v_desc >> 32), idesc_pv, 1u);
         }
-        __syncwarp();
+        ptx::mma_commit(bar(kODone + 2 * x + (j & 1)));
+        if (last) ptx::mma_commit(bar(kKVEmpty + buf));
+      }
+      __syncwarp();
+    };
+    if (split) {
+      if (live > 0) issue_qk(0, 0, 0);
+      if (live > 1) issue_qk(1, 1, 0);
+#pragma unroll 1
+      for (int k = 0; k < live; ++k) {
+        issue_pv(k, k & 1, k >> 1, true);
+        if (k + 2 < live) issue_qk(k + 2, k & 1, (k >> 1) + 1);
+      }
+    } else {
+      if (live > 0)
+        for (int x = 0; x < 2; ++x) issue_qk(0, x, 0);
+#pragma unroll 1
+      for (int k = 0; k < live; ++k) {
+        if (k + 1 < live)
+          for (int x = 0; x < 2; ++x) issue_qk(k + 1, x, k + 1);
+        for (int x = 0; x < 2; ++x) issue_pv(k, x, k, x == 1);
       }
     }
   }
