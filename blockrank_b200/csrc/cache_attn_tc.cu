@@ -11,9 +11,9 @@
 // columns are given their names as they are written.
 //
 // Bound by the integer instructions of softmax and unpacking together (of a page's 2,350 cycles with two tiles about 1,700; the products
-// take 1,950 of them beside it): 4 prompts of 100 documents of 160 tokens, 45 tokens by 4 heads in the longest: 110 us.  On the way there:
+// take 1,950 of them beside it): 4 prompts of 100 documents of 160 tokens, 45 tokens by 4 heads in the longest: 107 us.  On the way there:
 // products issued in a loop 131 us, unrolled 125; Q by asynchronous copies 120.6; one tile by both groups, outputs through
-// shared memory 117; no permutations 110.  (Q in tensor memory, one S to a tile: 124 where this took 125.)
+// shared memory 117; no permutations 110; of a page that ends in its first half only that half 107.  (Q in tensor memory, one S to a tile: 124 where this took 125.)
 //
 // Tensor memory: per tile S (64 columns) twice and O (D columns).  Shared memory at head_dim 128: Q 64 KB, K and V 3 x 32 KB, codes on
 // their way 4 x 12 KB.
@@ -159,14 +159,17 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attn_tc_kernel(CacheAttnArg
     for (int j = 0; j < pages; ++j) {
       const int k = split ? 2 * j + x : j, i = s_list[k], slot0 = (sh.page0 + i) * kPage;
       unsigned v0 = s_mask[2 * i], v1 = s_mask[2 * i + 1];
+      const uint32_t tm_s = tm + (uint32_t)(j & 1) * 64;
       const bool late = slot0 + kPage - 1 > first_lim;
       wait(kSFull + 2 * x + (j & 1), j >> 1);
       ptx::tc_fence_after_sync();
       __syncwarp();
-      uint32_t sr[64];
-      ptx::tmem_ld32(tm + (uint32_t)(j & 1) * 64, *reinterpret_cast<uint32_t (*)[32]>(&sr[0]));
-      ptx::tmem_ld32(tm + (uint32_t)(j & 1) * 64 + 32, *reinterpret_cast<uint32_t (*)[32]>(&sr[32]));
-      ptx::tmem_wait_ld(sr);
+      const bool two = v1 != 0;
+      uint32_t sr[2][32];
+      ptx::tmem_ld32(tm_s, sr[0]);
+      if (two) ptx::tmem_ld32(tm_s + 32, sr[1]);
+      ptx::tmem_wait_ld(sr[0]);
+      if (two) ptx::tmem_wait_ld(sr[1]);
       if (late || (v0 & v1) != ~0u) {  // (warp-uniform)
         if (late) {
           const int n = there ? max(0, min(64, lim - slot0 + 1)) : 64;
@@ -179,11 +182,19 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attn_tc_kernel(CacheAttnArg
           __syncwarp();
         }
 #pragma unroll
-        for (int c = 0; c < 64; ++c) sr[c] = ((c < 32 ? v0 : v1) & (1u << (c & 31))) ? sr[c] : 0xff800000u;
+        for (int c = 0; c < 32; ++c) sr[0][c] = (v0 & (1u << c)) ? sr[0][c] : 0xff800000u;
+        if (two) {
+#pragma unroll
+          for (int c = 0; c < 32; ++c) sr[1][c] = (v1 & (1u << c)) ? sr[1][c] : 0xff800000u;
+        }
       }
       float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-      for (int c = 0; c < 64; c += 2) mx4[(c >> 1) & 3] = ptx::max3(mx4[(c >> 1) & 3], __uint_as_float(sr[c]), __uint_as_float(sr[c + 1]));
+      for (int c = 0; c < 32; c += 2) mx4[(c >> 1) & 3] = ptx::max3(mx4[(c >> 1) & 3], __uint_as_float(sr[0][c]), __uint_as_float(sr[0][c + 1]));
+      if (two) {
+#pragma unroll
+        for (int c = 0; c < 32; c += 2) mx4[(c >> 1) & 3] = ptx::max3(mx4[(c >> 1) & 3], __uint_as_float(sr[1][c]), __uint_as_float(sr[1][c + 1]));
+      }
       const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * sl2;
       float m_new = fmaxf(m_run, mx);
       if (m_run != -INFINITY && m_new - m_run <= kLazy) m_new = m_run;
@@ -193,18 +204,21 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attn_tc_kernel(CacheAttnArg
       m_run = m_new;
       const ptx::f32x2 sc2 = ptx::pack2(sl2, sl2), nr2 = ptx::pack2(-ref, -ref);
       ptx::f32x2 sum2[2] = {0ull, 0ull};
-      uint32_t hi[32], lo[32];
 #pragma unroll
-      for (int c = 0; c < 64; c += 2) {
-        float t0, t1;
-        ptx::unpack2(ptx::fma2(ptx::pack2(__uint_as_float(sr[c]), __uint_as_float(sr[c + 1])), sc2, nr2), t0, t1);
-        const float p0 = ptx::ex2(t0), p1 = ptx::ex2(t1);
-        sum2[(c >> 1) & 1] = ptx::add2(sum2[(c >> 1) & 1], ptx::pack2(p0, p1));
-        hi[c >> 1] = pack_bf16(p0, p1);
-        lo[c >> 1] = low_part(hi[c >> 1], p0, p1);
+      for (int h = 0; h < 2; ++h) {
+        if (h == 1 && !two) break;
+        uint32_t parts[32];  // higher bits of 32 tokens, then what they leave
+#pragma unroll
+        for (int c = 0; c < 32; c += 2) {
+          float t0, t1;
+          ptx::unpack2(ptx::fma2(ptx::pack2(__uint_as_float(sr[h][c]), __uint_as_float(sr[h][c + 1])), sc2, nr2), t0, t1);
+          const float p0 = ptx::ex2(t0), p1 = ptx::ex2(t1);
+          sum2[(c >> 1) & 1] = ptx::add2(sum2[(c >> 1) & 1], ptx::pack2(p0, p1));
+          parts[c >> 1] = pack_bf16(p0, p1);
+          parts[16 + (c >> 1)] = low_part(parts[c >> 1], p0, p1);
+        }
+        ptx::tmem_st32(tm_s + 32 * h, parts);
       }
-      ptx::tmem_st32(tm + (uint32_t)(j & 1) * 64, hi);
-      ptx::tmem_st32(tm + (uint32_t)(j & 1) * 64 + 32, lo);
       if (j > 0 && __any_sync(0xffffffffu, changed)) {  // (rare)
         wait(kODone + 2 * x + ((j - 1) & 1), (j - 1) >> 1);
         ptx::tc_fence_after_sync();
@@ -364,15 +378,19 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attn_tc_kernel(CacheAttnArg
     unsigned char* const scale_cells = smem + SM::kCodes + 5 * 128 * SM::kCell + p * SM::kScales;
     auto request = [&](int k) {
       if (k < live) {
-        const unsigned char* const page = head + (int64_t)s_page[s_list[k]] * a.Nk * L::kBytes;
+        const int i = s_list[k];
+        const bool two = s_mask[2 * i + 1] != 0, pair = two || line < 16;
+        const unsigned char* const page = head + (int64_t)s_page[i] * a.Nk * L::kBytes;
         const int stage = k % kAhead * SM::kStage;
 #pragma unroll
         for (int y = 0; y < 2; ++y) {
-          cp_async<SM::kCell>(cells + stage + y * 128 * SM::kCell, page + L::k_word(key + 32 * y, 0, t));
-          cp_async<SM::kCell>(cells + stage + (2 + y) * 128 * SM::kCell, page + L::v_word(2 * line, 2 * t + (y ^ flip), 0));
-          cp_async<SM::kScales>(scale_cells + stage + y * 128 * SM::kScales, page + L::k_scale(key + 32 * y, 0));
+          if (y == 0 || two) {
+            cp_async<SM::kCell>(cells + stage + y * 128 * SM::kCell, page + L::k_word(key + 32 * y, 0, t));
+            cp_async<SM::kScales>(scale_cells + stage + y * 128 * SM::kScales, page + L::k_scale(key + 32 * y, 0));
+          }
+          if (pair) cp_async<SM::kCell>(cells + stage + (2 + y) * 128 * SM::kCell, page + L::v_word(2 * line, 2 * t + (y ^ flip), 0));
         }
-        cp_async<SM::kCell>(cells + stage + 4 * 128 * SM::kCell, page + L::v_scale(2 * line, 0));
+        if (pair) cp_async<SM::kCell>(cells + stage + 4 * 128 * SM::kCell, page + L::v_scale(2 * line, 0));
       }
       cp_async_commit();
     };
@@ -382,7 +400,7 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attn_tc_kernel(CacheAttnArg
     for (int k = 0; k < live; ++k) {
       const int buf = k % kBufs, i = s_list[k], slot0 = (sh.page0 + i) * kPage;
       const uint32_t in = s_mask[2 * i + (line >> 4)] >> (2 * line & 31);  // of this pair of tokens
-      const bool late = slot0 + kPage - 1 > first_lim;
+      const bool late = slot0 + kPage - 1 > first_lim, two = s_mask[2 * i + 1] != 0, pair = two || line < 16;
       request(k + kAhead - 1);
       cp_async_wait<kAhead - 1>();  // this thread's cells of page k have landed
       uint32_t kw[2][kG], ks[2][kG / 2], vw[2][kG], vs[kG];
@@ -401,12 +419,14 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attn_tc_kernel(CacheAttnArg
       unsigned char* const out_v = out_k + SM::kHalf;
       auto place = [&](int row, int unit) { return (unit >> 3) * SM::kChunk + row * 128 + (((unit & 7) ^ (row & 7)) << 4); };
 #pragma unroll
-      for (int y = 0; y < 2; ++y)
+      for (int y = 0; y < 2; ++y) {
+        if (y == 1 && !two) break;
 #pragma unroll
         for (int j = 0; j < kG; ++j) {
           const Pairs x = pairs_of(codes, kw[y][j], __byte_perm(ks[y][j / 2], 0, j % 2 ? 0x3232 : 0x1010));
           *reinterpret_cast<uint4*>(out_k + place(key + 32 * y, 4 * j + t)) = make_uint4(x.x[0], x.x[1], x.x[2], x.x[3]);
         }
+      }
       // values of tokens in no block are zeros (0 x NaN would reach every row); so are NaN that some rows see and others do not:
       // those rows are told
       const uint32_t keep = ((in & 1) ? 0xFFFFu : 0u) | ((in & 2) ? 0xFFFF0000u : 0u);
@@ -418,12 +438,13 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attn_tc_kernel(CacheAttnArg
 #pragma unroll
         for (int j = 0; j < kG; ++j) {
           const uint32_t is = __vcmpeq2(vs[j] & 0x7F807F80u, 0x7F807F80u);
-          if (is) atomicOr(&s_nan[buf][j][line >> 4], ((is & 1u) | ((is >> 31) << 1)) << (2 * line & 31));
+          if (is && pair) atomicOr(&s_nan[buf][j][line >> 4], ((is & 1u) | ((is >> 31) << 1)) << (2 * line & 31));
           vs[j] &= ~is;
         }
       }
+      if (pair) {
 #pragma unroll
-      for (int w = 0; w < kG / 2; ++w)
+        for (int w = 0; w < kG / 2; ++w)
 #pragma unroll
         for (int h = 0; h < 2; ++h) {  // the even and the odd token
           const uint32_t s2 = __byte_perm(vs[2 * w], vs[2 * w + 1], h ? 0x7632 : 0x5410), c2 = scale_offset(s2);
@@ -434,6 +455,7 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attn_tc_kernel(CacheAttnArg
                 make_uint4(held(codes, x, s2, c2), held(codes, rotr(x, 4), s2, c2), held(codes, rotr(x, 8), s2, c2), held(codes, rotr(x, 12), s2, c2));
           }
         }
+      }
       ptx::fence_proxy_async_smem();
       __syncwarp();
       ptx::mbar_arrive_warp(bar(kKVFull + buf));
@@ -441,12 +463,13 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attn_tc_kernel(CacheAttnArg
     cp_async_wait<0>();
   } else {
     // =============================== MMA ===========================================
-    const uint32_t idesc_qk = ptx::idesc_bf16(kTile, kPage, 0, 0), idesc_pv = ptx::idesc_bf16(kTile, D, 0, 1);
+    const uint32_t idesc_qk = ptx::idesc_bf16(kTile, kPage, 0, 0), idesc_half = ptx::idesc_bf16(kTile, kPage / 2, 0, 0), idesc_pv = ptx::idesc_bf16(kTile, D, 0, 1);
     const uint64_t q_desc = ptx::smem_desc_sw128(sbase, 16, 1024), k_desc = ptx::smem_desc_sw128(sbase + SM::kKV, 16, 1024);
     const uint64_t v_desc = ptx::smem_desc_sw128(sbase + SM::kKV + SM::kHalf, SM::kChunk, 1024);
     // Page k for group x's tile: its j-th.
     auto issue_qk = [&](int k, int x, int j) {
       const int buf = k % kBufs;
+      const uint32_t idesc = s_mask[2 * s_list[k] + 1] != 0 ? idesc_qk : idesc_half;
       wait(kKVFull + buf, k / kBufs);
       ptx::tc_fence_after_sync();
       __syncwarp();
@@ -456,13 +479,14 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attn_tc_kernel(CacheAttnArg
 #pragma unroll
         for (int s = 0; s < D / 16; ++s)
           ptx::mma_ss_lohi(d, q + (s >> 2) * (SM::kQChunk >> 4) + (s & 3) * 2, (uint32_t)(q_desc >> 32), key + (s >> 2) * (SM::kChunk >> 4) + (s & 3) * 2,
-                           (uint32_t)(k_desc >> 32), idesc_qk, s > 0);
+                           (uint32_t)(k_desc >> 32), idesc, s > 0);
         ptx::mma_commit(bar(kSFull + 2 * x + (j & 1)));
       }
       __syncwarp();
     };
     auto issue_pv = [&](int k, int x, int j, bool last) {
       const int buf = k % kBufs;
+      const bool two = s_mask[2 * s_list[k] + 1] != 0;
       wait(kPFull + 2 * x + (j & 1), j >> 1);
       ptx::tc_fence_after_sync();
       __syncwarp();
@@ -471,8 +495,10 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attn_tc_kernel(CacheAttnArg
         const uint32_t v = (uint32_t)v_desc + (uint32_t)buf * (2 * SM::kHalf >> 4);
 #pragma unroll
         for (int ks = 0; ks < kPage / 16; ++ks) {
-          ptx::mma_ts_lohi(d, s + ks * 8, v + ks * (16 * 128 >> 4), (uint32_t)(v_desc >> 32), idesc_pv, j > 0 || ks > 0);
-          ptx::mma_ts_lohi(d, s + 32 + ks * 8, v + ks * (16 * 128 >> 4), (uint32_t)(v_desc >> 32), idesc_pv, 1u);
+          if (ks == kPage / 32 && !two) break;
+          const uint32_t p = s + (ks >> 1) * 32 + (ks & 1) * 8;
+          ptx::mma_ts_lohi(d, p, v + ks * (16 * 128 >> 4), (uint32_t)(v_desc >> 32), idesc_pv, j > 0 || ks > 0);
+          ptx::mma_ts_lohi(d, p + 16, v + ks * (16 * 128 >> 4), (uint32_t)(v_desc >> 32), idesc_pv, 1u);
         }
         ptx::mma_commit(bar(kODone + 2 * x + (j & 1)));
         if (last) ptx::mma_commit(bar(kKVEmpty + buf));

@@ -755,3 +755,25 @@ def test_very_many_heads():
     assert torch.equal(gk.double().cpu(), torch.where(keep, ch.held(k).transpose(1, 2), 0.0))
     assert torch.equal(gv.double().cpu(), torch.where(keep, ch.held(v).transpose(1, 2), 0.0))
     ops.check_status()
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("rows", [9, 40])
+def test_pages_of_which_only_a_part_is_in_a_block(D, rows):
+    """Blocks in the first half of a page, in the second, across the middle, in single tokens at either end; NaN next to them."""
+    N, Nk = 8, 2
+    spans = [(0, 32), (96, 32), (128, 1), (191, 1), (220, 8), (256 + 31, 1), (320 + 32, 1), (384, 63), (449, 63), (576, 100 + rows)]
+    start, length = (torch.tensor([[s[i] for s in spans]], dtype=torch.int32) for i in (0, 1))
+    P = 14
+    cache, hk, hv = _filled(P, Nk, D, 211)
+    inside = torch.cat([torch.arange(a, a + n) for a, n in spans])
+    table = _table(1, P, P, 28)
+    at = ch.slots_of(table[0], inside)[None].int().cuda()
+    k, v = ops.cache_read(cache, at, F32)
+    cache.fill_(255)
+    ops.cache_write(k, v, cache, at)
+    q = _rand(1, rows, N, D, seed=29, dtype=BF16).transpose(1, 2)
+    out, lse = ops.cache_attention(q.cuda(), cache, table.cuda(), start.cuda(), length.cuda(), 0.1, return_lse=True)
+    ref, ref_lse, size = ch.attention(q, hk, hv, table, start, length, 0.1)
+    _check(out, lse, ref, ref_lse, size, hv, 64)
+    ops.check_status()
