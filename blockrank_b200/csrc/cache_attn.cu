@@ -27,7 +27,7 @@ constexpr int kWarps = 4;
 constexpr int kThreads = 32 * kWarps;
 constexpr int kShare = 128;       // pages a CTA takes at most
 constexpr int kParts = 3;         // K or V parts of pages that a warp has room for in shared memory: two K, one V
-constexpr int kCluster = 8;       // shares that a cluster joins, at most
+constexpr int kCluster = 8;       // shares that a cluster joins, at most (fp32, 3 prompts of 20 documents: 8.0 us, joined by a kernel 8.6)
 
 template <typename T, int kTiles>
 constexpr int ctas_per_sm = kTiles == 1 && sizeof(T) == 2 ? 3 : 2;

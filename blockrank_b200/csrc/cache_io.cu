@@ -147,7 +147,8 @@ __device__ __noinline__ uint32_t quantise_exactly(const Raw<T, kN> x, float s) {
 
 constexpr int kIoThreads = 256;
 constexpr int kTile = 32;  // tokens of a CTA, at most
-// Calls with at most this many tokens look for a later token with the same slot in the list itself; others go through `owner`.
+// Calls with at most this many tokens look for a later token with the same slot in the list itself; others go through `owner`, two
+// kernels more.  (8 heads of 128: 32 tokens 2.9 us, with `owner` 4.3; 1024 4.3 and 5.4; 2048 6.6 and 6.1; 4096 14.5 and 8.3.)
 constexpr int kScan = 1024;
 
 __global__ void __launch_bounds__(256) owner_clear_kernel(const int32_t* slots, int tokens, int64_t n_slots, int32_t* owner) {
@@ -170,18 +171,20 @@ struct Tile {
 
 __device__ __forceinline__ int token_of(const IoArgs& a, int row) { return a.Nk == 1 ? row : (int)__umulhi((uint32_t)row, a.per_head); }
 
-// One thread per token; the slots of a tile are looked for by all of the CTA.
+// One thread per token; that a later token names the same slot all of the CTA look for, in one pass over the list.
 template <int D, bool kWrite>
 __device__ __forceinline__ void find_tokens(const IoArgs& a, Tile& tile, int first, int n) {
-  __shared__ int later[kTile];
-  if (threadIdx.x < n) later[threadIdx.x] = 0;
+  __shared__ int own[kTile], later[kTile];
   if (kWrite && a.owner == nullptr) {  // a slot that several tokens name keeps the last one's values
+    if (threadIdx.x < n) {
+      own[threadIdx.x] = a.slots[first + threadIdx.x];
+      later[threadIdx.x] = 0;
+    }
     __syncthreads();
-    for (int i = 0; i < n; ++i) {
-      const int slot = a.slots[first + i];
-      bool seen = false;
-      for (int j = first + i + 1 + threadIdx.x; j < a.tokens; j += kIoThreads) seen |= a.slots[j] == slot;
-      if (seen) later[i] = 1;
+    for (int j = first + 1 + threadIdx.x; j < a.tokens; j += kIoThreads) {
+      const int slot = a.slots[j];
+      for (int i = 0; i < n; ++i)
+        if (own[i] == slot && first + i < j) later[i] = 1;
     }
     __syncthreads();
   }
@@ -374,9 +377,10 @@ IoArgs make_args(const brk_cache& c, const brk_view& k, const brk_view& v, int B
   a.S = S;
   a.Nk = c.Nk;
   a.per_head = (uint32_t)(((1ull << 32) + c.Nk - 1) / c.Nk);
-  // Tokens of a CTA: as many as give a warp four rounds, fewer where that leaves SMs without a CTA.
-  const int most = std::min(kTile, std::max(1, kIoThreads / a.Nk)), spread = a.tokens / (4 * std::max(1, sm_count()));
-  a.tile = std::max(1, std::min(most, spread));
+  // Tokens of a CTA: those that make it two CTAs an SM, at most as many as give a warp four rounds.  (bf16, 8 heads of 128; of 592 CTAs 512
+  // tokens took 4.9 us, now 3.4; 1024 7.7 and 4.2, 16384 24.1 and 23.1; of 148 CTAs 512 3.5, 1024 5.0.)
+  const int most = std::min(kTile, std::max(1, kIoThreads / a.Nk)), ctas = 2 * std::max(1, sm_count());
+  a.tile = std::min(most, (int)((a.tokens + (int64_t)ctas - 1) / ctas));
   return a;
 }
 dim3 grid_of(const IoArgs& a) { return dim3((unsigned)((a.tokens + (int64_t)a.tile - 1) / a.tile)); }
