@@ -1,8 +1,10 @@
 // Attention of a prompt's last tokens over its pages of the 4-bit cache, and the join of its parts.
 //
 // out = sum_j softmax_j(scale q . k_j) v_j over the slots j that row i sees: those of all blocks at or before its own slot.
-// Bound by the read of the cache (144 bytes per token and KV head at head_dim 128), with 72 % of the issue slots needed to keep up
-// with it (counted from the source: 287 instructions per 16 keys and warp).
+// The floor is the read of the cache (144 bytes per token and KV head at head_dim 128); bound by the instructions that bring the codes
+// into the products: from registers alone, 12 warps to an SM, a scheduler takes 364 cycles for 16 keys (K 139, softmax 40, V 206 where
+// they are timed one by one), which would be 7.1 TB/s.  One row each of 16 prompts of 100 documents (32 to 256 tokens), 32 heads
+// on 8: 82 us, 3.2 TB/s; of two contexts of 131,072 tokens 70 us, 4.3 TB/s; of one prompt of 5 documents 7.3 us, all of it latency.
 //
 // A CTA takes a share of one prompt's pages for one KV head and up to 8 kTiles rows (a row: a query head of the group at one
 // token).  Its warps take whole pages in turn and share nothing until the end: running maximum, sum and output of a warp
@@ -189,7 +191,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<T, kTiles>) cache_attn_k
     // ---- O^T += V^T P^T ----
     cp_async_wait<1>();
     __syncwarp();
-    const unsigned char* const page = ring + 2 * L::kHalf - L::kHalf;  // (offsets count from a page's beginning)
+    const unsigned char* const page = ring + 2 * L::kHalf - L::kHalf;  // (the third part; offsets count from a page's beginning)
     // The tensor cores cut a sum off rather than round it, so in 32 bits a page has sums of its own.
     float fresh[kF32 ? kTiles : 1][L::kGroups][2][4] = {};
     auto& sums = [&]() -> float (&)[kTiles][L::kGroups][2][4] {
@@ -198,7 +200,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<T, kTiles>) cache_attn_k
     }();
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-        uint32_t pt[kTiles][2][kMmas];
+      uint32_t pt[kTiles][2][kMmas];
 #pragma unroll
       for (int c = 0; c < kTiles; ++c)
 #pragma unroll
@@ -465,10 +467,12 @@ __global__ void __launch_bounds__(128) cache_join_kernel(CacheAttnArgs a) {
   if (a.lse && tid == 0) a.lse[row] = l != 0.f ? (ref + log2f(l)) * kLn2 : -INFINITY;
 }
 
-// More rows than this go to the tcgen05 kernel (bf16).
+// More rows than this go to the tcgen05 kernel (bf16).  (4 prompts of 100 documents of 160 tokens: 32 rows 84 us here, 36 rows 89 there;
+// 40 rows 174 here and 89 there.  One such prompt: 40 rows 38 and 32.)
 constexpr int kManyRows = 32;
 
-// Rows of a CTA: 4 (bf16), 8 or 16; 256 in the tcgen05 kernel.  (fp32 at head_dim 128 has no registers for 16: 2 prompts of 100 documents,
+// Rows of a CTA: 4 (bf16), 8 or 16; 256 in the tcgen05 kernel.  Fewer columns than rows would read the cache twice; 4 rows stand in 8 columns
+// so that one product takes both parts of P.  (fp32 at head_dim 128 has no registers for 16: 2 prompts of 100 documents,
 // 16 rows 47 us, with 8 to a CTA 36; 64 rows 135 and 113.  At head_dim 64 32 rows 35 and 42, 16 rows 23 and 24.)
 int rows_per_cta(const brk_cache_attn_params& p) {
   const int64_t rows = (int64_t)p.Lq * (p.N / p.cache.Nk);

@@ -446,15 +446,15 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attn_tc_kernel(CacheAttnArg
 #pragma unroll
         for (int w = 0; w < kG / 2; ++w)
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {  // the even and the odd token
-          const uint32_t s2 = __byte_perm(vs[2 * w], vs[2 * w + 1], h ? 0x7632 : 0x5410), c2 = scale_offset(s2);
+          for (int h = 0; h < 2; ++h) {  // the even and the odd token
+            const uint32_t s2 = __byte_perm(vs[2 * w], vs[2 * w + 1], h ? 0x7632 : 0x5410), c2 = scale_offset(s2);
 #pragma unroll
-          for (int y = 0; y < 2; ++y) {
-            const uint32_t x = vw[y][h * (kG / 2) + w];
-            *reinterpret_cast<uint4*>(out_v + place(2 * line + h, 8 * w + 2 * t + (y ^ flip))) =
-                make_uint4(held(codes, x, s2, c2), held(codes, rotr(x, 4), s2, c2), held(codes, rotr(x, 8), s2, c2), held(codes, rotr(x, 12), s2, c2));
+            for (int y = 0; y < 2; ++y) {
+              const uint32_t x = vw[y][h * (kG / 2) + w];
+              *reinterpret_cast<uint4*>(out_v + place(2 * line + h, 8 * w + 2 * t + (y ^ flip))) =
+                  make_uint4(held(codes, x, s2, c2), held(codes, rotr(x, 4), s2, c2), held(codes, rotr(x, 8), s2, c2), held(codes, rotr(x, 12), s2, c2));
+            }
           }
-        }
       }
       ptx::fence_proxy_async_smem();
       __syncwarp();

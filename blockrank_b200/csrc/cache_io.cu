@@ -176,13 +176,13 @@ template <int D, bool kWrite>
 __device__ __forceinline__ void find_tokens(const IoArgs& a, Tile& tile, int first, int n) {
   __shared__ int own[kTile], later[kTile];
   if (kWrite && a.owner == nullptr) {  // a slot that several tokens name keeps the last one's values
+    int j = first + 1 + threadIdx.x, slot = j < a.tokens ? a.slots[j] : -1;  // (requested together with the CTA's own)
     if (threadIdx.x < n) {
       own[threadIdx.x] = a.slots[first + threadIdx.x];
       later[threadIdx.x] = 0;
     }
     __syncthreads();
-    for (int j = first + 1 + threadIdx.x; j < a.tokens; j += kIoThreads) {
-      const int slot = a.slots[j];
+    for (; j < a.tokens; j += kIoThreads, slot = j < a.tokens ? a.slots[j] : -1) {
       for (int i = 0; i < n; ++i)
         if (own[i] == slot && first + i < j) later[i] = 1;
     }

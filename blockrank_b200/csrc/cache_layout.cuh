@@ -243,7 +243,8 @@ struct QueryRows {
         shift[n][0] = t == 0 ? w[0][0] : t == 1 ? w[1][0] : t == 2 ? w[2][0] : 0u;
         shift[n][1] = 0u;
       }
-      // 2^(133 - up), up >= -7: a row with NaN or an infinity has a unit of NaN, one from 2^121 on of infinity
+      // 2^(133 - up), up >= -7: a row with NaN or an infinity has a unit of NaN, one with a magnitude from 2^115 on of infinity (its logits
+      // are infinities or NaN)
       const float down = !finite ? NAN : 133 - up > 127 ? INFINITY : up > 133 + 126 ? 0.f : __uint_as_float((uint32_t)(133 - up + 127) << 23);
 #pragma unroll
       for (int y = 0; y < 2; ++y) unit[n][y] = __shfl_sync(0xffffffffu, down, 4 * (2 * t + y));

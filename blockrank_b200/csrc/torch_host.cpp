@@ -425,7 +425,7 @@ brk_view heads_view(const Tensor& t, bool bshd = false) {
   if (t.size(bshd ? 1 : 2) == 1) v.stride_s = 0;
   return v;
 }
-// at::empty without its dispatch: a step's call is as long as its host path (reading back one document 6.9 us of it, now XX)
+// at::empty without its dispatch: a step's call is as long as its host path (reading back one document: 6.9 us of it, now 5.2)
 Tensor fresh(at::IntArrayRef sizes, at::ScalarType type, const Tensor& like) { return at::detail::empty_cuda(sizes, type, like.device(), std::nullopt); }
 // (B, heads, S, D) with the memory layout (B, S, heads, D)
 Tensor fresh_heads(int64_t B, int64_t heads, int64_t S, int64_t D, at::ScalarType type, const Tensor& like) {

@@ -151,7 +151,7 @@ def cache_attention(q: torch.Tensor, cache: torch.Tensor, page_table: torch.Tens
     """Attention of the last tokens of every prompt over its pages: :func:`attention`'s query block, with the cache in the place
     of k and v (the tokens' own keys and values are written first).
 
-    q (B,N,L,D); page_table int32 (B,P); blk_start / blk_len int32 (B,M): the slots of the prompt's blocks, as for
+    q (B,N,L,D), magnitudes below 2^115; page_table int32 (B,P); blk_start / blk_len int32 (B,M): the slots of the prompt's blocks, as for
     :func:`attention` (slots between blocks have no influence; M = 1: one causal sequence).  Row i is the token at slot
     ``blk_start[b,-1] + blk_len[b,-1] - q_len[b] + i`` and sees every block's slots up to its own.  ``q_len`` int32 (B,): the number
     of rows of each prompt (None: L), from 0 to the last block's length.  Returns out (B,L,N,D) [and lse (B,N,L) fp32]; rows from
