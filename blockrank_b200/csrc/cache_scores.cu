@@ -3,7 +3,10 @@
 // A CTA takes some of a prompt's documents, about as many pages as every other CTA, for one KV head and up to 8 kTiles (head, signal
 // row) pairs; its warps take equal parts of those pages, whatever documents they belong to, and keep a running (maximum, sum) per
 // pair and document.  The pairs of a prompt's documents are merged by the kernel that merges those of doc_scores.
-// Bound by the read of the keys (72 bytes per token and KV head at head_dim 128).
+// The floor is the read of the keys (72 bytes per token and KV head at head_dim 128); bound by instructions, as the attention of few rows
+// is.  16 prompts of 100 documents of 32 to 256 tokens, two rows of 32 heads on 8: 49 us, 2.6 TB/s; one prompt of 5 documents
+// 8.6.  (Up to 64 documents at a time, not 32, so that no CTA has a second batch: 48.5 and 9.2; two batches as long as each other:
+// 49.6.)
 #include <algorithm>
 #include <atomic>
 #include <type_traits>
