@@ -386,32 +386,51 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<T, kTiles>) cache_attn_k
   }
   if (!a.cluster) return;
   ptx::cluster_sync();
-  for (int i = tid * a.shares + share; i < kRows * (D / 4); i += kThreads * a.shares) {
+  // Every CTA joins some of the rows' pieces of 4 channels: at most kPieces to a thread.
+  constexpr int kPieces = (kRows * (D / 4) / 2 + kThreads - 1) / kThreads;
+  float4 acc[kPieces];
+  float m[kPieces], l[kPieces];
+#pragma unroll
+  for (int n = 0; n < kPieces; ++n) {
+    const int i = (tid + n * kThreads) * a.shares + share;
+    if (i >= kRows * (D / 4)) break;
     const int col = i / (D / 4), d = i % (D / 4) * 4;
-    const int r = row0 + col, tok = r / G;
-    if (tok >= a.Lq) break;
     const uint32_t at_ml = ptx::smem_u32(reinterpret_cast<float2*>(s_part + kRows * D) + col), at_o = ptx::smem_u32(s_part + col * D + d);
     float2 ml[kCluster];
-    float m = -INFINITY;
+    float4 x[kCluster];
+    m[n] = -INFINITY;
+    l[n] = 0.f;
+    acc[n] = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
     for (int c = 0; c < kCluster; ++c) {
-      ml[c] = c < a.shares ? ptx::ld_cluster_f32x2(at_ml, c) : make_float2(-INFINITY, 0.f);
-      m = fmaxf(m, ml[c].x);
+      ml[c] = make_float2(-INFINITY, 0.f);
+      x[c] = acc[n];
+      if (c < a.shares) {
+        ml[c] = ptx::ld_cluster_f32x2(at_ml, c);
+        x[c] = ptx::ld_cluster_f32x4(at_o, c);
+      }
     }
-    const float ref = m == -INFINITY ? 0.f : m;
-    float l = 0.f;
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int c = 0; c < kCluster; ++c) m[n] = fmaxf(m[n], ml[c].x);
+    const float ref = m[n] == -INFINITY ? 0.f : m[n];
 #pragma unroll
     for (int c = 0; c < kCluster; ++c) {
-      if (c >= a.shares) continue;
       const float f = ptx::ex2(ml[c].x - ref);
-      const float4 x = ptx::ld_cluster_f32x4(at_o, c);
-      l = fmaf(ml[c].y, f, l);
-      acc.x = fmaf(x.x, f, acc.x); acc.y = fmaf(x.y, f, acc.y); acc.z = fmaf(x.z, f, acc.z); acc.w = fmaf(x.w, f, acc.w);
+      l[n] = fmaf(ml[c].y, f, l[n]);
+      acc[n].x = fmaf(x[c].x, f, acc[n].x); acc[n].y = fmaf(x[c].y, f, acc[n].y); acc[n].z = fmaf(x[c].z, f, acc[n].z); acc[n].w = fmaf(x[c].w, f, acc[n].w);
     }
-    write(tok, kvh * G + r % G, d, m, l, acc);
   }
-  ptx::cluster_sync();  // nobody leaves while its part is read
+  __syncwarp();
+  ptx::cluster_arrive();  // (this CTA has read what it needs)
+#pragma unroll
+  for (int n = 0; n < kPieces; ++n) {
+    const int i = (tid + n * kThreads) * a.shares + share, col = i / (D / 4), d = i % (D / 4) * 4;
+    const int r = row0 + col, tok = r / G;
+    if (i >= kRows * (D / 4) || tok >= a.Lq) break;
+    write(tok, kvh * G + r % G, d, m[n], l[n], acc[n]);
+  }
+  __syncwarp();
+  ptx::cluster_wait();  // nobody leaves while its part is read
 }
 
 // One CTA per row; D / 4 threads read a share's part, 4 channels each.  A share without pages has written its statistics alone.

@@ -46,14 +46,19 @@ __device__ __forceinline__ Share find_share(const CacheAttnArgs& a, int b, int r
   const int64_t slots = (int64_t)a.P * kPage;
   const int last_start = start[a.M - 1], last_len = len[a.M - 1], given = a.q_len ? a.q_len[b] : a.Lq;
   __shared__ int32_t s_table[kThreads];
+  __shared__ int2 s_span[kThreads];  // (start, length) of the first blocks
   s_table[tid] = tid < a.P ? table[tid] : -1;
   meanwhile();
   bool bad = given < 0 || given > a.Lq || given > last_len;
-  for (int m = tid; m < a.M; m += kThreads) bad |= span_is_bad(start, len, m, slots);
+  for (int m = tid; m < a.M; m += kThreads) {
+    bad |= span_is_bad(start, len, m, slots);
+    if (m < kThreads) s_span[m] = make_int2(start[m], len[m]);
+  }
   Share r;
   r.bad = __syncthreads_or(bad);
   if (r.bad && tid == 0 && a.status) atomicCAS(a.status, 0, kStatusBadCacheCall);
 
+  auto block = [&](int m) { return m < kThreads ? s_span[m] : make_int2(start[m], len[m]); };
   r.rows = r.bad ? 0 : given;
   r.n_rows = min(r.rows * G - row0, max_rows);
   r.first_slot = r.bad ? 0 : last_start + last_len - r.rows;
@@ -67,7 +72,8 @@ __device__ __forceinline__ Share find_share(const CacheAttnArgs& a, int b, int r
     int m = 0;  // the first block that ends behind the page's first token (blocks are in order)
     for (int size = a.M; size > 0;) {
       const int half = size / 2;
-      if (start[m + half] + len[m + half] <= lo) {
+      const int2 x = block(m + half);
+      if (x.x + x.y <= lo) {
         m += half + 1;
         size -= half + 1;
       } else {
@@ -75,8 +81,10 @@ __device__ __forceinline__ Share find_share(const CacheAttnArgs& a, int b, int r
       }
     }
     uint32_t w[2] = {0, 0};
-    for (; m < a.M && start[m] < lo + kPage; ++m) {
-      const int from = max(start[m] - lo, 0), to = min(start[m] + len[m] - lo, kPage);
+    for (; m < a.M; ++m) {
+      const int2 x = block(m);
+      if (x.x >= lo + kPage) break;
+      const int from = max(x.x - lo, 0), to = min(x.x + x.y - lo, kPage);
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const int f = max(from - 32 * h, 0), t = min(to - 32 * h, 32);

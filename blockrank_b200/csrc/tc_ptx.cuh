@@ -25,6 +25,9 @@ __device__ __forceinline__ void grid_dependency_launch() { asm volatile("griddep
 __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
+// Its two halves.
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 // The shared-memory word at this CTA's address `addr`, of CTA `rank` of the cluster.
 __device__ __forceinline__ float ld_cluster_f32(uint32_t addr, uint32_t rank) {
   float v;
