@@ -372,7 +372,7 @@ int brk_cache_doc_scores(const brk_cache_score_params* p, void* workspace, size_
   if (rc) return rc;
   BRK_REQUIRE(p->doc_mass != nullptr, BRK_E_ARG, "doc_mass is null");
   const size_t need = cache_scores_workspace(*p);
-  BRK_REQUIRE(workspace && workspace_bytes >= need && ((uintptr_t)workspace & 15) == 0, BRK_E_WORKSPACE,
+  BRK_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && ((uintptr_t)workspace & 15) == 0), BRK_E_WORKSPACE,
               "workspace %zu < %zu bytes (or not 16-byte aligned)", workspace_bytes, need);
   return cache_scores_launch(*p, workspace, (cudaStream_t)stream);
 }

@@ -2,10 +2,11 @@
 //
 // A CTA takes some of a prompt's documents, about as many pages as every other CTA, for one KV head and up to 8 kTiles (head, signal
 // row) pairs; its warps take equal parts of those pages, whatever documents they belong to, and keep a running (maximum, sum) per
-// pair and document.  The pairs of a prompt's documents are merged by the kernel that merges those of doc_scores.
+// pair and document.  The pairs of a prompt's documents are merged by the kernel that merges those of doc_scores, or, where a prompt
+// has few pages, at the end by the CTAs themselves: one per KV head with all documents, a cluster for a prompt.
 // The floor is the read of the keys (72 bytes per token and KV head at head_dim 128); bound by instructions, as the attention of few rows
 // is.  16 prompts of 100 documents of 32 to 256 tokens, two rows of 32 heads on 8: 49 us, 2.6 TB/s; one prompt of 5 documents
-// 8.6.  (Up to 64 documents at a time, not 32, so that no CTA has a second batch: 48.5 and 9.2; two batches as long as each other:
+// 7.6.  (Up to 64 documents at a time, not 32, so that no CTA has a second batch: 48.5 and 9.2; two batches as long as each other:
 // 49.6.)
 #include <algorithm>
 #include <atomic>
@@ -24,6 +25,7 @@ constexpr int kWarps = 4;
 constexpr int kThreads = 32 * kWarps;
 constexpr int kStages = 3;  // pages (their K parts) a warp has in shared memory
 constexpr int kDocs = 32;   // documents at a time: one per lane
+constexpr int kHeads = 8;   // KV heads of a prompt that a cluster has, at most
 constexpr float kLog2e = 1.4426950408889634f;
 
 struct CacheScoreArgs {
@@ -32,7 +34,11 @@ struct CacheScoreArgs {
   const int32_t* table;
   const int32_t* blk_start;
   const int32_t* blk_len;
-  float2* partial;  // [B, N, R, M - 2]
+  float2* partial;  // [B, N, R, M - 2], unless
+  bool whole;       // a CTA has all documents of a prompt, and a cluster all KV heads: masses and logits are made here
+  float* mass;      // [B, N, R, M - 2]
+  float* logits;    // [B, M - 2] or null
+  float inv_count_temp;
   int32_t* status;
   int n_pages, N, Nk, R, M, P, max_block_len;
   float scale;
@@ -50,12 +56,14 @@ __global__ void __launch_bounds__(kThreads, kTiles == 1 && sizeof(T) == 2 ? 3 : 
   extern __shared__ __align__(16) unsigned char smem[];  // [kWarps][kStages][K part of a page]
   __shared__ float2 s_ml[kWarps][kDocs][kCols];
   __shared__ int s_scan[kWarps], s_before[2];
+  __shared__ float s_mass[kWarps][kDocs], s_total[kDocs];
   __shared__ int2 s_span[kThreads];      // (start, length) of the first documents
   __shared__ int32_t s_table[kThreads];  // the first page numbers
   ptx::grid_dependency_wait();
   ptx::grid_dependency_launch();
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-  const int b = blockIdx.y / a.Nk, kvh = blockIdx.y % a.Nk, row0 = blockIdx.z * kCols;
+  const int b = a.whole ? blockIdx.y : blockIdx.y / a.Nk, kvh = a.whole ? blockIdx.x : blockIdx.y % a.Nk, row0 = blockIdx.z * kCols;
+  const int share = a.whole ? 0 : blockIdx.x, shares = a.whole ? 1 : gridDim.x;
   const int G = a.N / a.Nk, GR = G * a.R, nd = a.M - 2;
   const int32_t *const bs = a.blk_start + (int64_t)b * a.M, *const bl = a.blk_len + (int64_t)b * a.M;
 
@@ -113,12 +121,12 @@ __global__ void __launch_bounds__(kThreads, kTiles == 1 && sizeof(T) == 2 ? 3 : 
       }
       const bool only = nd <= kThreads;
       if (only) {
-        lo = (int64_t)sum * blockIdx.x / gridDim.x;
-        hi = (int64_t)sum * (blockIdx.x + 1) / gridDim.x;
+        lo = (int64_t)sum * share / shares;
+        hi = (int64_t)sum * (share + 1) / shares;
       }
       if (pass == 1 || only) {
         const unsigned below = __ballot_sync(0xffffffffu, d0 + tid < nd && before + first < lo);
-        const unsigned below_end = __ballot_sync(0xffffffffu, d0 + tid < nd && (before + first < hi || blockIdx.x + 1 == gridDim.x));
+        const unsigned below_end = __ballot_sync(0xffffffffu, d0 + tid < nd && (before + first < hi || share + 1 == shares));
         if (lane == 0) {
           atomicAdd(&s_before[0], __popc(below));
           atomicAdd(&s_before[1], __popc(below_end));
@@ -129,8 +137,8 @@ __global__ void __launch_bounds__(kThreads, kTiles == 1 && sizeof(T) == 2 ? 3 : 
       __syncthreads();
     }
     if (pass == 0) {
-      lo = before * blockIdx.x / gridDim.x;
-      hi = before * (blockIdx.x + 1) / gridDim.x;
+      lo = before * share / shares;
+      hi = before * (share + 1) / shares;
     }
   }
   const int doc_end = s_before[1];
@@ -268,21 +276,108 @@ __global__ void __launch_bounds__(kThreads, kTiles == 1 && sizeof(T) == 2 ? 3 : 
     }
     cp_async_wait<0>();
     __syncthreads();
+    if (a.whole) {  // (one batch) a warp has some of the rows, a lane a document
+      constexpr int kMine = kCols / kWarps;
+      float e[kMine], top[kMine], z[kMine], mine = 0.f;
+#pragma unroll
+      for (int i = 0; i < kMine; ++i) {
+        float2 ml[kWarps];
+        top[i] = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+          ml[w] = s_ml[w][lane][warp + kWarps * i];  // ((-infinity, 0) of documents that are not there)
+          top[i] = fmaxf(top[i], ml[w].x);
+        }
+#pragma unroll
+        for (int off = 16; off > 0; off >>= 1) top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], off));
+        const float ref = top[i] == -INFINITY ? 0.f : top[i];
+        e[i] = 0.f;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) e[i] = fmaf(ml[w].y, ptx::ex2(ml[w].x - ref), e[i]);
+        z[i] = e[i];
+#pragma unroll
+        for (int off = 16; off > 0; off >>= 1) z[i] += __shfl_xor_sync(0xffffffffu, z[i], off);
+      }
+#pragma unroll
+      for (int i = 0; i < kMine; ++i) {
+        const int r = warp + kWarps * i;
+        const float p = z[i] != 0.f ? e[i] / z[i] : 0.f;  // (NaN stays NaN)
+        if (r < GR && lane < nd) a.mass[(((int64_t)b * a.Nk + kvh) * GR + r) * nd + lane] = p;
+        if (r < GR) mine += p;
+      }
+      s_mass[warp][lane] = mine;
+      __syncthreads();
+      if (warp == 0) {
+        float total = 0.f;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) total += s_mass[w][lane];
+        s_total[lane] = total;
+      }
+      if (a.logits == nullptr) return;
+      __syncwarp();
+      if (a.Nk > 1) ptx::cluster_sync();
+      float total = 0.f;
+      if (kvh == 0 && warp == 0) {
+        float of[kHeads];
+#pragma unroll
+        for (int c = 0; c < kHeads; ++c) of[c] = c == 0 ? s_total[lane] : c < a.Nk ? ptx::ld_cluster_f32(ptx::smem_u32(&s_total[lane]), c) : 0.f;
+#pragma unroll
+        for (int c = 0; c < kHeads; ++c) total += of[c];
+        __syncwarp();
+      }
+      if (a.Nk > 1) ptx::cluster_arrive();
+      if (kvh == 0 && warp == 0 && lane < nd) a.logits[(int64_t)b * nd + lane] = total * a.inv_count_temp;
+      __syncwarp();
+      if (a.Nk > 1) ptx::cluster_wait();  // nobody leaves while its sums are read
+      return;
+    }
     for (int i = tid; i < kDocs * kCols; i += kThreads) {
       const int doc = i % kDocs, r = row0 + i / kDocs;
       if (doc >= n_docs || r >= GR) continue;
       float2 ml = s_ml[0][doc][i / kDocs];
 #pragma unroll
       for (int w = 1; w < kWarps; ++w) ml = merged(ml, s_ml[w][doc][i / kDocs]);
-      a.partial[(((int64_t)b * a.N + kvh * G + r / a.R) * a.R + r % a.R) * nd + doc0 + doc] = ml;
+      a.partial[(((int64_t)b * a.Nk + kvh) * GR + r) * nd + doc0 + doc] = ml;
     }
     __syncthreads();
   }
 }
 
+struct Split {
+  int tiles, z;    // of 8 rows; CTAs of a KV head's rows
+  int64_t shares;  // of a prompt's documents
+  bool whole;
+};
+// Shares of a prompt's documents, at least a page for each warp: a round of CTAs takes as long as its share, with about eight pages' time
+// for beginning and end, and the kernel that merges what they find about twelve; a cluster that has all of a prompt needs none.  (In
+// clusters and with the kernel: one prompt of 5 documents, 8 pages, 6.8 us and 8.1; 16 pages 8.6 and 8.4; 26 pages 10.3 and 9.1; 16
+// prompts of 18 pages 10.6 and 11.5, of 46 pages 18.5 and 15.0.)
+Split split_of(const brk_cache_score_params& p) {
+  const int nd = p.M - 2, Nk = p.cache.Nk, rows = p.N / Nk * p.R, tiles = rows > 8 ? 2 : 1, z = (rows + 8 * tiles - 1) / (8 * tiles);
+  Split r = {tiles, z, 1, false};
+  const int64_t ctas = (int64_t)p.B * Nk * z, room = (tiles == 1 && p.dtype == BRK_BF16 ? 3 : 2) * (int64_t)std::max(1, sm_count());
+  const int64_t most = std::min<int64_t>(nd, (p.P + kWarps - 1) / kWarps);
+  const bool may = z == 1 && nd <= kDocs && Nk <= kHeads;
+  int64_t best = may ? (ctas + room - 1) / room * (p.P + 8) : INT64_MAX;
+  r.whole = may;
+  for (int64_t round = 0; round <= 8; ++round) {  // (the most shares of so many rounds, and the fewest)
+    const int64_t s = std::min(most, std::max<int64_t>(1, round * room / ctas));
+    const int64_t cost = (ctas * s + room - 1) / room * ((p.P + s - 1) / s + 8) + 12;
+    if (cost < best) {
+      best = cost;
+      r.shares = s;
+      r.whole = false;
+    }
+  }
+  return r;
+}
+
 }  // namespace
 
-size_t cache_scores_workspace(const brk_cache_score_params& p) { return (size_t)p.B * p.N * p.R * (p.M - 2) * sizeof(float2); }
+
+size_t cache_scores_workspace(const brk_cache_score_params& p) {
+  return split_of(p).whole ? 0 : (size_t)p.B * p.N * p.R * (p.M - 2) * sizeof(float2);
+}
 
 int cache_scores_launch(const brk_cache_score_params& p, void* ws, cudaStream_t st) {
   CacheScoreArgs a;
@@ -296,22 +391,13 @@ int cache_scores_launch(const brk_cache_score_params& p, void* ws, cudaStream_t 
   a.n_pages = p.cache.n_pages; a.N = p.N; a.Nk = p.cache.Nk; a.R = p.R; a.M = p.M; a.P = p.P;
   a.max_block_len = p.max_block_len;
   a.scale = p.scale;
-  const int nd = p.M - 2, rows = p.N / a.Nk * p.R, tiles = rows > 8 ? 2 : 1;
-  const int z = (rows + 8 * tiles - 1) / (8 * tiles);
-  // Shares of a prompt's documents, at least a page for each warp: a round of CTAs takes as long as its share, with about eight pages' time
-  // for beginning and end.
-  const int64_t ctas = (int64_t)p.B * a.Nk * z, room = (tiles == 1 && p.dtype == BRK_BF16 ? 3 : 2) * (int64_t)std::max(1, sm_count());
-  const int64_t most = std::min<int64_t>(nd, (p.P + kWarps - 1) / kWarps);
-  int64_t shares = 1, best = INT64_MAX;
-  for (int64_t round = 0; round <= 8; ++round) {  // (the most shares of so many rounds, and the fewest)
-    const int64_t s = std::min(most, std::max<int64_t>(1, round * room / ctas));
-    const int64_t cost = (ctas * s + room - 1) / room * ((p.P + s - 1) / s + 8);
-    if (cost < best) {
-      best = cost;
-      shares = s;
-    }
-  }
-  const dim3 grid((unsigned)shares, p.B * a.Nk, z);
+  const Split split = split_of(p);
+  a.whole = split.whole;
+  a.mass = p.doc_mass;
+  a.logits = p.logits;
+  a.inv_count_temp = 1.f / ((float)(p.N * p.R) * p.temperature);
+  const int tiles = split.tiles;
+  const dim3 grid = split.whole ? dim3(a.Nk, p.B) : dim3((unsigned)split.shares, p.B * a.Nk, split.z);
   auto run = [&](auto kern, std::atomic<bool>* configured) -> int {
     const int bytes = kWarps * kStages * (int)head_page_bytes(p.cache.D) / 2;
     int dev = 0;
@@ -321,7 +407,7 @@ int cache_scores_launch(const brk_cache_score_params& p, void* ws, cudaStream_t 
       BRK_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributePreferredSharedMemoryCarveout, (int)cudaSharedmemCarveoutMaxShared));
       if (dev >= 0 && dev < 64) configured[dev].store(true, std::memory_order_release);
     }
-    return launch_dependent(kern, grid, dim3(kThreads), bytes, st, a);
+    return launch_dependent_clusters(a.whole ? a.Nk : 1, kern, grid, dim3(kThreads), bytes, st, a);
   };
   static std::atomic<bool> done[8][64] = {};
   auto of_head_dim = [&](auto d, std::atomic<bool>(*flags)[64]) -> int {
@@ -330,12 +416,13 @@ int cache_scores_launch(const brk_cache_score_params& p, void* ws, cudaStream_t 
     return tiles == 1 ? run(cache_scores_kernel<__nv_bfloat16, D, 1>, flags[2]) : run(cache_scores_kernel<__nv_bfloat16, D, 2>, flags[3]);
   };
   const int rc = p.cache.D == 128 ? of_head_dim(std::integral_constant<int, 128>(), done) : of_head_dim(std::integral_constant<int, 64>(), done + 4);
-  if (rc) return rc;
+  if (rc || a.whole) return rc;
   ScoreArgs m = {};
   m.partial = a.partial;
   m.mass = p.doc_mass;
   m.logits = p.logits;
-  m.inv_count_temp = 1.f / ((float)(p.N * p.R) * p.temperature);
+  m.inv_count_temp = a.inv_count_temp;
+  m.keep_nan = true;
   m.B = p.B; m.N = p.N; m.Nk = a.Nk; m.M = p.M; m.R = p.R;
   return doc_merge_launch(m, st);
 }

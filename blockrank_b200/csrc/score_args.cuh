@@ -15,6 +15,7 @@ struct ScoreArgs {
   float inv_count_temp;  // 1 / (N * R * temperature)
   int B, N, Nk, S, M, R;
   float scale;
+  bool keep_nan;  // a row with NaN among its documents' keys is NaN in all of them (otherwise 0 in the others)
 };
 
 inline ScoreArgs make_score_args(const brk_score_params& p) {
@@ -30,6 +31,7 @@ inline ScoreArgs make_score_args(const brk_score_params& p) {
   a.inv_count_temp = 0.f;
   a.B = p.B; a.N = p.N; a.Nk = p.Nk; a.S = p.S; a.M = p.M; a.R = p.R;
   a.scale = p.scale;
+  a.keep_nan = false;
   return a;
 }
 

@@ -106,7 +106,7 @@ __global__ void __launch_bounds__(merge_threads<kCluster>, kCluster ? 2 : 1) doc
       for (int d = lane + 32 * kHeld; d < n; d += 32) z[r] += p[d].y * exp2f(p[d].x - ref);
 #pragma unroll
       for (int off = 16; off > 0; off >>= 1) z[r] += __shfl_xor_sync(0xffffffffu, z[r], off);
-      const float inv = z[r] > 0.f ? 1.f / z[r] : 0.f;
+      const float inv = z[r] > 0.f || (a.keep_nan && z[r] != 0.f) ? 1.f / z[r] : 0.f;
       float* const mass = a.mass + (w0 + first + r * kWarps) * nd;
 #pragma unroll
       for (int i = 0; i < kHeld; ++i)

@@ -563,8 +563,9 @@ std::tuple<Tensor, Tensor> cache_doc_scores(const Tensor& q, const Tensor& cache
   p.logits = (float*)logits.data_ptr();
   p.status = status_ptr(cache);
   const size_t nbytes = brk_cache_doc_scores_workspace_bytes(&p);
-  Tensor ws = fresh({(int64_t)std::max<size_t>(nbytes, 16)}, at::kByte, cache);
-  check(brk_cache_doc_scores(&p, ws.data_ptr(), nbytes, stream_of(cache)), "brk_cache_doc_scores");
+  Tensor ws;
+  if (nbytes > 0) ws = fresh({(int64_t)nbytes}, at::kByte, cache);
+  check(brk_cache_doc_scores(&p, nbytes > 0 ? ws.data_ptr() : nullptr, nbytes, stream_of(cache)), "brk_cache_doc_scores");
   return {mass, logits};
 }
 

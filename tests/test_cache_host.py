@@ -73,7 +73,7 @@ def test_a_workspace_that_is_too_small_is_refused():
 
 
 @pytest.mark.parametrize("change,code", [
-    (dict(M=2), -1), (dict(R=65), -1), (dict(max_block_len=0), -1), (dict(temperature=0.0), -1), (dict(doc_mass=None), -1), (dict(N=3), -1), ({}, -3)])
+    (dict(M=2), -1), (dict(R=65), -1), (dict(max_block_len=0), -1), (dict(temperature=0.0), -1), (dict(doc_mass=None), -1), (dict(N=3), -1), (dict(M=40, P=40), -3)])
 def test_refusals_of_scores(change, code):
     L = _lib.lib()
     p = _lib.CacheScoreParams()

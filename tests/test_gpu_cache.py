@@ -777,3 +777,28 @@ def test_pages_of_which_only_a_part_is_in_a_block(D, rows):
     ref, ref_lse, size = ch.attention(q, hk, hv, table, start, length, 0.1)
     _check(out, lse, ref, ref_lse, size, hv, 64)
     ops.check_status()
+
+
+@pytest.mark.parametrize("docs,Nk", [(4, 2), (32, 8), (32, 1), (33, 2), (5, 12)])
+def test_scores_of_a_document_with_nan(docs, Nk):
+    """NaN in one head's keys of one document: NaN in all documents of that head's rows (a softmax over them), in the prompt's logits,
+    and nowhere else; with and without a kernel that merges."""
+    N, D, R, B = 2 * Nk, 64, 2, 3
+    start, length, P = ch.spans([[5] + [17] * docs + [9]] * B, False)
+    cache, hk, hv = _filled(B * P, Nk, D, 221)
+    table = _table(B, P, B * P, 30)
+    q = _rand(B, R, N, D, seed=31, dtype=BF16).transpose(1, 2)
+    args = (cache, table.cuda(), start.cuda(), length.cuda(), 0.1, 17)
+    ref = ch.doc_mass(q, hk, table, start, length, 0.1)
+    mass, out = ops.cache_doc_scores(q.cuda(), *args)
+    assert torch.allclose(mass.double().cpu(), ref, rtol=1e-4) and torch.allclose(out.double().cpu(), ref.mean((1, 2)) / 0.05, rtol=1e-4)
+    at = ch.slots_of(table[1], start[1, 2:3].long() + 3)[None].int().cuda()
+    k, v = ops.cache_read(cache, at, F32)
+    k[0, 0, 0, 7] = torch.nan
+    ops.cache_write(k, v, cache, at)
+    bad, bad_out = ops.cache_doc_scores(q.cuda(), *args)
+    assert bad[1, :2].isnan().all() and bad_out[1].isnan().all()
+    assert torch.equal(bad[1, 2:], mass[1, 2:])
+    for b in (0, 2):
+        assert torch.equal(bad[b], mass[b]) and torch.equal(bad_out[b], out[b])
+    ops.check_status()
