@@ -486,51 +486,56 @@ __global__ void __launch_bounds__(128) cache_join_kernel(CacheAttnArgs a) {
   if (a.lse && tid == 0) a.lse[row] = l != 0.f ? (ref + log2f(l)) * kLn2 : -INFINITY;
 }
 
-// More rows than this go to the tcgen05 kernel (bf16).  (4 prompts of 100 documents of 160 tokens: 32 rows 84 us here, 36 rows 89 there;
-// 40 rows 174 here and 89 there.  One such prompt: 40 rows 38 and 32.)
-constexpr int kManyRows = 32;
+// Which kernel, how many rows to a CTA, into how many shares a prompt's pages go (at most kShare pages each).
+struct Plan {
+  bool many;  // the tcgen05 kernel
+  int rows;   // of a CTA
+  int64_t groups, shares, cost;
+  // its cluster joins the parts of a prompt's shares; otherwise a kernel does
+  bool cluster() const { return shares > 1 && shares <= kCluster && !many; }
+};
 
-// Rows of a CTA: 4 (bf16), 8 or 16; 256 in the tcgen05 kernel.  Fewer columns than rows would read the cache twice; 4 rows stand in 8 columns
-// so that one product takes both parts of P.  (fp32 at head_dim 128 has no registers for 16: 2 prompts of 100 documents,
-// 16 rows 47 us, with 8 to a CTA 36; 64 rows 135 and 113.  At head_dim 64 32 rows 35 and 42, 16 rows 23 and 24.)
-int rows_per_cta(const brk_cache_attn_params& p) {
-  const int64_t rows = (int64_t)p.Lq * (p.N / p.cache.Nk);
-  if (p.dtype == BRK_BF16 && rows > kManyRows) return 256;
-  if (p.dtype == BRK_F32) return rows <= 8 || p.cache.D == 128 ? 8 : 16;
-  return rows <= 4 ? 4 : rows <= 8 ? 8 : 16;
-}
-int64_t row_groups(const brk_cache_attn_params& p) {
-  return ((int64_t)p.Lq * (p.N / p.cache.Nk) + rows_per_cta(p) - 1) / rows_per_cta(p);
-}
-
-// Shares of a prompt's pages, at most kShare pages each.  A round of CTAs takes as long as its share, with about six pages' time for
-// beginning and end (in the tcgen05 kernel four); what is left over of the SMs in the last round is lost.
-int shares_of(const brk_cache_attn_params& p) {
-  const bool many = rows_per_cta(p) == 256;
-  const int per_sm = many ? 1 : p.dtype == BRK_BF16 && rows_per_cta(p) <= 8 ? 3 : 2;
-  const int64_t ctas = (int64_t)p.B * p.cache.Nk * row_groups(p), room = per_sm * (int64_t)std::max(1, sm_count());
-  const int64_t largest = many ? kManyShare : kShare, least = (p.P + largest - 1) / largest, pages = many ? 4 : kWarps;
+// Shares: a round of CTAs takes as long as its share, with about six pages' time for beginning and end (in the tcgen05 kernel four); what is
+// left over of the SMs in the last round is lost.
+Plan plan_with(const brk_cache_attn_params& p, bool many, int per_cta) {
+  const int64_t rows = (int64_t)p.Lq * (p.N / p.cache.Nk), groups = (rows + per_cta - 1) / per_cta;
+  const int per_sm = many ? 1 : p.dtype == BRK_BF16 && per_cta <= 8 ? 3 : 2;
+  const int64_t ctas = (int64_t)p.B * p.cache.Nk * groups, room = per_sm * (int64_t)std::max(1, sm_count());
+  const int64_t largest = many ? kManyShare : kShare, least = (p.P + largest - 1) / largest, pages = many ? 2 : kWarps;
   const int64_t most = std::max<int64_t>(least, std::min<int64_t>(64, (p.P + pages - 1) / pages));
-  int64_t best = least, best_cost = INT64_MAX;
+  Plan best = {many, per_cta, groups, least, INT64_MAX};
   for (int64_t round = 0; round <= 8; ++round) {  // (the most shares of so many rounds, and the fewest)
     const int64_t s = std::min(most, std::max(least, round * room / ctas));
-    const int64_t join = s == 1 ? 0 : s > kCluster || many ? 6 + s / 8 : 2;
+    const int64_t join = s == 1 ? 0 : many ? 3 + s / 8 : s > kCluster ? 6 + s / 8 : 2;
     const int64_t cost = (ctas * s + room - 1) / room * ((p.P + s - 1) / s + (many ? 4 : 6)) + join;
-    if (cost < best_cost) {
-      best_cost = cost;
-      best = s;
+    if (cost < best.cost) {
+      best.cost = cost;
+      best.shares = s;
     }
   }
-  return (int)best;
+  return best;
 }
-// Its cluster joins the parts of a prompt's shares; otherwise a kernel does.
-bool cluster_joins(const brk_cache_attn_params& p, int shares) { return shares <= kCluster && rows_per_cta(p) != 256; }
+
+// Rows of a CTA: 4 (bf16), 8 or 16; 256 in the tcgen05 kernel.  Fewer columns than rows would read the cache twice; 4 rows stand in 8 columns
+// so that one product takes both parts of P.  (fp32 at head_dim 128 has no registers for 16: 2 prompts of 100 documents, 16 rows
+// 47 us, with 8 to a CTA 36; 64 rows 135 and 113.  At head_dim 64 32 rows 35 and 42, 16 rows 23 and 24.)
+// Of more than 16 rows in bf16 each kernel's cost is compared: a page takes 0.93 us (head_dim 64: 0.7) here and 1 us there, 1.45 for
+// more than 128 rows, and there are 5 us more in front and behind.  (One prompt of 2 documents of 128 tokens, 36 rows: 9.0 us here,
+// 14.1 there; of 100 documents 28.1 and 27.7, with 128 rows 55 and 29.  16 prompts of 2 documents, 36 rows 19.0 and 14.7.)
+Plan plan_of(const brk_cache_attn_params& p) {
+  const int64_t rows = (int64_t)p.Lq * (p.N / p.cache.Nk);
+  if (p.dtype == BRK_F32) return plan_with(p, false, rows <= 8 || p.cache.D == 128 ? 8 : 16);
+  const Plan few = plan_with(p, false, rows <= 4 ? 4 : rows <= 8 ? 8 : 16);
+  if (rows <= 16) return few;
+  const Plan many = plan_with(p, true, 256);
+  return few.cost * (p.cache.D == 128 ? 93 : 70) <= many.cost * (rows > 128 ? 145 : 100) + 500 ? few : many;
+}
 
 }  // namespace
 
 size_t cache_attn_workspace(const brk_cache_attn_params& p) {
-  const size_t n = shares_of(p);
-  return n > 1 && !cluster_joins(p, (int)n) ? (size_t)p.B * p.N * p.Lq * n * (p.cache.D * sizeof(float) + sizeof(float2)) : 0;
+  const Plan plan = plan_of(p);
+  return plan.shares > 1 && !plan.cluster() ? (size_t)p.B * p.N * p.Lq * plan.shares * (p.cache.D * sizeof(float) + sizeof(float2)) : 0;
 }
 
 int cache_attn_launch(const brk_cache_attn_params& p, void* ws, cudaStream_t st) {
@@ -545,15 +550,15 @@ int cache_attn_launch(const brk_cache_attn_params& p, void* ws, cudaStream_t st)
   a.lse = p.lse;
   a.status = p.status;
   a.n_pages = p.cache.n_pages; a.B = p.B; a.N = p.N; a.Nk = p.cache.Nk; a.Lq = p.Lq; a.M = p.M; a.P = p.P;
-  a.shares = shares_of(p);
+  const Plan plan = plan_of(p);
+  a.shares = (int)plan.shares;
   a.scale = p.scale;
-  a.cluster = a.shares > 1 && cluster_joins(p, a.shares);
+  a.cluster = plan.cluster();
   const size_t rows = (size_t)p.B * p.N * p.Lq;
   a.part_o = static_cast<float*>(ws);
   a.part_ml = reinterpret_cast<float2*>(a.part_o + rows * a.shares * p.cache.D);
-  const int64_t z = row_groups(p);
-  BRK_REQUIRE(z <= 65535, BRK_E_UNSUPPORTED, "Lq * N / Nk = %lld rows are too many for one call", (long long)p.Lq * (p.N / a.Nk));
-  const dim3 grid(a.shares, p.B * a.Nk, (unsigned)z);
+  BRK_REQUIRE(plan.groups <= 65535, BRK_E_UNSUPPORTED, "Lq * N / Nk = %lld rows are too many for one call", (long long)p.Lq * (p.N / a.Nk));
+  const dim3 grid(a.shares, p.B * a.Nk, (unsigned)plan.groups);
   auto run = [&](auto kern, std::atomic<bool>* configured) -> int {
     const int bytes = kWarps * kParts * (int)head_page_bytes(p.cache.D) / 2;
     int dev = 0;
@@ -567,16 +572,15 @@ int cache_attn_launch(const brk_cache_attn_params& p, void* ws, cudaStream_t st)
   };
   static std::atomic<bool> done[10][64] = {};
   const bool f32 = p.dtype == BRK_F32;
-  const int per = rows_per_cta(p);
   auto of_head_dim = [&](auto d, std::atomic<bool>(*flags)[64]) -> int {
     constexpr int D = decltype(d)::value;
     if constexpr (D == 64)
-      if (f32 && per == 16) return run(cache_attn_kernel<float, D, 2, false>, flags[1]);
+      if (f32 && plan.rows == 16) return run(cache_attn_kernel<float, D, 2, false>, flags[1]);
     if (f32) return run(cache_attn_kernel<float, D, 1, false>, flags[0]);
-    if (per == 4) return run(cache_attn_kernel<__nv_bfloat16, D, 1, true>, flags[2]);
-    return per == 8 ? run(cache_attn_kernel<__nv_bfloat16, D, 1, false>, flags[3]) : run(cache_attn_kernel<__nv_bfloat16, D, 2, false>, flags[4]);
+    if (plan.rows == 4) return run(cache_attn_kernel<__nv_bfloat16, D, 1, true>, flags[2]);
+    return plan.rows == 8 ? run(cache_attn_kernel<__nv_bfloat16, D, 1, false>, flags[3]) : run(cache_attn_kernel<__nv_bfloat16, D, 2, false>, flags[4]);
   };
-  const int rc = per == 256 ? cache_attn_tc_launch(a, p.cache.D, st)
+  const int rc = plan.many ? cache_attn_tc_launch(a, p.cache.D, st)
                  : p.cache.D == 128 ? of_head_dim(std::integral_constant<int, 128>(), done)
                                     : of_head_dim(std::integral_constant<int, 64>(), done + 5);
   if (rc || a.shares == 1 || a.cluster) return rc;
