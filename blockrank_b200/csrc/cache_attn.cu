@@ -29,6 +29,7 @@ constexpr int kWarps = 4;
 constexpr int kThreads = 32 * kWarps;
 constexpr int kShare = 128;       // pages a CTA takes at most
 constexpr int kParts = 3;         // K or V parts of pages that a warp has room for in shared memory: two K, one V
+constexpr int kFewJoins = 4;      // rows per SM that are joined by a CTA each
 constexpr int kCluster = 8;       // shares that a cluster joins, at most (fp32, 3 prompts of 20 documents: 8.0 us, joined by a kernel 8.6)
 
 template <typename T, int kTiles>
@@ -486,6 +487,51 @@ __global__ void __launch_bounds__(128) cache_join_kernel(CacheAttnArgs a) {
   if (a.lse && tid == 0) a.lse[row] = l != 0.f ? (ref + log2f(l)) * kLn2 : -INFINITY;
 }
 
+// The same for many rows: D / 4 threads a row, which share nothing; 8 parts at a time.  (A call of 18,432 rows in two parts 27.2 us, with a
+// CTA to a row 42.2; 6,144 rows in nine 88.6 and 93.8; 288 rows 28.1 and 27.6.)
+template <typename T, int D>
+__global__ void __launch_bounds__(128) cache_join_rows_kernel(CacheAttnArgs a, int64_t n_rows) {
+  constexpr int kLanes = D / 4, kHeld = 8;
+  const int lane = threadIdx.x % kLanes, d = lane * 4;
+  const int64_t at = (int64_t)blockIdx.x * (128 / kLanes) + threadIdx.x / kLanes, row = min(at, n_rows - 1);
+  ptx::grid_dependency_wait();
+  const int tok = (int)(row % a.Lq), hd = (int)(row / a.Lq % a.N), b = (int)(row / a.Lq / a.N);
+  const bool there = tok < (a.q_len ? a.q_len[b] : a.Lq);
+  const float2* const ml = a.part_ml + row * a.shares;
+  const float* const part = a.part_o + row * a.shares * D + d;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  float l = 0.f, m = -INFINITY;
+  for (int c0 = 0; c0 < (there ? a.shares : 0); c0 += kHeld) {
+    float2 w[kHeld];
+    float4 x[kHeld];
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i) {
+      const bool on = c0 + i < a.shares;
+      w[i] = on ? ml[c0 + i] : make_float2(-INFINITY, 0.f);
+      x[i] = on ? load4(part + (int64_t)(c0 + i) * D) : acc;
+    }
+    float top = m;
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i) top = fmaxf(top, w[i].x);
+    const float ref = top == -INFINITY ? 0.f : top, old = ptx::ex2(m - ref);
+    m = top;
+    l *= old;
+    acc.x *= old; acc.y *= old; acc.z *= old; acc.w *= old;
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i) {
+      if (w[i].y == 0.f) continue;  // (a share without pages has written its statistics alone)
+      const float f = ptx::ex2(w[i].x - ref);
+      l = fmaf(w[i].y, f, l);
+      acc.x = fmaf(x[i].x, f, acc.x); acc.y = fmaf(x[i].y, f, acc.y); acc.z = fmaf(x[i].z, f, acc.z); acc.w = fmaf(x[i].w, f, acc.w);
+    }
+  }
+  if (at >= n_rows) return;
+  const float inv = l != 0.f ? 1.f / l : 0.f;
+  store4(reinterpret_cast<T*>(a.o.ptr) + (int64_t)b * a.o.sb + (int64_t)hd * a.o.sh + (int64_t)tok * a.o.ss + d,
+         make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv));
+  if (a.lse && lane == 0) a.lse[row] = l != 0.f ? (m + log2f(l)) * kLn2 : -INFINITY;
+}
+
 // Which kernel, how many rows to a CTA, into how many shares a prompt's pages go (at most kShare pages each).
 struct Plan {
   bool many;  // the tcgen05 kernel
@@ -496,7 +542,9 @@ struct Plan {
 };
 
 // Shares: a round of CTAs takes as long as its share, with about six pages' time for beginning and end (in the tcgen05 kernel four); what is
-// left over of the SMs in the last round is lost.
+// left over of the SMs in the last round is lost.  Clusters find fewer places: each group of SMs that one cannot leave has up to s - 1 too few
+// for another (of 296 places 296 for clusters of 2, 279 of 3, 264 of 8; of 444 444, 426 and 384; ten groups assumed here are more).  Taken for
+// 296, 288 CTAs in clusters of 3 took 53 us, where 256 in clusters of 2 took 38.
 Plan plan_with(const brk_cache_attn_params& p, bool many, int per_cta) {
   const int64_t rows = (int64_t)p.Lq * (p.N / p.cache.Nk), groups = (rows + per_cta - 1) / per_cta;
   const int per_sm = many ? 1 : p.dtype == BRK_BF16 && per_cta <= 8 ? 3 : 2;
@@ -504,14 +552,21 @@ Plan plan_with(const brk_cache_attn_params& p, bool many, int per_cta) {
   const int64_t largest = many ? kManyShare : kShare, least = (p.P + largest - 1) / largest, pages = many ? 2 : kWarps;
   const int64_t most = std::max<int64_t>(least, std::min<int64_t>(64, (p.P + pages - 1) / pages));
   Plan best = {many, per_cta, groups, least, INT64_MAX};
-  for (int64_t round = 0; round <= 8; ++round) {  // (the most shares of so many rounds, and the fewest)
-    const int64_t s = std::min(most, std::max(least, round * room / ctas));
-    const int64_t join = s == 1 ? 0 : many ? 3 + s / 8 : s > kCluster ? 6 + s / 8 : 2;
-    const int64_t cost = (ctas * s + room - 1) / room * ((p.P + s - 1) / s + (many ? 4 : 6)) + join;
+  auto consider = [&](int64_t s) {
+    const bool cluster = s > 1 && s <= kCluster && !many;
+    const int64_t places = cluster ? std::max<int64_t>(s, s == 2 ? room : room - 10 * (s - 1)) : room;
+    const int64_t join = s == 1 ? 0 : many ? 3 + s / 8 : cluster ? 2 : 6 + s / 8;
+    const int64_t cost = (ctas * s + places - 1) / places * ((p.P + s - 1) / s + (many ? 4 : 6)) + join;
     if (cost < best.cost) {
       best.cost = cost;
       best.shares = s;
     }
+  };
+  for (int64_t round = 0; round <= 8; ++round) {  // (the most shares of so many rounds, and the fewest)
+    const int64_t s = std::min(most, std::max(least, round * room / ctas));
+    consider(s);
+    if (s > least) consider(s - 1);
+    if (s == most) break;
   }
   return best;
 }
@@ -584,12 +639,15 @@ int cache_attn_launch(const brk_cache_attn_params& p, void* ws, cudaStream_t st)
                  : p.cache.D == 128 ? of_head_dim(std::integral_constant<int, 128>(), done)
                                     : of_head_dim(std::integral_constant<int, 64>(), done + 5);
   if (rc || a.shares == 1 || a.cluster) return rc;
-  const dim3 joins((unsigned)rows), block(128);
-  if (p.cache.D == 128)
-    return f32 ? launch_dependent(cache_join_kernel<float, 128>, joins, block, 0, st, a)
-               : launch_dependent(cache_join_kernel<__nv_bfloat16, 128>, joins, block, 0, st, a);
-  return f32 ? launch_dependent(cache_join_kernel<float, 64>, joins, block, 0, st, a)
-             : launch_dependent(cache_join_kernel<__nv_bfloat16, 64>, joins, block, 0, st, a);
+  auto join = [&](auto d, auto t) -> int {
+    constexpr int D = decltype(d)::value;
+    using T = decltype(t);
+    if (rows <= (size_t)kFewJoins * std::max(1, sm_count())) return launch_dependent(cache_join_kernel<T, D>, dim3((unsigned)rows), dim3(128), 0, st, a);
+    const int per = 512 / D;  // rows of a CTA
+    return launch_dependent(cache_join_rows_kernel<T, D>, dim3((unsigned)((rows + per - 1) / per)), dim3(128), 0, st, a, (int64_t)rows);
+  };
+  if (p.cache.D == 128) return f32 ? join(std::integral_constant<int, 128>(), float()) : join(std::integral_constant<int, 128>(), __nv_bfloat16());
+  return f32 ? join(std::integral_constant<int, 64>(), float()) : join(std::integral_constant<int, 64>(), __nv_bfloat16());
 }
 
 }  // namespace brk

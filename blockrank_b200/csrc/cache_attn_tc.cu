@@ -11,9 +11,10 @@
 // columns are given their names as they are written.
 //
 // Bound by the integer instructions of softmax and unpacking together (of a page's 2,350 cycles with two tiles about 1,700; the products
-// take 1,950 of them beside it): 4 prompts of 100 documents of 160 tokens, 45 tokens by 4 heads in the longest: 107 us.  On the way there:
+// take 1,950 of them beside it): 4 prompts of 100 documents of 160 tokens, 45 tokens by 4 heads in the longest: 105 us.  On the way there:
 // products issued in a loop 131 us, unrolled 125; Q by asynchronous copies 120.6; one tile by both groups, outputs through
-// shared memory 117; no permutations 110; of a page that ends in its first half only that half 107.  (Q in tensor memory, one S to a tile: 124 where this took 125.)
+// shared memory 117; no permutations 110; of a page that ends in its first half only that half 107, the parts joined
+// by more rows to a CTA 105.  (Q in tensor memory, one S to a tile: 124 where this took 125.)
 //
 // Tensor memory: per tile S (64 columns) twice and O (D columns).  Shared memory at head_dim 128: Q 64 KB, K and V 3 x 32 KB, codes on
 // their way 4 x 12 KB.

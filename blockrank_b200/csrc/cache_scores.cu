@@ -348,7 +348,7 @@ struct Split {
   int64_t shares;  // of a prompt's documents
   bool whole;
 };
-// Shares of a prompt's documents, at least a page for each warp: a round of CTAs takes as long as its share, with about eight pages' time
+// Shares of a prompt's documents, at least a page (or short document) for each warp: a round of CTAs takes as long as its share, with about eight pages' time
 // for beginning and end, and the kernel that merges what they find about twelve; a cluster that has all of a prompt needs none.  (In
 // clusters and with the kernel: one prompt of 5 documents, 8 pages, 6.8 us and 8.1; 16 pages 8.6 and 8.4; 26 pages 10.3 and 9.1; 16
 // prompts of 18 pages 10.6 and 11.5, of 46 pages 18.5 and 15.0.)
@@ -356,13 +356,13 @@ Split split_of(const brk_cache_score_params& p) {
   const int nd = p.M - 2, Nk = p.cache.Nk, rows = p.N / Nk * p.R, tiles = rows > 8 ? 2 : 1, z = (rows + 8 * tiles - 1) / (8 * tiles);
   Split r = {tiles, z, 1, false};
   const int64_t ctas = (int64_t)p.B * Nk * z, room = (tiles == 1 && p.dtype == BRK_BF16 ? 3 : 2) * (int64_t)std::max(1, sm_count());
-  const int64_t most = std::min<int64_t>(nd, (p.P + kWarps - 1) / kWarps);
+  const int64_t pages = std::max(p.P, nd), most = std::min<int64_t>(nd, (pages + kWarps - 1) / kWarps);
   const bool may = z == 1 && nd <= kDocs && Nk <= kHeads;
-  int64_t best = may ? (ctas + room - 1) / room * (p.P + 8) : INT64_MAX;
+  int64_t best = may ? (ctas + room - 1) / room * (pages + 8) : INT64_MAX;
   r.whole = may;
   for (int64_t round = 0; round <= 8; ++round) {  // (the most shares of so many rounds, and the fewest)
     const int64_t s = std::min(most, std::max<int64_t>(1, round * room / ctas));
-    const int64_t cost = (ctas * s + room - 1) / room * ((p.P + s - 1) / s + 8) + 12;
+    const int64_t cost = (ctas * s + room - 1) / room * ((pages + s - 1) / s + 8) + 12;
     if (cost < best) {
       best = cost;
       r.shares = s;
