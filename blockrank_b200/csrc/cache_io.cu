@@ -148,8 +148,9 @@ __device__ __noinline__ uint32_t quantise_exactly(const Raw<T, kN> x, float s) {
 constexpr int kIoThreads = 256;
 constexpr int kTile = 32;  // tokens of a CTA, at most
 // Calls with at most this many tokens look for a later token with the same slot in the list itself; others go through `owner`, two
-// kernels more.  (8 heads of 128: 32 tokens 2.9 us, with `owner` 4.3; 1024 4.3 and 5.4; 2048 6.6 and 6.1; 4096 14.5 and 8.3.)
-constexpr int kScan = 1024;
+// kernels more.  (8 heads of 128: 32 tokens 2.9 us, with `owner` 4.3; 1024 4.3 and 5.4; 2048 6.6 and 6.1, but 4 us less from the host;
+// 4096 14.5 and 8.3.)
+constexpr int kScan = 2048;
 
 __global__ void __launch_bounds__(256) owner_clear_kernel(const int32_t* slots, int tokens, int64_t n_slots, int32_t* owner) {
   const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;

@@ -21,15 +21,15 @@ def test_sizes():
     assert L.brk_cache_page_bytes(1, 64) == 64 * 72 and L.brk_cache_page_bytes(8, 128) == 8 * 64 * 144
     assert L.brk_cache_page_bytes(1, 96) == 0 and L.brk_cache_page_bytes(0, 64) == 0
     c = _cache()
-    assert L.brk_cache_write_workspace_bytes(C.byref(c), 4, 256) == 0
-    assert L.brk_cache_write_workspace_bytes(C.byref(c), 4, 257) == 4 * 64 * 4
+    assert L.brk_cache_write_workspace_bytes(C.byref(c), 8, 256) == 0
+    assert L.brk_cache_write_workspace_bytes(C.byref(c), 8, 257) == 4 * 64 * 4
     assert L.brk_cache_attn_workspace_bytes(None) == 0 and L.brk_cache_doc_scores_workspace_bytes(None) == 0
 
 
 @pytest.mark.parametrize("change,code", [
     (dict(cache=None), -1), (dict(ptr=0), -1), (dict(ptr=72), -1), (dict(D=96), -2), (dict(n_pages=0), -1), (dict(Nk=0), -1),
     (dict(n_pages=2 ** 25), -1), (dict(dtype=2), -2), (dict(slots=None), -1), (dict(S=0), -1), (dict(B=2 ** 16, S=2 ** 16), -1),
-    (dict(view=0), -1), (dict(view=8), -1), (dict(S=2000), -3)])
+    (dict(view=0), -1), (dict(view=8), -1), (dict(S=2049), -3)])
 def test_refusals_of_write(change, code):
     """(every one of them is refused in front of any launch)"""
     L = _lib.lib()

@@ -32,6 +32,14 @@ def _table(B, P, pool, seed):
     return torch.randperm(pool, generator=torch.Generator().manual_seed(seed))[:B * P].reshape(B, P).to(torch.int32)
 
 
+def _wide(table, width=4000):
+    """The same table with room for far more pages: calls are split in other ways, and many rows go to the tcgen05 kernel however short
+    their prompts are."""
+    wide = torch.full((table.shape[0], width), -1, dtype=torch.int32)
+    wide[:, :table.shape[1]] = table
+    return wide
+
+
 def _check(out, lse, ref, ref_lse, size, v, steps):
     """Rounding of the output to its type (half a step), and in front of it: a logit is off by its products' and sums' roundings (at
     most 24 accumulations of 2^-23 of sum |q||k|), a probability by twice that, by its exponential (2^-21) and by what its bf16
@@ -100,7 +108,7 @@ def test_values_at_the_ends_of_the_range():
             assert torch.equal(got.nan_to_num(nan=0.0), ref.nan_to_num(nan=0.0))
 
 
-@pytest.mark.parametrize("S", [7, 1025, 3000])
+@pytest.mark.parametrize("S", [7, 1025, 2048, 2049, 3000])
 def test_of_tokens_with_the_same_slot_the_last_one_is_kept(S):
     Nk, D, pool = 2, 64, 3
     k, v = (_rand(1, S, Nk, D, seed=i, dtype=F32) for i in (0, 1))
@@ -115,7 +123,7 @@ def test_of_tokens_with_the_same_slot_the_last_one_is_kept(S):
     assert torch.equal(gk[0].transpose(0, 1).double().cpu(), hk) and torch.equal(gv[0].transpose(0, 1).double().cpu(), hv)
 
 
-@pytest.mark.parametrize("S", [9, 1500])
+@pytest.mark.parametrize("S", [9, 1500, 2500])
 def test_slots_outside_the_cache_are_left_out_and_reported(S):
     Nk, D, pool = 1, 128, S // PAGE + 1
     k, v = (_rand(1, S, Nk, D, seed=i, dtype=BF16) for i in (0, 1))
@@ -171,10 +179,11 @@ def test_several_rows_of_different_number(dtype, N, Nk, D, rows):
     cache, hk, hv = _filled(4 * P + 1, Nk, D, 21, dtype)
     table = _table(4, P, 4 * P + 1, 4)
     q = _rand(4, rows, N, D, seed=6, dtype=dtype).transpose(1, 2)
-    out, lse = ops.cache_attention(q.cuda(), cache, table.cuda(), start.cuda(), length.cuda(), D ** -0.5, q_len=q_len.cuda(), return_lse=True)
     ref, ref_lse, size = ch.attention(q, hk, hv, table, start, length, D ** -0.5, q_len)
-    _check(out, lse, ref, ref_lse, size, hv, 3 * P + 8)
-    assert not out[3].any() and not out[2, rows // 2:].any()
+    for tab in (table, _wide(table)):
+        out, lse = ops.cache_attention(q.cuda(), cache, tab.cuda(), start.cuda(), length.cuda(), D ** -0.5, q_len=q_len.cuda(), return_lse=True)
+        _check(out, lse, ref, ref_lse, size, hv, 3 * P + 8)
+        assert not out[3].any() and not out[2, rows // 2:].any()
     ops.check_status()
 
 
@@ -213,8 +222,9 @@ def test_views_and_a_given_output():
     assert (room[:, 0] == 7).all() and (room[:, -1] == 7).all() and (room[..., D:] == 7).all()
 
 
+@pytest.mark.parametrize("wide", [False, True])
 @pytest.mark.parametrize("dtype,N,R", [(BF16, 4, 5), (F32, 4, 5), (BF16, 4, 3), (BF16, 16, 5), (BF16, 4, 30)])
-def test_what_no_row_sees_has_no_influence(dtype, N, R):
+def test_what_no_row_sees_has_no_influence(dtype, N, R, wide):
     """Pages of NaN scales and arbitrary codes outside the blocks; NaN and infinities in tokens behind a row's own."""
     Nk, D, B = 2, 128, 2
     lens = [[3, 70, 9, R + 7], [64, 1, 0, R]]
@@ -229,7 +239,7 @@ def test_what_no_row_sees_has_no_influence(dtype, N, R):
     cache.fill_(255)
     ops.cache_write(kept_k, kept_v, cache, inside.nonzero().T.int().contiguous().cuda())  # (held values are held as they are)
     q = _rand(B, R, N, D, seed=9, dtype=dtype).transpose(1, 2)
-    args = (q.cuda(), cache, table.cuda(), start.cuda(), length.cuda(), D ** -0.5)
+    args = (q.cuda(), cache, (_wide(table) if wide else table).cuda(), start.cuda(), length.cuda(), D ** -0.5)
     ref, ref_lse, size = ch.attention(q, hk, hv, table, start, length, D ** -0.5)
     out, lse = ops.cache_attention(*args, return_lse=True)
     _check(out, lse, ref, ref_lse, size, hv, 3 * P + 8)
@@ -537,8 +547,9 @@ def test_refused_calls():
         ops.cache_read(cache, torch.zeros(1, 3, dtype=torch.int32))
 
 
+@pytest.mark.parametrize("wide", [False, True])
 @pytest.mark.parametrize("N,Nk,D,rows,tokens", [(8, 2, 128, 70, 700), (16, 2, 64, 33, 5000), (4, 1, 128, 9, 9000), (8, 1, 64, 100, 131)])
-def test_many_rows_over_shares_of_the_pages(N, Nk, D, rows, tokens):
+def test_many_rows_over_shares_of_the_pages(N, Nk, D, rows, tokens, wide):
     """Query blocks long enough for the tensor cores' rows, over as many pages as several CTAs take: the same every time."""
     lens = [[40, tokens // 3, tokens // 2, rows], [3, tokens // 4, 64, rows + 7]]
     start, length, P = ch.spans(lens, False)
@@ -546,7 +557,7 @@ def test_many_rows_over_shares_of_the_pages(N, Nk, D, rows, tokens):
     table = _table(2, P, 2 * P + 1, 14)
     q_len = torch.tensor([rows, rows - 5], dtype=torch.int32)
     q = 3 * _rand(2, rows, N, D, seed=15, dtype=BF16).transpose(1, 2)
-    args = (q.cuda(), cache, table.cuda(), start.cuda(), length.cuda(), D ** -0.5)
+    args = (q.cuda(), cache, (_wide(table, 600) if wide else table).cuda(), start.cuda(), length.cuda(), D ** -0.5)
     ref, ref_lse, size = ch.attention(q, hk, hv, table, start, length, D ** -0.5, q_len)
     first = None
     for _ in range(30):
@@ -567,9 +578,9 @@ def test_logits_that_keep_growing():
     hk = ch.held(k[0].transpose(0, 1).cpu())
     table = torch.arange(P, dtype=torch.int32)[None]
     start, length = torch.zeros(1, 1, dtype=torch.int32), torch.full((1, 1), P * PAGE - 3, dtype=torch.int32)
-    for rows in (1, 2, 9):
+    for rows, tab in ((1, table), (2, table), (9, table), (9, _wide(table))):
         q = _rand(1, rows, N, D, seed=16, dtype=BF16).transpose(1, 2)
-        out, lse = ops.cache_attention(q.cuda(), cache, table.cuda(), start.cuda(), length.cuda(), 0.05, return_lse=True)
+        out, lse = ops.cache_attention(q.cuda(), cache, tab.cuda(), start.cuda(), length.cuda(), 0.05, return_lse=True)
         ref, ref_lse, size = ch.attention(q, hk, hv, table, start, length, 0.05)
         _check(out, lse, ref, ref_lse, size, hv, 64)
 
@@ -583,9 +594,10 @@ def test_more_rows_than_a_cta_takes(dtype, N, Nk, D, rows):
     table = _table(3, P, 3 * P, 18)
     q_len = torch.tensor([rows, 0, max(1, rows - 9)], dtype=torch.int32)
     q = _rand(3, rows, N, D, seed=19, dtype=dtype).transpose(1, 2)
-    out, lse = ops.cache_attention(q.cuda(), cache, table.cuda(), start.cuda(), length.cuda(), D ** -0.5, q_len=q_len.cuda(), return_lse=True)
     ref, ref_lse, size = ch.attention(q, hk, hv, table, start, length, D ** -0.5, q_len)
-    _check(out, lse, ref, ref_lse, size, hv, 3 * P + 8)
+    for tab in (table, _wide(table, 300), _wide(table)):
+        out, lse = ops.cache_attention(q.cuda(), cache, tab.cuda(), start.cuda(), length.cuda(), D ** -0.5, q_len=q_len.cuda(), return_lse=True)
+        _check(out, lse, ref, ref_lse, size, hv, 3 * P + 8)
     ops.check_status()
 
 
@@ -598,9 +610,10 @@ def test_more_blocks_than_a_cta_has_threads(dtype, rows):
     cache, hk, hv = _filled(2 * P, Nk, D, 171, dtype)
     table = _table(2, P, 2 * P, 20)
     q = _rand(2, rows, N, D, seed=21, dtype=dtype).transpose(1, 2)
-    out, lse = ops.cache_attention(q.cuda(), cache, table.cuda(), start.cuda(), length.cuda(), 0.1, return_lse=True)
     ref, ref_lse, size = ch.attention(q, hk, hv, table, start, length, 0.1)
-    _check(out, lse, ref, ref_lse, size, hv, 3 * P + 8)
+    for tab in (table, _wide(table)):
+        out, lse = ops.cache_attention(q.cuda(), cache, tab.cuda(), start.cuda(), length.cuda(), 0.1, return_lse=True)
+        _check(out, lse, ref, ref_lse, size, hv, 3 * P + 8)
     ops.check_status()
 
 
@@ -666,10 +679,10 @@ def test_malformed_prompts_of_many_rows(width):
 
 
 def test_captured_prompts_replay_on_new_inputs():
-    """Calls that take workspaces, as one graph: over a thousand tokens written, read back, a block of many rows over a wide table, one row
+    """Calls that take workspaces, as one graph: over two thousand tokens written, read back, a block of many rows over a wide table, one row
     over a long one, scores."""
     N, Nk, D, B, rows = 8, 2, 128, 2, 40
-    start, length, P = ch.spans([[30, 500, 300, rows], [30, 64, 700, rows]], True)
+    start, length, P = ch.spans([[30, 800, 300, rows], [30, 64, 700, rows]], True)
     S = P * PAGE
     st, ln = start.cuda(), length.cuda()
     table = torch.full((B, 4000), -1, dtype=torch.int32)
@@ -685,7 +698,7 @@ def test_captured_prompts_replay_on_new_inputs():
         ops.cache_write(k, v, cache, slots)
         ck, _ = ops.cache_read(cache, slots)
         return (ck, ops.cache_attention(q, cache, tab, st, ln, 0.1), ops.cache_attention(q[:, :, :1], cache, tab, st, ln, 0.1),
-                ops.cache_doc_scores(q[:, :, :2], cache, tab, st, ln, 0.1, 700)[0])
+                ops.cache_doc_scores(q[:, :, :2], cache, tab, st, ln, 0.1, 800)[0])
     with torch.cuda.stream(torch.cuda.Stream()):
         run()
     torch.cuda.synchronize()
@@ -773,9 +786,10 @@ def test_pages_of_which_only_a_part_is_in_a_block(D, rows):
     cache.fill_(255)
     ops.cache_write(k, v, cache, at)
     q = _rand(1, rows, N, D, seed=29, dtype=BF16).transpose(1, 2)
-    out, lse = ops.cache_attention(q.cuda(), cache, table.cuda(), start.cuda(), length.cuda(), 0.1, return_lse=True)
     ref, ref_lse, size = ch.attention(q, hk, hv, table, start, length, 0.1)
-    _check(out, lse, ref, ref_lse, size, hv, 64)
+    for tab in (table, _wide(table)):
+        out, lse = ops.cache_attention(q.cuda(), cache, tab.cuda(), start.cuda(), length.cuda(), 0.1, return_lse=True)
+        _check(out, lse, ref, ref_lse, size, hv, 64)
     ops.check_status()
 
 
@@ -802,3 +816,25 @@ def test_scores_of_a_document_with_nan(docs, Nk):
     for b in (0, 2):
         assert torch.equal(bad[b], mass[b]) and torch.equal(bad_out[b], out[b])
     ops.check_status()
+
+
+@pytest.mark.parametrize("N,Nk,D", [(32, 8, 128), (16, 8, 64), (8, 8, 128)])
+@pytest.mark.parametrize("rows", [40, 70])
+def test_query_blocks_of_a_batch(N, Nk, D, rows):
+    """So many prompts that each has a CTA of the tcgen05 kernel for a KV head: one tile of rows, two, and more; no parts to join."""
+    B = 40
+    g = torch.Generator().manual_seed(6)
+    lens = [torch.randint(0, 130, (3,), generator=g).tolist() + [rows + b % 3] for b in range(B)]
+    start, length, P = ch.spans(lens, True)
+    cache, hk, hv = _filled(B * P, Nk, D, 231)
+    table = _table(B, P, B * P, 32)
+    q_len = torch.tensor([rows - b % 5 if b % 7 else 0 for b in range(B)], dtype=torch.int32)
+    start[11, 2] = start[11, 1] + length[11, 1] - 1 if lens[11][1] else -1  # malformed
+    q = _rand(B, rows, N, D, seed=33, dtype=BF16).transpose(1, 2)
+    ops.check_status()
+    out, lse = ops.cache_attention(q.cuda(), cache, table.cuda(), start.cuda(), length.cuda(), D ** -0.5, q_len=q_len.cuda(), return_lse=True)
+    with pytest.raises(ValueError, match="of a call on the cache"):
+        ops.check_status()
+    q_len[11] = 0
+    ref, ref_lse, size = ch.attention(q, hk, hv, table, start, length, D ** -0.5, q_len)
+    _check(out, lse, ref, ref_lse, size, hv, 3 * P + 8)
