@@ -838,3 +838,24 @@ def test_query_blocks_of_a_batch(N, Nk, D, rows):
     q_len[11] = 0
     ref, ref_lse, size = ch.attention(q, hk, hv, table, start, length, D ** -0.5, q_len)
     _check(out, lse, ref, ref_lse, size, hv, 3 * P + 8)
+
+
+@pytest.mark.parametrize("dtype,N,Nk,D,T", [(BF16, 4, 1, 64, 2500), (F32, 4, 1, 64, 1100), (BF16, 2, 2, 128, 1300)])
+def test_a_whole_sequence_at_once(dtype, N, Nk, D, T):
+    """As many rows as there are tokens: each sees those up to its own."""
+    P = -(-T // PAGE)
+    cache, hk, hv = _filled(P, Nk, D, 241, dtype)
+    table = _table(1, P, P, 34)
+    start, length = torch.zeros(1, 1, dtype=torch.int32), torch.full((1, 1), T, dtype=torch.int32)
+    q = _rand(1, T, N, D, seed=35, dtype=dtype).transpose(1, 2)
+    at = ch.slots_of(table[0], torch.arange(T))
+    k, v = (x[at].repeat_interleave(N // Nk, 1).transpose(0, 1) for x in (hk, hv))
+    x = q[0].double() @ k.transpose(1, 2) * 0.1
+    late = torch.ones(T, T).triu(1).bool()
+    ref_lse = torch.logsumexp(x.masked_fill(late, -torch.inf), -1)[None]
+    ref = (torch.softmax(x.masked_fill(late, -torch.inf), -1) @ v).transpose(0, 1)[None]
+    size = (q[0].double().abs() @ k.abs().transpose(1, 2) * 0.1).amax()
+    for tab in (table, _wide(table)):
+        out, lse = ops.cache_attention(q.cuda(), cache, tab.cuda(), start.cuda(), length.cuda(), 0.1, return_lse=True)
+        _check(out, lse, ref, ref_lse, size, hv, 3 * P + 8)
+    ops.check_status()
