@@ -5,7 +5,8 @@
 // largest value off: 7 / (1 - 2^-5) < 7.5.
 // Both decisions are those of exact arithmetic.  A border of n is (k + 1/2) s, 4 bits times 5; of s, a 6-bit number times 7:
 // representable, so a 32-bit x is either equal to it or off by more than half a last place of the quotient, and a correctly
-// rounded quotient lies on the border only if x does.  Where that costs too much, see quantise().
+// rounded quotient lies on the border only if x does.  (Of a quotient that is a normal number; for others see group_scale().)  Where
+// that costs too much, see quantise().
 #include <algorithm>
 
 #include "cache_layout.cuh"
@@ -98,14 +99,19 @@ __device__ __forceinline__ void reduce_largest(uint32_t (&m)[kGroups]) {
 }
 
 // The scale of a group whose largest magnitude has these bits, NaN where it holds NaN or an infinity.
+// fp32 below 7 * 2^-126, where amax / 7 is subnormal and would be rounded before it is brought to the grid of 2^-130: the quotient is
+// taken 2^32 times as large, and a sum with 1.5 * 2^-75, whose last place is 2^-98, rounds it once.
 template <typename T>
 __device__ __forceinline__ float group_scale(uint32_t top) {
   constexpr bool kBf16 = sizeof(T) == 2;
   if (kBf16) top <<= 16;
   const float amax = __uint_as_float(top);
-  uint32_t b = __float_as_uint(kBf16 ? amax * 0x1.24924ap-3f : __fdiv_rn(amax, 7.f));
+  const bool fine = !kBf16 && amax < 0x1.cp-124f;
+  uint32_t b = __float_as_uint(kBf16 ? amax * 0x1.24924ap-3f : __fdiv_rn(fine ? amax * 0x1p32f : amax, 7.f));
   if (kBf16) b = (b + 0x200u) & ~0x3FFu;
-  return top < 0x7F800000u ? fminf(__uint_as_float((b + 0x3FFFFu + ((b >> 19) & 1u)) & ~0x7FFFFu), kLargestScale) : NAN;
+  float s = fminf(__uint_as_float((b + 0x3FFFFu + ((b >> 19) & 1u)) & ~0x7FFFFu), kLargestScale);
+  if (fine) s = __fadd_rn(__fadd_rn(__uint_as_float(b), 0x1.8p-75f), -0x1.8p-75f) * 0x1p-32f;
+  return top < 0x7F800000u ? s : NAN;
 }
 
 // kN values over a scale, as codes, value i in bits 4 i .. 4 i + 3; r: the reciprocal of the scale, 0 for a scale that is 0 or NaN.

@@ -859,3 +859,21 @@ def test_a_whole_sequence_at_once(dtype, N, Nk, D, T):
         out, lse = ops.cache_attention(q.cuda(), cache, tab.cuda(), start.cuda(), length.cuda(), 0.1, return_lse=True)
         _check(out, lse, ref, ref_lse, size, hv, 3 * P + 8)
     ops.check_status()
+
+
+def test_scales_next_to_the_borders_of_the_smallest_ones():
+    """fp32 groups whose largest magnitude is 7 (k + 1/2) 2^-130 or up to three last places of it away: the scale's grid is that of 2^-130
+    there, and a seventh of such a magnitude is no normal number."""
+    k = torch.arange(0, 17, dtype=torch.float64) + 0.5
+    top = torch.ldexp(7 * k, torch.tensor(-130)).float()
+    top = (top.view(torch.int32)[:, None] + torch.arange(-3, 4, dtype=torch.int32)).flatten().view(F32)
+    g = torch.linspace(-1, 1, 32, dtype=torch.float64)
+    x = (top.double()[:, None] * g).float()
+    x[:, 0] = top
+    x = torch.cat([x, x.flip(-1)], -1)[None, None]  # (B, Nk, S, D)
+    slots = torch.arange(x.shape[2], dtype=torch.int32)[None]
+    cache = ops.cache_alloc(2, 1, 64, "cuda")
+    ops.cache_write(x.cuda(), -x.cuda(), cache, slots.cuda())
+    for got, src in zip(ops.cache_read(cache, slots.cuda(), F32), (x, -x)):
+        assert torch.equal(got.double().cpu(), ch.held(src))
+    ops.check_status()
