@@ -69,14 +69,12 @@ __global__ void __launch_bounds__(kThreads, kTiles == 1 && sizeof(T) == 2 ? 3 : 
 
   const int32_t* const table = a.table + (int64_t)b * a.P;
 
-  // document d's span (length 0 if it is malformed) and its pages
+  // document d's span (length 0 in a prompt with a malformed block, which has no documents) and its pages
+  bool bad = false;
   auto span = [&](int d, int& start, int& len) {
-    start = bs[d + 1];
-    len = bl[d + 1];
-    if (span_is_bad(bs, bl, d + 1, (int64_t)a.P * kPage) || len > a.max_block_len) {
-      if (a.status) atomicCAS(a.status, 0, kStatusBadCacheCall);
-      len = 0;
-    }
+    const int2 x = d < kThreads ? s_span[d] : make_int2(bs[d + 1], bl[d + 1]);
+    start = x.x;
+    len = bad ? 0 : x.y;
   };
   auto pages_of = [](int start, int len) { return len > 0 ? (start + len - 1) / kPage - start / kPage + 1 : 0; };
   auto warp_scan = [&](int x) {
@@ -89,10 +87,12 @@ __global__ void __launch_bounds__(kThreads, kTiles == 1 && sizeof(T) == 2 ? 3 : 
   };
 
   // ---- this CTA's documents: those whose first page is in its share of all documents' pages ----
-  int my_start = 0, my_len = 0;
   s_table[tid] = tid < a.P ? table[tid] : -1;
-  if (tid < nd) span(tid, my_start, my_len);
-  s_span[tid] = make_int2(my_start, my_len);
+  for (int m = tid; m < a.M; m += kThreads) {
+    const bool doc = m > 0 && m < a.M - 1;
+    bad |= span_is_bad(bs, bl, m, (int64_t)a.P * kPage) || (doc && bl[m] > a.max_block_len);
+    if (doc && m <= kThreads) s_span[m - 1] = make_int2(bs[m], bl[m]);
+  }
   typename QueryRows<T, D, kTiles>::Raw raw;
   QueryRows<T, D, kTiles>::fetch([&](int c) -> const T* {
     const int r = row0 + c;
@@ -101,6 +101,8 @@ __global__ void __launch_bounds__(kThreads, kTiles == 1 && sizeof(T) == 2 ? 3 : 
   }, g, t, raw);
   int64_t lo = 0, hi = 0;
   if (tid < 2) s_before[tid] = 0;
+  bad = __syncthreads_or(bad);
+  if (bad && tid == 0 && a.status) atomicCAS(a.status, 0, kStatusBadCacheCall);
   // All pages (pass 0); then the number of documents that begin before the share, and before its end.  Up to kThreads documents are
   // looked at once.
 #pragma unroll 1
@@ -108,8 +110,8 @@ __global__ void __launch_bounds__(kThreads, kTiles == 1 && sizeof(T) == 2 ? 3 : 
     int64_t before = 0;
 #pragma unroll 1
     for (int d0 = 0; d0 < nd; d0 += kThreads) {
-      int st = my_start, ln = my_len;
-      if (d0 > 0 && d0 + tid < nd) span(d0 + tid, st, ln);
+      int st = 0, ln = 0;
+      if (d0 + tid < nd) span(d0 + tid, st, ln);
       const int n = d0 + tid < nd ? pages_of(st, ln) : 0, x = warp_scan(n);
       if (lane == 31) s_scan[warp] = x;
       __syncthreads();
@@ -162,14 +164,7 @@ __global__ void __launch_bounds__(kThreads, kTiles == 1 && sizeof(T) == 2 ? 3 : 
   for (int doc0 = s_before[0]; doc0 < doc_end; doc0 += kDocs) {
     const int n_docs = min(kDocs, doc_end - doc0);
     int start = 0, len = 0;  // lane l: of document doc0 + l
-    if (lane < n_docs) {
-      if (doc0 + lane < kThreads) {
-        start = s_span[doc0 + lane].x;
-        len = s_span[doc0 + lane].y;
-      } else {
-        span(doc0 + lane, start, len);
-      }
-    }
+    if (lane < n_docs) span(doc0 + lane, start, len);
     const int n = pages_of(start, len);
     const int end = warp_scan(n), pages = __shfl_sync(0xffffffffu, end, 31);
     const int from = (int)((int64_t)pages * warp / kWarps), to = (int)((int64_t)pages * (warp + 1) / kWarps);

@@ -167,7 +167,9 @@ def cache_doc_scores(q: torch.Tensor, cache: torch.Tensor, page_table: torch.Ten
     """:func:`doc_scores` with the document keys from the cache.
 
     q (B,N,R,D): the signal rows' queries; page table and spans as for :func:`cache_attention` (blocks 1..M-2 are the documents), of
-    documents of up to ``max_block_len`` tokens.  Returns (doc_mass (B,N,R,num_docs) fp32, logits (B,num_docs) fp32).
+    documents of up to ``max_block_len`` tokens.  Returns (doc_mass (B,N,R,num_docs) fp32, logits (B,num_docs) fp32).  A prompt with
+    malformed spans (of whichever block) or a longer document gets zeros, a page that does not exist takes its tokens away; both raise
+    at the next :func:`check_status`.
     """
     return _lib.host().cache_doc_scores(q, cache, page_table, blk_start, blk_len, scale, int(max_block_len), temperature)
 

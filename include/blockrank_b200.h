@@ -255,9 +255,10 @@ BRK_API int brk_raw_scores_bwd(const brk_score_params* p, const void* d_raw, con
  * nearest integer (ties to even) within -7..7 (0 where s is 0).  The value is n s, exact in bf16: 4.5 bits per channel.  A group
  * that holds NaN or an infinity reads as NaN in all its channels.  The order of the bytes in a page is the library's own.
  *
- * The device checks what a call reads there: a slot outside the pool, a page number outside [0, n_pages) that a block needs,
- * spans that overlap, are out of order or reach past the page table, too many rows -- it sets the status word (BRK_E_ARG at
- * brk_status_poll) and leaves that token, page or prompt out. */
+ * The device checks what a call reads there and sets the status word (BRK_E_ARG at brk_status_poll).  A slot outside the pool
+ * leaves its token out, a page number outside [0, n_pages) that a block needs the page's tokens.  A prompt with a malformed block --
+ * blocks that overlap, are out of order or reach past the page table, whether the call reads them or not; in the scores a
+ * document longer than max_block_len; in the attention too many rows -- is left out whole: zeros. */
 #define BRK_CACHE_PAGE 64
 typedef struct brk_cache {
   void* pages;

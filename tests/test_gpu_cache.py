@@ -877,3 +877,77 @@ def test_scales_next_to_the_borders_of_the_smallest_ones():
     for got, src in zip(ops.cache_read(cache, slots.cuda(), F32), (x, -x)):
         assert torch.equal(got.double().cpu(), ch.held(src))
     ops.check_status()
+
+
+@pytest.mark.parametrize("docs", [3, 40, 200])
+def test_scores_of_a_prompt_with_a_malformed_block(docs):
+    """One malformed block, whichever it is, leaves its whole prompt without documents; a page that does not exist only takes its own tokens
+    away.  Each is reported by itself; the other prompts have their masses and logits.  (Prompts whose CTAs make the logits
+    themselves, prompts that are merged, more documents than a CTA has threads.)"""
+    N, Nk, D, R, most = 4, 2, 64, 2, 70
+    lens = [9] + [most - (i % 7) for i in range(docs)] + [12]
+    start, length, P = ch.spans([lens], True)
+    broken = {
+        "none": None,
+        "a document that runs into the next one": lambda st, ln: st[docs].fill_(int(st[docs - 1] + ln[docs - 1]) - 1),
+        "a document that is too long": lambda st, ln: ln[2].fill_(most + 1),
+        "the last document runs into the query block": lambda st, ln: st[-1].fill_(int(st[-2] + ln[-2]) - 1),
+        "an instruction block of negative length": lambda st, ln: ln[0].fill_(-1),
+        "an instruction block in front of the first slot": lambda st, ln: st[0].fill_(-1),
+        "an instruction block that runs into the first document": lambda st, ln: ln[0].fill_(int(st[1]) + 1),
+        "a query block behind the page table": lambda st, ln: st[-1].fill_(P * PAGE - 11),
+        "no page": "page",
+    }
+    B = len(broken)
+    pool = B * P + 1
+    cache, hk, _ = _filled(pool, Nk, D, 251)
+    table = _table(B, P, pool, 36)
+    q = _rand(B, R, N, D, seed=37, dtype=BF16).transpose(1, 2)
+    st, ln, tab = start.repeat(B, 1), length.repeat(B, 1), table.clone()
+    seen_st, seen_ln = st.clone(), ln.clone()  # what is left to be seen
+    for b, (name, how) in enumerate(broken.items()):
+        if how == "page":  # of the second document's two pages the last one
+            tab[b, int(start[0, 2]) // PAGE + 1] = pool
+            seen_ln[b, 2] = PAGE
+        elif how is not None:
+            how(st[b], ln[b])
+            seen_ln[b] = 0
+    ref = ch.doc_mass(q, hk, table, seen_st, seen_ln, 0.2)
+    assert bool((ref[0] > 0).all()) and bool((ref[-1] > 0).all())
+    size = float(torch.einsum("bnrd,snd->bnrs", q.double().abs(), hk.abs().repeat_interleave(N // Nk, 1)).max()) * 0.2
+    rel = 2 * size * 24 * 2.0 ** -23 + 64 * 2.0 ** -23  # (as in test_document_scores)
+    assert rel < 1 / (4 * docs)  # (a document too many or too few shows)
+    ops.check_status()
+
+    def check(of):
+        mass, logits = ops.cache_doc_scores(q[of].cuda(), cache, tab[of].cuda(), st[of].cuda(), ln[of].cuda(), 0.2, most)
+        assert torch.allclose(mass.double().cpu(), ref[of], rtol=rel, atol=0)
+        assert torch.allclose(logits.double().cpu(), ref[of].mean((1, 2)) / 0.05, rtol=2 * rel, atol=0)
+    for b in range(B):
+        check(slice(b, b + 1))
+        if b == 0:
+            ops.check_status()
+        else:
+            with pytest.raises(ValueError, match="of a call on the cache"):
+                ops.check_status()
+    check(slice(0, B))
+    with pytest.raises(ValueError, match="of a call on the cache"):
+        ops.check_status()
+
+
+def test_a_document_behind_one_that_is_too_long_only():
+    """Overlap and length each alone: a document longer than max_block_len that touches no other."""
+    N, Nk, D = 4, 2, 64
+    start, length, P = ch.spans([[3, 70, 60, 9]], True, gap=PAGE)
+    cache, hk, _ = _filled(P, Nk, D, 261)
+    table = _table(1, P, P, 38)
+    q = _rand(1, 1, N, D, seed=39, dtype=BF16).transpose(1, 2)
+    args = (q.cuda(), cache, table.cuda(), start.cuda(), length.cuda(), 0.2)
+    ops.check_status()
+    mass, logits = ops.cache_doc_scores(*args, 70)
+    ops.check_status()
+    assert torch.allclose(mass.double().cpu(), ch.doc_mass(q, hk, table, start, length, 0.2), rtol=1e-4)
+    mass, logits = ops.cache_doc_scores(*args, 69)
+    with pytest.raises(ValueError, match="of a call on the cache"):
+        ops.check_status()
+    assert not mass.any() and not logits.any()
