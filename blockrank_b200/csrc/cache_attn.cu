@@ -27,7 +27,8 @@ using namespace cache;
 
 constexpr int kWarps = 4;
 constexpr int kThreads = 32 * kWarps;
-constexpr int kShare = 128;       // pages a CTA takes at most
+constexpr int kAtOnce = 128;      // pages of its share that a CTA knows of at a time
+constexpr int kWorthwhile = 128;  // pages that are worth a share of their own where there are more than 64
 constexpr int kParts = 3;         // K or V parts of pages that a warp has room for in shared memory: two K, one V
 constexpr int kFewJoins = 4;      // rows per SM that are joined by a CTA each
 constexpr int kCluster = 8;       // shares that a cluster joins, at most (fp32, 3 prompts of 20 documents: 8.0 us, joined by a kernel 8.6)
@@ -37,15 +38,18 @@ constexpr int ctas_per_sm = kTiles == 1 && sizeof(T) == 2 ? 3 : 2;
 
 // kTwice: up to 4 rows, each in columns c and c + 4: the higher 8 bits of P go into one, the rest into the other, and one MMA takes
 // both.
-template <typename T, int D, int kTiles, bool kTwice>
+// kLong: a share can have more than kAtOnce pages.  (The code for that costs the others a little: one row each of 16 prompts of 100 documents
+// 81.4 us, without it 80.9; of 4 in fp32 40.7 and 40.0.)
+template <typename T, int D, int kTiles, bool kTwice, bool kLong>
 __global__ void __launch_bounds__(kThreads, ctas_per_sm<T, kTiles>) cache_attn_kernel(CacheAttnArgs a) {
   using L = Layout<D>;
   constexpr bool kF32 = sizeof(T) == 4;
   constexpr int kP = kF32 ? 3 : 2, kMmas = kTwice ? 1 : kP;
   constexpr int kCols = 8 * kTiles, kRows = kTwice ? 4 : kCols;
   extern __shared__ __align__(16) unsigned char smem[];  // [kWarps][kParts][part]; at the end the warps' outputs
-  __shared__ uint32_t s_mask[2 * kShare];                // which tokens of the CTA's pages lie in a block
-  __shared__ int32_t s_page[kShare];
+  __shared__ uint32_t s_mask[2 * kAtOnce];               // which tokens of the CTA's pages lie in a block
+  __shared__ int32_t s_page[kAtOnce];
+  __shared__ Prompt<kThreads> s_prompt;
   __shared__ float2 s_ml[kWarps][kCols];
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
@@ -55,14 +59,15 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<T, kTiles>) cache_attn_k
   ptx::grid_dependency_wait();  // (inputs of this call; the workspace of the one in front)
 
   typename QueryRows<T, D, kTiles>::Raw raw;
-  const Share sh = find_share<kThreads, kShare>(a, b, row0, kRows, share, kWarps, s_mask, s_page, [&] {
+  const Share sh = find_share<kAtOnce>(a, b, row0, kRows, share, kWarps, s_prompt, s_mask, s_page, [&] {
     QueryRows<T, D, kTiles>::fetch([&](int c) -> const T* {  // (rows from q_len on among them: they are not used)
       const int r = row0 + (kTwice ? c & 3 : c);
       if (r >= a.Lq * G) return nullptr;
       return reinterpret_cast<const T*>(a.q.ptr) + (int64_t)b * a.q.sb + (int64_t)(kvh * G + r % G) * a.q.sh + (int64_t)(r / G) * a.q.ss;
     }, g, t, raw);
   });
-  const int n = sh.n, n_rows = sh.n_rows, page0 = sh.page0, first_slot = sh.first_slot;
+  const int n_rows = sh.n_rows, first_slot = sh.first_slot;
+  int page0 = sh.page0, n = kLong ? min(sh.n, kAtOnce) : sh.n;  // the pages at hand
 
   // Copies are requested in the order K0 K1 V0 K2 V1 K3 ..., each into the place of the part that has just been used.
   unsigned char* const ring = smem + warp * kParts * L::kHalf;
@@ -82,9 +87,12 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<T, kTiles>) cache_attn_k
     cp_async_commit();
   };
   int i = next(warp), ahead = next(i + kWarps);  // the page in hand, and the one whose K is requested next
-  request(i, 0, 0);
-  request(ahead, 0, 1);
-  request(i, 1, 2);
+  auto begin = [&] {
+    request(i, 0, 0);
+    request(ahead, 0, 1);
+    request(i, 1, 2);
+  };
+  begin();
 
   // ---- the rows ----
   QueryRows<T, D, kTiles> q;
@@ -112,206 +120,218 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<T, kTiles>) cache_attn_k
     }
 
   int place = 0;  // of the page's K
-  while (i < n) {
-    const int i1 = ahead;
-    ahead = next(ahead + kWarps);
-    cp_async_wait<2>();
-    __syncwarp();
-    const int slot0 = (page0 + i) * kPage;
-    const uint32_t m_lo = s_mask[2 * i], m_hi = s_mask[2 * i + 1];
-    const bool ragged = (m_lo & m_hi) != ~0u, late = slot0 + kPage - 1 > first_lim;  // tokens that no row sees, that some do not see
-    float s[kTiles][4][4];
-    q.logits(ring + place * L::kHalf, g, t, s);
-    __syncwarp();
-    request(ahead, 0, place);
-    place ^= 1;
+  for (;;) {
+    while (i < n) {
+      const int i1 = ahead;
+      ahead = next(ahead + kWarps);
+      cp_async_wait<2>();
+      __syncwarp();
+      const int slot0 = (page0 + i) * kPage;
+      const uint32_t m_lo = s_mask[2 * i], m_hi = s_mask[2 * i + 1];
+      const bool ragged = (m_lo & m_hi) != ~0u, late = slot0 + kPage - 1 > first_lim;  // tokens that no row sees, that some do not see
+      float s[kTiles][4][4];
+      q.logits(ring + place * L::kHalf, g, t, s);
+      __syncwarp();
+      request(ahead, 0, place);
+      place ^= 1;
 
-    // ---- softmax ----
-    // (A page's last tokens are worked on whether they count or not: left out 16 at a time, with a branch each, two contexts of
-    // 131,072 tokens took 77 us, not 69; with code of their own for pages that end early 16 prompts of 100 documents 100, not 87.)
-    if (ragged) {
-      const uint32_t lo = m_lo >> g, hi = m_hi >> g;  // this lane's keys: every eighth bit
+      // ---- softmax ----
+      // (A page's last tokens are worked on whether they count or not: left out 16 at a time, with a branch each, two contexts of
+      // 131,072 tokens took 77 us, not 69; with code of their own for pages that end early 16 prompts of 100 documents 100, not 87.)
+      if (ragged) {
+        const uint32_t lo = m_lo >> g, hi = m_hi >> g;  // this lane's keys: every eighth bit
 #pragma unroll
-      for (int k = 0; k < 4; ++k)
+        for (int k = 0; k < 4; ++k)
 #pragma unroll
-        for (int y = 0; y < 2; ++y)
-          if (!((k < 2 ? lo : hi) & (1u << (16 * (k & 1) + 8 * y)))) {
+          for (int y = 0; y < 2; ++y)
+            if (!((k < 2 ? lo : hi) & (1u << (16 * (k & 1) + 8 * y)))) {
 #pragma unroll
-            for (int c = 0; c < kTiles; ++c) s[c][k][2 * y] = s[c][k][2 * y + 1] = -INFINITY;
+              for (int c = 0; c < kTiles; ++c) s[c][k][2 * y] = s[c][k][2 * y + 1] = -INFINITY;
+            }
+      }
+      if (late) {
+#pragma unroll
+        for (int c = 0; c < kTiles; ++c)
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            const int last = lim[c][x] - slot0 - g;
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+#pragma unroll
+              for (int y = 0; y < 2; ++y)
+                if (16 * k + 8 * y > last) s[c][k][2 * y + x] = -INFINITY;
           }
-    }
-    if (late) {
+      }
+      float scale_o[kTiles][2];
+      bool grown = false;
 #pragma unroll
       for (int c = 0; c < kTiles; ++c)
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
-          const int last = lim[c][x] - slot0 - g;
+          float top = mx[c][x];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) top = fmaxf(top, fmaxf(s[c][k][x], s[c][k][2 + x]));
+#pragma unroll
+          for (int off = 4; off <= 16; off <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+          const float ref = top == -INFINITY ? 0.f : top * sl2[c][x];
+          scale_o[c][x] = ptx::ex2(mx[c][x] * sl2[c][x] - ref);  // (2^-inf = 0 in front of the first page)
+          grown |= top > mx[c][x];
+          mx[c][x] = top;
+          sum[c][x] *= scale_o[c][x];
 #pragma unroll
           for (int k = 0; k < 4; ++k)
 #pragma unroll
-            for (int y = 0; y < 2; ++y)
-              if (16 * k + 8 * y > last) s[c][k][2 * y + x] = -INFINITY;
+            for (int y = 0; y < 2; ++y) {
+              const float p = ptx::ex2(fmaf(s[c][k][2 * y + x], sl2[c][x], -ref));
+              s[c][k][2 * y + x] = p;
+              sum[c][x] += p;
+            }
         }
-    }
-    float scale_o[kTiles][2];
-    bool grown = false;
+      if (__any_sync(0xffffffffu, grown)) {
 #pragma unroll
-    for (int c = 0; c < kTiles; ++c)
+        for (int c = 0; c < kTiles; ++c)
 #pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        float top = mx[c][x];
+          for (int j = 0; j < L::kGroups; ++j)
 #pragma unroll
-        for (int k = 0; k < 4; ++k) top = fmaxf(top, fmaxf(s[c][k][x], s[c][k][2 + x]));
+            for (int y = 0; y < 2; ++y)
 #pragma unroll
-        for (int off = 4; off <= 16; off <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
-        const float ref = top == -INFINITY ? 0.f : top * sl2[c][x];
-        scale_o[c][x] = ptx::ex2(mx[c][x] * sl2[c][x] - ref);  // (2^-inf = 0 in front of the first page)
-        grown |= top > mx[c][x];
-        mx[c][x] = top;
-        sum[c][x] *= scale_o[c][x];
+              for (int x = 0; x < 4; ++x) o[c][j][y][x] *= scale_o[c][x & 1];
+      }
+
+      // ---- O^T += V^T P^T ----
+      cp_async_wait<1>();
+      __syncwarp();
+      const unsigned char* const page = ring + 2 * L::kHalf - L::kHalf;  // (the third part; offsets count from a page's beginning)
+      // The tensor cores cut a sum off rather than round it, so in 32 bits a page has sums of its own.
+      float fresh[kF32 ? kTiles : 1][L::kGroups][2][4] = {};
+      auto& sums = [&]() -> float (&)[kTiles][L::kGroups][2][4] {
+        if constexpr (kF32) return fresh;
+        else return o;
+      }();
 #pragma unroll
-        for (int k = 0; k < 4; ++k)
+      for (int k = 0; k < 4; ++k) {
+        uint32_t pt[kTiles][2][kMmas];
+#pragma unroll
+        for (int c = 0; c < kTiles; ++c)
 #pragma unroll
           for (int y = 0; y < 2; ++y) {
-            const float p = ptx::ex2(fmaf(s[c][k][2 * y + x], sl2[c][x], -ref));
-            s[c][k][2 * y + x] = p;
-            sum[c][x] += p;
+            uint32_t piece[kP];
+            split2<kP>(s[c][k][2 * y], s[c][k][2 * y + 1], piece);
+            if constexpr (kTwice) {
+              pt[c][y][0] = transpose8(t < 2 ? piece[0] : piece[1]);
+            } else {
+#pragma unroll
+              for (int x = 0; x < kP; ++x) pt[c][y][x] = transpose8(piece[x]);
+            }
           }
-      }
-    if (__any_sync(0xffffffffu, grown)) {
-#pragma unroll
-      for (int c = 0; c < kTiles; ++c)
-#pragma unroll
-        for (int j = 0; j < L::kGroups; ++j)
-#pragma unroll
-          for (int y = 0; y < 2; ++y)
-#pragma unroll
-            for (int x = 0; x < 4; ++x) o[c][j][y][x] *= scale_o[c][x & 1];
-    }
-
-    // ---- O^T += V^T P^T ----
-    cp_async_wait<1>();
-    __syncwarp();
-    const unsigned char* const page = ring + 2 * L::kHalf - L::kHalf;  // (the third part; offsets count from a page's beginning)
-    // The tensor cores cut a sum off rather than round it, so in 32 bits a page has sums of its own.
-    float fresh[kF32 ? kTiles : 1][L::kGroups][2][4] = {};
-    auto& sums = [&]() -> float (&)[kTiles][L::kGroups][2][4] {
-      if constexpr (kF32) return fresh;
-      else return o;
-    }();
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      uint32_t pt[kTiles][2][kMmas];
-#pragma unroll
-      for (int c = 0; c < kTiles; ++c)
-#pragma unroll
-        for (int y = 0; y < 2; ++y) {
-          uint32_t piece[kP];
-          split2<kP>(s[c][k][2 * y], s[c][k][2 * y + 1], piece);
-          if constexpr (kTwice) {
-            pt[c][y][0] = transpose8(t < 2 ? piece[0] : piece[1]);
-          } else {
-#pragma unroll
-            for (int x = 0; x < kP; ++x) pt[c][y][x] = transpose8(piece[x]);
-          }
-        }
-      // pairs of tokens 16 k + 2 t (v[0]) and 16 k + 8 + 2 t (v[1]); words of the even token, then of the odd one
-      uint32_t v[2][2 * (L::kGroups / 2)], sv[2][L::kGroups];
-#pragma unroll
-      for (int y = 0; y < 2; ++y) {
-        const int tok = 16 * k + 8 * y + 2 * t;
-        const unsigned char *pv = page + L::v_word(tok, g, 0), *ps = page + L::v_scale(tok, 0);
-        if constexpr (D == 128) {
-          *reinterpret_cast<uint4*>(v[y]) = *reinterpret_cast<const uint4*>(pv);
-          *reinterpret_cast<uint4*>(sv[y]) = *reinterpret_cast<const uint4*>(ps);
-        } else {
-          *reinterpret_cast<uint2*>(v[y]) = *reinterpret_cast<const uint2*>(pv);
-          *reinterpret_cast<uint2*>(sv[y]) = *reinterpret_cast<const uint2*>(ps);
-        }
-      }
-      if (ragged) {  // values of tokens that no row sees are zeros: 0 x NaN would reach every row
+        // pairs of tokens 16 k + 2 t (v[0]) and 16 k + 8 + 2 t (v[1]); words of the even token, then of the odd one
+        uint32_t v[2][2 * (L::kGroups / 2)], sv[2][L::kGroups];
 #pragma unroll
         for (int y = 0; y < 2; ++y) {
           const int tok = 16 * k + 8 * y + 2 * t;
-          const uint32_t in = (tok < 32 ? m_lo : m_hi) >> (tok & 31);
-          const uint32_t keep = ((in & 1) ? 0xFFFFu : 0u) | ((in & 2) ? 0xFFFF0000u : 0u);
-#pragma unroll
-          for (int j = 0; j < L::kGroups; ++j) sv[y][j] &= keep;
+          const unsigned char *pv = page + L::v_word(tok, g, 0), *ps = page + L::v_scale(tok, 0);
+          if constexpr (D == 128) {
+            *reinterpret_cast<uint4*>(v[y]) = *reinterpret_cast<const uint4*>(pv);
+            *reinterpret_cast<uint4*>(sv[y]) = *reinterpret_cast<const uint4*>(ps);
+          } else {
+            *reinterpret_cast<uint2*>(v[y]) = *reinterpret_cast<const uint2*>(pv);
+            *reinterpret_cast<uint2*>(sv[y]) = *reinterpret_cast<const uint2*>(ps);
+          }
         }
-      }
-      if (late) {
-        uint32_t nan = 0;  // (a scale of all ones in the exponent is NaN)
+        if (ragged) {  // values of tokens that no row sees are zeros: 0 x NaN would reach every row
 #pragma unroll
-        for (int y = 0; y < 2; ++y)
+          for (int y = 0; y < 2; ++y) {
+            const int tok = 16 * k + 8 * y + 2 * t;
+            const uint32_t in = (tok < 32 ? m_lo : m_hi) >> (tok & 31);
+            const uint32_t keep = ((in & 1) ? 0xFFFFu : 0u) | ((in & 2) ? 0xFFFF0000u : 0u);
 #pragma unroll
-          for (int j = 0; j < L::kGroups; ++j) nan |= __vcmpeq2(sv[y][j] & 0x7F807F80u, 0x7F807F80u);
-        if (__any_sync(0xffffffffu, nan != 0)) {
-          // A value that is NaN belongs to the rows that see it and to no other: out of the product, into their outputs.
+            for (int j = 0; j < L::kGroups; ++j) sv[y][j] &= keep;
+          }
+        }
+        if (late) {
+          uint32_t nan = 0;  // (a scale of all ones in the exponent is NaN)
 #pragma unroll
           for (int y = 0; y < 2; ++y)
 #pragma unroll
-            for (int j = 0; j < L::kGroups; ++j) {
-              const uint32_t is = __vcmpeq2(sv[y][j] & 0x7F807F80u, 0x7F807F80u);
-              sv[y][j] &= ~is;
-              int earliest = INT_MAX;  // slot of the first such token of these 8
-              const int at = slot0 + 16 * k + 8 * y + 2 * t;
-              if (is & 0xFFFF0000u) earliest = at + 1;
-              if (is & 0xFFFFu) earliest = at;
-              earliest = min(earliest, __shfl_xor_sync(0xffffffffu, earliest, 1));
-              earliest = min(earliest, __shfl_xor_sync(0xffffffffu, earliest, 2));
+            for (int j = 0; j < L::kGroups; ++j) nan |= __vcmpeq2(sv[y][j] & 0x7F807F80u, 0x7F807F80u);
+          if (__any_sync(0xffffffffu, nan != 0)) {
+            // A value that is NaN belongs to the rows that see it and to no other: out of the product, into their outputs.
+#pragma unroll
+            for (int y = 0; y < 2; ++y)
+#pragma unroll
+              for (int j = 0; j < L::kGroups; ++j) {
+                const uint32_t is = __vcmpeq2(sv[y][j] & 0x7F807F80u, 0x7F807F80u);
+                sv[y][j] &= ~is;
+                int earliest = INT_MAX;  // slot of the first such token of these 8
+                const int at = slot0 + 16 * k + 8 * y + 2 * t;
+                if (is & 0xFFFF0000u) earliest = at + 1;
+                if (is & 0xFFFFu) earliest = at;
+                earliest = min(earliest, __shfl_xor_sync(0xffffffffu, earliest, 1));
+                earliest = min(earliest, __shfl_xor_sync(0xffffffffu, earliest, 2));
+#pragma unroll
+                for (int c = 0; c < kTiles; ++c)
+#pragma unroll
+                  for (int x = 0; x < 4; ++x)
+                    if (earliest <= lim[c][x & 1]) o[c][j][0][x] = o[c][j][1][x] = NAN;
+              }
+          }
+        }
+#pragma unroll
+        for (int w = 0; w < L::kGroups / 2; ++w) {
+          // the four bytes of each token, shifted by bytes: codes 2 i and 2 i + 1 of both in bits 3..6 and 7..10 of their halves
+          uint32_t x[2][4];
+#pragma unroll
+          for (int y = 0; y < 2; ++y) {
+            const uint32_t even = v[y][w], odd = v[y][L::kGroups / 2 + w];
+            x[y][0] = __byte_perm(even, odd, 0x5410);
+            x[y][1] = __byte_perm(even, odd, 0x6521);
+            x[y][2] = __byte_perm(even, odd, 0x7632);
+            x[y][3] = __byte_perm(even, odd, 0x4703);
+          }
+#pragma unroll
+          for (int z = 0; z < 2; ++z) {
+            const int j = 2 * w + z;
+            uint32_t c2[2];
+#pragma unroll
+            for (int y = 0; y < 2; ++y) c2[y] = scale_offset(sv[y][j]);
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {  // channels 4 g + 2 u, 4 g + 2 u + 1 of group j
+              const uint32_t e0 = held(codes, x[0][2 * z + u], sv[0][j], c2[0]), e1 = held(codes, x[0][2 * z + u] >> 4, sv[0][j], c2[0]);
+              const uint32_t f0 = held(codes, x[1][2 * z + u], sv[1][j], c2[1]), f1 = held(codes, x[1][2 * z + u] >> 4, sv[1][j], c2[1]);
 #pragma unroll
               for (int c = 0; c < kTiles; ++c)
 #pragma unroll
-                for (int x = 0; x < 4; ++x)
-                  if (earliest <= lim[c][x & 1]) o[c][j][0][x] = o[c][j][1][x] = NAN;
+                for (int p = kMmas - 1; p >= 0; --p) mma(sums[c][j][u], e0, e1, f0, f1, pt[c][0][p], pt[c][1][p]);
             }
-        }
-      }
-#pragma unroll
-      for (int w = 0; w < L::kGroups / 2; ++w) {
-        // the four bytes of each token, shifted by bytes: codes 2 i and 2 i + 1 of both in bits 3..6 and 7..10 of their halves
-        uint32_t x[2][4];
-#pragma unroll
-        for (int y = 0; y < 2; ++y) {
-          const uint32_t even = v[y][w], odd = v[y][L::kGroups / 2 + w];
-          x[y][0] = __byte_perm(even, odd, 0x5410);
-          x[y][1] = __byte_perm(even, odd, 0x6521);
-          x[y][2] = __byte_perm(even, odd, 0x7632);
-          x[y][3] = __byte_perm(even, odd, 0x4703);
-        }
-#pragma unroll
-        for (int z = 0; z < 2; ++z) {
-          const int j = 2 * w + z;
-          uint32_t c2[2];
-#pragma unroll
-          for (int y = 0; y < 2; ++y) c2[y] = scale_offset(sv[y][j]);
-#pragma unroll
-          for (int u = 0; u < 2; ++u) {  // channels 4 g + 2 u, 4 g + 2 u + 1 of group j
-            const uint32_t e0 = held(codes, x[0][2 * z + u], sv[0][j], c2[0]), e1 = held(codes, x[0][2 * z + u] >> 4, sv[0][j], c2[0]);
-            const uint32_t f0 = held(codes, x[1][2 * z + u], sv[1][j], c2[1]), f1 = held(codes, x[1][2 * z + u] >> 4, sv[1][j], c2[1]);
-#pragma unroll
-            for (int c = 0; c < kTiles; ++c)
-#pragma unroll
-              for (int p = kMmas - 1; p >= 0; --p) mma(sums[c][j][u], e0, e1, f0, f1, pt[c][0][p], pt[c][1][p]);
           }
         }
       }
+      if constexpr (kF32) {
+#pragma unroll
+        for (int c = 0; c < kTiles; ++c)
+#pragma unroll
+          for (int j = 0; j < L::kGroups; ++j)
+#pragma unroll
+            for (int y = 0; y < 2; ++y)
+#pragma unroll
+              for (int x = 0; x < 4; ++x) o[c][j][y][x] += fresh[c][j][y][x];
+      }
+      __syncwarp();
+      request(i1, 1, 2);
+      i = i1;
     }
-    if constexpr (kF32) {
-#pragma unroll
-      for (int c = 0; c < kTiles; ++c)
-#pragma unroll
-        for (int j = 0; j < L::kGroups; ++j)
-#pragma unroll
-          for (int y = 0; y < 2; ++y)
-#pragma unroll
-            for (int x = 0; x < 4; ++x) o[c][j][y][x] += fresh[c][j][y][x];
-    }
-    __syncwarp();
-    request(i1, 1, 2);
-    i = i1;
+    cp_async_wait<0>();
+    if (!kLong || page0 + n >= sh.page0 + sh.n) break;
+    __syncthreads();  // every warp is through with these pages
+    page0 += n;
+    n = min(sh.page0 + sh.n - page0, kAtOnce);
+    find_pages(a, lists_of(a, b), s_prompt, page0, n, tid, kThreads, s_mask, s_page);
+    __syncthreads();
+    i = next(warp);
+    ahead = next(i + kWarps);
+    place = 0;
+    begin();
   }
-  cp_async_wait<0>();
 
   // ---- the warps' parts ----
 #pragma unroll
@@ -379,7 +399,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<T, kTiles>) cache_attn_k
     } else if (a.shares > 1) {
       if (col >= n_rows && !sh.bad) continue;  // (the join looks at q_len: a malformed prompt's rows get statistics, of nothing)
       const int64_t row = ((int64_t)b * a.N + hd) * a.Lq + tok;
-      if (n > 0) store4(a.part_o + (row * a.shares + share) * D + d, acc);
+      if (sh.n > 0) store4(a.part_o + (row * a.shares + share) * D + d, acc);
       if (d == 0) a.part_ml[row * a.shares + share] = make_float2(m, l);
     } else {
       write(tok, hd, d, m, l, acc);
@@ -532,7 +552,7 @@ __global__ void __launch_bounds__(128) cache_join_rows_kernel(CacheAttnArgs a, i
   if (a.lse && lane == 0) a.lse[row] = l != 0.f ? (m + log2f(l)) * kLn2 : -INFINITY;
 }
 
-// Which kernel, how many rows to a CTA, into how many shares a prompt's pages go (at most kShare pages each).
+// Which kernel, how many rows to a CTA, into how many shares a prompt's pages go.
 struct Plan {
   bool many;  // the tcgen05 kernel
   int rows;   // of a CTA
@@ -545,13 +565,15 @@ struct Plan {
 // left over of the SMs in the last round is lost.  Clusters find fewer places: each group of SMs that one cannot leave has up to s - 1 too few
 // for another (of 296 places 296 for clusters of 2, 279 of 3, 264 of 8; of 444 444, 426 and 384; ten groups assumed here are more).  Taken for
 // 296, 288 CTAs in clusters of 3 took 53 us, where 256 in clusters of 2 took 38.
+// There are never more than eight rounds of CTAs that have shares, so the parts that a kernel joins are those of 8 x 148 CTAs of the tcgen05
+// kernel at most (256 rows each: 158 MB at head_dim 128), however long the call.
 Plan plan_with(const brk_cache_attn_params& p, bool many, int per_cta) {
   const int64_t rows = (int64_t)p.Lq * (p.N / p.cache.Nk), groups = (rows + per_cta - 1) / per_cta;
-  const int per_sm = many ? 1 : p.dtype == BRK_BF16 && per_cta <= 8 ? 3 : 2;
-  const int64_t ctas = (int64_t)p.B * p.cache.Nk * groups, room = per_sm * (int64_t)std::max(1, sm_count());
-  const int64_t largest = many ? kManyShare : kShare, least = (p.P + largest - 1) / largest, pages = many ? 2 : kWarps;
-  const int64_t most = std::max<int64_t>(least, std::min<int64_t>(64, (p.P + pages - 1) / pages));
-  Plan best = {many, per_cta, groups, least, INT64_MAX};
+  const int per_sm = many ? 1 : p.dtype == BRK_BF16 && per_cta <= 8 ? 3 : 2, sms = sm_count();
+  const int64_t ctas = (int64_t)p.B * p.cache.Nk * groups, room = per_sm * (int64_t)(sms > 0 ? sms : 148);  // (workspaces are asked for without a device too)
+  const int64_t pages = many ? 2 : kWarps;
+  const int64_t most = std::max<int64_t>(1, std::min<int64_t>(std::max(64, p.P / kWorthwhile), (p.P + pages - 1) / pages));
+  Plan best = {many, per_cta, groups, 1, INT64_MAX};
   auto consider = [&](int64_t s) {
     const bool cluster = s > 1 && s <= kCluster && !many;
     const int64_t places = cluster ? std::max<int64_t>(s, s == 2 ? room : room - 10 * (s - 1)) : room;
@@ -563,9 +585,9 @@ Plan plan_with(const brk_cache_attn_params& p, bool many, int per_cta) {
     }
   };
   for (int64_t round = 0; round <= 8; ++round) {  // (the most shares of so many rounds, and the fewest)
-    const int64_t s = std::min(most, std::max(least, round * room / ctas));
+    const int64_t s = std::min(most, std::max<int64_t>(1, round * room / ctas));
     consider(s);
-    if (s > least) consider(s - 1);
+    if (s > 1) consider(s - 1);
     if (s == most) break;
   }
   return best;
@@ -625,19 +647,24 @@ int cache_attn_launch(const brk_cache_attn_params& p, void* ws, cudaStream_t st)
     }
     return launch_dependent_clusters(a.cluster ? a.shares : 1, kern, grid, dim3(kThreads), bytes, st, a);
   };
-  static std::atomic<bool> done[10][64] = {};
+  static std::atomic<bool> done[20][64] = {};
   const bool f32 = p.dtype == BRK_F32;
-  auto of_head_dim = [&](auto d, std::atomic<bool>(*flags)[64]) -> int {
+  auto of = [&](auto d, auto is_long, std::atomic<bool>(*flags)[64]) -> int {
     constexpr int D = decltype(d)::value;
+    constexpr bool kLong = decltype(is_long)::value;
     if constexpr (D == 64)
-      if (f32 && plan.rows == 16) return run(cache_attn_kernel<float, D, 2, false>, flags[1]);
-    if (f32) return run(cache_attn_kernel<float, D, 1, false>, flags[0]);
-    if (plan.rows == 4) return run(cache_attn_kernel<__nv_bfloat16, D, 1, true>, flags[2]);
-    return plan.rows == 8 ? run(cache_attn_kernel<__nv_bfloat16, D, 1, false>, flags[3]) : run(cache_attn_kernel<__nv_bfloat16, D, 2, false>, flags[4]);
+      if (f32 && plan.rows == 16) return run(cache_attn_kernel<float, D, 2, false, kLong>, flags[1]);
+    if (f32) return run(cache_attn_kernel<float, D, 1, false, kLong>, flags[0]);
+    if (plan.rows == 4) return run(cache_attn_kernel<__nv_bfloat16, D, 1, true, kLong>, flags[2]);
+    return plan.rows == 8 ? run(cache_attn_kernel<__nv_bfloat16, D, 1, false, kLong>, flags[3])
+                          : run(cache_attn_kernel<__nv_bfloat16, D, 2, false, kLong>, flags[4]);
+  };
+  auto of_head_dim = [&](auto d, std::atomic<bool>(*flags)[64]) -> int {
+    return (p.P + a.shares - 1) / a.shares > kAtOnce ? of(d, std::true_type(), flags + 5) : of(d, std::false_type(), flags);
   };
   const int rc = plan.many ? cache_attn_tc_launch(a, p.cache.D, st)
                  : p.cache.D == 128 ? of_head_dim(std::integral_constant<int, 128>(), done)
-                                    : of_head_dim(std::integral_constant<int, 64>(), done + 5);
+                                    : of_head_dim(std::integral_constant<int, 64>(), done + 10);
   if (rc || a.shares == 1 || a.cluster) return rc;
   auto join = [&](auto d, auto t) -> int {
     constexpr int D = decltype(d)::value;

@@ -29,7 +29,7 @@ namespace {
 
 using namespace cache;
 
-constexpr int kShare = kManyShare;
+constexpr int kAtOnce = 256;               // pages of its share that a CTA knows of at a time
 constexpr int kTile = 128;                 // rows of a tile
 constexpr int kSoftWarps = 8, kUnpackWarps = 4;
 constexpr int kMmaWarp = kSoftWarps + kUnpackWarps;
@@ -64,15 +64,21 @@ __device__ __forceinline__ void cp_async_or_zero(uint32_t dst, const void* src, 
 }
 __device__ __forceinline__ uint32_t low_part(uint32_t hi, float x, float y) { return pack_bf16(x - bf_lo(hi), y - bf_hi(hi)); }
 
-template <int D>
+// kLong: a share can have more than kAtOnce pages.  (The code for that costs the others something: query blocks of 4 prompts of 100
+// documents 108 us, without it 104.)
+template <int D, bool kLong>
 __global__ void __launch_bounds__(kThreads, 1) cache_attn_tc_kernel(CacheAttnArgs a) {
   using L = Layout<D>;
   using SM = Smem<D>;
   constexpr int kG = L::kGroups;
   extern __shared__ unsigned char smem_raw[];
-  __shared__ uint32_t s_mask[2 * kShare];
-  __shared__ int32_t s_page[kShare];
-  __shared__ int s_list[kShare], s_live;  // the pages with a token in a block, in order
+  __shared__ uint32_t s_mask[2 * kAtOnce];
+  __shared__ int32_t s_page[kAtOnce];
+  __shared__ Prompt<kThreads> s_prompt;
+  // The pages with a token in a block, in order, are numbered over the whole share: number k is page s_list[k % kAtOnce] of those at hand,
+  // which begin with entry s_page0 of the page table and end with page s_known - 1.
+  __shared__ int s_list[kAtOnce], s_known, s_page0;
+  __shared__ bool s_more;  // there are entries behind them
   __shared__ uint32_t s_nan[kBufs][kG][2];  // pages that some rows see in part: tokens whose value is NaN, by group
   unsigned char* const smem = smem_raw + ((1024u - (ptx::smem_u32(smem_raw) & 1023u)) & 1023u);
   const uint32_t sbase = ptx::smem_u32(smem);
@@ -99,7 +105,7 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attn_tc_kernel(CacheAttnArg
   auto q_place = [&](int rr) {
     return smem + (rr / kTile) * SM::kQ + (q_unit >> 3) * SM::kQChunk + (rr % kTile) * 128 + (((q_unit & 7) ^ (rr & 7)) << 4);
   };
-  const Share sh = find_share<kThreads, kShare>(a, b, row0, 2 * kTile, share, 1, s_mask, s_page, [&] {
+  const Share sh = find_share<kAtOnce>(a, b, row0, 2 * kTile, share, 1, s_prompt, s_mask, s_page, [&] {
     // Q as the K-major A operand: rows of 128 bytes, their 16-byte units swizzled
     const __nv_bfloat16* const q = reinterpret_cast<const __nv_bfloat16*>(a.q.ptr);
     const int step_tok = kQStep / G, step_head = kQStep % G;
@@ -118,15 +124,22 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attn_tc_kernel(CacheAttnArg
     }
     cp_async_commit();
   });
-  if (warp == 0) {
-    int live = 0;
-    for (int i = lane; i - lane < sh.n; i += 32) {
-      const unsigned there = __ballot_sync(0xffffffffu, i < sh.n && s_page[i] >= 0);
-      if (i < sh.n && s_page[i] >= 0) s_list[live + __popc(there & ((1u << lane) - 1))] = i;
-      live += __popc(there);
+  auto place = [](int k) { return kLong ? k & (kAtOnce - 1) : k; };
+  auto make_list = [&](int page0, int known) {  // by a warp
+    const int n = kLong ? min(sh.page0 + sh.n - page0, kAtOnce) : sh.n;
+    for (int i = lane; i - lane < n; i += 32) {
+      const bool there = i < n && s_page[i] >= 0;
+      const unsigned all = __ballot_sync(0xffffffffu, there);
+      if (there) s_list[place(known + __popc(all & ((1u << lane) - 1)))] = i;
+      known += __popc(all);
     }
-    if (lane == 0) s_live = live;
-  }
+    if (lane == 0) {
+      s_known = known;
+      s_page0 = page0;
+      s_more = page0 + n < sh.page0 + sh.n;
+    }
+  };
+  if (warp == 0) make_list(sh.page0, 0);
   cp_async_wait<0>();
 #pragma unroll 2
   for (int rr = tid / kQUnits; rr < 2 * kTile; rr += kQStep) {  // (what this thread has copied) channels in the order of K's
@@ -139,11 +152,15 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attn_tc_kernel(CacheAttnArg
   __syncthreads();
   ptx::tc_fence_after_sync();
   const uint32_t tmem = *tmem_slot;
-  const int live = s_live;
   const bool split = sh.n_rows <= kTile;  // one tile: the softmax groups take its pages in turn
   const int first_lim = sh.first_slot + row0 / G;  // the last slot that the CTA's first row sees
   ptx::BoundedWaits waits(kWaitBudget);
   auto wait = [&](int i, uint32_t parity) { waits(bar(i), parity & 1u, 1); };
+  // When all that is known of has been worked on, the warps that unpack look at the next kAtOnce entries, between two of these.
+  auto meet = [] {
+    __syncwarp();
+    asm volatile("bar.sync 3, %0;" ::"n"(kThreads) : "memory");
+  };
 
   if (warp < kSoftWarps) {
     // =============================== softmax: a thread per row ===========================================
@@ -155,93 +172,101 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attn_tc_kernel(CacheAttnArg
     const float sl2 = a.scale * kLog2e;
     float m_run = -INFINITY, l_run = 0.f;
     unsigned poison = 0;  // groups of channels in which this row has seen NaN
-    int pages = split ? (live + 1 - x) / 2 : live;
+    int pages = 0;  // that this group has worked on
 #pragma unroll 1
-    for (int j = 0; j < pages; ++j) {
-      const int k = split ? 2 * j + x : j, i = s_list[k], slot0 = (sh.page0 + i) * kPage;
-      unsigned v0 = s_mask[2 * i], v1 = s_mask[2 * i + 1];
-      const uint32_t tm_s = tm + (uint32_t)(j & 1) * 64;
-      const bool late = slot0 + kPage - 1 > first_lim;
-      wait(kSFull + 2 * x + (j & 1), j >> 1);
-      ptx::tc_fence_after_sync();
-      __syncwarp();
-      const bool two = v1 != 0;
-      uint32_t sr[2][32];
-      ptx::tmem_ld32(tm_s, sr[0]);
-      if (two) ptx::tmem_ld32(tm_s + 32, sr[1]);
-      ptx::tmem_wait_ld(sr[0]);
-      if (two) ptx::tmem_wait_ld(sr[1]);
-      if (late || (v0 & v1) != ~0u) {  // (warp-uniform)
-        if (late) {
-          const int n = there ? max(0, min(64, lim - slot0 + 1)) : 64;
-          v0 &= n >= 32 ? ~0u : (1u << n) - 1u;
-          v1 &= n >= 64 ? ~0u : n > 32 ? (1u << (n - 32)) - 1u : 0u;
-          wait(kKVFull + k % kBufs, k / kBufs);  // (long since: what the unpacking warps wrote beside K and V is visible behind it)
-#pragma unroll
-          for (int c = 0; c < kG; ++c)
-            if ((s_nan[k % kBufs][c][0] & v0) | (s_nan[k % kBufs][c][1] & v1)) poison |= 1u << c;
-          __syncwarp();
-        }
-#pragma unroll
-        for (int c = 0; c < 32; ++c) sr[0][c] = (v0 & (1u << c)) ? sr[0][c] : 0xff800000u;
-        if (two) {
-#pragma unroll
-          for (int c = 0; c < 32; ++c) sr[1][c] = (v1 & (1u << c)) ? sr[1][c] : 0xff800000u;
-        }
-      }
-      float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-      for (int c = 0; c < 32; c += 2) mx4[(c >> 1) & 3] = ptx::max3(mx4[(c >> 1) & 3], __uint_as_float(sr[0][c]), __uint_as_float(sr[0][c + 1]));
-      if (two) {
-#pragma unroll
-        for (int c = 0; c < 32; c += 2) mx4[(c >> 1) & 3] = ptx::max3(mx4[(c >> 1) & 3], __uint_as_float(sr[1][c]), __uint_as_float(sr[1][c + 1]));
-      }
-      const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * sl2;
-      float m_new = fmaxf(m_run, mx);
-      if (m_run != -INFINITY && m_new - m_run <= kLazy) m_new = m_run;
-      const float ref = m_new == -INFINITY ? 0.f : m_new;
-      const float corr = ptx::ex2(m_run - ref);
-      const bool changed = m_new != m_run;
-      m_run = m_new;
-      const ptx::f32x2 sc2 = ptx::pack2(sl2, sl2), nr2 = ptx::pack2(-ref, -ref);
-      ptx::f32x2 sum2[2] = {0ull, 0ull};
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        if (h == 1 && !two) break;
-        uint32_t parts[32];  // higher bits of 32 tokens, then what they leave
-#pragma unroll
-        for (int c = 0; c < 32; c += 2) {
-          float t0, t1;
-          ptx::unpack2(ptx::fma2(ptx::pack2(__uint_as_float(sr[h][c]), __uint_as_float(sr[h][c + 1])), sc2, nr2), t0, t1);
-          const float p0 = ptx::ex2(t0), p1 = ptx::ex2(t1);
-          sum2[(c >> 1) & 1] = ptx::add2(sum2[(c >> 1) & 1], ptx::pack2(p0, p1));
-          parts[c >> 1] = pack_bf16(p0, p1);
-          parts[16 + (c >> 1)] = low_part(parts[c >> 1], p0, p1);
-        }
-        ptx::tmem_st32(tm_s + 32 * h, parts);
-      }
-      if (j > 0 && __any_sync(0xffffffffu, changed)) {  // (rare)
-        wait(kODone + 2 * x + ((j - 1) & 1), (j - 1) >> 1);
+    for (;;) {
+      const int to = split ? (s_known + 1 - x) / 2 : s_known, page0 = kLong ? s_page0 : sh.page0;
+#pragma unroll 1
+      for (; pages < to; ++pages) {
+        const int j = pages;
+        const int k = split ? 2 * j + x : j, i = s_list[place(k)], slot0 = (page0 + i) * kPage;
+        unsigned v0 = s_mask[2 * i], v1 = s_mask[2 * i + 1];
+        const uint32_t tm_s = tm + (uint32_t)(j & 1) * 64;
+        const bool late = slot0 + kPage - 1 > first_lim;
+        wait(kSFull + 2 * x + (j & 1), j >> 1);
         ptx::tc_fence_after_sync();
         __syncwarp();
-#pragma unroll 1
-        for (int ch = 0; ch < D / 32; ++ch) {
-          uint32_t o[32];
-          ptx::tmem_ld32(tm + kColO + (uint32_t)ch * 32, o);
-          ptx::tmem_wait_ld(o);
+        const bool two = v1 != 0;
+        uint32_t sr[2][32];
+        ptx::tmem_ld32(tm_s, sr[0]);
+        if (two) ptx::tmem_ld32(tm_s + 32, sr[1]);
+        ptx::tmem_wait_ld(sr[0]);
+        if (two) ptx::tmem_wait_ld(sr[1]);
+        if (late || (v0 & v1) != ~0u) {  // (warp-uniform)
+          if (late) {
+            const int n = there ? max(0, min(64, lim - slot0 + 1)) : 64;
+            v0 &= n >= 32 ? ~0u : (1u << n) - 1u;
+            v1 &= n >= 64 ? ~0u : n > 32 ? (1u << (n - 32)) - 1u : 0u;
+            wait(kKVFull + k % kBufs, k / kBufs);  // (long since: what the unpacking warps wrote beside K and V is visible behind it)
 #pragma unroll
-          for (int c = 0; c < 32; ++c) o[c] = __float_as_uint(__uint_as_float(o[c]) * corr);
-          ptx::tmem_st32(tm + kColO + (uint32_t)ch * 32, o);
+            for (int c = 0; c < kG; ++c)
+              if ((s_nan[k % kBufs][c][0] & v0) | (s_nan[k % kBufs][c][1] & v1)) poison |= 1u << c;
+            __syncwarp();
+          }
+#pragma unroll
+          for (int c = 0; c < 32; ++c) sr[0][c] = (v0 & (1u << c)) ? sr[0][c] : 0xff800000u;
+          if (two) {
+#pragma unroll
+            for (int c = 0; c < 32; ++c) sr[1][c] = (v1 & (1u << c)) ? sr[1][c] : 0xff800000u;
+          }
         }
+        float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int c = 0; c < 32; c += 2) mx4[(c >> 1) & 3] = ptx::max3(mx4[(c >> 1) & 3], __uint_as_float(sr[0][c]), __uint_as_float(sr[0][c + 1]));
+        if (two) {
+#pragma unroll
+          for (int c = 0; c < 32; c += 2) mx4[(c >> 1) & 3] = ptx::max3(mx4[(c >> 1) & 3], __uint_as_float(sr[1][c]), __uint_as_float(sr[1][c + 1]));
+        }
+        const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * sl2;
+        float m_new = fmaxf(m_run, mx);
+        if (m_run != -INFINITY && m_new - m_run <= kLazy) m_new = m_run;
+        const float ref = m_new == -INFINITY ? 0.f : m_new;
+        const float corr = ptx::ex2(m_run - ref);
+        const bool changed = m_new != m_run;
+        m_run = m_new;
+        const ptx::f32x2 sc2 = ptx::pack2(sl2, sl2), nr2 = ptx::pack2(-ref, -ref);
+        ptx::f32x2 sum2[2] = {0ull, 0ull};
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          if (h == 1 && !two) break;
+          uint32_t parts[32];  // higher bits of 32 tokens, then what they leave
+#pragma unroll
+          for (int c = 0; c < 32; c += 2) {
+            float t0, t1;
+            ptx::unpack2(ptx::fma2(ptx::pack2(__uint_as_float(sr[h][c]), __uint_as_float(sr[h][c + 1])), sc2, nr2), t0, t1);
+            const float p0 = ptx::ex2(t0), p1 = ptx::ex2(t1);
+            sum2[(c >> 1) & 1] = ptx::add2(sum2[(c >> 1) & 1], ptx::pack2(p0, p1));
+            parts[c >> 1] = pack_bf16(p0, p1);
+            parts[16 + (c >> 1)] = low_part(parts[c >> 1], p0, p1);
+          }
+          ptx::tmem_st32(tm_s + 32 * h, parts);
+        }
+        if (j > 0 && __any_sync(0xffffffffu, changed)) {  // (rare)
+          wait(kODone + 2 * x + ((j - 1) & 1), (j - 1) >> 1);
+          ptx::tc_fence_after_sync();
+          __syncwarp();
+#pragma unroll 1
+          for (int ch = 0; ch < D / 32; ++ch) {
+            uint32_t o[32];
+            ptx::tmem_ld32(tm + kColO + (uint32_t)ch * 32, o);
+            ptx::tmem_wait_ld(o);
+#pragma unroll
+            for (int c = 0; c < 32; ++c) o[c] = __float_as_uint(__uint_as_float(o[c]) * corr);
+            ptx::tmem_st32(tm + kColO + (uint32_t)ch * 32, o);
+          }
+        }
+        float s0, s1, s2, s3;
+        ptx::unpack2(sum2[0], s0, s1);
+        ptx::unpack2(sum2[1], s2, s3);
+        l_run = l_run * corr + ((s0 + s1) + (s2 + s3));
+        ptx::tmem_wait_st();
+        ptx::tc_fence_before_sync();
+        __syncwarp();
+        ptx::mbar_arrive_warp(bar(kPFull + 2 * x + (j & 1)));
       }
-      float s0, s1, s2, s3;
-      ptx::unpack2(sum2[0], s0, s1);
-      ptx::unpack2(sum2[1], s2, s3);
-      l_run = l_run * corr + ((s0 + s1) + (s2 + s3));
-      ptx::tmem_wait_st();
-      ptx::tc_fence_before_sync();
-      __syncwarp();
-      ptx::mbar_arrive_warp(bar(kPFull + 2 * x + (j & 1)));
+      if (!kLong || !s_more) break;
+      meet();
+      meet();
     }
     if (pages > 0) {
       wait(kODone + 2 * x + ((pages - 1) & 1), (pages - 1) >> 1);
@@ -298,7 +323,7 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attn_tc_kernel(CacheAttnArg
     if (tok < a.Lq) {
       if (a.shares == 1)
         to = reinterpret_cast<char*>(reinterpret_cast<__nv_bfloat16*>(a.o.ptr) + (int64_t)b * a.o.sb + (int64_t)hd * a.o.sh + (int64_t)tok * a.o.ss);
-      else if (there && live > 0) to = reinterpret_cast<char*>(a.part_o + (row * a.shares + share) * D);
+      else if (there && s_known > 0) to = reinterpret_cast<char*>(a.part_o + (row * a.shares + share) * D);
     }
     char* line_to[8];
 #pragma unroll
@@ -377,9 +402,9 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attn_tc_kernel(CacheAttnArg
     const Codes codes = a.codes;
     unsigned char* const cells = smem + SM::kCodes + p * SM::kCell;  // cell c of stage s: s kStage + c 128 kCell on
     unsigned char* const scale_cells = smem + SM::kCodes + 5 * 128 * SM::kCell + p * SM::kScales;
-    auto request = [&](int k) {
-      if (k < live) {
-        const int i = s_list[k];
+    auto request = [&](int k, int known) {
+      if (k < known) {
+        const int i = s_list[place(k)];
         const bool two = s_mask[2 * i + 1] != 0, pair = two || line < 16;
         const unsigned char* const page = head + (int64_t)s_page[i] * a.Nk * L::kBytes;
         const int stage = k % kAhead * SM::kStage;
@@ -395,82 +420,96 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attn_tc_kernel(CacheAttnArg
       }
       cp_async_commit();
     };
+    int k = 0, page0 = sh.page0;
 #pragma unroll 1
-    for (int k = 0; k < kAhead - 1; ++k) request(k);
+    for (;;) {
+      const int known = s_known;
 #pragma unroll 1
-    for (int k = 0; k < live; ++k) {
-      const int buf = k % kBufs, i = s_list[k], slot0 = (sh.page0 + i) * kPage;
-      const uint32_t in = s_mask[2 * i + (line >> 4)] >> (2 * line & 31);  // of this pair of tokens
-      const bool late = slot0 + kPage - 1 > first_lim, two = s_mask[2 * i + 1] != 0, pair = two || line < 16;
-      request(k + kAhead - 1);
-      cp_async_wait<kAhead - 1>();  // this thread's cells of page k have landed
-      uint32_t kw[2][kG], ks[2][kG / 2], vw[2][kG], vs[kG];
-      {
-        const int stage = k % kAhead * SM::kStage;
+      for (int i = 0; i < kAhead - 1; ++i) request(k + i, known);
+#pragma unroll 1
+      for (; k < known; ++k) {
+        const int buf = k % kBufs, i = s_list[place(k)], slot0 = (page0 + i) * kPage;
+        const uint32_t in = s_mask[2 * i + (line >> 4)] >> (2 * line & 31);  // of this pair of tokens
+        const bool late = slot0 + kPage - 1 > first_lim, two = s_mask[2 * i + 1] != 0, pair = two || line < 16;
+        request(k + kAhead - 1, known);
+        cp_async_wait<kAhead - 1>();  // this thread's cells of page k have landed
+        uint32_t kw[2][kG], ks[2][kG / 2], vw[2][kG], vs[kG];
+        {
+          const int stage = k % kAhead * SM::kStage;
+#pragma unroll
+          for (int y = 0; y < 2; ++y) {
+            load_words<D>(cells + stage + y * 128 * SM::kCell, kw[y]);
+            load_words<D>(cells + stage + (2 + y) * 128 * SM::kCell, vw[y]);  // the even token's words, then the odd one's
+            load_scales<D>(scale_cells + stage + y * 128 * SM::kScales, ks[y]);
+          }
+          load_words<D>(cells + stage + 4 * 128 * SM::kCell, vs);
+        }
+        if (k >= kBufs) wait(kKVEmpty + buf, k / kBufs - 1);
+        unsigned char* const out_k = smem + SM::kKV + buf * 2 * SM::kHalf;
+        unsigned char* const out_v = out_k + SM::kHalf;
+        auto place = [&](int row, int unit) { return (unit >> 3) * SM::kChunk + row * 128 + (((unit & 7) ^ (row & 7)) << 4); };
 #pragma unroll
         for (int y = 0; y < 2; ++y) {
-          load_words<D>(cells + stage + y * 128 * SM::kCell, kw[y]);
-          load_words<D>(cells + stage + (2 + y) * 128 * SM::kCell, vw[y]);  // the even token's words, then the odd one's
-          load_scales<D>(scale_cells + stage + y * 128 * SM::kScales, ks[y]);
-        }
-        load_words<D>(cells + stage + 4 * 128 * SM::kCell, vs);
-      }
-      if (k >= kBufs) wait(kKVEmpty + buf, k / kBufs - 1);
-      unsigned char* const out_k = smem + SM::kKV + buf * 2 * SM::kHalf;
-      unsigned char* const out_v = out_k + SM::kHalf;
-      auto place = [&](int row, int unit) { return (unit >> 3) * SM::kChunk + row * 128 + (((unit & 7) ^ (row & 7)) << 4); };
+          if (y == 1 && !two) break;
 #pragma unroll
-      for (int y = 0; y < 2; ++y) {
-        if (y == 1 && !two) break;
-#pragma unroll
-        for (int j = 0; j < kG; ++j) {
-          const Pairs x = pairs_of(codes, kw[y][j], __byte_perm(ks[y][j / 2], 0, j % 2 ? 0x3232 : 0x1010));
-          *reinterpret_cast<uint4*>(out_k + place(key + 32 * y, 4 * j + t)) = make_uint4(x.x[0], x.x[1], x.x[2], x.x[3]);
-        }
-      }
-      // values of tokens in no block are zeros (0 x NaN would reach every row); so are NaN that some rows see and others do not:
-      // those rows are told
-      const uint32_t keep = ((in & 1) ? 0xFFFFu : 0u) | ((in & 2) ? 0xFFFF0000u : 0u);
-#pragma unroll
-      for (int j = 0; j < kG; ++j) vs[j] &= keep;
-      if (late) {
-        if (p < 2 * kG) s_nan[buf][p / 2][p % 2] = 0;
-        asm volatile("bar.sync 1, 128;" ::: "memory");
-#pragma unroll
-        for (int j = 0; j < kG; ++j) {
-          const uint32_t is = __vcmpeq2(vs[j] & 0x7F807F80u, 0x7F807F80u);
-          if (is && pair) atomicOr(&s_nan[buf][j][line >> 4], ((is & 1u) | ((is >> 31) << 1)) << (2 * line & 31));
-          vs[j] &= ~is;
-        }
-      }
-      if (pair) {
-#pragma unroll
-        for (int w = 0; w < kG / 2; ++w)
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {  // the even and the odd token
-            const uint32_t s2 = __byte_perm(vs[2 * w], vs[2 * w + 1], h ? 0x7632 : 0x5410), c2 = scale_offset(s2);
-#pragma unroll
-            for (int y = 0; y < 2; ++y) {
-              const uint32_t x = vw[y][h * (kG / 2) + w];
-              *reinterpret_cast<uint4*>(out_v + place(2 * line + h, 8 * w + 2 * t + (y ^ flip))) =
-                  make_uint4(held(codes, x, s2, c2), held(codes, rotr(x, 4), s2, c2), held(codes, rotr(x, 8), s2, c2), held(codes, rotr(x, 12), s2, c2));
-            }
+          for (int j = 0; j < kG; ++j) {
+            const Pairs x = pairs_of(codes, kw[y][j], __byte_perm(ks[y][j / 2], 0, j % 2 ? 0x3232 : 0x1010));
+            *reinterpret_cast<uint4*>(out_k + place(key + 32 * y, 4 * j + t)) = make_uint4(x.x[0], x.x[1], x.x[2], x.x[3]);
           }
+        }
+        // values of tokens in no block are zeros (0 x NaN would reach every row); so are NaN that some rows see and others do not:
+        // those rows are told
+        const uint32_t keep = ((in & 1) ? 0xFFFFu : 0u) | ((in & 2) ? 0xFFFF0000u : 0u);
+#pragma unroll
+        for (int j = 0; j < kG; ++j) vs[j] &= keep;
+        if (late) {
+          if (p < 2 * kG) s_nan[buf][p / 2][p % 2] = 0;
+          asm volatile("bar.sync 1, 128;" ::: "memory");
+#pragma unroll
+          for (int j = 0; j < kG; ++j) {
+            const uint32_t is = __vcmpeq2(vs[j] & 0x7F807F80u, 0x7F807F80u);
+            if (is && pair) atomicOr(&s_nan[buf][j][line >> 4], ((is & 1u) | ((is >> 31) << 1)) << (2 * line & 31));
+            vs[j] &= ~is;
+          }
+        }
+        if (pair) {
+#pragma unroll
+          for (int w = 0; w < kG / 2; ++w)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {  // the even and the odd token
+              const uint32_t s2 = __byte_perm(vs[2 * w], vs[2 * w + 1], h ? 0x7632 : 0x5410), c2 = scale_offset(s2);
+#pragma unroll
+              for (int y = 0; y < 2; ++y) {
+                const uint32_t x = vw[y][h * (kG / 2) + w];
+                *reinterpret_cast<uint4*>(out_v + place(2 * line + h, 8 * w + 2 * t + (y ^ flip))) =
+                    make_uint4(held(codes, x, s2, c2), held(codes, rotr(x, 4), s2, c2), held(codes, rotr(x, 8), s2, c2), held(codes, rotr(x, 12), s2, c2));
+              }
+            }
+        }
+        ptx::fence_proxy_async_smem();
+        __syncwarp();
+        ptx::mbar_arrive_warp(bar(kKVFull + buf));
       }
-      ptx::fence_proxy_async_smem();
+      cp_async_wait<0>();
+      if (!kLong || !s_more) break;
+      meet();
+      page0 += kAtOnce;
+      find_pages(a, lists_of(a, b), s_prompt, page0, min(sh.page0 + sh.n - page0, kAtOnce), p, 32 * kUnpackWarps, s_mask, s_page);
       __syncwarp();
-      ptx::mbar_arrive_warp(bar(kKVFull + buf));
+      asm volatile("bar.sync 1, 128;" ::: "memory");
+      if (warp == kSoftWarps) make_list(page0, known);
+      meet();
     }
-    cp_async_wait<0>();
   } else {
     // =============================== MMA ===========================================
     const uint32_t idesc_qk = ptx::idesc_bf16(kTile, kPage, 0, 0), idesc_half = ptx::idesc_bf16(kTile, kPage / 2, 0, 0), idesc_pv = ptx::idesc_bf16(kTile, D, 0, 1);
     const uint64_t q_desc = ptx::smem_desc_sw128(sbase, 16, 1024), k_desc = ptx::smem_desc_sw128(sbase + SM::kKV, 16, 1024);
     const uint64_t v_desc = ptx::smem_desc_sw128(sbase + SM::kKV + SM::kHalf, SM::kChunk, 1024);
+    auto is_long = [&](int k) { return s_mask[2 * s_list[place(k)] + 1] != 0; };  // page k, beyond its first half
     // Page k for group x's tile: its j-th.
     auto issue_qk = [&](int k, int x, int j) {
       const int buf = k % kBufs;
-      const uint32_t idesc = s_mask[2 * s_list[k] + 1] != 0 ? idesc_qk : idesc_half;
+      const uint32_t idesc = is_long(k) ? idesc_qk : idesc_half;
       wait(kKVFull + buf, k / kBufs);
       ptx::tc_fence_after_sync();
       __syncwarp();
@@ -487,7 +526,7 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attn_tc_kernel(CacheAttnArg
     };
     auto issue_pv = [&](int k, int x, int j, bool last) {
       const int buf = k % kBufs;
-      const bool two = s_mask[2 * s_list[k] + 1] != 0;
+      const bool two = is_long(k);
       wait(kPFull + 2 * x + (j & 1), j >> 1);
       ptx::tc_fence_after_sync();
       __syncwarp();
@@ -506,23 +545,31 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attn_tc_kernel(CacheAttnArg
       }
       __syncwarp();
     };
-    if (split) {
-      if (live > 0) issue_qk(0, 0, 0);
-      if (live > 1) issue_qk(1, 1, 0);
+    int k = 0;
 #pragma unroll 1
-      for (int k = 0; k < live; ++k) {
-        issue_pv(k, k & 1, k >> 1, true);
-        if (k + 2 < live) issue_qk(k + 2, k & 1, (k >> 1) + 1);
-      }
-    } else {
-      if (live > 0)
-        for (int x = 0; x < 2; ++x) issue_qk(0, x, 0);
+    for (;;) {
+      const int known = s_known;
+      if (split) {
 #pragma unroll 1
-      for (int k = 0; k < live; ++k) {
-        if (k + 1 < live)
-          for (int x = 0; x < 2; ++x) issue_qk(k + 1, x, k + 1);
-        for (int x = 0; x < 2; ++x) issue_pv(k, x, k, x == 1);
+        for (int n = k; n < min(known, k + 2); ++n) issue_qk(n, n & 1, n >> 1);
+#pragma unroll 1
+        for (; k < known; ++k) {
+          issue_pv(k, k & 1, k >> 1, true);
+          if (k + 2 < known) issue_qk(k + 2, k & 1, (k >> 1) + 1);
+        }
+      } else {
+        if (k < known)
+          for (int x = 0; x < 2; ++x) issue_qk(k, x, k);
+#pragma unroll 1
+        for (; k < known; ++k) {
+          if (k + 1 < known)
+            for (int x = 0; x < 2; ++x) issue_qk(k + 1, x, k + 1);
+          for (int x = 0; x < 2; ++x) issue_pv(k, x, k, x == 1);
+        }
       }
+      if (!kLong || !s_more) break;
+      meet();
+      meet();
     }
   }
   ptx::tc_fence_before_sync();
@@ -544,8 +591,11 @@ int cache_attn_tc_launch(const cache::CacheAttnArgs& a, int D, cudaStream_t st) 
     }
     return launch_dependent(kern, grid, dim3(kThreads), bytes, st, a);
   };
-  static std::atomic<bool> done128[64] = {}, done64[64] = {};
-  return D == 128 ? run(cache_attn_tc_kernel<128>, Smem<128>::kBytes + 1024, done128) : run(cache_attn_tc_kernel<64>, Smem<64>::kBytes + 1024, done64);
+  static std::atomic<bool> done[4][64] = {};
+  constexpr int k128 = Smem<128>::kBytes + 1024, k64 = Smem<64>::kBytes + 1024;
+  if ((a.P + a.shares - 1) / a.shares > kAtOnce)
+    return D == 128 ? run(cache_attn_tc_kernel<128, true>, k128, done[0]) : run(cache_attn_tc_kernel<64, true>, k64, done[1]);
+  return D == 128 ? run(cache_attn_tc_kernel<128, false>, k128, done[2]) : run(cache_attn_tc_kernel<64, false>, k64, done[3]);
 }
 
 }  // namespace brk

@@ -1,4 +1,5 @@
 // What the kernels of the cache's attention share: their arguments, and a CTA's share of a prompt's pages.
+// A share can be as long as a page table: what a CTA needs to know of its pages it finds out for so many at a time as it has room for.
 #pragma once
 #include "cache_layout.cuh"
 #include "tc_ptx.cuh"
@@ -6,7 +7,6 @@
 namespace brk {
 namespace cache {
 
-constexpr int kManyShare = 256;  // pages a CTA of the tcgen05 kernel takes at most
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 struct CacheAttnArgs {
@@ -26,6 +26,13 @@ struct CacheAttnArgs {
   Codes codes;
 };
 
+// Shared memory: the first entries of the prompt's page table and of its block spans (start, length).
+template <int kThreads>
+struct Prompt {
+  int32_t table[kThreads];
+  int2 span[kThreads];
+};
+
 struct Share {
   int rows;        // of the prompt
   int n_rows;      // of this CTA; none is left where it is not positive
@@ -34,41 +41,22 @@ struct Share {
   bool bad;        // spans or number of rows malformed: the prompt has no rows
 };
 
-// Rows row0 .. row0 + max_rows - 1 of prompt b (query heads of a group at one token after the other) against an even share, of at
-// least min_pages, of the pages up to the last row's slot.  s_mask [2 kShare]: which tokens of these pages lie in a block; s_page [kShare]: the pages'
-// numbers, -1 for one without such a token.  The latencies are paid once each: spans and number of rows, with what `meanwhile` requests and
-// the first entries of the page table; the other entries.
-template <int kThreads, int kShare, typename F>
-__device__ __forceinline__ Share find_share(const CacheAttnArgs& a, int b, int row0, int max_rows, int share, int min_pages, uint32_t* s_mask,
-                                            int32_t* s_page, F meanwhile) {
-  const int tid = threadIdx.x, G = a.N / a.Nk;
-  const int32_t *start = a.blk_start + (int64_t)b * a.M, *len = a.blk_len + (int64_t)b * a.M, *table = a.table + (int64_t)b * a.P;
-  const int64_t slots = (int64_t)a.P * kPage;
-  const int last_start = start[a.M - 1], last_len = len[a.M - 1], given = a.q_len ? a.q_len[b] : a.Lq;
-  __shared__ int32_t s_table[kThreads];
-  __shared__ int2 s_span[kThreads];  // (start, length) of the first blocks
-  s_table[tid] = tid < a.P ? table[tid] : -1;
-  meanwhile();
-  bool bad = given < 0 || given > a.Lq || given > last_len;
-  for (int m = tid; m < a.M; m += kThreads) {
-    bad |= span_is_bad(start, len, m, slots);
-    if (m < kThreads) s_span[m] = make_int2(start[m], len[m]);
-  }
-  Share r;
-  r.bad = __syncthreads_or(bad);
-  if (r.bad && tid == 0 && a.status) atomicCAS(a.status, 0, kStatusBadCacheCall);
+struct Lists {  // of a prompt
+  const int32_t *start, *len, *table;
+};
+__device__ __forceinline__ Lists lists_of(const CacheAttnArgs& a, int b) {
+  return {a.blk_start + (int64_t)b * a.M, a.blk_len + (int64_t)b * a.M, a.table + (int64_t)b * a.P};
+}
 
-  auto block = [&](int m) { return m < kThreads ? s_span[m] : make_int2(start[m], len[m]); };
-  r.rows = r.bad ? 0 : given;
-  r.n_rows = min(r.rows * G - row0, max_rows);
-  r.first_slot = r.bad ? 0 : last_start + last_len - r.rows;
-  const int live = r.n_rows > 0 ? (r.first_slot + (row0 + r.n_rows - 1) / G) / kPage + 1 : 0;
-  const int per = max((live + a.shares - 1) / a.shares, min(live, min_pages));
-  r.page0 = min(live, share * per);
-  r.n = min(live, r.page0 + per) - r.page0;
-  for (int i = tid; i < r.n; i += kThreads) {
-    const int at = r.page0 + i, lo = at * kPage;
-    int page = at < kThreads ? s_table[at] : table[at];
+// What n entries of the page table from number `from` on say, by `threads` threads of which this is number `me`.  s_mask [2 n]: which tokens
+// of the page lie in a block; s_page [n]: its number, -1 for one without such a token.
+template <int kThreads>
+__device__ __forceinline__ void find_pages(const CacheAttnArgs& a, const Lists& lists, const Prompt<kThreads>& prompt, int from, int n, int me,
+                                           int threads, uint32_t* s_mask, int32_t* s_page) {
+  auto block = [&](int m) { return m < kThreads ? prompt.span[m] : make_int2(lists.start[m], lists.len[m]); };
+  for (int i = me; i < n; i += threads) {
+    const int at = from + i, lo = at * kPage;
+    int page = at < kThreads ? prompt.table[at] : lists.table[at];
     int m = 0;  // the first block that ends behind the page's first token (blocks are in order)
     for (int size = a.M; size > 0;) {
       const int half = size / 2;
@@ -100,6 +88,38 @@ __device__ __forceinline__ Share find_share(const CacheAttnArgs& a, int b, int r
     s_mask[2 * i + 1] = w[1];
     s_page[i] = needed ? page : -1;
   }
+}
+
+// Rows row0 .. row0 + max_rows - 1 of prompt b (query heads of a group at one token after the other) against an even share, of at
+// least min_pages, of the pages up to the last row's slot; of the first kAtOnce of them what find_pages says.  The latencies are paid once
+// each: spans and number of rows, with what `meanwhile` requests and the first entries of the page table; the other entries.
+template <int kAtOnce, int kThreads, typename F>
+__device__ __forceinline__ Share find_share(const CacheAttnArgs& a, int b, int row0, int max_rows, int share, int min_pages,
+                                            Prompt<kThreads>& prompt, uint32_t* s_mask, int32_t* s_page, F meanwhile) {
+  const int tid = threadIdx.x, G = a.N / a.Nk;
+  const Lists lists = lists_of(a, b);
+  const int32_t *start = lists.start, *len = lists.len;
+  const int64_t slots = (int64_t)a.P * kPage;
+  const int last_start = start[a.M - 1], last_len = len[a.M - 1], given = a.q_len ? a.q_len[b] : a.Lq;
+  prompt.table[tid] = tid < a.P ? lists.table[tid] : -1;
+  meanwhile();
+  bool bad = given < 0 || given > a.Lq || given > last_len;
+  for (int m = tid; m < a.M; m += kThreads) {
+    bad |= span_is_bad(start, len, m, slots);
+    if (m < kThreads) prompt.span[m] = make_int2(start[m], len[m]);
+  }
+  Share r;
+  r.bad = __syncthreads_or(bad);
+  if (r.bad && tid == 0 && a.status) atomicCAS(a.status, 0, kStatusBadCacheCall);
+
+  r.rows = r.bad ? 0 : given;
+  r.n_rows = min(r.rows * G - row0, max_rows);
+  r.first_slot = r.bad ? 0 : last_start + last_len - r.rows;
+  const int live = r.n_rows > 0 ? (r.first_slot + (row0 + r.n_rows - 1) / G) / kPage + 1 : 0;
+  const int per = max((live + a.shares - 1) / a.shares, min(live, min_pages));
+  r.page0 = (int)min((int64_t)live, (int64_t)share * per);
+  r.n = min(live, r.page0 + per) - r.page0;
+  find_pages(a, lists, prompt, r.page0, min(r.n, kAtOnce), tid, kThreads, s_mask, s_page);
   __syncthreads();
   return r;
 }

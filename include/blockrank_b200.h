@@ -296,6 +296,7 @@ typedef struct brk_cache_attn_params {
   float* lse;             /* optional [B, N, Lq] natural-log sum-exp of scaled logits */
   int32_t* status;        /* optional, see brk_status_poll */
 } brk_cache_attn_params;
+/* (parts of rows that several CTAs make; 158 MB at most, however long the call) */
 BRK_API size_t brk_cache_attn_workspace_bytes(const brk_cache_attn_params* p);
 BRK_API int brk_cache_attn(const brk_cache_attn_params* p, void* workspace, size_t workspace_bytes, void* stream);
 

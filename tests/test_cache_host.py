@@ -104,3 +104,14 @@ def test_what_is_held():
     assert torch.equal(ch.held(h), h)
     s = ch.scales(x).repeat_interleave(32, -1)
     assert bool(((h - x.double()).abs() <= s / 2 + 1e-300).all())
+
+
+@pytest.mark.parametrize("dtype,N,Nk,D,Lq,tokens,B", [
+    (0, 32, 8, 128, 131072, 131072, 1), (0, 32, 8, 128, 32768, 32768, 1), (0, 32, 8, 128, 4096, 131072, 1), (1, 32, 8, 128, 4096, 131072, 1),
+    (1, 8, 8, 64, 65536, 65536, 1), (0, 128, 1, 128, 1, 2 ** 22, 1), (0, 32, 8, 128, 1, 131072, 1024), (0, 32, 8, 128, 48, 2 ** 24, 64)])
+def test_workspaces_do_not_grow_with_the_call(dtype, N, Nk, D, Lq, tokens, B):
+    """Whole sequences, long caches, many prompts: parts of 8 x 148 CTAs of 256 rows at most (include/blockrank_b200.h)."""
+    view = _lib.View(64, Lq * N * D, D, N * D)
+    p = _attn(dtype=dtype, N=N, Lq=Lq, B=B, P=-(-tokens // 64), cache=_cache(2 ** 18, Nk, D), q=view, o=view)
+    need = _lib.lib().brk_cache_attn_workspace_bytes(C.byref(p))
+    assert need <= 8 * 148 * 256 * (4 * D + 8), need

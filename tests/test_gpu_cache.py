@@ -951,3 +951,91 @@ def test_a_document_behind_one_that_is_too_long_only():
     with pytest.raises(ValueError, match="of a call on the cache"):
         ops.check_status()
     assert not mass.any() and not logits.any()
+
+
+def _attention_of_long(q, hk, hv, table, start, length, scale, q_len):
+    """ch.attention for long prompts of many rows (a prompt's rows together, on the GPU); entries of -1 in the table do not exist."""
+    B, N, R, D = q.shape
+    outs, lses, sizes = [], [], []
+    for b in range(B):
+        rows, slot = int(q_len[b]), torch.cat([torch.arange(a, a + n) for a, n in zip(start[b].tolist(), length[b].tolist())])
+        slot = slot[table[b][slot // PAGE] >= 0]
+        at = ch.slots_of(table[b], slot)
+        k, v = (x[at].repeat_interleave(N // x.shape[1], 1).transpose(0, 1).cuda() for x in (hk, hv))
+        own = int(start[b, -1] + length[b, -1]) - rows + torch.arange(rows)
+        qq = q[b, :, :rows].double().cuda()
+        x = (qq @ k.transpose(1, 2) * scale).masked_fill((slot > own[:, None]).cuda(), -torch.inf)
+        pad = (0, R - rows)
+        outs.append(torch.nn.functional.pad((torch.softmax(x, -1) @ v).transpose(0, 1), (0, 0, 0, 0) + pad))
+        lses.append(torch.nn.functional.pad(torch.logsumexp(x, -1), pad, value=-torch.inf))
+        sizes.append((qq.abs() @ k.abs().transpose(1, 2) * scale).amax())
+    return torch.stack(outs).cpu(), torch.stack(lses).cpu(), torch.stack(sizes).cpu()
+
+
+@pytest.mark.parametrize("dtype,N,Nk,D,R,pages,B", [
+    (BF16, 4, 2, 64, 1, 300, 1800), (BF16, 4, 2, 128, 2, 300, 1800), (BF16, 8, 2, 128, 2, 300, 1800), (BF16, 6, 2, 64, 5, 300, 1200),
+    (F32, 4, 2, 64, 1, 300, 1200), (F32, 2, 1, 64, 8, 300, 2400), (F32, 6, 2, 128, 2, 300, 1200),
+    (BF16, 4, 2, 128, 20, 700, 600), (BF16, 4, 2, 64, 70, 700, 600)])
+def test_shares_of_more_pages_than_a_cta_knows_of_at_a_time(dtype, N, Nk, D, R, pages, B):
+    """So many prompts that each is one share, of pages that are looked at in several goes: blocks that end and begin where those do,
+    a whole go without a token, prompts far shorter than the table, a page that does not exist.  (The prompts are 10 in turn.)"""
+    T, at = pages * PAGE, lambda page, more=0: page * PAGE + more
+    go = 256 if pages > 300 else 128
+    prompts = [  # (start, length) of three blocks
+        [(0, 50), (at(1), at(pages - 4)), (at(pages - 2), 2 * PAGE)],
+        [(0, at(go)), (at(go), at(go)), (at(2 * go), R + 1)],
+        [(0, at(go, -1)), (at(go, 1), 3), (at(2 * go, -1), R + 2)],
+        [(0, 1), (at(2 * go), 1), (at(pages - 2, 3), R + 40)],          # a go with nothing
+        [(at(2 * go, 5), 1), (at(2 * go, 6), 0), (at(2 * go + 1), R)],  # nothing before the last go
+        [(0, 5), (7, 0), (9, R)],
+        [(0, at(go)), (at(go), 0), (at(go), R + 63)],
+        [(3, at(1)), (at(5), at(go, 17)), (T - R, R)],
+        [(1, 31), (at(go, 32), 32), (T - R - 9, R + 9)],
+        [(0, T - 70), (T - 70, 0), (T - 70, 70)],
+    ]
+    start, length = (torch.tensor([[s[i] for s in p] for p in prompts], dtype=torch.int32) for i in (0, 1))
+    K = len(prompts)
+    cache, hk, hv = _filled(pages, Nk, D, 271, dtype)
+    table = _table(1, pages, pages, 40).repeat(K, 1)
+    q_len = torch.tensor([R - b % 3 if R > 3 else R for b in range(K)], dtype=torch.int32)
+    q = _rand(K, R, N, D, seed=41, dtype=dtype).transpose(1, 2)
+    ref, ref_lse, size = _attention_of_long(q, hk, hv, table, start, length, D ** -0.5, q_len)
+    rep = lambda x: x.repeat(-(-B // K), *[1] * (x.dim() - 1))[:B].cuda()
+    args = (rep(q), cache, rep(table), rep(start), rep(length), D ** -0.5)
+    ops.check_status()
+    out, lse = ops.cache_attention(*args, q_len=rep(q_len), return_lse=True)
+    ops.check_status()
+    _check(out[:K], lse[:K], ref, ref_lse, size, hv, 3 * pages + 8)
+    assert torch.equal(out, rep(out[:K])) and torch.equal(lse, rep(lse[:K]))
+    # the last page of one prompt does not exist, nor a page of another's second go
+    tab, kept = args[2].clone(), table[[0, 1]].clone()
+    tab[K, pages - 1], kept[0, pages - 1] = pages, -1
+    tab[K + 1, go + 7], kept[1, go + 7] = -5, -1
+    out2, lse2 = ops.cache_attention(args[0], cache, tab, *args[3:], q_len=rep(q_len), return_lse=True)
+    with pytest.raises(ValueError, match="of a call on the cache"):
+        ops.check_status()
+    same = (torch.arange(B) - K) // 2 != 0
+    assert torch.equal(out2[same.cuda()], out[same.cuda()]) and torch.equal(lse2[same.cuda()], lse[same.cuda()])
+    ref, ref_lse, size = _attention_of_long(q[:2], hk, hv, kept, start[:2], length[:2], D ** -0.5, q_len[:2])
+    _check(out2[K:K + 2], lse2[K:K + 2], ref, ref_lse, size, hv, 3 * pages + 8)
+
+
+@pytest.mark.parametrize("dtype,N,Nk,D,T", [(BF16, 4, 1, 64, 40000), (BF16, 8, 2, 128, 18000), (F32, 2, 1, 64, 20000)])
+def test_a_long_sequence_at_once(dtype, N, Nk, D, T):
+    """As many rows as tokens, longer than a CTA knows the pages of at a time; rows here and there against 64 bits."""
+    P = -(-T // PAGE)
+    cache, hk, hv = _filled(P, Nk, D, 281, dtype)
+    table = _table(1, P, P, 42)
+    start, length = torch.zeros(1, 1, dtype=torch.int32), torch.full((1, 1), T, dtype=torch.int32)
+    q = _rand(1, T, N, D, seed=43, dtype=dtype).transpose(1, 2)
+    out, lse = ops.cache_attention(q.cuda(), cache, table.cuda(), start.cuda(), length.cuda(), 0.1, return_lse=True)
+    at = ch.slots_of(table[0], torch.arange(T))
+    k, v = (x[at].repeat_interleave(N // Nk, 1).transpose(0, 1).cuda() for x in (hk, hv))
+    rows = torch.cat([torch.arange(0, T, 997), torch.tensor([63, 64, 127, 8191, 8192, 16383, 16384, T - 2, T - 1])]).cuda()
+    qq = q[0].cuda()[:, rows].double()
+    x = (qq @ k.transpose(1, 2) * 0.1).masked_fill(torch.arange(T, device="cuda") > rows[:, None], -torch.inf)
+    ref, ref_lse = (torch.softmax(x, -1) @ v).transpose(0, 1)[None], torch.logsumexp(x, -1)[None]
+    size = (qq.abs() @ k.abs().transpose(1, 2) * 0.1).amax()
+    _check(out[:, rows], lse[:, :, rows], ref.cpu(), ref_lse.cpu(), size, hv, 3 * P + 8)
+    assert bool(torch.isfinite(out).all()) and bool(torch.isfinite(lse).all())
+    ops.check_status()
