@@ -21,7 +21,9 @@ struct IoArgs {
   unsigned char* pages;
   View k, v;
   const int32_t* slots;
-  int32_t* owner;  // [slots of the pool]: the last token of the call that names the slot; null: looked up in `slots`
+  int32_t* owner;  // where owner_place says: the last token of the call that names the slot; null: looked up in `slots`
+  int32_t* key;    // a table by hash: the slot that a place is for, -1 for none; null: a place per slot of the pool
+  int hash_shift;  // 32 - log2 of the table's places
   int32_t* status;
   int64_t n_slots;
   int tokens;  // B S
@@ -158,15 +160,43 @@ constexpr int kTile = 32;  // tokens of a CTA, at most
 // 4096 14.5 and 8.3.)
 constexpr int kScan = 2048;
 
-__global__ void __launch_bounds__(256) owner_clear_kernel(const int32_t* slots, int tokens, int64_t n_slots, int32_t* owner) {
-  const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
-  ptx::grid_dependency_wait();
-  if (i < tokens && slots[i] >= 0 && slots[i] < n_slots) owner[slots[i]] = -1;
+// Places of a table by hash for so many tokens: a power of two, at most half of them taken.  It takes longer (16,384 tokens 32 us, with a
+// place per slot of the pool 23.5; 78,720 91 and 83), so it is used for pools of more than 2^24 slots (64 MB of places) alone, where it is
+// smaller: a pool has as many slots as the memory has room for.
+int64_t hash_places(int64_t tokens) {
+  int64_t n = 1;
+  while (n < 2 * tokens) n *= 2;
+  return n;
 }
-__global__ void __launch_bounds__(256) owner_claim_kernel(const int32_t* slots, int tokens, int64_t n_slots, int32_t* owner) {
+bool by_hash(int64_t tokens, int64_t n_slots) { return n_slots > 1 << 24 && 2 * hash_places(tokens) < n_slots; }
+
+// The place of a slot: in a table by hash the first one from the hash on that has its key, or none.
+template <bool kEnter>
+__device__ __forceinline__ int32_t* owner_place(const IoArgs& a, int slot) {
+  if (a.key == nullptr) return a.owner + slot;
+  const uint32_t last = ~0u >> a.hash_shift;
+  uint32_t at = (uint32_t)slot * 0x9E3779B1u >> a.hash_shift;  // (2^32 over the golden ratio: neighbours lie far apart)
+  for (;; at = (at + 1) & last) {
+    const int there = kEnter ? atomicCAS(a.key + at, -1, slot) : a.key[at];
+    if (there == slot || there < 0) return a.owner + at;
+  }
+}
+__global__ void __launch_bounds__(256) owner_clear_kernel(IoArgs a) {
   const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
   ptx::grid_dependency_wait();
-  if (i < tokens && slots[i] >= 0 && slots[i] < n_slots) atomicMax(owner + slots[i], (int)i);
+  if (a.key) {
+    if (i <= ~0u >> a.hash_shift) a.key[i] = a.owner[i] = -1;
+  } else if (i < a.tokens) {
+    const int slot = a.slots[i];
+    if (slot >= 0 && slot < a.n_slots) a.owner[slot] = -1;
+  }
+}
+__global__ void __launch_bounds__(256) owner_claim_kernel(IoArgs a) {
+  const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
+  ptx::grid_dependency_wait();
+  if (i >= a.tokens) return;
+  const int slot = a.slots[i];
+  if (slot >= 0 && slot < a.n_slots) atomicMax(owner_place<true>(a, slot), (int)i);
 }
 
 // Where the CTA's tokens are: element offsets of their rows in k and v, and the byte offset of head 0's page and the place in it
@@ -202,7 +232,7 @@ __device__ __forceinline__ void find_tokens(const IoArgs& a, Tile& tile, int fir
       if (a.status) atomicCAS(a.status, 0, kStatusBadSlot);
       slot = -1;
     }
-    if (kWrite && slot >= 0 && (a.owner ? a.owner[slot] != tok : later[threadIdx.x] != 0)) slot = -1;
+    if (kWrite && slot >= 0 && (a.owner ? *owner_place<false>(a, slot) != tok : later[threadIdx.x] != 0)) slot = -1;
     const int b = tok / a.S, s = tok % a.S;
     tile.k[threadIdx.x] = b * a.k.sb + s * a.k.ss;
     tile.v[threadIdx.x] = b * a.v.sb + s * a.v.ss;
@@ -380,7 +410,8 @@ IoArgs make_args(const brk_cache& c, const brk_view& k, const brk_view& v, int B
   a.k = make_view(k);
   a.v = make_view(v);
   a.slots = slots;
-  a.owner = nullptr;
+  a.owner = a.key = nullptr;
+  a.hash_shift = 0;
   a.status = status;
   a.n_slots = (int64_t)c.n_pages * kPage;
   a.tokens = B * S;
@@ -398,7 +429,9 @@ dim3 grid_of(const IoArgs& a) { return dim3((unsigned)((a.tokens + (int64_t)a.ti
 }  // namespace
 
 size_t cache_write_workspace(const brk_cache& c, int B, int S) {
-  return (int64_t)B * S <= kScan ? 0 : (size_t)c.n_pages * kPage * sizeof(int32_t);
+  const int64_t tokens = (int64_t)B * S, n_slots = (int64_t)c.n_pages * kPage;
+  if (tokens <= kScan) return 0;
+  return sizeof(int32_t) * (by_hash(tokens, n_slots) ? 2 * hash_places(tokens) : n_slots);
 }
 
 int cache_write_launch(int dtype, const brk_cache& c, const brk_view& k, const brk_view& v, int B, int S, const int32_t* slots, void* ws,
@@ -406,9 +439,15 @@ int cache_write_launch(int dtype, const brk_cache& c, const brk_view& k, const b
   IoArgs a = make_args(c, k, v, B, S, slots, status);
   if (a.tokens > kScan) {
     a.owner = static_cast<int32_t*>(ws);
-    const dim3 n((unsigned)((a.tokens + 255ll) / 256));
-    int rc = launch_dependent(owner_clear_kernel, n, dim3(256), 0, st, slots, a.tokens, a.n_slots, a.owner);
-    if (rc || (rc = launch_dependent(owner_claim_kernel, n, dim3(256), 0, st, slots, a.tokens, a.n_slots, a.owner))) return rc;
+    int64_t cleared = a.tokens;
+    if (by_hash(a.tokens, a.n_slots)) {
+      cleared = hash_places(a.tokens);
+      a.key = a.owner + cleared;
+      for (a.hash_shift = 32; (int64_t)1 << (32 - a.hash_shift) < cleared;) --a.hash_shift;
+    }
+    auto of = [](int64_t n) { return dim3((unsigned)((n + 255) / 256)); };
+    int rc = launch_dependent(owner_clear_kernel, of(cleared), dim3(256), 0, st, a);
+    if (rc || (rc = launch_dependent(owner_claim_kernel, of(a.tokens), dim3(256), 0, st, a))) return rc;
   }
   auto run = [&](auto kern) { return launch_dependent(kern, grid_of(a), dim3(kIoThreads), 0, st, a); };
   if (dtype == BRK_BF16) return c.D == 128 ? run(cache_write_kernel<__nv_bfloat16, 128>) : run(cache_write_kernel<__nv_bfloat16, 64>);

@@ -269,7 +269,8 @@ BRK_API size_t brk_cache_page_bytes(int32_t Nk, int32_t D);
 
 /* Quantises k and v ((B, Nk, S, D) views, dtype BRK_BF16 or BRK_F32) into slots[B * S] (page * BRK_CACHE_PAGE + offset;
  * negative: skip).  Slots that no token names keep what they hold; one that several tokens name gets the last one's (in the order of
- * `slots`).  Workspace: brk_cache_write_workspace_bytes (0 for up to 2048 tokens). */
+ * `slots`).  Workspace: brk_cache_write_workspace_bytes (0 for up to 2048 tokens; otherwise 4 bytes per slot of the pool, of
+ * more than 2^24 slots fewer than 32 bytes per token if that is less). */
 BRK_API size_t brk_cache_write_workspace_bytes(const brk_cache* c, int32_t B, int32_t S);
 BRK_API int brk_cache_write(int32_t dtype, const brk_cache* c, const brk_view* k, const brk_view* v, int32_t B, int32_t S,
                             const int32_t* slots, void* workspace, size_t workspace_bytes, int32_t* status, void* stream);

@@ -115,3 +115,11 @@ def test_workspaces_do_not_grow_with_the_call(dtype, N, Nk, D, Lq, tokens, B):
     p = _attn(dtype=dtype, N=N, Lq=Lq, B=B, P=-(-tokens // 64), cache=_cache(2 ** 18, Nk, D), q=view, o=view)
     need = _lib.lib().brk_cache_attn_workspace_bytes(C.byref(p))
     assert need <= 8 * 148 * 256 * (4 * D + 8), need
+
+
+@pytest.mark.parametrize("tokens", [2049, 4096, 4097, 100000, 2 ** 26 + 1])
+def test_the_workspace_of_a_write_to_a_large_pool_goes_by_its_tokens(tokens):
+    """(156 million slots of 8 heads of 128 are a GPU's memory: 4 bytes of each were 625 MB for 2,049 tokens)"""
+    for n_pages in (1, 33, 50000, 2 ** 18, 2 ** 18 + 1, 2 ** 21, 2 ** 25 - 1):
+        need = _lib.lib().brk_cache_write_workspace_bytes(C.byref(_cache(n_pages)), 1, tokens)
+        assert 0 < need <= min(4 * 64 * n_pages, max(2 ** 26, 32 * tokens))

@@ -1039,3 +1039,35 @@ def test_a_long_sequence_at_once(dtype, N, Nk, D, T):
     _check(out[:, rows], lse[:, :, rows], ref.cpu(), ref_lse.cpu(), size, hv, 3 * P + 8)
     assert bool(torch.isfinite(out).all()) and bool(torch.isfinite(lse).all())
     ops.check_status()
+
+
+@pytest.mark.parametrize("S,different", [(2049, 40), (4096, 4096), (20000, 5000)])
+@pytest.mark.parametrize("step", [1, 64, 8191, 1048573])
+def test_of_tokens_with_the_same_slot_the_last_one_is_kept_in_a_large_pool(S, different, step):
+    """A pool so much larger than the call that the tokens of its slots are looked up by hash; slots side by side, page by page, far apart."""
+    Nk, D, pool = 1, 64, 2 ** 18 + 1000
+    n_slots = pool * PAGE
+    c = _lib.Cache(64, pool, Nk, D)
+    assert _lib.lib().brk_cache_write_workspace_bytes(c, 1, S) < 4 * n_slots
+    k, v = (_rand(1, S, Nk, D, seed=i, dtype=BF16) for i in (0, 1))
+    g = torch.Generator().manual_seed(S)
+    slots = (torch.randint(0, different, (1, S), generator=g) * step % n_slots).int()
+    slots[0, ::17] = -1
+    slots[0, 5::97] = n_slots + 3
+    last = {s: i for i, s in enumerate(slots[0].tolist()) if 0 <= s < n_slots}
+    cache = ops.cache_alloc(pool, Nk, D, "cuda")
+    ops.check_status()
+    ops.cache_write(k.transpose(1, 2).cuda(), v.transpose(1, 2).cuda(), cache, slots.cuda())
+    with pytest.raises(ValueError, match="slot lies outside the cache"):
+        ops.check_status()
+    at, tok = torch.tensor(list(last), dtype=torch.int32)[None], torch.tensor(list(last.values()))
+    for got, x in zip(ops.cache_read(cache, at.cuda(), F32), (k, v)):
+        assert torch.equal(got[0].transpose(0, 1).double().cpu(), ch.held(x[0, tok]))
+    pages = torch.ones(pool, dtype=torch.bool)
+    pages[at[0].long() // PAGE] = False
+    assert not cache[pages.cuda()].any()
+    others = torch.ones(n_slots, dtype=torch.bool)
+    others[at[0].long()] = False
+    rest = (others.view(pool, PAGE) & ~pages[:, None]).view(-1).nonzero().T.int().cuda()
+    assert not any(x.any() for x in ops.cache_read(cache, rest, F32))
+    ops.check_status()
