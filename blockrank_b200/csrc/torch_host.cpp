@@ -417,6 +417,14 @@ void need_device(const Tensor& of, std::initializer_list<const Tensor*> ts) {
   for (const Tensor* t : ts)
     if (t != nullptr && t->defined()) BRK_VALUE(t->device() == of.device(), "tensors on ", of.device(), " and ", t->device());
 }
+// A call on the cache has no derivative: inputs that want one are refused, as the attention function refuses them for its fused scores.
+void need_no_grad(std::initializer_list<const Tensor*> ts) {
+  for (const Tensor* t : ts)
+    if (t != nullptr && t->defined())
+      TORCH_CHECK_NOT_IMPLEMENTED(!(at::GradMode::is_enabled() && t->requires_grad()) && !t->_fw_grad(/*level=*/0).defined(),
+                                  "the 4-bit cache is inference-only: a tensor of this call requires a gradient (call it under torch.no_grad(), or "
+                                  "detach the tensor)");
+}
 // view_of (view_bshd), for any stride of a dimension of one
 brk_view heads_view(const Tensor& t, bool bshd = false) {
   brk_view v = bshd ? view_bshd(t) : view_of(t);
@@ -442,6 +450,7 @@ Tensor cache_alloc(int64_t n_pages, int64_t kv_heads, int64_t head_dim, const c1
 }
 
 void cache_write(const Tensor& k, const Tensor& v, const Tensor& cache, const Tensor& slots_in) {
+  need_no_grad({&k, &v});
   need_cuda({&k, &v, &cache, &slots_in});
   need_device(cache, {&k, &v, &slots_in});
   const brk_cache c = cache_of(cache);
@@ -496,6 +505,7 @@ void need_prompts(const Tensor& q, const brk_cache& c, const Tensor& table, cons
 
 std::tuple<Tensor, Tensor> cache_attention(const Tensor& q, const Tensor& cache, const Tensor& table_in, const Tensor& blk_start, const Tensor& blk_len,
                                            double scale, const OptTensor& q_len_in, const OptTensor& out_in, bool return_lse) {
+  need_no_grad({&q, opt(out_in)});
   need_cuda({&q, &cache, &table_in, &blk_start, &blk_len, opt(q_len_in), opt(out_in)});
   need_device(cache, {&q, &table_in, &blk_start, &blk_len, opt(q_len_in), opt(out_in)});
   const brk_cache c = cache_of(cache);
@@ -538,6 +548,7 @@ std::tuple<Tensor, Tensor> cache_attention(const Tensor& q, const Tensor& cache,
 
 std::tuple<Tensor, Tensor> cache_doc_scores(const Tensor& q, const Tensor& cache, const Tensor& table_in, const Tensor& blk_start, const Tensor& blk_len,
                                             double scale, int64_t max_block_len, double temperature) {
+  need_no_grad({&q});
   need_cuda({&q, &cache, &table_in, &blk_start, &blk_len});
   need_device(cache, {&q, &table_in, &blk_start, &blk_len});
   const brk_cache c = cache_of(cache);

@@ -121,7 +121,8 @@ def cache_alloc(n_pages: int, kv_heads: int, head_dim: int, device=None) -> torc
 
     A prompt is a row of a page table, int32: its slot s lies in page ``page_table[b, s // 64]`` at offset ``s % 64``.  A
     document's keys and values depend on the instruction block and the document alone: any number of prompts can share its
-    pages.  None of the cache functions records a gradient.
+    pages.  The cache is for inference: a call with keys, values or queries that require a gradient raises NotImplementedError unless
+    it is made under ``torch.no_grad()``.
     """
     device = torch.device("cuda" if device is None else device)
     if device.type == "cuda" and device.index is None:

@@ -123,3 +123,19 @@ def test_the_workspace_of_a_write_to_a_large_pool_goes_by_its_tokens(tokens):
     for n_pages in (1, 33, 50000, 2 ** 18, 2 ** 18 + 1, 2 ** 21, 2 ** 25 - 1):
         need = _lib.lib().brk_cache_write_workspace_bytes(C.byref(_cache(n_pages)), 1, tokens)
         assert 0 < need <= min(4 * 64 * n_pages, max(2 ** 26, 32 * tokens))
+
+
+def test_tensors_that_require_a_gradient_are_refused():
+    i = torch.zeros(1, 1, dtype=torch.int32)
+    x, c = torch.zeros(1, 1, 1, 64), torch.zeros(1, 1, 64 * 72, dtype=torch.uint8)
+    p = x.clone().requires_grad_()
+    calls = (lambda g: ops.cache_write(g, x, c, i), lambda g: ops.cache_write(x, g, c, i), lambda g: ops.cache_attention(g, c, i, i, i, 1.0),
+             lambda g: ops.cache_attention(x, c, i, i, i, 1.0, out=g), lambda g: ops.cache_doc_scores(g, c, i, i, i, 1.0, 1))
+    for call in calls:
+        for t in (p, p * 2):
+            with pytest.raises(NotImplementedError, match="inference-only"):
+                call(t)
+            with torch.no_grad(), pytest.raises(RuntimeError, match="CUDA tensors"):  # (the next refusal: there is no GPU)
+                call(t)
+    with torch.autograd.forward_ad.dual_level(), pytest.raises(NotImplementedError, match="inference-only"):
+        ops.cache_attention(torch.autograd.forward_ad.make_dual(x, x), c, i, i, i, 1.0)

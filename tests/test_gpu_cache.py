@@ -1071,3 +1071,24 @@ def test_of_tokens_with_the_same_slot_the_last_one_is_kept_in_a_large_pool(S, di
     rest = (others.view(pool, PAGE) & ~pages[:, None]).view(-1).nonzero().T.int().cuda()
     assert not any(x.any() for x in ops.cache_read(cache, rest, F32))
     ops.check_status()
+
+
+def test_gradients_are_refused_and_not_dropped():
+    cache, _, _ = _filled(2, 2, 64, 301)
+    z = lambda *s: torch.zeros(*s, dtype=torch.int32, device="cuda")
+    x, one = (torch.ones(1, n, 1, 64, dtype=BF16, device="cuda") for n in (4, 2))
+    spans = z(1, 1), torch.arange(3, dtype=torch.int32, device="cuda")[None], z(1, 3) + 1  # the page table, three blocks of one token
+    attend, score = lambda: ops.cache_attention(x, cache, *spans, 1.0), lambda: ops.cache_doc_scores(x, cache, *spans, 1.0, 1)
+    want = attend(), score()
+    before = cache.clone()
+    x.requires_grad_(), one.requires_grad_()
+    for call in (attend, score, lambda: ops.cache_write(one, one, cache, z(1, 1))):
+        with pytest.raises(NotImplementedError, match="inference-only"):
+            call()
+    assert torch.equal(cache, before)
+    with torch.no_grad():
+        got = attend(), score()
+        ops.cache_write(one, one, cache, z(1, 1))
+    assert torch.equal(got[0], want[0]) and all(torch.equal(a, b) for a, b in zip(got[1], want[1]))
+    assert not torch.equal(cache, before)
+    ops.check_status()
