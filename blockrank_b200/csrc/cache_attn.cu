@@ -406,6 +406,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<T, kTiles>) cache_attn_k
     }
   }
   if (!a.cluster) return;
+  __syncwarp();  // (at head_dim 64 a warp has pieces of two rows, of which only one may exist)
   ptx::cluster_sync();
   // Every CTA joins some of the rows' pieces of 4 channels: at most kPieces to a thread.
   constexpr int kPieces = (kRows * (D / 4) / 2 + kThreads - 1) / kThreads;

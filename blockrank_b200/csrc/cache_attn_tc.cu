@@ -161,6 +161,10 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attn_tc_kernel(CacheAttnArg
     __syncwarp();
     asm volatile("bar.sync 3, %0;" ::"n"(kThreads) : "memory");
   };
+  auto unpackers_meet = [] {
+    __syncwarp();
+    asm volatile("bar.sync 1, 128;" ::: "memory");
+  };
 
   if (warp < kSoftWarps) {
     // =============================== softmax: a thread per row ===========================================
@@ -464,7 +468,7 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attn_tc_kernel(CacheAttnArg
         for (int j = 0; j < kG; ++j) vs[j] &= keep;
         if (late) {
           if (p < 2 * kG) s_nan[buf][p / 2][p % 2] = 0;
-          asm volatile("bar.sync 1, 128;" ::: "memory");
+          unpackers_meet();
 #pragma unroll
           for (int j = 0; j < kG; ++j) {
             const uint32_t is = __vcmpeq2(vs[j] & 0x7F807F80u, 0x7F807F80u);
@@ -495,8 +499,7 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attn_tc_kernel(CacheAttnArg
       meet();
       page0 += kAtOnce;
       find_pages(a, lists_of(a, b), s_prompt, page0, min(sh.page0 + sh.n - page0, kAtOnce), p, 32 * kUnpackWarps, s_mask, s_page);
-      __syncwarp();
-      asm volatile("bar.sync 1, 128;" ::: "memory");
+      unpackers_meet();
       if (warp == kSoftWarps) make_list(page0, known);
       meet();
     }
