@@ -105,7 +105,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<T, kTiles>) cache_attn_k
     for (int x = 0; x < 2; ++x) {
       const int col = 8 * c + (kTwice ? 2 * (t & 1) : 2 * t) + x;
       lim[c][x] = col < n_rows ? first_slot + (row0 + col) / G : INT_MAX;
-      sl2[c][x] = a.scale * kLog2e * q.unit[c][x];
+      sl2[c][x] = q.exponent_scale(a.scale, c, x);
     }
   const int first_lim = first_slot + row0 / G;  // the least of the CTA's rows
   const Codes codes = a.codes;

@@ -250,6 +250,12 @@ struct QueryRows {
       for (int y = 0; y < 2; ++y) unit[n][y] = __shfl_sync(0xffffffffu, down, 4 * (2 * t + y));
     }
   }
+  // What logits of tile n's columns x are multiplied by to be exponents of 2.  Never 0 (a row of zeros has the smallest unit, 2^-113, and a
+  // scale can be smaller still): the running maximum begins at -infinity.
+  __device__ __forceinline__ float exponent_scale(float scale, int n, int x) const {
+    const float f = scale * 1.4426950408889634f * unit[n][x];
+    return f == 0.f ? 0x1p-149f : f;
+  }
   // s[n][i]: the C fragment of keys 16 i .. 16 i + 15 of the page and the columns of tile n
   __device__ __forceinline__ void logits(const unsigned char* page, int g, int t, float (&s)[kTiles][4][4]) const {
 #pragma unroll

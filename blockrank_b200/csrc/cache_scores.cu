@@ -152,7 +152,7 @@ __global__ void __launch_bounds__(kThreads, kTiles == 1 && sizeof(T) == 2 ? 3 : 
   for (int c = 0; c < kTiles; ++c)
 #pragma unroll
     for (int x = 0; x < 2; ++x) {
-      sl2[c][x] = a.scale * kLog2e * q.unit[c][x];
+      sl2[c][x] = q.exponent_scale(a.scale, c, x);
       mx[c][x] = -INFINITY;
       sum[c][x] = 0.f;
     }

@@ -1092,3 +1092,26 @@ def test_gradients_are_refused_and_not_dropped():
     assert torch.equal(got[0], want[0]) and all(torch.equal(a, b) for a, b in zip(got[1], want[1]))
     assert not torch.equal(cache, before)
     ops.check_status()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("rows", [1, 3, 5, 20])
+@pytest.mark.parametrize("scale", [1e-12, 1e-30, 1.2e-38])
+def test_queries_of_zeros_and_scales_next_to_nothing(dtype, rows, scale):
+    """Every slot counts the same: the mean of the values, the logarithm of their number, documents by their tokens."""
+    N, Nk, D = 4, 2, 64
+    start, length, P = ch.spans([[5, 64, 1, 100, rows + 30], [1, 63, 65, 0, rows]], False, gap=3)
+    cache, hk, hv = _filled(2 * P, Nk, D, 311, dtype)
+    table = _table(2, P, 2 * P, 44)
+    q = _rand(2, rows, N, D, seed=45, dtype=dtype).transpose(1, 2).contiguous()
+    q[:, 1] = 0
+    q[:, 2] = torch.finfo(dtype).tiny / 4
+    ref, ref_lse, size = ch.attention(q, hk, hv, table, start, length, scale)
+    for tab in (table, _wide(table)):
+        out, lse = ops.cache_attention(q.cuda(), cache, tab.cuda(), start.cuda(), length.cuda(), scale, return_lse=True)
+        _check(out, lse, ref, ref_lse, size, hv, 3 * P + 8)
+    mass, logits = ops.cache_doc_scores(q[:, :, :3].cuda(), cache, table.cuda(), start.cuda(), length.cuda(), scale, 100)
+    want = ch.doc_mass(q[:, :, :3], hk, table, start, length, scale)
+    assert torch.allclose(mass.double().cpu(), want, rtol=2.0 ** -16, atol=0)  # (64 accumulations of 2^-23, as in test_document_scores)
+    assert torch.allclose(logits.double().cpu(), want.mean((1, 2)) / 0.05, rtol=2.0 ** -16, atol=0)
+    ops.check_status()
