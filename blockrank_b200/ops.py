@@ -152,7 +152,7 @@ def cache_attention(q: torch.Tensor, cache: torch.Tensor, page_table: torch.Tens
     """Attention of the last tokens of every prompt over its pages: :func:`attention`'s query block, with the cache in the place
     of k and v (the tokens' own keys and values are written first).
 
-    q (B,N,L,D), magnitudes below 2^115; page_table int32 (B,P); blk_start / blk_len int32 (B,M): the slots of the prompt's blocks, as for
+    q (B,N,L,D), magnitudes below 2^114, also times ``scale``; page_table int32 (B,P); blk_start / blk_len int32 (B,M): the slots of the prompt's blocks, as for
     :func:`attention` (slots between blocks have no influence; M = 1: one causal sequence).  Row i is the token at slot
     ``blk_start[b,-1] + blk_len[b,-1] - q_len[b] + i`` and sees every block's slots up to its own.  ``q_len`` int32 (B,): the number
     of rows of each prompt (None: L), from 0 to the last block's length.  Returns out (B,L,N,D) [and lse (B,N,L) fp32]; rows from
@@ -167,7 +167,7 @@ def cache_doc_scores(q: torch.Tensor, cache: torch.Tensor, page_table: torch.Ten
                      scale: float, max_block_len: int, temperature: float = 0.05) -> Tuple[torch.Tensor, torch.Tensor]:
     """:func:`doc_scores` with the document keys from the cache.
 
-    q (B,N,R,D): the signal rows' queries; page table and spans as for :func:`cache_attention` (blocks 1..M-2 are the documents), of
+    q (B,N,R,D): the signal rows' queries, magnitudes as there; page table and spans as for :func:`cache_attention` (blocks 1..M-2 are the documents), of
     documents of up to ``max_block_len`` tokens.  Returns (doc_mass (B,N,R,num_docs) fp32, logits (B,num_docs) fp32).  A prompt with
     malformed spans (of whichever block) or a longer document gets zeros, a page that does not exist takes its tokens away; both raise
     at the next :func:`check_status`.

@@ -282,7 +282,9 @@ BRK_API int brk_cache_read(int32_t dtype, const brk_cache* c, const brk_view* k,
  * the tokens' own among them).  Row i < q_len[b] of q is the token at slot
  *   blk_start[b, M-1] + blk_len[b, M-1] - q_len[b] + i
  * and sees the slots of all blocks at or before its own.  Rows from q_len[b] on, and rows that see nothing, get zeros (lse:
- * -infinity).  M == 1: one causal sequence.  The slots between blocks, and what their pages hold, have no influence. */
+ * -infinity).  M == 1: one causal sequence.  The slots between blocks, and what their pages hold, have no influence.
+ * Magnitudes of q, and those times scale, are below 2^114 (rows with NaN, infinities or larger ones have no meaning), here and in
+ * brk_cache_doc_scores. */
 typedef struct brk_cache_attn_params {
   int32_t dtype;          /* BRK_BF16 or BRK_F32 (q, o) */
   int32_t B, N, Lq;       /* prompts, query heads, rows per prompt */

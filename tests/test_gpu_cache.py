@@ -1115,3 +1115,27 @@ def test_queries_of_zeros_and_scales_next_to_nothing(dtype, rows, scale):
     assert torch.allclose(mass.double().cpu(), want, rtol=2.0 ** -16, atol=0)  # (64 accumulations of 2^-23, as in test_document_scores)
     assert torch.allclose(logits.double().cpu(), want.mean((1, 2)) / 0.05, rtol=2.0 ** -16, atol=0)
     ops.check_status()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("rows", [1, 5, 20])
+@pytest.mark.parametrize("e,scale", [(114, 1.0), (112, 4.0), (114, 1e-3), (60, 1.0), (-100, 1.0)])
+def test_queries_as_large_as_they_may_be(dtype, rows, e, scale):
+    """Largest magnitude next to 2^e, of keys that make ordinary logits of them."""
+    N, Nk, D = 4, 2, 64
+    start, length, P = ch.spans([[5, 64, 1, 100, rows + 30]], False)
+    k, v = (_rand(P * PAGE, Nk, D, seed=321 + i, dtype=F32) for i in (0, 1))
+    k, v = (k.clamp(-4, 4) * 2.0 ** -e / scale).to(dtype), v.to(dtype)
+    cache = ops.cache_alloc(P, Nk, D, "cuda")
+    ops.cache_write(*(x[None].transpose(1, 2).cuda() for x in (k, v)), cache, torch.arange(P * PAGE, dtype=torch.int32, device="cuda")[None])
+    hk, hv, table = ch.held(k), ch.held(v), torch.arange(P, dtype=torch.int32)[None]
+    q = _rand(1, rows, N, D, seed=46, dtype=F32)
+    q = (q / q.abs().max() * 2.0 ** e * 0.99).to(dtype).transpose(1, 2)
+    ref, ref_lse, size = ch.attention(q, hk, hv, table, start, length, scale)
+    for tab in (table, _wide(table)):
+        out, lse = ops.cache_attention(q.cuda(), cache, tab.cuda(), start.cuda(), length.cuda(), scale, return_lse=True)
+        _check(out, lse, ref, ref_lse, size, hv, 3 * P + 8)
+    mass, _ = ops.cache_doc_scores(q[:, :, :2].cuda(), cache, table.cuda(), start.cuda(), length.cuda(), scale, 100)
+    want = ch.doc_mass(q[:, :, :2], hk, table, start, length, scale)
+    assert torch.allclose(mass.double().cpu(), want, rtol=2 * float(size.max()) * 24 * 2.0 ** -23 + 2.0 ** -17, atol=0)
+    ops.check_status()
