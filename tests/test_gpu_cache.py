@@ -1139,3 +1139,24 @@ def test_queries_as_large_as_they_may_be(dtype, rows, e, scale):
     want = ch.doc_mass(q[:, :, :2], hk, table, start, length, scale)
     assert torch.allclose(mass.double().cpu(), want, rtol=2 * float(size.max()) * 24 * 2.0 ** -23 + 2.0 ** -17, atol=0)
     ops.check_status()
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_properties_of_what_the_kernels_hold(dtype, D):
+    """Read back, values are exact in bf16, half a step of their scale off at most, and held as the same bytes when written again."""
+    Nk, pool = 3, 8
+    g = torch.Generator().manual_seed(9)
+    x = [(torch.randn(pool * PAGE, Nk, D, generator=g) * torch.exp(8 * torch.randn(pool * PAGE, Nk, 1, generator=g))).to(dtype) for _ in range(2)]
+    every = torch.arange(pool * PAGE, dtype=torch.int32, device="cuda")[None]
+    caches = [ops.cache_alloc(pool, Nk, D, "cuda") for _ in range(3)]
+    ops.cache_write(*(t[None].transpose(1, 2).cuda() for t in x), caches[0], every)
+    wide, narrow = (ops.cache_read(caches[0], every, t) for t in (F32, BF16))
+    for w, n, t in zip(wide, narrow, x):
+        assert torch.equal(w, n.float())
+        half = ch.scales(t).repeat_interleave(32, -1) / 2
+        assert bool(((w[0].transpose(0, 1).double().cpu() - t.double()).abs() <= half).all())
+    for held, c in zip((wide, narrow), caches[1:]):
+        ops.cache_write(*held, c, every)
+        assert torch.equal(c, caches[0])
+    ops.check_status()
