@@ -1,10 +1,14 @@
 // Attention of a prompt's last tokens over its pages of the 4-bit cache, and the join of its parts.
 //
 // out = sum_j softmax_j(scale q . k_j) v_j over the slots j that row i sees: those of all blocks at or before its own slot.
-// The floor is the read of the cache (144 bytes per token and KV head at head_dim 128); bound by the instructions that bring the codes
-// into the products: from registers alone, 12 warps to an SM, a scheduler takes 364 cycles for 16 keys (K 139, softmax 40, V 206 where
-// they are timed one by one), which would be 7.1 TB/s.  One row each of 16 prompts of 100 documents (32 to 256 tokens), 32 heads
-// on 8: 82 us, 3.2 TB/s; of two contexts of 131,072 tokens 70 us, 4.3 TB/s; of one prompt of 5 documents 7.3 us, all of it latency.
+// The floor is the read of the cache (144 bytes per token and KV head at head_dim 128).  Bound by latency: a page's products, softmax and
+// unpacking are one chain in a warp, which two or three warps to a scheduler cover in part.  From registers alone, 12 warps to an SM, a
+// scheduler takes 364 cycles for 16 keys (K 139, softmax 40, V 206 where they are timed one by one), which would be 7.1 TB/s; in the kernel it
+// takes 507 (5.3 TB/s at 1,965 MHz: two contexts of twice the tokens take 57.2 us more), 287 of them with an instruction; the ALU pipe, the
+// busiest unit, is at 52 %.  One row each of two contexts of 131,072 tokens, 32 heads on 8: 69 us, 4.4 TB/s, of which 12 are beginning, end and
+// join (kept up, the board's 1000 W bring the clock to 1,820 MHz: 73.5 us); of 16 prompts of 100 documents (32 to 256 tokens) 81 us, 3.2 TB/s:
+// some SMs have two CTAs and some three, and 21 % more slots are worked on than there are tokens, because a document's last page is taken
+// whole; of one prompt of 5 documents 7.3 us, all of it latency.
 //
 // A CTA takes a share of one prompt's pages for one KV head and up to 8 kTiles rows (a row: a query head of the group at one
 // token).  Its warps take whole pages in turn and share nothing until the end: running maximum, sum and output of a warp

@@ -10,8 +10,11 @@
 // Channels stand in K and V in whatever order the codes come out in, without a permutation: Q's are brought into K's order once, O's
 // columns are given their names as they are written.
 //
-// Bound by the integer instructions of softmax and unpacking together (of a page's 2,350 cycles with two tiles about 1,700; the products
-// take 1,950 of them beside it): 4 prompts of 100 documents of 160 tokens, 45 tokens by 4 heads in the longest: 105 us.  On the way there:
+// Bound by the chain that a page is for a softmax thread (S out of tensor memory, maximum, exponentials, P into it: 2,200 of a page's
+// 2,350 cycles by clocks read inside, 45 tokens by 4 heads), which two such warps and one that unpacks to a scheduler cover in part.  Two
+// tiles of 192 rows, 64 pages more to a CTA: 1.41 us a page, under the profiler 2,590 cycles, in which a scheduler has 1,385 instructions; ALU
+// pipe 41 %, special functions 40 %, tensor pipe 56 %.  One tile: 1.0 us.  4 prompts of 100 documents of 160 tokens, up to 45 tokens by 4 heads: 104 us, of
+// which a CTA has 18,000 cycles in front of its pages and behind them.  On the way there:
 // products issued in a loop 131 us, unrolled 125; Q by asynchronous copies 120.6; one tile by both groups, outputs through
 // shared memory 117; no permutations 110; of a page that ends in its first half only that half 107, the parts joined
 // by more rows to a CTA 105.  (Q in tensor memory, one S to a tile: 124 where this took 125.)

@@ -242,8 +242,9 @@ __device__ __forceinline__ void find_tokens(const IoArgs& a, Tile& tile, int fir
   __syncthreads();
 }
 
-// Bound by the reads (4 D bytes a token and head in bf16) and, close behind, by the arithmetic of quantising: 62 % of the ALU pipe.  Every token of
-// 4 prompts of 100 documents, 8 heads of 128: 71 us, 4.0 TB/s; with a warp to a row and one channel at a time 199.
+// The floor is the read (4 D bytes a token and head in bf16) and what is held.  Bound by the wait for the loads, at 21 warps to an SM, and by
+// the arithmetic of quantising, 60 % of the ALU pipe.  Every token of 4 prompts of 100 documents, 8 heads of 128: 71 us, its bytes 52; in fp32
+// 114 and 92; with a warp to a row and one channel at a time 199.
 // Eight lanes take two rows (a token's key and value in one head).  K: four lanes a row, lane t the channels 32 j + 8 t + 0..7, its
 // codes one access.  V: all eight both rows, lane g the channels 32 j + 4 g + 0..3.  Each lane makes one scale of either
 // and hands its reciprocal round.
@@ -348,7 +349,7 @@ __device__ __forceinline__ void write8(float* p, uint2 x, uint2 y) {
 }
 
 // Bound by the writes: 4 prompts of 100 documents of 32 to 256 tokens in bf16 60 us, 93 % of the copy bandwidth (a lane's stores 16 bytes; with a
-// warp to a row 99).  Lanes as in the write.
+// warp to a row 99); in fp32 133, 76 %.  Lanes as in the write.
 template <typename T, int D>
 __global__ void __launch_bounds__(kIoThreads) cache_read_kernel(IoArgs a) {
   using L = Layout<D>;

@@ -4,10 +4,13 @@
 // row) pairs; its warps take equal parts of those pages, whatever documents they belong to, and keep a running (maximum, sum) per
 // pair and document.  The pairs of a prompt's documents are merged by the kernel that merges those of doc_scores, or, where a prompt
 // has few pages, at the end by the CTAs themselves: one per KV head with all documents, a cluster for a prompt.
-// The floor is the read of the keys (72 bytes per token and KV head at head_dim 128); bound by instructions, as the attention of few rows
-// is.  16 prompts of 100 documents of 32 to 256 tokens, two rows of 32 heads on 8: 49 us, 2.6 TB/s; one prompt of 5 documents
-// 7.6.  (Up to 64 documents at a time, not 32, so that no CTA has a second batch: 48.5 and 9.2; two batches as long as each other:
-// 49.6.)
+// The floor is the read of the keys (72 bytes per token and KV head at head_dim 128).  Bound by latency, as the attention of few rows is: 50 %
+// of the issue slots, 45 % of the ALU pipe, where the instructions of products and softmax alone (cache_attn.cu) would take 22 us.
+// 16 prompts of 100 documents of 32 to 256 tokens, two rows of 32 heads on 8: 50 us, 2.6 TB/s; one prompt of 5 documents 7.9.  (Up to 64
+// documents at a time, not 32, so that no CTA has a second batch: 48.5 and 9.2, where these took 49 and 7.6; two batches as long as each
+// other: 49.6.)
+// A document is never divided between CTAs: few long ones take as long as the longest does on a CTA per KV head (one prompt of a document
+// of 100,000 tokens 317 us, its bytes 9; of four of 8,000 34 us, its bytes 3).
 #include <algorithm>
 #include <atomic>
 #include <type_traits>
