@@ -975,9 +975,11 @@ def _attention_of_long(q, hk, hv, table, start, length, scale, q_len):
 @pytest.mark.parametrize("dtype,N,Nk,D,R,pages,B", [
     (BF16, 4, 2, 64, 1, 300, 1800), (BF16, 4, 2, 128, 2, 300, 1800), (BF16, 8, 2, 128, 2, 300, 1800), (BF16, 6, 2, 64, 5, 300, 1200),
     (F32, 4, 2, 64, 1, 300, 1200), (F32, 2, 1, 64, 8, 300, 2400), (F32, 6, 2, 128, 2, 300, 1200),
-    (BF16, 4, 2, 128, 20, 700, 600), (BF16, 4, 2, 64, 70, 700, 600)])
+    (BF16, 4, 2, 128, 20, 700, 600), (BF16, 4, 2, 64, 70, 700, 600),
+    # fewer prompts: two long shares each, joined by a cluster (few rows) or a kernel (many), or ten, joined by a kernel
+    (BF16, 4, 2, 64, 1, 300, 111), (F32, 4, 2, 128, 3, 300, 74), (BF16, 4, 2, 128, 20, 1100, 37), (BF16, 4, 2, 64, 70, 1100, 37), (BF16, 2, 1, 64, 1, 1500, 44)])
 def test_shares_of_more_pages_than_a_cta_knows_of_at_a_time(dtype, N, Nk, D, R, pages, B):
-    """So many prompts that each is one share, of pages that are looked at in several goes: blocks that end and begin where those do,
+    """Shares of pages that are looked at in several goes, first so many prompts that each is one share: blocks that end and begin where those do,
     a whole go without a token, prompts far shorter than the table, a page that does not exist.  (The prompts are 10 in turn.)"""
     T, at = pages * PAGE, lambda page, more=0: page * PAGE + more
     go = 256 if pages > 300 else 128
@@ -1018,6 +1020,20 @@ def test_shares_of_more_pages_than_a_cta_knows_of_at_a_time(dtype, N, Nk, D, R, 
     assert torch.equal(out2[same.cuda()], out[same.cuda()]) and torch.equal(lse2[same.cuda()], lse[same.cuda()])
     ref, ref_lse, size = _attention_of_long(q[:2], hk, hv, kept, start[:2], length[:2], D ** -0.5, q_len[:2])
     _check(out2[K:K + 2], lse2[K:K + 2], ref, ref_lse, size, hv, 3 * pages + 8)
+    # NaN in the value of the last slot but one, in one head and 32 channels: in the rows that see it, and in nothing else of theirs
+    at = ch.slots_of(table[0], torch.tensor([T - 2]))[None].int().cuda()
+    k1, v1 = ops.cache_read(cache, at, F32)
+    v1[:, 0, 0, 5] = torch.nan
+    ops.cache_write(k1, v1, cache, at)
+    bad, bad_lse = ops.cache_attention(*args, q_len=rep(q_len), return_lse=True)
+    ends, i = (start + length)[:, -1:], torch.arange(R)[None]
+    sees = (start[:, -1:] <= T - 2) & (ends - q_len[:, None] + i >= T - 2) & (i < q_len[:, None])  # (K, R)
+    want = out[:K].clone()
+    want[:, :, :N // Nk, :32] = torch.where(sees[:, :, None, None].cuda(), torch.nan, want[:, :, :N // Nk, :32])
+    assert bool(sees.any()) and torch.equal(bad_lse, lse)
+    assert torch.equal(bad[:K].isnan(), want.isnan()) and torch.equal(bad[:K].nan_to_num(), want.nan_to_num())
+    assert torch.equal(bad.nan_to_num(), rep(bad[:K]).nan_to_num())
+    ops.check_status()
 
 
 @pytest.mark.parametrize("dtype,N,Nk,D,T", [(BF16, 4, 1, 64, 40000), (BF16, 8, 2, 128, 18000), (F32, 2, 1, 64, 20000)])
